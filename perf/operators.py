@@ -143,11 +143,11 @@ def _quantized(W, group, zeros):
     w = torch.nn.functional.pad(W.float(), (0, groups * group - K)).view(N, groups, group)
     if zeros:
         lo, hi = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
-        scale = ((hi - lo) / 15).to(W.dtype)
+        scale = ((hi - lo) * (1 / 15)).to(W.dtype)
         s = scale.float()
         zero = torch.where(s > 0, torch.round(-lo / s), 0.0).clamp(0, 15)
     else:
-        scale = (w.abs().amax(-1) / 7).to(W.dtype)
+        scale = (w.abs().amax(-1) * (1 / 7)).to(W.dtype)
         s = scale.float()
         zero = torch.full_like(s, 8.0)
     q = torch.where(s[..., None] > 0, torch.round(w / s[..., None]), 0.0) + zero[..., None]
