@@ -64,7 +64,8 @@ enum {
                                  whose conversion maps NaN to 0: there C is 0, and
                                  only this status tells it from a valid result */
     OZK_ERR_TOO_LARGE = -10   /* (ozk_matmul_static) the call needs more scratch than
-                                 OZK_STATIC_SCRATCH_BYTES */
+                                 OZK_STATIC_SCRATCH_BYTES; (products for linear
+                                 layers) rows too far apart or too many tiles */
 };
 
 /* The reference's ozaki_matmul asserts num_splits <= 4 (ozaki_triton.py:563),
@@ -251,6 +252,94 @@ int ozk_matmul_static(const void *A, const int64_t a_strides[3], const void *B,
                       const int64_t b_strides[3], int dtype, int64_t batch, int64_t M,
                       int64_t N, int64_t K, int num_splits, int slice_dtype, void *C,
                       const int64_t c_strides[3], void *const events[4], void *stream);
+
+/*
+ * Products for a model's linear layers -- no counterpart in the reference.
+ * The same conventions: device pointers, sizes and strides in elements, an
+ * asynchronous call on `stream`, a status; nothing is allocated.
+ *
+ * Grouped matmul: rows offsets[g] .. offsets[g + 1] of A are multiplied with
+ * matrix g of B (a layer of experts, the rows sorted by expert).
+ *   A [T, K], rows a_stride apart, K contiguous; B [G, K, N], strides
+ *   b_strides, N or K contiguous; C [T, N], rows c_stride apart; all of
+ *   dtype OZK_F16 or OZK_BF16, summed in fp32 and rounded once.
+ *   offsets [G + 1] on the device, not decreasing, of 4 or 8 bytes each
+ *   (offset_bytes); rows of no group get zeros.  Values outside [0, T] are
+ *   taken as 0 or T.
+ * The gradient to A is the same call with C's gradient and the transposed
+ * strides of B; ozk_grouped_matmul_wgrad gives the one to B:
+ *   dB[g] = A[rows of g]^T D[rows of g], D [T, N] the gradient of C; dB
+ *   [G, K, N] with N contiguous, strides db_strides[2] of group and row, zeros
+ *   for a group without rows.  Workspace: partial sums where few tiles share
+ *   many rows, 0 bytes otherwise.
+ * Rows longer than 2^22 elements apart return OZK_ERR_TOO_LARGE.
+ */
+int ozk_grouped_matmul(const void *A, int64_t a_stride, const void *B, const int64_t b_strides[3],
+                       const void *offsets, int offset_bytes, int64_t T, int64_t K, int64_t N,
+                       int64_t G, int dtype, void *C, int64_t c_stride, void *stream);
+
+int ozk_grouped_matmul_wgrad_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t G,
+                                             size_t *bytes_out);
+
+int ozk_grouped_matmul_wgrad(const void *A, int64_t a_stride, const void *D, int64_t d_stride,
+                             const void *offsets, int offset_bytes, int64_t T, int64_t K,
+                             int64_t N, int64_t G, int dtype, void *dB,
+                             const int64_t db_strides[2], void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/*
+ * 4-bit weights: W[n, k] = (q[n, k] - z[n, k / group]) s[n, k / group].
+ *   packed  [N] rows of packed_stride bytes, 16-byte aligned, at least K / 2
+ *           rounded up to whole 16 bytes: q of 0 .. 15, k even in the low half
+ *           of byte k / 2
+ *   scales  [N, ceil(K / group)], rows s_stride apart
+ *   zeros   the same of uint8 (0 .. 15), or NULL: z = 8
+ *   group   32, 64 or 128
+ * ozk_quantize_w4 makes it from W [N, K] (OZK_F32, OZK_F16 or OZK_BF16, K
+ * contiguous): s = max |w| / 7, or with zeros the range of w with 0 over 15,
+ * rounded to W's type, which is the scales'; ozk_dequantize_w4 gives W back,
+ * rounded to its type (scales of that type or fp32).  NaN weights count as 0.
+ * ozk_matmul_w4: y [M, N] = x [M, K] W^T, x and y of one type, scales of that
+ * type or fp32, summed in fp32 (fp32 x as three bf16 slices), rounded once.  A
+ * row of x with an infinity or NaN gives a row of NaN.
+ * Workspace: partial sums where a few rows of W share a long K.
+ */
+int ozk_quantize_w4(const void *W, int dtype, int64_t N, int64_t K, int64_t w_stride, int group,
+                    void *packed, int64_t packed_stride, void *scales, int64_t s_stride,
+                    void *zeros, int64_t z_stride, void *stream);
+
+int ozk_dequantize_w4(const void *packed, int64_t packed_stride, const void *scales,
+                      int scale_dtype, int64_t s_stride, const void *zeros, int64_t z_stride,
+                      int group, int64_t N, int64_t K, void *W, int dtype, int64_t w_stride,
+                      void *stream);
+
+int ozk_matmul_w4_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K, int group,
+                                  size_t *bytes_out);
+
+int ozk_matmul_w4(const void *x, int dtype, int64_t x_stride, const void *packed,
+                  int64_t packed_stride, const void *scales, int scale_dtype, int64_t s_stride,
+                  const void *zeros, int64_t z_stride, int group, int64_t M, int64_t N, int64_t K,
+                  void *y, int64_t y_stride, void *workspace, size_t workspace_bytes,
+                  void *stream);
+
+/*
+ * Orthogonalisation by Newton-Schulz products (an optimiser's update of a
+ * weight matrix): X = G / (|G|_F + eps), then for every step with its
+ * coefficients (a, b, c)
+ *   A = X X^T,  X <- a X + (b A + c A A) X      (X transposed where M > N)
+ *   G, out  [batch, M, N] of OZK_F32, OZK_F16 or OZK_BF16, N contiguous,
+ *           strides of batch and row
+ *   coefficients  host memory, 3 * steps
+ * The products are fp32-grade: two fp16 slices of each matrix, three of the
+ * four slice pairs, sums in fp32.
+ */
+int ozk_orthogonalize_workspace_bytes(int64_t batch, int64_t M, int64_t N, int steps,
+                                      size_t *bytes_out);
+
+int ozk_orthogonalize(const void *G, int dtype, int64_t batch, int64_t M, int64_t N,
+                      const int64_t g_strides[2], const double *coefficients, int steps,
+                      double eps, void *out, const int64_t o_strides[2], void *workspace,
+                      size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

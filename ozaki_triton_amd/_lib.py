@@ -43,6 +43,15 @@ EXPORTED = (
     "ozk_matmul_static",
     "ozk_cross_gemm_pairs",
     "ozk_matmul_pairs",
+    "ozk_grouped_matmul",
+    "ozk_grouped_matmul_wgrad_workspace_bytes",
+    "ozk_grouped_matmul_wgrad",
+    "ozk_quantize_w4",
+    "ozk_dequantize_w4",
+    "ozk_matmul_w4_workspace_bytes",
+    "ozk_matmul_w4",
+    "ozk_orthogonalize_workspace_bytes",
+    "ozk_orthogonalize",
 )
 
 # the test hooks of include/ozaki_amd_debug.h
@@ -116,6 +125,22 @@ def load() -> ctypes.CDLL:
     L.ozk_matmul_pairs.argtypes = [vp, p64, vp, p64, i32, i64, i64, i64, i64, i32, i32, i32, vp,
                                    p64, vp, sz, ctypes.POINTER(ctypes.c_void_p), vp]
     L.ozk_matmul_pairs.restype = i32
+    psz, pd = ctypes.POINTER(sz), ctypes.POINTER(ctypes.c_double)
+    for name, args in (
+            ("ozk_grouped_matmul", [vp, i64, vp, p64, vp, i32, i64, i64, i64, i64, i32, vp, i64, vp]),
+            ("ozk_grouped_matmul_wgrad_workspace_bytes", [i64, i64, i64, i64, psz]),
+            ("ozk_grouped_matmul_wgrad", [vp, i64, vp, i64, vp, i32, i64, i64, i64, i64, i32, vp,
+                                          p64, vp, sz, vp]),
+            ("ozk_quantize_w4", [vp, i32, i64, i64, i64, i32, vp, i64, vp, i64, vp, i64, vp]),
+            ("ozk_dequantize_w4", [vp, i64, vp, i32, i64, vp, i64, i32, i64, i64, vp, i32, i64, vp]),
+            ("ozk_matmul_w4_workspace_bytes", [i32, i64, i64, i64, i32, psz]),
+            ("ozk_matmul_w4", [vp, i32, i64, vp, i64, vp, i32, i64, vp, i64, i32, i64, i64, i64, vp,
+                               i64, vp, sz, vp]),
+            ("ozk_orthogonalize_workspace_bytes", [i64, i64, i64, i32, psz]),
+            ("ozk_orthogonalize", [vp, i32, i64, i64, i64, p64, pd, i32, ctypes.c_double, vp, p64,
+                                   vp, sz, vp])):
+        fn = getattr(L, name)
+        fn.argtypes, fn.restype = args, i32
     cp = ctypes.c_char_p
     L.ozk_debug_force_gemm_kernel.argtypes = [cp]
     L.ozk_debug_force_gemm_kernel.restype = i32

@@ -27,7 +27,8 @@ ARCH = os.environ.get("OZK_OFFLOAD_ARCH", "gfx950")
 # (the int8 cross-GEMM one is the largest), so that they compile in parallel
 SOURCES = ["ozk_gemm_i8.hip", "ozk_gemm_f16.hip", "ozk_gemm_bf16.hip", "ozk_gemm_f32.hip",
            "ozk_split_i8.hip", "ozk_split_f16.hip", "ozk_split_bf16.hip", "ozk_split_f32.hip",
-           "ozk_split.hip", "ozk_api.cpp", "ozk_gemm.hip"]
+           "ozk_split.hip", "ozk_api.cpp", "ozk_gemm.hip",
+           "ozk_grouped.hip", "ozk_w4.hip", "ozk_orth.hip", "ozk_linear_api.cpp"]
 
 COMMON_FLAGS = [
     f"--offload-arch={ARCH}",

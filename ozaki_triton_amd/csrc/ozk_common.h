@@ -1,6 +1,6 @@
-// ozk_common.h -- device arithmetic shared by the split and cross-GEMM kernels.
+// ozk_common.h -- device arithmetic and waits shared by the kernels.
 //
-// Every helper reproduces one rounding step of the reference exactly (IEEE
+// Every arithmetic helper reproduces one rounding step of the reference exactly (IEEE
 // binary32/binary64, round-to-nearest-even, denormals kept).  The library is
 // compiled with -ffp-contract=off so that no multiply-add pair is fused where
 // the reference rounds the product.
@@ -91,5 +91,18 @@ OZK_DEV uint32_t f32_to_bf16_bits(float x) {
     return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
 }
 OZK_DEV float bf16_bits_to_f32(uint32_t h) { return __uint_as_float(h << 16); }
+
+// s_waitcnt with only the vector-memory counter limited to n
+template <int N> OZK_DEV void wait_vmcnt() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0xF << 8) | ((N >> 4) << 14));
+}
+
+// Workgroup execution barrier without the release fence of __syncthreads()
+// (which would wait for every outstanding global load, i.e. drain the DMA
+// prefetch ring).  Callers make their own DMA writes complete with
+// wait_vmcnt first; the memory clobber keeps the compiler from moving LDS
+// accesses across the barrier.
+OZK_DEV void exec_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 }  // namespace ozk

@@ -438,19 +438,6 @@ template <int RB> OZK_DEV int rswz(int r, int c) {
     else return r * 128 + ((c ^ ((r >> 1) & 7)) << 4);
 }
 
-// s_waitcnt with only the vector-memory counter limited to n
-template <int N> OZK_DEV void wait_vmcnt() {
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0xF << 8) | ((N >> 4) << 14));
-}
-
-// Workgroup execution barrier without the release fence of __syncthreads()
-// (which would wait for every outstanding global load, i.e. drain the DMA
-// prefetch ring).  Callers make their own DMA writes complete with
-// wait_vmcnt first; the memory clobber keeps the compiler from moving LDS
-// accesses across the barrier.
-OZK_DEV void exec_barrier() { asm volatile("s_barrier" ::: "memory"); }
-
 // ---------------------------------------------------------------------------
 // Split-K hand-off (ring and wide kernels on grids too small to fill the
 // chip).  A tile's 128-byte K stages are cut into p.ksplit ranges of

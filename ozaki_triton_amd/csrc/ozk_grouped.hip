@@ -1,0 +1,269 @@
+// ozk_grouped.hip -- matrix products grouped by expert, with ragged groups.
+//
+// Rows offsets[g] .. offsets[g + 1] of A belong to group g, whose matrix they
+// are multiplied with; the offsets stay on the device, so the grid is the most
+// tiles that T rows in G groups can need and a workgroup finds its group from
+// the offsets (one wave-wide prefix sum of the groups' tile counts).
+// Workgroups past the last tile end at once.
+#include "ozk_linear.h"
+#include "ozk_tile.h"
+
+namespace ozk {
+
+// offsets[i] clamped to [0, T]: whatever the tensor holds, no row outside the
+// operands is touched
+OZK_DEV int64_t offset_at(const void *offsets, int wide, int64_t i, int64_t T) {
+    const int64_t v = wide ? ((const int64_t *)offsets)[i] : (int64_t)((const int32_t *)offsets)[i];
+    return v < 0 ? 0 : v > T ? T : v;
+}
+
+OZK_DEV int wave_sum_before(int v, int lane) {   // inclusive prefix sum over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(v, d);
+        if (lane >= d) v += u;
+    }
+    return v;
+}
+
+// The groups with the rows before the first (segment 0) and after the last
+// (segment G + 1), which have no group: segment s spans lo .. hi.
+struct Segment {
+    int64_t s, lo, hi;
+};
+OZK_DEV Segment segment_at(const GroupedParams &p, int64_t s) {
+    const int64_t lo = s == 0 ? 0 : offset_at(p.offsets, p.offsets64, s - 1, p.T);
+    const int64_t hi = s == p.G + 1 ? p.T : offset_at(p.offsets, p.offsets64, s, p.T);
+    return {s, lo, hi < lo ? lo : hi};
+}
+
+template <typename ST, typename Sh, bool DMA>
+__global__ __launch_bounds__(Sh::THREADS) void grouped_kernel(GroupedParams p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63;
+    constexpr int BM = Sh::BM, BN = Sh::BN;
+    const uint32_t tiles_n = (uint32_t)((p.N + BN - 1) / BN);
+
+    // tiles along the rows, all segments
+    const int64_t segs = p.G + 2;
+    uint32_t total = 0;
+    for (int64_t s0 = 0; s0 < segs; s0 += 64) {
+        int n = 0;
+        if (s0 + lane < segs) {
+            const Segment g = segment_at(p, s0 + lane);
+            n = (int)((g.hi - g.lo + BM - 1) / BM);
+        }
+        total += (uint32_t)__builtin_amdgcn_readlane(wave_sum_before(n, lane), 63);
+    }
+    const int64_t tile = xcd_tile(blockIdx.x, total * tiles_n);
+    if (tile < 0) return;
+    const uint32_t tm = (uint32_t)tile / tiles_n, tn = (uint32_t)tile - tm * tiles_n;
+
+    // the segment that holds tile row tm
+    int64_t seg = 0, lo = 0, hi = 0;
+    uint32_t before = 0;
+    for (int64_t s0 = 0; s0 < segs; s0 += 64) {
+        Segment g = {0, 0, 0};
+        int n = 0;
+        if (s0 + lane < segs) {
+            g = segment_at(p, s0 + lane);
+            n = (int)((g.hi - g.lo + BM - 1) / BM);
+        }
+        const int upto = wave_sum_before(n, lane);
+        const uint64_t past = __ballot(before + (uint32_t)upto > tm);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            seg = s0 + l;
+            lo = __shfl(g.lo, l);
+            hi = __shfl(g.hi, l);
+            lo += (int64_t)(tm - before - (uint32_t)__shfl(upto - n, l)) * BM;
+            break;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+    }
+    const int rows = (int)(hi - lo < BM ? hi - lo : BM);
+    const int64_t n0 = (int64_t)tn * BN;
+    const int cols = (int)(p.N - n0 < BN ? p.N - n0 : BN);
+
+    TileLoop<ST, Sh, DMA> t;
+    const bool none = seg == 0 || seg == p.G + 1;
+    TileSrc A = {p.A + lo * p.a_pitch, p.a_pitch, rows, none ? 0 : p.K * 2};
+    const char *Bg = p.B + (none ? 0 : seg - 1) * p.b_group;
+    TileSrc B = Sh::BCOLS ? TileSrc{Bg + n0 * 2, p.b_pitch, cols * 2, none ? 0 : p.K}
+                          : TileSrc{Bg + n0 * p.b_pitch, p.b_pitch, cols, none ? 0 : p.K * 2};
+    t.run(A, B, smem);
+
+    char *C = p.C + lo * p.c_pitch + n0 * 2;
+    const bool wide = ((p.c_pitch | (int64_t)(uintptr_t)C) & 7) == 0;
+    t.each([&](int m, int n, f32x4 v) {
+        if (m >= rows || n >= cols) return;
+        uint16_t e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = to_bits16(v[i], ST{});
+        uint16_t *to = (uint16_t *)(C + m * p.c_pitch) + n;
+        if (wide && n + 4 <= cols) {
+            i32x2 u;
+            __builtin_memcpy(&u, e, 8);
+            *(i32x2 *)to = u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < cols) to[i] = e[i];
+        }
+    });
+}
+
+// dB: the rows of a group are the contraction, both operands "cols".  With
+// splits > 1 workgroup s of a tile sums the s-th part of the group's rows into
+// the workspace, and grouped_join_kernel adds the parts in order.
+template <typename ST, typename Sh, bool DMA>
+__global__ __launch_bounds__(Sh::THREADS) void grouped_grad_kernel(GroupedGradParams p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int BM = Sh::BM, BN = Sh::BN;
+    const uint32_t tiles_k = (uint32_t)((p.K + BM - 1) / BM);
+    const uint32_t tiles_n = (uint32_t)((p.N + BN - 1) / BN);
+    const uint32_t each = tiles_k * tiles_n;
+    const int64_t tile = xcd_tile(blockIdx.x, each * (uint32_t)p.G * (uint32_t)p.splits);
+    if (tile < 0) return;
+    const uint32_t gs = (uint32_t)tile / each, in = (uint32_t)tile - gs * each;
+    const uint32_t g = gs / (uint32_t)p.splits, s = gs - g * (uint32_t)p.splits;
+    const uint32_t tk = in / tiles_n, tn = in - tk * tiles_n;
+
+    int64_t lo = offset_at(p.offsets, p.offsets64, g, p.T);
+    int64_t hi = offset_at(p.offsets, p.offsets64, g + 1, p.T);
+    if (hi < lo) hi = lo;
+    if (p.splits > 1) {
+        // whole stages each
+        const int64_t stages = (hi - lo + Sh::KS - 1) / Sh::KS;
+        const int64_t per = (stages + p.splits - 1) / p.splits * Sh::KS;
+        lo += per * s;
+        if (lo > hi) lo = hi;
+        if (hi > lo + per) hi = lo + per;
+    }
+    const int64_t k0 = (int64_t)tk * BM, n0 = (int64_t)tn * BN;
+    const int rows = (int)(p.K - k0 < BM ? p.K - k0 : BM);
+    const int cols = (int)(p.N - n0 < BN ? p.N - n0 : BN);
+
+    TileLoop<ST, Sh, DMA> t;
+    const TileSrc A = {p.A + lo * p.a_pitch + k0 * 2, p.a_pitch, rows * 2, hi - lo};
+    const TileSrc B = {p.D + lo * p.d_pitch + n0 * 2, p.d_pitch, cols * 2, hi - lo};
+    t.run(A, B, smem);
+
+    if (p.splits > 1) {
+        float *P = p.part + ((int64_t)s * p.G + g) * p.K * p.N + k0 * p.N + n0;
+        t.each([&](int m, int n, f32x4 v) {
+            if (m >= rows) return;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < cols) P[(int64_t)m * p.N + n + i] = v[i];
+        });
+        return;
+    }
+    char *C = p.dB + (int64_t)g * p.db_group + k0 * p.db_pitch + n0 * 2;
+    const bool wide = ((p.db_pitch | (int64_t)(uintptr_t)C) & 7) == 0;
+    t.each([&](int m, int n, f32x4 v) {
+        if (m >= rows || n >= cols) return;
+        uint16_t e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = to_bits16(v[i], ST{});
+        uint16_t *to = (uint16_t *)(C + m * p.db_pitch) + n;
+        if (wide && n + 4 <= cols) {
+            i32x2 u;
+            __builtin_memcpy(&u, e, 8);
+            *(i32x2 *)to = u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < cols) to[i] = e[i];
+        }
+    });
+}
+
+template <typename ST>
+__global__ __launch_bounds__(256) void grouped_join_kernel(GroupedGradParams p) {
+    const int64_t each = p.K * p.N, all = p.G * each;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all;
+         i += (int64_t)gridDim.x * 256) {
+        float v = 0.f;
+        for (int s = 0; s < p.splits; ++s) v += p.part[s * all + i];
+        const int64_t g = i / each, r = (i - g * each) / p.N, c = i - g * each - r * p.N;
+        ((uint16_t *)(p.dB + g * p.db_group + r * p.db_pitch))[c] = to_bits16(v, ST{});
+    }
+}
+
+namespace {
+
+template <typename ST, typename Sh, bool DMA>
+hipError_t grouped_go(const GroupedParams &p, hipStream_t st) {
+    // most tiles: every segment may end inside one
+    const int64_t segs = p.G + 2 < p.T ? p.G + 2 : p.T;
+    const int64_t tiles = (p.T / Sh::BM + segs) * ((p.N + Sh::BN - 1) / Sh::BN);
+    if (tiles >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
+    if (hipError_t e = allow_lds<&grouped_kernel<ST, Sh, DMA>>(Sh::LDS_BYTES); e != hipSuccess)
+        return e;
+    grouped_kernel<ST, Sh, DMA><<<dim3((uint32_t)((tiles + 7) / 8 * 8)), Sh::THREADS, Sh::LDS_BYTES, st>>>(p);
+    return hipGetLastError();
+}
+
+template <typename ST, typename Sh, bool DMA>
+hipError_t grad_go(const GroupedGradParams &p, hipStream_t st) {
+    const int64_t tiles = ((p.K + Sh::BM - 1) / Sh::BM) * ((p.N + Sh::BN - 1) / Sh::BN) * p.G *
+                          p.splits;
+    if (tiles >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
+    if (hipError_t e = allow_lds<&grouped_grad_kernel<ST, Sh, DMA>>(Sh::LDS_BYTES);
+        e != hipSuccess)
+        return e;
+    grouped_grad_kernel<ST, Sh, DMA><<<dim3((uint32_t)((tiles + 7) / 8 * 8)), Sh::THREADS, Sh::LDS_BYTES, st>>>(p);
+    return hipGetLastError();
+}
+
+template <typename ST, bool BCOLS> hipError_t grouped_plan(const GroupedParams &p, hipStream_t st) {
+    const bool pieces = (((uintptr_t)p.A | (uintptr_t)p.B | p.a_pitch | p.b_pitch | p.b_group |
+                          p.K * 2 | (BCOLS ? p.N * 2 : 0)) & 15) == 0;
+    const int64_t rows = p.T / (p.G > 0 ? p.G : 1);
+    if (pieces) {
+        if (rows >= 256) return grouped_go<ST, TileShape<1, false, BCOLS, 256, 256, 2, 4, 2>, true>(p, st);
+        if (rows >= 48) return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 2, 2>, true>(p, st);
+        return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 4>, true>(p, st);
+    }
+    if (rows >= 48) return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 2, 2>, false>(p, st);
+    return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 2>, false>(p, st);
+}
+
+template <typename ST> hipError_t grad_plan(const GroupedGradParams &p, hipStream_t st) {
+    const bool pieces = (((uintptr_t)p.A | (uintptr_t)p.D | p.a_pitch | p.d_pitch | p.K * 2 |
+                          p.N * 2) & 15) == 0;
+    hipError_t e;
+    if (pieces && p.K * p.N * p.G >= (int64_t)256 * 256 * 256)
+        e = grad_go<ST, TileShape<1, true, true, 256, 256, 2, 4, 2>, true>(p, st);
+    else if (pieces)
+        e = grad_go<ST, TileShape<1, true, true, 128, 128, 2, 2, 2>, true>(p, st);
+    else
+        e = grad_go<ST, TileShape<1, true, true, 128, 128, 2, 2, 2>, false>(p, st);
+    if (e != hipSuccess || p.splits == 1) return e;
+    const int64_t all = p.G * p.K * p.N;
+    const int64_t blocks = (all + 255) / 256 < 2048 ? (all + 255) / 256 : 2048;
+    grouped_join_kernel<ST><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_grouped(const GroupedParams &p, int dtype, hipStream_t st) {
+    if (dtype == 2) return p.b_cols ? grouped_plan<_Float16, true>(p, st) : grouped_plan<_Float16, false>(p, st);
+    return p.b_cols ? grouped_plan<__bf16, true>(p, st) : grouped_plan<__bf16, false>(p, st);
+}
+
+int grouped_grad_splits(int64_t T, int64_t K, int64_t N, int64_t G) {
+    const int64_t tiles = ((K + 127) / 128) * ((N + 127) / 128) * G;
+    const int64_t stages = (T / (G > 0 ? G : 1) + 63) / 64;
+    int s = 1;
+    while (s < 16 && tiles * s < 256 && stages / (2 * s) >= 8) s *= 2;
+    return s;
+}
+
+hipError_t launch_grouped_grad(const GroupedGradParams &p, int dtype, hipStream_t st) {
+    return dtype == 2 ? grad_plan<_Float16>(p, st) : grad_plan<__bf16>(p, st);
+}
+
+}  // namespace ozk

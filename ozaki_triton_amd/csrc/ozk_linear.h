@@ -1,0 +1,111 @@
+// ozk_linear.h -- parameter blocks and launchers of the operators for linear
+// layers, shared between their C entry points (ozk_linear_api.cpp) and their
+// kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <atomic>
+
+namespace ozk {
+
+// Raises kernel K's dynamic-LDS limit where `bytes` needs it, once per device.
+template <auto K> hipError_t allow_lds(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    if (bytes <= 64 * 1024) return hipSuccess;
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(
+        (const void *)K, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+// C[t, n] = sum_k A[t, k] B[g(t), k, n] with rows offsets[g] .. offsets[g + 1]
+// of group g; rows of no group get zeros.
+struct GroupedParams {
+    const char *A;          // [T, K], rows of a_pitch bytes
+    const char *B;          // [G] matrices, b_group bytes apart; rows of b_pitch bytes:
+    char *C;                // K rows of N (b_cols) or N rows of K
+    const void *offsets;    // [G + 1], int32 or int64
+    int64_t T, K, N, G;
+    int64_t a_pitch, b_group, b_pitch, c_pitch;
+    int b_cols, offsets64;
+};
+// dB[g, k, n] = sum over the rows t of group g of A[t, k] D[t, n]
+struct GroupedGradParams {
+    const char *A;          // [T, K]
+    const char *D;          // [T, N]
+    char *dB;               // [G, K, N], matrices db_group bytes apart
+    const void *offsets;
+    int64_t T, K, N, G;
+    int64_t a_pitch, d_pitch, db_group, db_pitch;
+    int offsets64;
+    float *part;            // workspace: partial sums of the row ranges (splits > 1)
+    int splits;
+};
+// dtype: 2 fp16, 3 bf16
+hipError_t launch_grouped(const GroupedParams &p, int dtype, hipStream_t st);
+hipError_t launch_grouped_grad(const GroupedGradParams &p, int dtype, hipStream_t st);
+int grouped_grad_splits(int64_t T, int64_t K, int64_t N, int64_t G);
+
+
+// y[m, n] = sum_k x[m, k] (q[n, k] - z[n, k / group]) s[n, k / group]
+struct W4Params {
+    const char *x;            // [M, K], rows of x_pitch elements
+    const uint8_t *packed;    // [N], rows of w_pitch bytes, k even in the low half of byte k / 2
+    const void *scales;       // [N, groups], rows of s_pitch elements
+    const uint8_t *zeros;     // [N, groups], rows of z_pitch; null: every zero point is 8
+    char *y;                  // [M, N], rows of y_pitch elements
+    int64_t M, N, K;
+    int64_t x_pitch, w_pitch, s_pitch, z_pitch, y_pitch;
+    int scales32;             // scales are fp32 (else x's type)
+    int group;                // 32, 64 or 128
+    float *part;              // workspace [splits, M, N] where splits > 1
+    int splits, range;        // K ranges and elements of one (whole chunks of 128)
+    int held;                 // elements of K of x in the LDS at a time
+};
+// dtype: 1 fp32, 2 fp16, 3 bf16
+void plan_w4(W4Params &p, int dtype);
+hipError_t launch_w4(const W4Params &p, int dtype, hipStream_t st);
+
+struct QuantParams {
+    const char *W;            // [N, K], rows of w_pitch elements (null: dequantise into out)
+    char *out;
+    uint8_t *packed;
+    char *scales;             // W's type
+    uint8_t *zeros;           // null: symmetric, zero point 8
+    int64_t N, K, w_pitch, p_pitch, groups, s_pitch, z_pitch;
+    int group;
+};
+hipError_t launch_quantize_w4(const QuantParams &p, int dtype, hipStream_t st);
+hipError_t launch_dequantize_w4(const QuantParams &p, int dtype, int scale_dtype, hipStream_t st);
+
+// Newton-Schulz orthogonalisation of batch matrices G [M, N]; inside, X is
+// [m, n] with m <= n (G transposed where M > N).
+struct OrthStep {            // factors of the products and of what is added, scales included
+    float a_acc;             // A = X X^T
+    float b_a, b_acc;        // B = b A + c A A
+    float x_x, x_acc;        // X' = a X + B X
+};
+struct OrthParams {
+    const char *G;
+    char *out;
+    int64_t batch, M, N;
+    int64_t g_batch, g_row, o_batch, o_row;    // elements
+    double eps;
+    float start_scale;                         // of X's slices at the start, a power of two
+    // workspace
+    double *sums;                              // [batch, blocks] partial sums of squares
+    int blocks;
+    char *X[2], *A, *B;                        // slices
+};
+int orth_blocks(int64_t batch, int64_t M, int64_t N);
+hipError_t launch_orth(const OrthParams &p, const OrthStep *steps, int count, int dtype,
+                       hipStream_t st);
+
+}  // namespace ozk
