@@ -38,13 +38,13 @@ OZK_DEV Segment segment_at(const GroupedParams &p, int64_t s) {
 }
 
 template <typename ST, typename Sh, bool DMA>
-__global__ __launch_bounds__(Sh::THREADS) void grouped_kernel(GroupedParams p) {
+__global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_kernel(GroupedParams p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63;
     constexpr int BM = Sh::BM, BN = Sh::BN;
     const uint32_t tiles_n = (uint32_t)((p.N + BN - 1) / BN);
 
-    // tiles along the rows, all segments
+    // tile rows of all segments
     const int64_t segs = p.G + 2;
     uint32_t total = 0;
     for (int64_t s0 = 0; s0 < segs; s0 += 64) {
@@ -57,11 +57,12 @@ __global__ __launch_bounds__(Sh::THREADS) void grouped_kernel(GroupedParams p) {
     }
     const int64_t tile = xcd_tile(blockIdx.x, total * tiles_n);
     if (tile < 0) return;
-    const uint32_t tm = (uint32_t)tile / tiles_n, tn = (uint32_t)tile - tm * tiles_n;
 
-    // the segment that holds tile row tm
+    // the segment that holds the tile, and in it the order: 8 tile rows at a
+    // time, column by column, so that the workgroups of an XCD share a square
+    // block of both operands in its L2
     int64_t seg = 0, lo = 0, hi = 0;
-    uint32_t before = 0;
+    uint32_t before = 0, tn = 0;
     for (int64_t s0 = 0; s0 < segs; s0 += 64) {
         Segment g = {0, 0, 0};
         int n = 0;
@@ -70,17 +71,26 @@ __global__ __launch_bounds__(Sh::THREADS) void grouped_kernel(GroupedParams p) {
             n = (int)((g.hi - g.lo + BM - 1) / BM);
         }
         const int upto = wave_sum_before(n, lane);
-        const uint64_t past = __ballot(before + (uint32_t)upto > tm);
+        const uint64_t past = __ballot((before + (uint32_t)upto) * tiles_n > (uint32_t)tile);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             seg = s0 + l;
             lo = __shfl(g.lo, l);
             hi = __shfl(g.hi, l);
-            lo += (int64_t)(tm - before - (uint32_t)__shfl(upto - n, l)) * BM;
+            const uint32_t have = (uint32_t)__shfl(n, l);
+            const uint32_t in = (uint32_t)tile - (before + (uint32_t)__shfl(upto, l) - have) * tiles_n;
+            const uint32_t first = in / tiles_n / 8 * 8;
+            const uint32_t high = have - first < 8 ? have - first : 8, at = in - first * tiles_n;
+            tn = at / high;
+            lo += (int64_t)(first + at - tn * high) * BM;
             break;
         }
         before += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
     }
+    seg = uniform(seg);
+    lo = uniform(lo);
+    hi = uniform(hi);
+    tn = (uint32_t)uniform((int)tn);
     const int rows = (int)(hi - lo < BM ? hi - lo : BM);
     const int64_t n0 = (int64_t)tn * BN;
     const int cols = (int)(p.N - n0 < BN ? p.N - n0 : BN);
@@ -117,7 +127,7 @@ __global__ __launch_bounds__(Sh::THREADS) void grouped_kernel(GroupedParams p) {
 // splits > 1 workgroup s of a tile sums the s-th part of the group's rows into
 // the workspace, and grouped_join_kernel adds the parts in order.
 template <typename ST, typename Sh, bool DMA>
-__global__ __launch_bounds__(Sh::THREADS) void grouped_grad_kernel(GroupedGradParams p) {
+__global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_grad_kernel(GroupedGradParams p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int BM = Sh::BM, BN = Sh::BN;
     const uint32_t tiles_k = (uint32_t)((p.K + BM - 1) / BM);
@@ -129,8 +139,8 @@ __global__ __launch_bounds__(Sh::THREADS) void grouped_grad_kernel(GroupedGradPa
     const uint32_t g = gs / (uint32_t)p.splits, s = gs - g * (uint32_t)p.splits;
     const uint32_t tk = in / tiles_n, tn = in - tk * tiles_n;
 
-    int64_t lo = offset_at(p.offsets, p.offsets64, g, p.T);
-    int64_t hi = offset_at(p.offsets, p.offsets64, g + 1, p.T);
+    int64_t lo = uniform(offset_at(p.offsets, p.offsets64, g, p.T));
+    int64_t hi = uniform(offset_at(p.offsets, p.offsets64, g + 1, p.T));
     if (hi < lo) hi = lo;
     if (p.splits > 1) {
         // whole stages each

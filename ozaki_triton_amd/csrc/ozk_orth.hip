@@ -109,7 +109,7 @@ struct OrthGemm {
 };
 
 template <typename T, int KIND, typename Sh>
-__global__ __launch_bounds__(Sh::THREADS) void orth_gemm_kernel(OrthGemm p) {
+__global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(OrthGemm p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int BM = Sh::BM, BN = Sh::BN;
     constexpr bool kSym = KIND == kOrthA || KIND == kOrthB;
@@ -124,6 +124,7 @@ __global__ __launch_bounds__(Sh::THREADS) void orth_gemm_kernel(OrthGemm p) {
         tm = (uint32_t)((sqrtf(8.f * (float)in + 1.f) - 1.f) * 0.5f);
         while ((uint64_t)tm * (tm + 1) / 2 > in) --tm;
         while ((uint64_t)(tm + 1) * (tm + 2) / 2 <= in) ++tm;
+        tm = (uint32_t)uniform((int)tm);
         tn = in - tm * (tm + 1) / 2;
     } else {
         // 8 tile rows at a time, column by column

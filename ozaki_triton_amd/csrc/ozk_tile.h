@@ -75,7 +75,14 @@ struct TileShape {
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
     static constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
     static constexpr int LP = STAGE / 1024 / WAVES;   // windows per wave and stage
+    // a wave's windows are all A's or all B's where that comes out even, else
+    // LPA of A's and the others of B's
+    static constexpr bool ONE = BM / 8 % LP == 0;
+    static constexpr int LPA = ONE ? 0 : BM / 8 / WAVES;
+    static_assert(ONE || (BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0), "windows per operand");
     static constexpr int LDS_BYTES = NST * STAGE;
+    // waves per SIMD that the registers have to leave room for
+    static constexpr int PER_SIMD = 2;
     static_assert(LP * WAVES * 1024 == STAGE, "windows split evenly over the waves");
     static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "whole 16 x 16 blocks");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS");
@@ -93,25 +100,55 @@ template <int RB> OZK_DEV int cols_swz(int k) {
     else return (k >> 3) & 1;
 }
 
+// a value that is the same in every lane, in scalar registers: the DMA's buffer
+// descriptor and destination have to be there
+OZK_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+OZK_DEV int64_t uniform(int64_t v) {
+    const uint32_t lo = (uint32_t)uniform((int)(uint32_t)v);
+    return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | lo);
+}
+
 // Where lane `lane` of 1 KB window w of an operand reads: byte offset from the
-// stage's base, and its place along K (bytes of the 128 for "rows", the row
-// for "cols") with which the last stage is cut.
+// stage's base, its place along K (bytes of the 128 for "rows", the row for
+// "cols") with which the last stage is cut, and how many bytes there are
+// ("rows": before that cut).
 struct WindowAt {
     uint32_t off;
-    int k;
+    int k, n;
 };
 template <int S, bool COLS, int BX> OZK_DEV WindowAt window_at(const TileSrc &s, int w, int lane) {
     if constexpr (!COLS) {
         const int row = 8 * w + (lane >> 3);
         const int k = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
-        return {row < s.rows ? (uint32_t)(row * s.pitch) + k : kTileOOB, k};
+        const bool ok = row < s.rows;
+        return {ok ? (uint32_t)(row * s.pitch) + k : kTileOOB, k, ok ? 16 : 0};
     } else {
         constexpr int RB = ColsRow<S, BX>::RB;
         const int pos = w * 64 + lane;
         const int k = pos / (RB / 16), c16 = pos % (RB / 16);
         const int col = (((c16 >> 1) ^ cols_swz<RB>(k)) << 5) + (c16 & 1) * 16;
-        return {col < s.rows ? (uint32_t)(k * s.pitch) + col : kTileOOB, k};
+        const int n = s.rows - col < 0 ? 0 : s.rows - col < 16 ? s.rows - col : 16;
+        return {n > 0 ? (uint32_t)(k * s.pitch) + col : kTileOOB, k, n};
     }
+}
+
+// One LDS-DMA instruction: 16 bytes per lane from `base` + off to LDS byte `to`
+// + 16 * lane; zeros where off is past the 2 GiB behind base.  Written in
+// assembly because behind the builtin the compiler waits for every DMA on its
+// way before a ds_read_b64_tr_b16 (measured: 1028 us against 815 without the
+// read-ahead below, 32768 x 2048 x 4096).  It has no register result; its LDS
+// writes are waited for by wait_vmcnt and a barrier like the builtin's.
+OZK_DEV void dma_piece(const char *base, uint32_t off, uint32_t to) {
+    const uint64_t at = (uint64_t)(uintptr_t)base;
+    const i32x4 desc = {uniform((int)(uint32_t)at), uniform((int)(uint32_t)(at >> 32)), 0x7FFFFFFF,
+                        0x00020000};
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 holds nothing else in these kernels
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(uniform((int)to)), "v"(off), "s"(desc)
+                 : "memory", "m0");
+#pragma clang diagnostic pop
 }
 
 // 16 bytes at an address of any alignment, of which the first `n` exist
@@ -131,6 +168,13 @@ OZK_DEV i32x4 load_piece(const char *p, int n) {
     return v;
 }
 
+template <int N, typename F> OZK_DEV void static_for_tile(F &&f) {
+    if constexpr (N > 0) {
+        static_for_tile<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+
 template <typename ST, typename Sh, bool DMA> struct TileLoop {
     static constexpr int S = Sh::S, LP = Sh::LP, MI = Sh::MI, NI = Sh::NI;
     f32x4 acc[MI][NI];
@@ -144,68 +188,87 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-        const int64_t ka = Sh::ACOLS ? Sh::KS : 128, kb_ = Sh::BCOLS ? Sh::KS : 128;
-        const int nka = (int)((A.klen + ka - 1) / ka), nkb_b = (int)((B.klen + kb_ - 1) / kb_);
+        constexpr int ua = Sh::ACOLS ? Sh::KS : 128, ub = Sh::BCOLS ? Sh::KS : 128;
+        const int nka = (int)((A.klen + ua - 1) / ua), nkb_b = (int)((B.klen + ub - 1) / ub);
         const int nkb = nka < nkb_b ? nka : nkb_b;
-        const int64_t stepA = Sh::ACOLS ? Sh::KS * A.pitch : 128;
-        const int64_t stepB = Sh::BCOLS ? Sh::KS * B.pitch : 128;
 
+        // the operands as this wave stages them: base of the stage it is at, and
+        // what is left of K from there on
+        struct Feed {
+            const char *base;
+            int64_t step, left;
+            int unit;
+        };
+        const Feed fa = {A.base, Sh::ACOLS ? Sh::KS * A.pitch : 128, A.klen, ua};
+        const Feed fb = {B.base, Sh::BCOLS ? Sh::KS * B.pitch : 128, B.klen, ub};
+        const bool onlyA = Sh::ONE && wave * LP < Sh::BM / 8;
+        Feed feed[Sh::ONE ? 1 : 2];
+        if constexpr (Sh::ONE) {
+            feed[0] = onlyA ? fa : fb;
+        } else {
+            feed[0] = fa;
+            feed[1] = fb;
+        }
+        constexpr auto of = [](int q) { return Sh::ONE || q < Sh::LPA ? 0 : 1; };   // window q's feed
         WindowAt win[LP];
+        int slot_at[LP];   // its place in a stage
 #pragma unroll
         for (int q = 0; q < LP; ++q) {
-            const int w = wave * LP + q;
-            win[q] = w < Sh::BM / 8
-                         ? window_at<S, Sh::ACOLS, Sh::BM>(A, w, lane)
-                         : window_at<S, Sh::BCOLS, Sh::BN>(B, w - Sh::BM / 8, lane);
+            if constexpr (Sh::ONE) {
+                const int w = wave * LP + q;
+                win[q] = onlyA ? window_at<S, Sh::ACOLS, Sh::BM>(A, w, lane)
+                               : window_at<S, Sh::BCOLS, Sh::BN>(B, w - Sh::BM / 8, lane);
+                slot_at[q] = w * 1024;
+            } else {
+                constexpr int LPB = LP - Sh::LPA;
+                const int w = of(q) == 0 ? wave * Sh::LPA + q : wave * LPB + q - Sh::LPA;
+                win[q] = of(q) == 0 ? window_at<S, Sh::ACOLS, Sh::BM>(A, w, lane)
+                                    : window_at<S, Sh::BCOLS, Sh::BN>(B, w, lane);
+                slot_at[q] = (of(q) == 0 ? w : Sh::BM / 8 + w) * 1024;
+            }
         }
+        auto advance = [&] {
+#pragma unroll
+            for (Feed &f : feed) {
+                f.base += f.step;
+                f.left -= f.unit;
+            }
+        };
 
-        // what is left of K from stage kb on, as win[].k counts it
-        auto left_a = [&](int kb) { return A.klen - kb * ka; };
-        auto left_b = [&](int kb) { return B.klen - kb * kb_; };
-
-        auto issue = [&](int kb) {
-            char *dst = smem + (kb % Sh::NST) * Sh::STAGE + wave * LP * 1024;
-            const __amdgpu_buffer_rsrc_t rA = __builtin_amdgcn_make_buffer_rsrc(
-                (void *)(A.base + kb * stepA), (short)0, 0x7FFFFFFF, 0x00020000);
-            const __amdgpu_buffer_rsrc_t rB = __builtin_amdgcn_make_buffer_rsrc(
-                (void *)(B.base + kb * stepB), (short)0, 0x7FFFFFFF, 0x00020000);
-            const int la = (int)(left_a(kb) < ka ? left_a(kb) : ka);
-            const int lb = (int)(left_b(kb) < kb_ ? left_b(kb) : kb_);
+        // windows q0 .. q1 of stage kb, if there is one; stages come in order
+        const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+        auto issue = [&](int kb, int q0, int q1) {
+            if (kb >= nkb) return;
+            if (q0 == 0 && kb > 0) advance();
+            const uint32_t dst = lds + (uint32_t)(kb % Sh::NST) * Sh::STAGE;
 #pragma unroll
             for (int q = 0; q < LP; ++q) {
-                const bool isA = wave * LP + q < Sh::BM / 8;
-                const uint32_t off = win[q].k < (isA ? la : lb) ? win[q].off : kTileOOB;
-                auto *to = (__attribute__((address_space(3))) void *)(dst + q * 1024);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(isA ? rA : rB, to, 16, off, 0, 0, 0);
+                if (q < q0 || q >= q1) continue;
+                const Feed &f = feed[of(q)];
+                uint32_t off = win[q].off;
+                if (f.left < f.unit && win[q].k >= (int)f.left) off = kTileOOB;
+                dma_piece(f.base, off, dst + slot_at[q]);
             }
         };
         // the same through registers, for rows of any alignment
         i32x4 held[DMA ? 1 : LP];
         auto fetch = [&](int kb) {
+            if (kb > 0) advance();
 #pragma unroll
             for (int q = 0; q < LP; ++q) {
-                const bool isA = wave * LP + q < Sh::BM / 8;
-                const char *base = isA ? A.base + kb * stepA : B.base + kb * stepB;
-                const int64_t left = isA ? left_a(kb) : left_b(kb);
-                const bool cols = isA ? Sh::ACOLS : Sh::BCOLS;
-                int n = 0;
-                if (win[q].off != kTileOOB && win[q].k < left) {
-                    if (cols) {
-                        // the column is what is left of the offset after its row
-                        const int col = (int)(win[q].off - (uint32_t)(win[q].k *
-                                                                      (isA ? A.pitch : B.pitch)));
-                        n = (isA ? A.rows : B.rows) - col;
-                    } else {
-                        n = (int)(left - win[q].k < 16 ? left - win[q].k : 16);
-                    }
-                }
-                held[q] = load_piece(base + (n > 0 ? win[q].off : 0u), n);
+                const Feed &f = feed[of(q)];
+                const bool cols = Sh::ONE ? (onlyA ? Sh::ACOLS : Sh::BCOLS)
+                                          : (of(q) == 0 ? Sh::ACOLS : Sh::BCOLS);
+                const int64_t left = f.left - win[q].k;
+                int n = left > 0 ? win[q].n : 0;
+                if (!cols && left < n) n = (int)left;
+                held[q] = load_piece(f.base + (n > 0 ? win[q].off : 0u), n);
             }
         };
         auto put = [&](int kb) {
-            char *dst = smem + (kb % Sh::NST) * Sh::STAGE + wave * LP * 1024 + lane * 16;
+            char *dst = smem + (kb % Sh::NST) * Sh::STAGE + lane * 16;
 #pragma unroll
-            for (int q = 0; q < LP; ++q) *(i32x4 *)(dst + q * 1024) = held[q];
+            for (int q = 0; q < LP; ++q) *(i32x4 *)(dst + slot_at[q]) = held[q];
         };
 
         const int g = lane >> 4, i16 = lane & 15;
@@ -230,68 +293,131 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 return i32x4{a.x, a.y, b.x, b.y};
             }
         };
-        auto compute = [&](int kb) {
-            const char *bufA = smem + (kb % Sh::NST) * Sh::STAGE;
-            const char *bufB = bufA + Sh::A_BYTES;
-            i32x4 a[2][MI], b[2][NI];
-            auto read = [&](int ks) {
+        // A stage is 2 MI groups of MFMAs: group n multiplies A's fragment (step n
+        // / MI, block n % MI) with B's.  S = 1: a step is one K step, B's fragments
+        // of the step.  S = 2: step 0 is slice h of A with both slices of B, step 1
+        // slice l of A with slice h of B.  A's fragments are read two groups ahead
+        // into a ring of 4; behind the last read of a stage, two groups before its
+        // end, comes the barrier that hands the slot back and the next stage over,
+        // so the next stage's first reads run under the last MFMAs.
+        constexpr int G = 2 * MI, BG = G - 2;
+        static_assert(G % 4 == 0, "the ring goes on from stage to stage");
+        i32x4 a[4], b[2][NI], bn[NI];
+        auto readA = [&](const char *buf, int n, auto n_) {
+            constexpr int N_ = decltype(n_)::value;   // ring place
+            a[N_] = frag(buf, std::integral_constant<bool, Sh::ACOLS>{},
+                         std::integral_constant<int, Sh::BM>{}, wm * MI, n % MI, n / MI);
+        };
+        auto readB = [&](const char *buf, int j, int ks) -> i32x4 {
+            return frag(buf + Sh::A_BYTES, std::integral_constant<bool, Sh::BCOLS>{},
+                        std::integral_constant<int, Sh::BN>{}, wn * NI, j, ks);
+        };
+        auto first = [&](const char *buf) {   // what group 0 of a stage needs
 #pragma unroll
-                for (int j = 0; j < NI; ++j)
-                    b[ks][j] = frag(bufB, std::integral_constant<bool, Sh::BCOLS>{},
-                                    std::integral_constant<int, Sh::BN>{}, wn * NI, j, ks);
+            for (int j = 0; j < NI; ++j) b[0][j] = readB(buf, j, 0);
+            if constexpr (S == 2)
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
-                    a[ks][i] = frag(bufA, std::integral_constant<bool, Sh::ACOLS>{},
-                                    std::integral_constant<int, Sh::BM>{}, wm * MI, i, ks);
-            };
-            auto mul = [&](int ka_, int kb2) {
+                for (int j = 0; j < NI; ++j) b[1][j] = readB(buf, j, 1);
+            readA(buf, 0, std::integral_constant<int, 0>{});
+            readA(buf, 1, std::integral_constant<int, 1>{});
+        };
+        // ready(): stage kb + 1 has landed and every wave has read stage kb;
+        // during(n): what else group n issues
+        auto stage = [&](int kb, auto &&ready, auto &&during) {
+            const char *buf = smem + (kb % Sh::NST) * Sh::STAGE;
+            const char *next = smem + ((kb + 1) % Sh::NST) * Sh::STAGE;
+            static_for_tile<G>([&](auto n_) {
+                constexpr int n = decltype(n_)::value, i = n % MI;
+                if constexpr (n == BG) ready();
+                if constexpr (n + 2 < G) {
+                    readA(buf, n + 2, std::integral_constant<int, (n + 2) % 4>{});
+                    if constexpr (S == 1 && n < MI) {
+                        constexpr int on = MI < BG ? MI : BG, per = (NI + on - 1) / on;
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+                        for (int j = n * per; j < (n + 1) * per && j < NI; ++j)
+                            b[1][j] = readB(buf, j, 1);
+                    }
+                } else {
+                    // the next stage's first fragments
+                    readA(next, n + 2 - G, std::integral_constant<int, (n + 2) % 4>{});
 #pragma unroll
                     for (int j = 0; j < NI; ++j)
-                        acc[i][j] = mfma16(b[kb2][j], a[ka_][i], acc[i][j], ST{});
-            };
-            read(0);
-            if constexpr (S == 1) {
-                mul(0, 0);
-                read(1);
-                mul(1, 1);
-            } else {
-                read(1);
-                mul(0, 0);
-                mul(0, 1);
-                mul(1, 0);
-            }
+                        if (j * 2 / NI == n - BG) {
+                            (S == 1 ? b[0][j] : bn[j]) = readB(next, j, 0);
+                            if (S == 2) b[1][j] = readB(next, j, 1);
+                        }
+                }
+                during(n_);
+                constexpr int r = n % 4;
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    acc[i][j] = mfma16(b[S == 1 ? n / MI : 0][j], a[r], acc[i][j], ST{});
+                if constexpr (S == 2 && n < MI)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j)
+                        acc[i][j] = mfma16(b[1][j], a[r], acc[i][j], ST{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            if constexpr (S == 2)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) b[0][j] = bn[j];
         };
 
         if constexpr (DMA) {
-#pragma unroll
-            for (int s = 0; s < Sh::NST - 1; ++s)
-                if (s < nkb) issue(s);
-            for (int kb = 0; kb < nkb; ++kb) {
-                // the stages issued after kb may still be on their way
-                const int after = nkb - 1 - kb < Sh::NST - 2 ? nkb - 1 - kb : Sh::NST - 2;
-                if (after >= 3) wait_vmcnt<(Sh::NST > 4 ? 3 : 0) * LP>();
-                else if (after == 2) wait_vmcnt<(Sh::NST > 3 ? 2 : 0) * LP>();
-                else if (after == 1) wait_vmcnt<(Sh::NST > 2 ? 1 : 0) * LP>();
+            auto wait = [&](int stages) {   // all but the last `stages` issued ones have landed
+                if (stages >= 4) wait_vmcnt<(Sh::NST > 4 ? 4 : 0) * LP>();
+                else if (stages == 3) wait_vmcnt<(Sh::NST > 3 ? 3 : 0) * LP>();
+                else if (stages == 2) wait_vmcnt<(Sh::NST > 2 ? 2 : 0) * LP>();
+                else if (stages == 1) wait_vmcnt<LP>();
                 else wait_vmcnt<0>();
-                static_assert(Sh::NST <= 5 && 3 * LP < 64, "wait table");
-                __builtin_amdgcn_s_waitcnt(0xC07F);   // this wave's reads of the slot refilled next
+                static_assert(Sh::NST <= 5 && 4 * LP < 64, "wait table");
+            };
+            constexpr int NOW = LP < 2 ? LP : 2;   // windows issued right after the barrier
+#pragma unroll
+            for (int s = 0; s < Sh::NST; ++s) issue(s, 0, LP);
+            if (nkb > 0) {
+                wait(nkb - 1 < Sh::NST - 1 ? nkb - 1 : Sh::NST - 1);
                 exec_barrier();
-                if (kb + Sh::NST - 1 < nkb) issue(kb + Sh::NST - 1);
-                compute(kb);
+                first(smem);
             }
+            for (int kb = 0; kb < nkb; ++kb)
+                stage(
+                    kb,
+                    [&] {
+                        const int left = nkb - 2 - kb;
+                        wait(left < 0 ? 0 : left < Sh::NST - 2 ? left : Sh::NST - 2);
+                        __builtin_amdgcn_s_waitcnt(0xC07F);   // this wave's reads of the slot
+                        exec_barrier();
+                        issue(kb + Sh::NST, 0, NOW);
+                    },
+                    [&](auto n_) {
+                        // the rest of the stage begun behind the last barrier
+                        constexpr int n = decltype(n_)::value;
+                        constexpr int groups = BG > 1 ? BG : 1;
+                        constexpr int per = (LP - NOW + groups - 1) / groups;
+                        if constexpr (n < BG && NOW + n * per < LP)
+                            if (kb > 0) issue(kb - 1 + Sh::NST, NOW + n * per,
+                                              NOW + (n + 1) * per < LP ? NOW + (n + 1) * per : LP);
+                    });
         } else {
             if (nkb > 0) {
                 fetch(0);
                 put(0);
-            }
-            for (int kb = 0; kb < nkb; ++kb) {
                 __syncthreads();
-                if (kb + 1 < nkb) fetch(kb + 1);
-                compute(kb);
-                // (the slot of kb + 1 was read last in step kb - 1, before the barrier)
-                if (kb + 1 < nkb) put(kb + 1);
+                if (nkb > 1) fetch(1);
+                first(smem);
+            }
+            static_assert(DMA || Sh::NST == 2, "two slots");
+            for (int kb = 0; kb < nkb; ++kb) {
+                // stage kb + 1 goes into the slot of kb - 1, read before the last barrier
+                stage(
+                    kb,
+                    [&] {
+                        if (kb + 1 < nkb) put(kb + 1);
+                        __syncthreads();
+                        if (kb + 2 < nkb) fetch(kb + 2);
+                    },
+                    [](auto) {});
             }
         }
     }
