@@ -227,29 +227,53 @@ hipError_t grad_go(const GroupedGradParams &p, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Tiles for T rows in G groups, the counts themselves being on the device: a
+// group is taken to leave half a tile row unused.  The largest tile reads the
+// least per product but wants two rounds of workgroups; smaller groups take
+// the tile that covers most groups whole (each tile row reads the group's
+// matrix again), with more stages in flight where a CU has one workgroup.
+// Measured (us, T x G x K x N, counts uneven, bf16; 256 x 256 / 128 x 128 of 8
+// waves and 4 stages / 64 x 128 of 2 stages / 64 x 64 of 4 / 32 x 64 of 4):
+//     32768 x 16 x 2048 x 4096   570 /  789 /  800 / 1068 / 1357
+//     16384 x 32 x 1024 x 2048   101 /  128 /  112 /  161 /  203
+//     4096 x 8 x 1024 x 4096      69 /   72 /   58 /   85 /  104
+//     1999 x 7 x 1000 x 520       28 /   14 /   13 /   12 /   14
+//     512 x 8 x 1024 x 2048       32 /   16 /   17 /   15 /   14
+//     300 x 8 x 4096 x 4096       96 /   46 /   65 /   64 /   70
+//     200 x 32 x 1024 x 2048      30 /   29 /   23 /   27 /   26
+//     16 x 16 x 1024 x 2048       26 /   13 /   12 /   10 /    9
 template <typename ST, bool BCOLS> hipError_t grouped_plan(const GroupedParams &p, hipStream_t st) {
     const bool pieces = (((uintptr_t)p.A | (uintptr_t)p.B | p.a_pitch | p.b_pitch | p.b_group |
                           p.K * 2 | (BCOLS ? p.N * 2 : 0)) & 15) == 0;
-    const int64_t rows = p.T / (p.G > 0 ? p.G : 1);
-    if (pieces) {
-        if (rows >= 256) return grouped_go<ST, TileShape<1, false, BCOLS, 256, 256, 2, 4, 2>, true>(p, st);
-        if (rows >= 48) return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 2, 2>, true>(p, st);
-        return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 4>, true>(p, st);
+    const int64_t groups = p.G < 1 ? 1 : p.G < p.T ? p.G : p.T, rows = p.T / groups;
+    auto tiles = [&](int64_t bm, int64_t bn) {
+        return (p.T / bm + (groups + 1) / 2) * ((p.N + bn - 1) / bn);
+    };
+    if (!pieces) {
+        if (rows >= 48) return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 2, 2>, false>(p, st);
+        return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 2>, false>(p, st);
     }
-    if (rows >= 48) return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 2, 2>, false>(p, st);
-    return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 2>, false>(p, st);
+    if (rows >= 192 && tiles(256, 256) >= 512)
+        return grouped_go<ST, TileShape<1, false, BCOLS, 256, 256, 2, 4, 2>, true>(p, st);
+    if (rows > 24 && rows <= 128 && p.K * p.N >= (int64_t)1 << 22 && tiles(128, 128) >= 128)
+        return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 4, 4>, true>(p, st);
+    if (tiles(64, 128) >= 256)
+        return grouped_go<ST, TileShape<1, false, BCOLS, 64, 128, 1, 4, 2>, true>(p, st);
+    if (rows >= 8) return grouped_go<ST, TileShape<1, false, BCOLS, 64, 64, 2, 2, 4>, true>(p, st);
+    return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 4>, true>(p, st);
 }
 
 template <typename ST> hipError_t grad_plan(const GroupedGradParams &p, hipStream_t st) {
     const bool pieces = (((uintptr_t)p.A | (uintptr_t)p.D | p.a_pitch | p.d_pitch | p.K * 2 |
                           p.N * 2) & 15) == 0;
+    const int64_t large = ((p.K + 255) / 256) * ((p.N + 255) / 256) * p.G;
     hipError_t e;
-    if (pieces && p.K * p.N * p.G >= (int64_t)256 * 256 * 256)
-        e = grad_go<ST, TileShape<1, true, true, 256, 256, 2, 4, 2>, true>(p, st);
-    else if (pieces)
-        e = grad_go<ST, TileShape<1, true, true, 128, 128, 2, 2, 2>, true>(p, st);
-    else
+    if (!pieces)
         e = grad_go<ST, TileShape<1, true, true, 128, 128, 2, 2, 2>, false>(p, st);
+    else if (large >= 192)
+        e = grad_go<ST, TileShape<1, true, true, 256, 256, 2, 4, 2>, true>(p, st);
+    else
+        e = grad_go<ST, TileShape<1, true, true, 64, 128, 1, 4, 2>, true>(p, st);
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t all = p.G * p.K * p.N;
     const int64_t blocks = (all + 255) / 256 < 2048 ? (all + 255) / 256 : 2048;

@@ -203,9 +203,9 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
 
 namespace {
 
-template <typename T, int KIND, int BM, int WM, int WN>
+template <typename T, int KIND, int BM, int WM, int WN, int NST>
 hipError_t orth_gemm(OrthGemm q, int64_t batch, hipStream_t st) {
-    using Sh = TileShape<2, false, KIND >= kOrthX, BM, BM, WM, WN, 2>;
+    using Sh = TileShape<2, false, KIND >= kOrthX, BM, BM, WM, WN, NST>;
     q.tiles_m = (q.m + BM - 1) / BM;
     q.tiles_n = ((KIND >= kOrthX ? q.n : q.m) + BM - 1) / BM;
     const int64_t tiles = batch * (KIND >= kOrthX ? q.tiles_m * q.tiles_n
@@ -226,9 +226,17 @@ hipError_t orth_product(const OrthGemm &q, int64_t batch, hipStream_t st) {
         const int64_t tm = (q.m + bm - 1) / bm, tn = (cols + bm - 1) / bm;
         return batch * (KIND >= kOrthX ? tm * tn : tm * (tm + 1) / 2);
     };
-    if (tiles(256) >= 192) return orth_gemm<T, KIND, 256, 2, 4>(q, batch, st);
-    if (tiles(128) >= 128) return orth_gemm<T, KIND, 128, 2, 2>(q, batch, st);
-    return orth_gemm<T, KIND, 64, 2, 2>(q, batch, st);
+    // the largest tile that still gives the CUs enough workgroups; where each has
+    // one at most, more stages in flight.  Measured (us, A = X X^T / B X of
+    // 2048 x 8192, then of 1024 x 1024, then of 8 matrices 256 x 512):
+    //     256 x 256                452 / 200    76 / 84    44 / 38
+    //     128 x 128                265 / 200    41 / 44    21 / 16
+    //     64 x 64, two stages      168 / 249    23 / 24    11 / 8.4
+    //     64 x 64, four stages     205 / 274    16 / 17    10 / 8.1
+    if (tiles(256) >= 192) return orth_gemm<T, KIND, 256, 2, 4, 2>(q, batch, st);
+    if (tiles(128) >= 256) return orth_gemm<T, KIND, 128, 2, 2, 2>(q, batch, st);
+    if (tiles(64) >= 384) return orth_gemm<T, KIND, 64, 2, 2, 2>(q, batch, st);
+    return orth_gemm<T, KIND, 64, 2, 2, 4>(q, batch, st);
 }
 
 template <typename T>

@@ -192,15 +192,18 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
         const int nka = (int)((A.klen + ua - 1) / ua), nkb_b = (int)((B.klen + ub - 1) / ub);
         const int nkb = nka < nkb_b ? nka : nkb_b;
 
-        // the operands as this wave stages them: base of the stage it is at, and
-        // what is left of K from there on
+        // the operands as this wave stages them, `base` that of the stage it is at
         struct Feed {
             const char *base;
-            int64_t step, left;
-            int unit;
+            int64_t step;
+            int whole, rest;   // whole stages, and what the one behind them has of K
+            // what stage kb has of K, as WindowAt counts it
+            OZK_DEV int left(int kb) const { return kb < whole ? 128 : rest; }
         };
-        const Feed fa = {A.base, Sh::ACOLS ? Sh::KS * A.pitch : 128, A.klen, ua};
-        const Feed fb = {B.base, Sh::BCOLS ? Sh::KS * B.pitch : 128, B.klen, ub};
+        const Feed fa = {A.base, Sh::ACOLS ? Sh::KS * A.pitch : 128, (int)(A.klen / ua),
+                         (int)(A.klen % ua)};
+        const Feed fb = {B.base, Sh::BCOLS ? Sh::KS * B.pitch : 128, (int)(B.klen / ub),
+                         (int)(B.klen % ub)};
         const bool onlyA = Sh::ONE && wave * LP < Sh::BM / 8;
         Feed feed[Sh::ONE ? 1 : 2];
         if constexpr (Sh::ONE) {
@@ -229,10 +232,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
         }
         auto advance = [&] {
 #pragma unroll
-            for (Feed &f : feed) {
-                f.base += f.step;
-                f.left -= f.unit;
-            }
+            for (Feed &f : feed) f.base += f.step;
         };
 
         // windows q0 .. q1 of stage kb, if there is one; stages come in order
@@ -245,9 +245,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
             for (int q = 0; q < LP; ++q) {
                 if (q < q0 || q >= q1) continue;
                 const Feed &f = feed[of(q)];
-                uint32_t off = win[q].off;
-                if (f.left < f.unit && win[q].k >= (int)f.left) off = kTileOOB;
-                dma_piece(f.base, off, dst + slot_at[q]);
+                dma_piece(f.base, win[q].k < f.left(kb) ? win[q].off : kTileOOB, dst + slot_at[q]);
             }
         };
         // the same through registers, for rows of any alignment
@@ -259,9 +257,9 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 const Feed &f = feed[of(q)];
                 const bool cols = Sh::ONE ? (onlyA ? Sh::ACOLS : Sh::BCOLS)
                                           : (of(q) == 0 ? Sh::ACOLS : Sh::BCOLS);
-                const int64_t left = f.left - win[q].k;
+                const int left = f.left(kb) - win[q].k;
                 int n = left > 0 ? win[q].n : 0;
-                if (!cols && left < n) n = (int)left;
+                if (!cols && left < n) n = left;
                 held[q] = load_piece(f.base + (n > 0 ? win[q].off : 0u), n);
             }
         };
@@ -364,19 +362,13 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
         };
 
         if constexpr (DMA) {
-            auto wait = [&](int stages) {   // all but the last `stages` issued ones have landed
-                if (stages >= 4) wait_vmcnt<(Sh::NST > 4 ? 4 : 0) * LP>();
-                else if (stages == 3) wait_vmcnt<(Sh::NST > 3 ? 3 : 0) * LP>();
-                else if (stages == 2) wait_vmcnt<(Sh::NST > 2 ? 2 : 0) * LP>();
-                else if (stages == 1) wait_vmcnt<LP>();
-                else wait_vmcnt<0>();
-                static_assert(Sh::NST <= 5 && 4 * LP < 64, "wait table");
-            };
             constexpr int NOW = LP < 2 ? LP : 2;   // windows issued right after the barrier
 #pragma unroll
             for (int s = 0; s < Sh::NST; ++s) issue(s, 0, LP);
             if (nkb > 0) {
-                wait(nkb - 1 < Sh::NST - 1 ? nkb - 1 : Sh::NST - 1);
+                // the first has landed; few stages: all have
+                if (nkb >= Sh::NST) wait_vmcnt<(Sh::NST - 1) * LP>();
+                else wait_vmcnt<0>();
                 exec_barrier();
                 first(smem);
             }
@@ -384,8 +376,11 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 stage(
                     kb,
                     [&] {
-                        const int left = nkb - 2 - kb;
-                        wait(left < 0 ? 0 : left < Sh::NST - 2 ? left : Sh::NST - 2);
+                        // kb + 1 has landed; the last stages, on their way for a
+                        // while, all have
+                        if (kb + Sh::NST <= nkb) wait_vmcnt<(Sh::NST - 2) * LP>();
+                        else wait_vmcnt<0>();
+                        static_assert((Sh::NST - 1) * LP < 64, "vmcnt");
                         __builtin_amdgcn_s_waitcnt(0xC07F);   // this wave's reads of the slot
                         exec_barrier();
                         issue(kb + Sh::NST, 0, NOW);

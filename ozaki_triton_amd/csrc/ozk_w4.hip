@@ -61,139 +61,262 @@ OZK_DEV void transpose_words(uint32_t (&r)[4]) {
     swap16(r[2], r[3]);
 }
 
-OZK_DEV float scale_at(const W4Params &p, int64_t i, int dtype16) {
-    if (p.scales32) return ((const float *)p.scales)[i];
-    const uint16_t u = ((const uint16_t *)p.scales)[i];
-    return dtype16 == 2 ? (float)__builtin_bit_cast(_Float16, u) : bf16_bits_to_f32(u);
+// 16 bytes built element by element, the last first: a rolled loop, since code
+// that is fetched and skipped costs these short kernels more than it would
+OZK_DEV void push16(i32x4 &v, uint32_t e) {
+    v.w = (int)__builtin_amdgcn_alignbit((uint32_t)v.w, (uint32_t)v.z, 16);
+    v.z = (int)__builtin_amdgcn_alignbit((uint32_t)v.z, (uint32_t)v.y, 16);
+    v.y = (int)__builtin_amdgcn_alignbit((uint32_t)v.y, (uint32_t)v.x, 16);
+    v.x = (int)(((uint32_t)v.x << 16) | e);
+}
+OZK_DEV void push32(i32x4 &lo, i32x4 &hi, int e) {
+    hi = i32x4{lo.w, hi.x, hi.y, hi.z};
+    lo = i32x4{e, lo.x, lo.y, lo.z};
 }
 
-template <typename XT> OZK_DEV float x_value(const char *p) {
-    if constexpr (sizeof(XT) == 4) {
-        return *(const float *)p;
-    } else {
-        return from_bits16(*(const uint16_t *)p, XT{});
+// 8 scales and zero points of a row of W, of which the first n exist
+struct SPiece {
+    i32x4 s[2];      // fp32, or 16 bits in the first
+    i32x2 z;
+    OZK_DEV void load(const W4Params &p, int64_t row, int64_t g, int n) {
+        const int64_t at = row * p.s_pitch + g;
+        const uint8_t *zf = p.zeros ? p.zeros + row * p.z_pitch + g : nullptr;
+        z = i32x2{0, 0};
+        if (n >= 8) {
+            if (p.scales32) __builtin_memcpy(s, (const float *)p.scales + at, 32);
+            else __builtin_memcpy(s, (const uint16_t *)p.scales + at, 16);
+            if (zf) __builtin_memcpy(&z, zf, 8);
+        } else {
+            s[0] = s[1] = i32x4{0, 0, 0, 0};
+#pragma unroll 1
+            for (int i = n - 1; i >= 0; --i) {
+                if (p.scales32) push32(s[0], s[1], ((const int *)p.scales)[at + i]);
+                else push16(s[0], ((const uint16_t *)p.scales)[at + i]);
+                if (zf) {
+                    z.y = (int)__builtin_amdgcn_alignbit((uint32_t)z.y, (uint32_t)z.x, 24);
+                    z.x = (int)(((uint32_t)z.x << 8) | zf[i]);
+                }
+            }
+        }
     }
+    OZK_DEV float2 at(const W4Params &p, int i, int dtype16) const {   // (s, 16 + z)
+        float f;
+        if (p.scales32) {
+            f = __int_as_float(s[i >> 2][i & 3]);
+        } else {
+            const uint16_t u = (uint16_t)((uint32_t)s[0][i >> 1] >> (16 * (i & 1)));
+            f = dtype16 == 2 ? (float)__builtin_bit_cast(_Float16, u) : bf16_bits_to_f32(u);
+        }
+        const uint32_t q = ((uint32_t)z[i >> 2] >> (8 * (i & 3))) & 255u;
+        return float2{f, p.zeros ? 16.f + (float)q : 24.f};
+    }
+};
+
+// i / n for 0 <= i < 2^22, n a small part of it: (i + 1/2) / n is at least 1 / 2n
+// away from a whole number, the two roundings of rcp * (i + 1/2) less
+OZK_DEV int part_of(int i, int n, float rcp) { return (int)(((float)i + 0.5f) * rcp); }
+
+// the sum over 4, 8 or 16 consecutive lanes, in each of them
+template <int CTRL> OZK_DEV float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
 }
+template <int N> OZK_DEV float sum_lanes(float v) {
+    v = dpp_add<0xB1>(v);                      // lane ^ 1
+    v = dpp_add<0x4E>(v);                      // lane ^ 2
+    if constexpr (N > 4) v = dpp_add<0x141>(v);   // the other four of 8
+    if constexpr (N > 8) v = dpp_add<0x140>(v);   // the other eight of 16
+    return v;
+}
+
+// 8 values of a row of x, of which the first n exist
+template <typename XT> struct XPiece {
+    static constexpr int W = sizeof(XT) / 2;   // 16-byte words
+    i32x4 raw[W];
+    OZK_DEV void load(const char *from, int n) {
+        if (n >= 8) {
+            __builtin_memcpy(raw, from, sizeof(raw));   // rows of any alignment
+            return;
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) raw[w] = i32x4{0, 0, 0, 0};
+#pragma unroll 1
+        for (int i = n - 1; i >= 0; --i) {
+            if constexpr (W == 2) push32(raw[0], raw[1], ((const int *)from)[i]);
+            else push16(raw[0], ((const uint16_t *)from)[i]);
+        }
+    }
+    OZK_DEV void values(float (&v)[8]) const {
+        if constexpr (W == 2) {
+            __builtin_memcpy(v, raw, 32);
+        } else {
+            uint16_t e[8];
+            __builtin_memcpy(e, raw, 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = from_bits16(e[i], XT{});
+        }
+    }
+};
 
 // Waves: WN along n, WK along the chunks of K; a wave has RT blocks of 16 n
-// and TT blocks of 16 rows of x; GPC groups per chunk of 128 k.
+// and TT blocks of 16 rows of x; GPC groups per chunk of 128 k.  The LDS holds
+// x, its sums over the groups, and scale and zero point of the workgroup's
+// rows of W, for p.held of K.  The loads of x, then of the scales, then of the
+// wave's first U chunks of W are all on their way before the first is used.
 template <typename XT, int WN, int WK, int RT, int TT, int GPC>
 __global__ __launch_bounds__(64 * WN * WK) void w4_kernel(W4Params p) {
     using MT = typename W4Type<XT>::M;
-    constexpr int SL = W4Type<XT>::SL, NT = 64 * WN * WK, U = RT == 1 ? 4 : 2;
+    constexpr int SL = W4Type<XT>::SL, NT = 64 * WN * WK, U = 8 / RT, NR = 16 * RT * WN;
     constexpr int AC = SL > 1 ? 2 : 1;   // sums of the first slice and of the others, apart
     constexpr int D16 = std::is_same<XT, _Float16>::value ? 2 : 3;
+    // pieces of x and scales a lane loads at once, before its first chunks of W:
+    // loads return in order, so one issued behind W's waits for W
+    constexpr int XB = SL > 1 ? 4 : TT > 1 ? 8 : 4, SB = 1;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wn = wave / WK, wk = wave % WK, g = lane >> 4, i16 = lane & 15;
 
-    const int64_t nb = (int64_t)blockIdx.x * (16 * RT * WN) + wn * 16 * RT;
+    const int64_t n0 = (int64_t)blockIdx.x * NR;
+    const int64_t nb = n0 + wn * 16 * RT;
     const int64_t m0 = (int64_t)blockIdx.y * (16 * TT);
     const int rows = (int)(p.M - m0 < 16 * TT ? p.M - m0 : 16 * TT);
     const int64_t kbeg = (int64_t)blockIdx.z * p.range;
     const int64_t kend = kbeg + p.range < p.K ? kbeg + p.range : p.K;
 
-    // x in the LDS: [slice][row][k], then the groups' sums [group][16 TT rows]
+    // x [slice][row][k]; its sums [AC][group][16 TT rows]; (s, 16 + z) [row][group]
     const int pitch = p.held * 2 + 16;
     const int slice_bytes = rows * pitch;
+    const int gheld = p.held / p.group, sums_each = gheld * 16 * TT;
     float *sums = (float *)(smem + SL * slice_bytes);
-    const int sums_each = p.held / p.group * 16 * TT;   // [AC] of them
+    float2 *scales = (float2 *)(sums + AC * sums_each);
+    const int spitch = gheld + 1;
 
-    int64_t nrow[RT];
     const uint8_t *wrow[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int64_t n = nb + 16 * r + i16;
-        nrow[r] = n < p.N ? n : p.N - 1;
-        wrow[r] = p.packed + nrow[r] * p.w_pitch;
+        wrow[r] = p.packed + (n < p.N ? n : p.N - 1) * p.w_pitch;
     }
-
     f32x4 acc[RT][TT];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int t = 0; t < TT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    const int64_t pieces = (p.K + 31) / 32;          // 16-byte pieces of a row of W
+    const int64_t groups = (p.K + p.group - 1) / p.group;
     struct Chunk {
         i32x4 w[RT];
-        float s[RT][GPC], z[RT][GPC];
     };
-    const int64_t pieces = (p.K + 31) / 32;          // 16-byte pieces of a row
-    const int64_t groups = (p.K + p.group - 1) / p.group;
     auto load = [&](int64_t c, Chunk &ch) {          // chunk c: k from 128 c on
         const int64_t piece = c * 4 + g;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
+        for (int r = 0; r < RT; ++r)
             ch.w[r] = piece < pieces ? *(const i32x4 *)(wrow[r] + piece * 16) : i32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int q = 0; q < GPC; ++q) {
-                const int64_t gi = c * GPC + q < groups ? c * GPC + q : groups - 1;
-                ch.s[r][q] = scale_at(p, nrow[r] * p.s_pitch + gi, D16);
-                ch.z[r][q] = p.zeros ? 16.f + (float)p.zeros[nrow[r] * p.z_pitch + gi] : 24.f;
-            }
-        }
     };
 
     for (int64_t k0 = kbeg; k0 < kend; k0 += p.held) {
         const int64_t kstop = k0 + p.held < kend ? k0 + p.held : kend;
-        const int64_t c0 = k0 / 128 + wk, c1 = (kstop + 127) / 128;
-        Chunk cur[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c0 + u * WK < c1) load(c0 + u * WK, cur[u]);
+        // the wave's chunk t: pairs of chunks (a 128-byte line of each row) in turn
+        const int64_t c0 = k0 / 128, c1 = (kstop + 127) / 128;
+        auto chunk = [&](int t) { return c0 + ((t >> 1) * WK + wk) * 2 + (t & 1); };
 
-        if (k0 != kbeg) __syncthreads();             // the last part of x has been read
-        // x: 8 elements a lane, in the order of the unpacked weights, zeros past K
-        const int per_row = (int)((kstop - k0 + 127) / 128 * 16);
-        const int all = rows * per_row;
-        for (int i = threadIdx.x; i < (all + NT - 1) / NT * NT; i += NT) {
-            const int row = i < all ? i / per_row : rows - 1, at = i - row * per_row;
+        // x: pieces of 8 of whole chunks, zeros past K
+        const int per_row = (int)((kstop - k0 + 127) / 128 * 16), all = rows * per_row;
+        const int gcount = (int)((kstop - k0 + p.group - 1) / p.group);
+        const int gpieces = (gcount + 7) / 8, sall = NR * gpieces;
+        const float x_rcp = 1.f / (float)per_row, s_rcp = 1.f / (float)gpieces;
+        XPiece<XT> xp[XB];
+        SPiece sp[SB];
+        auto load_x = [&](int i, XPiece<XT> &x) {
+            const int row = i < all ? part_of(i, per_row, x_rcp) : 0;
+            const int at = i < all ? i - row * per_row : 0;
+            const int64_t k = k0 + at * 8;
+            const int64_t n = i < all ? p.K - k : 0;
+            x.load(p.x + ((m0 + row) * p.x_pitch + k) * (int64_t)sizeof(XT),
+                   n < 0 ? 0 : n < 8 ? (int)n : 8);
+        };
+        auto put_x = [&](int i, const XPiece<XT> &x) {
+            const int row = i < all ? part_of(i, per_row, x_rcp) : 0;
+            const int at = i < all ? i - row * per_row : 0;
             float v[8], sum[AC] = {};
-            const char *from = p.x + ((m0 + row) * p.x_pitch + k0 + at * 8) * (int64_t)sizeof(XT);
+            x.values(v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = i < all && k0 + at * 8 + e < p.K ? x_value<XT>(from + e * sizeof(XT)) : 0.f;
-                if constexpr (SL > 1) {
-                    const float h = from_bits16(to_bits16(v[e], MT{}), MT{});
-                    sum[0] += h;
-                    sum[1] += v[e] - h;
-                } else {
-                    sum[0] += v[e];
-                }
-            }
-            if (i < all) {
+            for (int s = 0; s < SL; ++s) {
+                uint16_t h[8];
+                if constexpr (SL == 1) __builtin_memcpy(h, x.raw, 16);
 #pragma unroll
-                for (int s = 0; s < SL; ++s) {
-                    uint16_t h[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        h[(e & 3) * 2 + (e >> 2)] = to_bits16(v[e], MT{});
-                        if (SL > 1) v[e] -= from_bits16(h[(e & 3) * 2 + (e >> 2)], MT{});
+                for (int e = 0; e < 8; ++e) {
+                    float f = v[e];
+                    if constexpr (SL > 1) {
+                        h[e] = to_bits16(v[e], MT{});
+                        f = from_bits16(h[e], MT{});
+                        v[e] -= f;
                     }
-                    i32x4 u;
-                    __builtin_memcpy(&u, h, 16);
-                    *(i32x4 *)(smem + s * slice_bytes + row * pitch + at * 16) = u;
+                    if (s == 0) {
+                        sum[0] += f;
+                        if constexpr (AC > 1) sum[1] += v[e];
+                    }
                 }
+                // in the order of the unpacked weights
+                const uint16_t o[8] = {h[0], h[4], h[1], h[5], h[2], h[6], h[3], h[7]};
+                i32x4 u;
+                __builtin_memcpy(&u, o, 16);
+                if (i < all) *(i32x4 *)(smem + s * slice_bytes + row * pitch + at * 16) = u;
             }
 #pragma unroll
             for (int a = 0; a < AC; ++a) {
-#pragma unroll
-                for (int d = 1; d < 16 / GPC; d <<= 1) sum[a] += __shfl_xor(sum[a], d);
+                const float t = sum_lanes<16 / GPC>(sum[a]);
                 if (i < all && at % (16 / GPC) == 0)
-                    sums[a * sums_each + at / (16 / GPC) * 16 * TT + row] = sum[a];
+                    sums[a * sums_each + at / (16 / GPC) * 16 * TT + row] = t;
             }
+        };
+        auto load_s = [&](int i, SPiece &s) {
+            if (i >= sall) return;
+            const int row = part_of(i, gpieces, s_rcp), at = (i - row * gpieces) * 8;
+            const int64_t n = n0 + row < p.N ? n0 + row : p.N - 1, gi = k0 / p.group + at;
+            s.load(p, n, gi, (int)(groups - gi < 8 ? groups - gi : 8));
+        };
+        auto put_s = [&](int i, const SPiece &s) {
+            if (i >= sall) return;
+            const int row = part_of(i, gpieces, s_rcp), at = (i - row * gpieces) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (at + e < gcount) scales[row * spitch + at + e] = s.at(p, e, D16);
+        };
+
+#pragma unroll
+        for (int u = 0; u < XB; ++u) load_x(threadIdx.x + u * NT, xp[u]);
+#pragma unroll
+        for (int u = 0; u < SB; ++u) load_s(threadIdx.x + u * NT, sp[u]);
+        Chunk cur[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (chunk(u) < c1) load(chunk(u), cur[u]);
+
+        if (k0 != kbeg) __syncthreads();             // the last part of x has been read
+#pragma unroll
+        for (int u = 0; u < XB; ++u) put_x(threadIdx.x + u * NT, xp[u]);
+#pragma unroll
+        for (int u = 0; u < SB; ++u) put_s(threadIdx.x + u * NT, sp[u]);
+        for (int i = threadIdx.x + XB * NT; i < (all + NT - 1) / NT * NT; i += XB * NT) {
+#pragma unroll
+            for (int u = 0; u < XB; ++u) load_x(i + u * NT, xp[u]);
+#pragma unroll
+            for (int u = 0; u < XB; ++u) put_x(i + u * NT, xp[u]);
+        }
+        for (int i = threadIdx.x + SB * NT; i < sall; i += SB * NT) {
+#pragma unroll
+            for (int u = 0; u < SB; ++u) load_s(i + u * NT, sp[u]);
+#pragma unroll
+            for (int u = 0; u < SB; ++u) put_s(i + u * NT, sp[u]);
         }
         __syncthreads();
 
-        for (int64_t c = c0; c < c1; c += U * WK) {
-            Chunk nxt[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (c + (U + u) * WK < c1) load(c + (U + u) * WK, nxt[u]);
+        for (int t0 = 0; chunk(t0) < c1; t0 += U) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t cu = c + u * WK;
+                const int64_t cu = chunk(t0 + u);
                 if (cu >= c1) break;
                 const int kl = (int)(cu * 128 - k0);   // of the chunk, in the LDS
                 uint32_t w[RT][4];
@@ -203,6 +326,8 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_kernel(W4Params p) {
                     for (int j = 0; j < 4; ++j) w[r][j] = (uint32_t)cur[u].w[r][j];
                     transpose_words(w[r]);
                 }
+                // the registers are free again: the chunk U rounds on
+                if (chunk(t0 + u + U) < c1) load(chunk(t0 + u + U), cur[u]);
 #pragma unroll
                 for (int q = 0; q < GPC; ++q) {
                     f32x4 part[AC][RT][TT];
@@ -230,26 +355,30 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_kernel(W4Params p) {
                                     part[s > 0][r][t] = mfma16(xf, wf[r], part[s > 0][r][t], MT{});
                             }
                     }
+                    const int gl = kl / 128 * GPC + q;
+                    float2 sz[RT];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+                        sz[r] = scales[(wn * 16 * RT + 16 * r + i16) * spitch +
+                                       (gl < gcount ? gl : gcount - 1)];
 #pragma unroll
                     for (int t = 0; t < TT; ++t) {
-                        const float *xs = sums + (kl / 128 * GPC + q) * 16 * TT + 16 * t + 4 * g;
-                        f32x4 x0 = *(const f32x4 *)xs, x1 = x0;
+                        const float *xs = sums + gl * 16 * TT + 16 * t + 4 * g;
+                        const f32x4 x0 = *(const f32x4 *)xs;
+                        f32x4 x1 = x0;
                         if constexpr (AC > 1) x1 = *(const f32x4 *)(xs + sums_each);
 #pragma unroll
                         for (int r = 0; r < RT; ++r)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float z = cur[u].z[r][q];
-                                float v = __builtin_fmaf(-z, x0[e], part[0][r][t][e]);
+                                float v = __builtin_fmaf(-sz[r].y, x0[e], part[0][r][t][e]);
                                 if constexpr (AC > 1)
-                                    v += __builtin_fmaf(-z, x1[e], part[1][r][t][e]);
-                                acc[r][t][e] = __builtin_fmaf(cur[u].s[r][q], v, acc[r][t][e]);
+                                    v += __builtin_fmaf(-sz[r].y, x1[e], part[1][r][t][e]);
+                                acc[r][t][e] = __builtin_fmaf(sz[r].x, v, acc[r][t][e]);
                             }
                     }
                 }
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) cur[u] = nxt[u];
         }
     }
 
@@ -328,44 +457,72 @@ template <typename T> OZK_DEV float rounded(float v) {
     else return from_bits16(to_bits16(v, T{}), T{});
 }
 
-// 8 weights a lane: a group is 4, 8 or 16 lanes, a wave 512 weights of a row
+// smallest and largest over 4, 8 or 16 consecutive lanes, in each of them (of a
+// number and NaN the number)
+template <int CTRL> OZK_DEV void dpp_range(float &lo, float &hi) {
+    lo = fminf(lo, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(lo), CTRL, 0xF, 0xF, true)));
+    hi = fmaxf(hi, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(hi), CTRL, 0xF, 0xF, true)));
+}
+
+// 8 weights a lane: a group is 4, 8 or 16 lanes, a wave takes 512 weights of a
+// row at a time and kQuantParts such parts, whose loads are all on their way
+// before the first is used (one part a wave: 8192 x 8192 bf16 in 64 us).
+constexpr int kQuantParts = 4;
 template <typename T> __global__ __launch_bounds__(256) void quantize_w4_kernel(QuantParams p) {
-    const int64_t per_row = (p.p_pitch * 2 + 511) / 512;
-    const int64_t wave = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 6;
+    const uint32_t per_row = (uint32_t)((p.p_pitch * 2 + 511) / 512);
+    const uint32_t parts = (uint32_t)p.N * per_row;
+    const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kQuantParts;
     const int lane = threadIdx.x & 63;
-    const int64_t n = wave / per_row, k = (wave - n * per_row) * 512 + lane * 8;
-    if (n >= p.N) return;
-    float v[8], lo = 0.f, hi = 0.f;
+    XPiece<T> x[kQuantParts];
+    auto place = [&](int u, int64_t &n, int64_t &k) {
+        const uint32_t part = first + u < parts ? first + u : parts - 1;
+        n = part / per_row;
+        k = (int64_t)(part - (uint32_t)n * per_row) * 512 + lane * 8;
+    };
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        v[e] = k + e < p.K ? load_value<T>(p.W, n * p.w_pitch + k + e) : 0.f;
-        lo = fminf(lo, v[e]);     // (of a number and NaN the number)
-        hi = fmaxf(hi, v[e]);
+    for (int u = 0; u < kQuantParts; ++u) {
+        int64_t n, k;
+        place(u, n, k);
+        x[u].load(p.W + (n * p.w_pitch + k) * (int64_t)sizeof(T),
+                  k + 8 <= p.K ? 8 : k < p.K ? (int)(p.K - k) : 0);
     }
-    for (int d = 1; d < p.group / 8; d <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, d));
-        hi = fmaxf(hi, __shfl_xor(hi, d));
-    }
-    float s, z = 8.f;
-    if (p.zeros) {
-        s = rounded<T>((hi - lo) * (1.f / 15.f));
-        z = s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
-    } else {
-        s = rounded<T>(fmaxf(hi, -lo) * (1.f / 7.f));
-    }
-    uint32_t word = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float q = s > 0.f ? rintf(v[e] / s) : 0.f;
-        if (q != q) q = 0.f;
-        q = fminf(fmaxf(q + z, 0.f), 15.f);
-        word |= (uint32_t)(int)q << (4 * e);
+    for (int u = 0; u < kQuantParts; ++u) {
+        if (first + u >= parts) return;
+        int64_t n, k;
+        place(u, n, k);
+        float v[8], lo = 0.f, hi = 0.f;
+        x[u].values(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            lo = fminf(lo, v[e]);
+            hi = fmaxf(hi, v[e]);
+        }
+        dpp_range<0xB1>(lo, hi);                           // lane ^ 1
+        dpp_range<0x4E>(lo, hi);                           // lane ^ 2
+        if (p.group >= 64) dpp_range<0x141>(lo, hi);       // the other four of 8
+        if (p.group == 128) dpp_range<0x140>(lo, hi);      // the other eight of 16
+        float s, z = 8.f;
+        if (p.zeros) {
+            s = rounded<T>((hi - lo) * (1.f / 15.f));
+            z = s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
+        } else {
+            s = rounded<T>(fmaxf(hi, -lo) * (1.f / 7.f));
+        }
+        uint32_t word = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float q = s > 0.f ? rintf(v[e] / s) : 0.f;
+            if (q != q) q = 0.f;
+            word |= (uint32_t)(int)fminf(fmaxf(q + z, 0.f), 15.f) << (4 * e);
+        }
+        if (k < p.K && k % p.group == 0) {
+            const int64_t g = k / p.group;
+            store_value<T>(p.scales, n * p.s_pitch + g, s);
+            if (p.zeros) p.zeros[n * p.z_pitch + g] = (uint8_t)(int)z;
+        }
+        if (k / 2 < p.p_pitch) *(uint32_t *)(p.packed + n * p.p_pitch + k / 2) = word;
     }
-    if (k < p.K && k % p.group == 0) {
-        store_value<T>(p.scales, n * p.s_pitch + k / p.group, s);
-        if (p.zeros) p.zeros[n * p.z_pitch + k / p.group] = (uint8_t)(int)z;
-    }
-    if (k / 2 < p.p_pitch) *(uint32_t *)(p.packed + n * p.p_pitch + k / 2) = word;
 }
 
 template <typename T, typename ST>
@@ -397,39 +554,53 @@ __global__ __launch_bounds__(256) void dequantize_w4_kernel(QuantParams p) {
 
 namespace {
 
-constexpr int kHeldBytes = 64 * 1024;   // of x in the LDS: two workgroups a CU
-
-struct W4Shape { int wn, wk, rt, tt; };
-W4Shape w4_shape(int64_t M) {
-    if (M <= 4) return {1, 4, 1, 1};
-    if (M <= 16) return {4, 1, 1, 1};
-    if (M <= 32) return {4, 1, 2, 2};
-    return {4, 1, 2, 4};
+// Waves along n and K, blocks of n and of rows of x per wave; bytes of the LDS
+// for x and the scales.  Few rows of x: one block of 16 n and its whole K to a
+// workgroup, nothing to join.  More rows of x: more n to a workgroup, since
+// each stages x for itself, and K cut to have a workgroup per CU.  Measured
+// (us, HIP graph of 40 calls on several weights, M x N x K, group):
+//     1 x 4096 x 4096, 128    {1,8,1,1} 7.7   {2,4,2,1} 10.2   {8,1,2,2} > 11
+//     1 x 16384 x 4096, 128   {1,8,1,1} 16.8  {2,4,2,1} 14.3   {4,2,2,1} 17.0
+//     2 x 8192 x 8192, 32     {1,8,1,1} 21.0  {2,4,2,1} 21.7   {4,2,2,1} 23.4
+//     16 x 8192 x 8192, 128   {4,2,2,1} 22.6  {8,1,2,2} 21.4
+//     32 x 8192 x 8192, 128   {4,2,2,2} 26.0  {8,1,2,2} 21.9   {8,1,2,4} 24.8
+//     64 x 8192 x 8192, 128   {4,2,2,4} > 40  {8,1,2,2} 35.3   {8,1,2,4} 31.6
+struct W4Shape {
+    int wn, wk, rt, tt, lds;
+};
+constexpr W4Shape kW4Shapes[] = {
+    {1, 8, 1, 1, 64 << 10}, {2, 4, 2, 1, 64 << 10}, {8, 1, 2, 2, 128 << 10}, {8, 1, 2, 4, 150 << 10}};
+int w4_shape(const W4Params &p, int slices) {
+    if (p.M <= 16 && p.N <= (p.M <= 4 ? 8192 : 4096)) return 0;
+    if (p.M <= 4) return 1;
+    return p.M <= 32 || slices > 1 ? 2 : 3;   // (3 with three slices of x leaves no registers)
 }
+int64_t w4_rows(const W4Params &p, const W4Shape &s) { return p.M < 16 * s.tt ? p.M : 16 * s.tt; }
 int lds_of(const W4Params &p, const W4Shape &s, int slices) {
-    const int rows = (int)(p.M < 16 * s.tt ? p.M : 16 * s.tt);
-    const int sums = p.held / p.group * 16 * s.tt * 4 * (slices > 1 ? 2 : 1);
-    const int x = slices * rows * (p.held * 2 + 16) + sums;
-    const int join = (s.wk - 1) * s.wn * s.rt * s.tt * 64 * 16;
-    return x > join ? x : join;
+    const int groups = p.held / p.group;
+    const int64_t x = slices * w4_rows(p, s) * (p.held * 2 + 16);
+    const int64_t sums = (int64_t)groups * 16 * s.tt * 4 * (slices > 1 ? 2 : 1);
+    const int64_t scales = (int64_t)16 * s.rt * s.wn * (groups + 1) * 8;
+    const int64_t join = (int64_t)(s.wk - 1) * s.wn * s.rt * s.tt * 64 * 16;
+    return (int)(x + sums + scales > join ? x + sums + scales : join);
 }
 
-template <typename XT, int WN, int WK, int RT, int TT, int GPC>
-hipError_t w4_start(const W4Params &p, hipStream_t st) {
-    const dim3 grid((uint32_t)((p.N + 16 * RT * WN - 1) / (16 * RT * WN)),
-                    (uint32_t)((p.M + 16 * TT - 1) / (16 * TT)), (uint32_t)p.splits);
-    const int lds = lds_of(p, {WN, WK, RT, TT}, W4Type<XT>::SL);
-    if (hipError_t e = allow_lds<&w4_kernel<XT, WN, WK, RT, TT, GPC>>(lds); e != hipSuccess)
+template <typename XT, int I, int GPC> hipError_t w4_start(const W4Params &p, hipStream_t st) {
+    constexpr W4Shape s = kW4Shapes[I];
+    const dim3 grid((uint32_t)((p.N + 16 * s.rt * s.wn - 1) / (16 * s.rt * s.wn)),
+                    (uint32_t)((p.M + 16 * s.tt - 1) / (16 * s.tt)), (uint32_t)p.splits);
+    if (grid.y > 65535) return hipErrorInvalidConfiguration;
+    const int lds = lds_of(p, s, W4Type<XT>::SL);
+    if (hipError_t e = allow_lds<&w4_kernel<XT, s.wn, s.wk, s.rt, s.tt, GPC>>(lds); e != hipSuccess)
         return e;
-    w4_kernel<XT, WN, WK, RT, TT, GPC><<<grid, 64 * WN * WK, lds, st>>>(p);
+    w4_kernel<XT, s.wn, s.wk, s.rt, s.tt, GPC><<<grid, 64 * s.wn * s.wk, lds, st>>>(p);
     return hipGetLastError();
 }
 
-template <typename XT, int WN, int WK, int RT, int TT>
-hipError_t w4_go(const W4Params &p, hipStream_t st) {
-    const hipError_t e = p.group == 32   ? w4_start<XT, WN, WK, RT, TT, 4>(p, st)
-                         : p.group == 64 ? w4_start<XT, WN, WK, RT, TT, 2>(p, st)
-                                         : w4_start<XT, WN, WK, RT, TT, 1>(p, st);
+template <typename XT, int I> hipError_t w4_go(const W4Params &p, hipStream_t st) {
+    const hipError_t e = p.group == 32   ? w4_start<XT, I, 4>(p, st)
+                         : p.group == 64 ? w4_start<XT, I, 2>(p, st)
+                                         : w4_start<XT, I, 1>(p, st);
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t blocks = (p.M * p.N + 255) / 256;
     w4_join_kernel<XT><<<dim3((uint32_t)(blocks < 1024 ? blocks : 1024)), 256, 0, st>>>(p);
@@ -437,31 +608,41 @@ hipError_t w4_go(const W4Params &p, hipStream_t st) {
 }
 
 template <typename XT> hipError_t w4_run(const W4Params &p, hipStream_t st) {
-    if (p.M <= 4) return w4_go<XT, 1, 4, 1, 1>(p, st);
-    if (p.M <= 16) return w4_go<XT, 4, 1, 1, 1>(p, st);
-    if (p.M <= 32) return w4_go<XT, 4, 1, 2, 2>(p, st);
-    return w4_go<XT, 4, 1, 2, 4>(p, st);
+    switch (w4_shape(p, W4Type<XT>::SL)) {
+    case 0: return w4_go<XT, 0>(p, st);
+    case 1: return w4_go<XT, 1>(p, st);
+    case 2: return w4_go<XT, 2>(p, st);
+    }
+    if constexpr (W4Type<XT>::SL == 1) return w4_go<XT, 3>(p, st);
+    return hipErrorInvalidConfiguration;
 }
 
 }  // namespace
 
 void plan_w4(W4Params &p, int dtype) {
-    const W4Shape s = w4_shape(p.M);
     const int slices = dtype == 1 ? 3 : 1;
-    const int64_t rows = p.M < 16 * s.tt ? p.M : 16 * s.tt;
+    const W4Shape s = kW4Shapes[w4_shape(p, slices)];
     const int64_t blocks = (p.N + 16 * s.rt * s.wn - 1) / (16 * s.rt * s.wn) *
                            ((p.M + 16 * s.tt - 1) / (16 * s.tt));
     const int64_t chunks = (p.K + 127) / 128;
-    // enough workgroups for every CU, two chunks of work per wave at least
+    // workgroups for the CUs, two chunks of work per wave at least
     int64_t splits = 1;
-    while (splits < 32 && blocks * splits < 256 && chunks / (2 * splits) >= 2 * s.wk) splits *= 2;
+    while (splits < 32 && blocks * splits < 160 && chunks / (2 * splits) >= 2 * s.wk) splits *= 2;
     const int64_t per = (chunks + splits - 1) / splits;
     p.range = (int)(per * 128);
     p.splits = (int)((chunks + per - 1) / per);
-    int64_t held = kHeldBytes / (slices * rows * 2 + 2 * s.tt) / (128 * s.wk) * (128 * s.wk);
-    if (held < 128 * s.wk) held = 128 * s.wk;
-    p.held = (int)(held < p.range ? held : p.range);
     p.part = nullptr;
+    // as much of K as the LDS takes, in whole rounds of the waves
+    const int step = 128 * s.wk;
+    p.held = step;
+    while (p.held < p.range) {
+        p.held += step;
+        if (lds_of(p, s, slices) > s.lds) {
+            p.held -= step;
+            break;
+        }
+    }
+    if (p.held > p.range) p.held = p.range;
 }
 
 hipError_t launch_w4(const W4Params &p, int dtype, hipStream_t st) {
@@ -470,9 +651,9 @@ hipError_t launch_w4(const W4Params &p, int dtype, hipStream_t st) {
 }
 
 hipError_t launch_quantize_w4(const QuantParams &p, int dtype, hipStream_t st) {
-    const int64_t waves = p.N * ((p.p_pitch * 2 + 511) / 512);
-    const int64_t blocks = (waves + 3) / 4;
-    if (blocks >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
+    const int64_t parts = p.N * ((p.p_pitch * 2 + 511) / 512);
+    const int64_t blocks = (parts + 4 * kQuantParts - 1) / (4 * kQuantParts);
+    if (parts >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
     auto *k = dtype == 1   ? quantize_w4_kernel<float>
               : dtype == 2 ? quantize_w4_kernel<_Float16>
                            : quantize_w4_kernel<__bf16>;
