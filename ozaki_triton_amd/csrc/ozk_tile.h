@@ -50,9 +50,7 @@ OZK_DEV f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c, __bf16) {
 
 // fp32 -> 16 bits, to nearest even (NaN stays NaN)
 OZK_DEV uint16_t to_bits16(float v, _Float16) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
-OZK_DEV uint16_t to_bits16(float v, __bf16) {
-    return (uint16_t)(v != v ? 0x7FC0u : f32_to_bf16_bits(v));
-}
+OZK_DEV uint16_t to_bits16(float v, __bf16) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 OZK_DEV float from_bits16(uint16_t v, _Float16) { return (float)__builtin_bit_cast(_Float16, v); }
 OZK_DEV float from_bits16(uint16_t v, __bf16) { return bf16_bits_to_f32(v); }
 

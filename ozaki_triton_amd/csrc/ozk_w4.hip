@@ -241,28 +241,36 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_kernel(W4Params p) {
             const int at = i < all ? i - row * per_row : 0;
             float v[8], sum[AC] = {};
             x.values(v);
-#pragma unroll
-            for (int s = 0; s < SL; ++s) {
+            if constexpr (SL == 1) {
                 uint16_t h[8];
-                if constexpr (SL == 1) __builtin_memcpy(h, x.raw, 16);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float f = v[e];
-                    if constexpr (SL > 1) {
-                        h[e] = to_bits16(v[e], MT{});
-                        f = from_bits16(h[e], MT{});
-                        v[e] -= f;
-                    }
-                    if (s == 0) {
-                        sum[0] += f;
-                        if constexpr (AC > 1) sum[1] += v[e];
-                    }
-                }
+                __builtin_memcpy(h, x.raw, 16);
                 // in the order of the unpacked weights
                 const uint16_t o[8] = {h[0], h[4], h[1], h[5], h[2], h[6], h[3], h[7]};
                 i32x4 u;
                 __builtin_memcpy(&u, o, 16);
-                if (i < all) *(i32x4 *)(smem + s * slice_bytes + row * pitch + at * 16) = u;
+                if (i < all) *(i32x4 *)(smem + row * pitch + at * 16) = u;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[0] += v[e];
+            } else {
+                // 8, 8 and 8 bits of the 24: a slice is the upper half of what is left
+#pragma unroll
+                for (int s = 0; s < SL; ++s) {
+                    i32x4 u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        u[e] = (int)__builtin_amdgcn_perm(__float_as_uint(v[e + 4]),
+                                                          __float_as_uint(v[e]), 0x07060302u);
+                    if (i < all) *(i32x4 *)(smem + s * slice_bytes + row * pitch + at * 16) = u;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float h = __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
+                        if (s + 1 < SL) v[e] -= h;
+                        if (s == 0) {
+                            sum[0] += h;
+                            sum[AC - 1] += v[e];
+                        }
+                    }
+                }
             }
 #pragma unroll
             for (int a = 0; a < AC; ++a) {
@@ -464,65 +472,71 @@ template <int CTRL> OZK_DEV void dpp_range(float &lo, float &hi) {
     hi = fmaxf(hi, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(hi), CTRL, 0xF, 0xF, true)));
 }
 
-// 8 weights a lane: a group is 4, 8 or 16 lanes, a wave takes 512 weights of a
-// row at a time and kQuantParts such parts, whose loads are all on their way
-// before the first is used (one part a wave: 8192 x 8192 bf16 in 64 us).
-constexpr int kQuantParts = 4;
+// 8 weights a lane: a group is 4, 8 or 16 lanes, a wave 512 weights of a row.
+// The divisions and roundings bound it (8192 x 8192 bf16: 64 us with v / s and
+// rint per weight), so a group divides once, y = fl(1 / s), and each quotient is
+// corrected twice by its exact remainder, which gives fl(v / s) (Markstein,
+// 1990: one correction of a quotient within a unit does where y is fl(1 / s));
+// adding 1.5 2^23 rounds it to a whole number, ties to even.
 template <typename T> __global__ __launch_bounds__(256) void quantize_w4_kernel(QuantParams p) {
     const uint32_t per_row = (uint32_t)((p.p_pitch * 2 + 511) / 512);
-    const uint32_t parts = (uint32_t)p.N * per_row;
-    const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kQuantParts;
+    const uint32_t part = blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    XPiece<T> x[kQuantParts];
-    auto place = [&](int u, int64_t &n, int64_t &k) {
-        const uint32_t part = first + u < parts ? first + u : parts - 1;
-        n = part / per_row;
-        k = (int64_t)(part - (uint32_t)n * per_row) * 512 + lane * 8;
-    };
+    const int64_t n = part / per_row, k = (int64_t)(part - (uint32_t)n * per_row) * 512 + lane * 8;
+    if (n >= p.N) return;
+    XPiece<T> x;
+    x.load(p.W + (n * p.w_pitch + k) * (int64_t)sizeof(T),
+           k + 8 <= p.K ? 8 : k < p.K ? (int)(p.K - k) : 0);
+    float v[8], lo = 0.f, hi = 0.f;
+    x.values(v);
 #pragma unroll
-    for (int u = 0; u < kQuantParts; ++u) {
-        int64_t n, k;
-        place(u, n, k);
-        x[u].load(p.W + (n * p.w_pitch + k) * (int64_t)sizeof(T),
-                  k + 8 <= p.K ? 8 : k < p.K ? (int)(p.K - k) : 0);
+    for (int e = 0; e < 8; ++e) {
+        lo = fminf(lo, v[e]);
+        hi = fmaxf(hi, v[e]);
     }
+    dpp_range<0xB1>(lo, hi);                           // lane ^ 1
+    dpp_range<0x4E>(lo, hi);                           // lane ^ 2
+    if (p.group >= 64) dpp_range<0x141>(lo, hi);       // the other four of 8
+    if (p.group == 128) dpp_range<0x140>(lo, hi);      // the other eight of 16
+    float s, z = 8.f;
+    if (p.zeros) {
+        s = rounded<T>((hi - lo) * (1.f / 15.f));
+        z = s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
+    } else {
+        s = rounded<T>(fmaxf(hi, -lo) * (1.f / 7.f));
+    }
+    uint32_t word = 0;
+    bool nan = false;
 #pragma unroll
-    for (int u = 0; u < kQuantParts; ++u) {
-        if (first + u >= parts) return;
-        int64_t n, k;
-        place(u, n, k);
-        float v[8], lo = 0.f, hi = 0.f;
-        x[u].values(v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            lo = fminf(lo, v[e]);
-            hi = fmaxf(hi, v[e]);
-        }
-        dpp_range<0xB1>(lo, hi);                           // lane ^ 1
-        dpp_range<0x4E>(lo, hi);                           // lane ^ 2
-        if (p.group >= 64) dpp_range<0x141>(lo, hi);       // the other four of 8
-        if (p.group == 128) dpp_range<0x140>(lo, hi);      // the other eight of 16
-        float s, z = 8.f;
-        if (p.zeros) {
-            s = rounded<T>((hi - lo) * (1.f / 15.f));
-            z = s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
-        } else {
-            s = rounded<T>(fmaxf(hi, -lo) * (1.f / 7.f));
-        }
-        uint32_t word = 0;
+    for (int e = 0; e < 8; e += 2) nan = nan || __builtin_isunordered(v[e], v[e + 1]);
+    // remainders stay clear of the subnormals
+    if (s > 0x1p-90f && s < 0x1p90f && !nan) {
+        const float y = 1.f / s;
+        const int zi = (int)z - 0x4B400000;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float q = s > 0.f ? rintf(v[e] / s) : 0.f;
+            float q = v[e] * y;
+            q = __builtin_fmaf(__builtin_fmaf(-q, s, v[e]), y, q);
+            q = __builtin_fmaf(__builtin_fmaf(-q, s, v[e]), y, q);
+            const int i = __float_as_int(q + 12582912.f) + zi;
+            word |= (uint32_t)(i < 0 ? 0 : i > 15 ? 15 : i) << (4 * e);
+        }
+    } else {
+#pragma unroll 1
+        for (int e = 7; e >= 0; --e) {
+            float q = s > 0.f ? rintf(v[7] / s) : 0.f;
             if (q != q) q = 0.f;
-            word |= (uint32_t)(int)fminf(fmaxf(q + z, 0.f), 15.f) << (4 * e);
+            word = (word << 4) | (uint32_t)(int)fminf(fmaxf(q + z, 0.f), 15.f);
+#pragma unroll
+            for (int i = 7; i > 0; --i) v[i] = v[i - 1];
         }
-        if (k < p.K && k % p.group == 0) {
-            const int64_t g = k / p.group;
-            store_value<T>(p.scales, n * p.s_pitch + g, s);
-            if (p.zeros) p.zeros[n * p.z_pitch + g] = (uint8_t)(int)z;
-        }
-        if (k / 2 < p.p_pitch) *(uint32_t *)(p.packed + n * p.p_pitch + k / 2) = word;
     }
+    if (k < p.K && k % p.group == 0) {
+        const int64_t g = k / p.group;
+        store_value<T>(p.scales, n * p.s_pitch + g, s);
+        if (p.zeros) p.zeros[n * p.z_pitch + g] = (uint8_t)(int)z;
+    }
+    if (k / 2 < p.p_pitch) *(uint32_t *)(p.packed + n * p.p_pitch + k / 2) = word;
 }
 
 template <typename T, typename ST>
@@ -652,7 +666,7 @@ hipError_t launch_w4(const W4Params &p, int dtype, hipStream_t st) {
 
 hipError_t launch_quantize_w4(const QuantParams &p, int dtype, hipStream_t st) {
     const int64_t parts = p.N * ((p.p_pitch * 2 + 511) / 512);
-    const int64_t blocks = (parts + 4 * kQuantParts - 1) / (4 * kQuantParts);
+    const int64_t blocks = (parts + 3) / 4;
     if (parts >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
     auto *k = dtype == 1   ? quantize_w4_kernel<float>
               : dtype == 2 ? quantize_w4_kernel<_Float16>

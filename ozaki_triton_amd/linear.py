@@ -15,11 +15,12 @@ NotImplementedError, tensors off the GPU RuntimeError.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
-from .ozaki import _TORCH_TO_OZK, _on_device, _require_gpu, _stream
+from .ozaki import _TORCH_TO_OZK, _require_gpu, _stream
 
 _HALF = (torch.float16, torch.bfloat16)
 _FLOAT = (torch.float32, torch.float16, torch.bfloat16)
@@ -31,6 +32,55 @@ def _require_dtype(name: str, dtype: torch.dtype, allowed) -> None:
         raise NotImplementedError(
             f"{name}: {dtype} is not implemented by the MI355X kernels (implemented: "
             f"{', '.join(str(d).replace('torch.', '') for d in allowed)})")
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _on_one_gpu(a: torch.Tensor, *others) -> None:
+    """_require_gpu's check without its sets: host time counts in calls of a few us."""
+    if a.is_cuda:
+        dev = a.device
+        for t in others:
+            if t is not None and t.device != dev:
+                break
+        else:
+            return
+    _require_gpu(a, *(t for t in others if t is not None))
+
+
+def _call(name: str, dev: torch.device, *args) -> None:
+    """Library call `name` on dev's current stream, its last argument."""
+    fn = getattr(_lib.load(), name)
+    if dev.index == _current_device():
+        st = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, _stream(dev))
+    if st:
+        _lib.check(name, st)
+
+
+@functools.lru_cache(maxsize=1024)
+def _bytes(name: str, *args) -> int:
+    """Workspace query `name`: it depends on nothing but its arguments."""
+    n = ctypes.c_size_t(0)
+    _lib.check(name, getattr(_lib.load(), name)(*args, ctypes.byref(n)))
+    return n.value
+
+
+def _workspace(nbytes: int, dev: torch.device):
+    """Scratch on dev's current stream, the one the kernels run on (so it needs no
+    record_stream), and its address."""
+    if not nbytes:
+        return None, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _i64(*vals):
+    return _lib.i64arr(vals)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -50,7 +100,7 @@ def _grouped_checks(A, B, offsets):
     assert A.shape[1] == B.shape[1], f"contraction dim mismatch: A K={A.shape[1]}, B K={B.shape[1]}"
     assert A.dtype == B.dtype, f"A/B dtype mismatch: {A.dtype} vs {B.dtype}"
     _offset_checks(offsets, B.shape[0])
-    _require_gpu(A, B, offsets)
+    _on_one_gpu(A, B, offsets)
     _require_dtype("grouped_matmul", A.dtype, _HALF)
 
 
@@ -71,13 +121,11 @@ def _grouped_forward(A, B, offsets):
         sb = B.stride()
     if offsets.stride(0) != 1:
         offsets = offsets.contiguous()
-    C = torch.empty((T, N), dtype=A.dtype, device=A.device)
-    with _on_device(A.device):
-        st = _lib.load().ozk_grouped_matmul(
-            A.data_ptr(), A.stride(0), B.data_ptr(), _lib.i64arr(sb), offsets.data_ptr(),
-            offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[A.dtype], C.data_ptr(), N,
-            _stream(A.device))
-    _lib.check("ozk_grouped_matmul", st)
+    dtype, dev = A.dtype, A.device
+    C = torch.empty((T, N), dtype=dtype, device=dev)
+    _call("ozk_grouped_matmul", dev, A.data_ptr(), A.stride(0), B.data_ptr(), _i64(*sb),
+          offsets.data_ptr(), offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype],
+          C.data_ptr(), N)
     return C
 
 
@@ -87,19 +135,14 @@ def _grouped_wgrad(A, D, offsets, G):
     A, D = _rows(A), _rows(D)
     if offsets.stride(0) != 1:
         offsets = offsets.contiguous()
-    dB = torch.empty((G, K, N), dtype=A.dtype, device=A.device)
-    L = _lib.load()
-    nbytes = ctypes.c_size_t(0)
-    _lib.check("ozk_grouped_matmul_wgrad_workspace_bytes",
-               L.ozk_grouped_matmul_wgrad_workspace_bytes(T, K, N, G, ctypes.byref(nbytes)))
-    n = nbytes.value
-    ws = torch.empty(n, dtype=torch.uint8, device=A.device) if n else None
-    with _on_device(A.device):
-        st = L.ozk_grouped_matmul_wgrad(
-            A.data_ptr(), A.stride(0), D.data_ptr(), D.stride(0), offsets.data_ptr(),
-            offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[A.dtype], dB.data_ptr(),
-            _lib.i64arr((K * N, N)), ws.data_ptr() if n else None, n, _stream(A.device))
-    _lib.check("ozk_grouped_matmul_wgrad", st)
+    dtype, dev = A.dtype, A.device
+    dB = torch.empty((G, K, N), dtype=dtype, device=dev)
+    n = _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", T, K, N, G)
+    ws, wsp = _workspace(n, dev)
+    _call("ozk_grouped_matmul_wgrad", dev, A.data_ptr(), A.stride(0), D.data_ptr(), D.stride(0),
+          offsets.data_ptr(), offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype],
+          dB.data_ptr(), _i64(K * N, N), wsp, n)
+    del ws
     return dB
 
 
@@ -146,7 +189,7 @@ def grouped_matmul_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     assert dC.shape == (A.shape[0], B.shape[2]), \
         f"dC must be {(A.shape[0], B.shape[2])}, got {tuple(dC.shape)}"
     assert dC.dtype == A.dtype, f"dC/A dtype mismatch: {dC.dtype} vs {A.dtype}"
-    _require_gpu(dC, A)
+    _on_one_gpu(dC, A)
     return _grouped_forward(dC, B.mT, offsets), _grouped_wgrad(A, dC, offsets, B.shape[0])
 
 
@@ -203,7 +246,7 @@ def quantize_w4(W: torch.Tensor, group_size: int = 128, *, zeros: bool = False):
     """
     assert W.dim() == 2, f"W must be [N, K], got {tuple(W.shape)}"
     assert group_size in _GROUPS, f"group_size must be 32, 64 or 128, got {group_size}"
-    _require_gpu(W)
+    _on_one_gpu(W)
     _require_dtype("quantize_w4", W.dtype, _FLOAT)
     _no_grad("quantize_w4", W)
     N, K = W.shape
@@ -213,12 +256,9 @@ def quantize_w4(W: torch.Tensor, group_size: int = 128, *, zeros: bool = False):
     packed = torch.empty((N, (K + 31) // 32 * 16), dtype=torch.uint8, device=dev)
     scales = torch.empty((N, groups), dtype=W.dtype, device=dev)
     z = torch.empty((N, groups), dtype=torch.uint8, device=dev) if zeros else None
-    with _on_device(dev):
-        st = _lib.load().ozk_quantize_w4(
-            W.data_ptr(), _TORCH_TO_OZK[W.dtype], N, K, W.stride(0), group_size,
-            packed.data_ptr(), packed.shape[1], scales.data_ptr(), groups,
-            z.data_ptr() if zeros else None, groups, _stream(dev))
-    _lib.check("ozk_quantize_w4", st)
+    _call("ozk_quantize_w4", dev, W.data_ptr(), _TORCH_TO_OZK[W.dtype], N, K, W.stride(0),
+          group_size, packed.data_ptr(), packed.shape[1], scales.data_ptr(), groups,
+          z.data_ptr() if zeros else None, groups)
     return packed, scales, z
 
 
@@ -231,20 +271,17 @@ def dequantize_w4(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tenso
     K = packed.shape[-1] * 2 if K is None else K
     _w4_checks(packed, scales, zeros, group_size, K)
     dtype = scales.dtype if dtype is None else dtype
-    _require_gpu(packed, scales, *(() if zeros is None else (zeros,)))
+    _on_one_gpu(packed, scales, zeros)
     _require_dtype("dequantize_w4", dtype, _FLOAT)
     assert scales.dtype in (dtype, torch.float32), \
         f"scales must be {dtype} or float32, got {scales.dtype}"
     packed, scales, zeros = _w4_operands(packed, scales, zeros)
     N, dev = packed.shape[0], packed.device
     W = torch.empty((N, K), dtype=dtype, device=dev)
-    with _on_device(dev):
-        st = _lib.load().ozk_dequantize_w4(
-            packed.data_ptr(), packed.stride(0), scales.data_ptr(), _TORCH_TO_OZK[scales.dtype],
-            scales.stride(0), None if zeros is None else zeros.data_ptr(),
-            0 if zeros is None else zeros.stride(0), group_size, N, K, W.data_ptr(),
-            _TORCH_TO_OZK[dtype], K, _stream(dev))
-    _lib.check("ozk_dequantize_w4", st)
+    _call("ozk_dequantize_w4", dev, packed.data_ptr(), packed.stride(0), scales.data_ptr(),
+          _TORCH_TO_OZK[scales.dtype], scales.stride(0),
+          None if zeros is None else zeros.data_ptr(), 0 if zeros is None else zeros.stride(0),
+          group_size, N, K, W.data_ptr(), _TORCH_TO_OZK[dtype], K)
     return W
 
 
@@ -265,7 +302,7 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     _w4_checks(packed, scales, zeros, group_size, K)
     assert scales.dtype in (x.dtype, torch.float32), \
         f"scales must be {x.dtype} or float32, got {scales.dtype}"
-    _require_gpu(x, packed, scales, *(() if zeros is None else (zeros,)))
+    _on_one_gpu(x, packed, scales, zeros)
     dtype = x.dtype
     _require_dtype("matmul_w4", dtype, _FLOAT)
     _no_grad("matmul_w4", x, scales)
@@ -275,20 +312,14 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
         x2 = x2.contiguous()
     M, N, dev = x2.shape[0], packed.shape[0], x.device
     y = torch.empty((M, N), dtype=dtype, device=dev)
-    L = _lib.load()
     code = _TORCH_TO_OZK[dtype]
-    nbytes = ctypes.c_size_t(0)
-    _lib.check("ozk_matmul_w4_workspace_bytes",
-               L.ozk_matmul_w4_workspace_bytes(code, M, N, K, group_size, ctypes.byref(nbytes)))
-    n = nbytes.value
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    with _on_device(dev):
-        st = L.ozk_matmul_w4(
-            x2.data_ptr(), code, x2.stride(0), packed.data_ptr(), packed.stride(0),
-            scales.data_ptr(), _TORCH_TO_OZK[scales.dtype], scales.stride(0),
-            None if zeros is None else zeros.data_ptr(), 0 if zeros is None else zeros.stride(0),
-            group_size, M, N, K, y.data_ptr(), N, ws.data_ptr() if n else None, n, _stream(dev))
-    _lib.check("ozk_matmul_w4", st)
+    n = _bytes("ozk_matmul_w4_workspace_bytes", code, M, N, K, group_size)
+    ws, wsp = _workspace(n, dev)
+    _call("ozk_matmul_w4", dev, x2.data_ptr(), code, x2.stride(0), packed.data_ptr(),
+          packed.stride(0), scales.data_ptr(), _TORCH_TO_OZK[scales.dtype], scales.stride(0),
+          None if zeros is None else zeros.data_ptr(), 0 if zeros is None else zeros.stride(0),
+          group_size, M, N, K, y.data_ptr(), N, wsp, n)
+    del ws
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
@@ -316,7 +347,7 @@ def orthogonalize(G: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750
     triples = [co] * steps if len(co) == 3 and not hasattr(co[0], "__len__") else co
     assert len(triples) == steps and all(len(t) == 3 for t in triples), \
         f"coefficients must be one triple or {steps}, got {coefficients!r}"
-    _require_gpu(G)
+    _on_one_gpu(G)
     _require_dtype("orthogonalize", G.dtype, _FLOAT)
     _no_grad("orthogonalize", G)
     M, N = G.shape[-2:]
@@ -327,16 +358,10 @@ def orthogonalize(G: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750
     out = torch.empty((B, M, N), dtype=G.dtype, device=dev)
     if out.numel() == 0:
         return out.view(G.shape)
-    L = _lib.load()
-    nbytes = ctypes.c_size_t(0)
-    _lib.check("ozk_orthogonalize_workspace_bytes",
-               L.ozk_orthogonalize_workspace_bytes(B, M, N, steps, ctypes.byref(nbytes)))
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+    n = _bytes("ozk_orthogonalize_workspace_bytes", B, M, N, steps)
+    ws, wsp = _workspace(n, dev)
     flat = (ctypes.c_double * (3 * steps))(*[float(v) for t in triples for v in t])
-    with _on_device(dev):
-        st = L.ozk_orthogonalize(
-            G3.data_ptr(), _TORCH_TO_OZK[G.dtype], B, M, N, _lib.i64arr(G3.stride()[:2]), flat,
-            steps, float(eps), out.data_ptr(), _lib.i64arr((M * N, N)), ws.data_ptr(),
-            nbytes.value, _stream(dev))
-    _lib.check("ozk_orthogonalize", st)
+    _call("ozk_orthogonalize", dev, G3.data_ptr(), _TORCH_TO_OZK[G.dtype], B, M, N,
+          _i64(*G3.stride()[:2]), flat, steps, float(eps), out.data_ptr(), _i64(M * N, N), wsp, n)
+    del ws
     return out.view(G.shape)
