@@ -37,6 +37,51 @@ OZK_DEV Segment segment_at(const GroupedParams &p, int64_t s) {
     return {s, lo, hi < lo ? lo : hi};
 }
 
+// The tile's values, rounded, to C [rows, cols]
+template <typename ST, typename Loop>
+OZK_DEV void store_tile(const Loop &t, char *C, int64_t pitch, int rows, int cols) {
+    const bool wide = ((pitch | (int64_t)(uintptr_t)C) & 15) == 0;
+    auto bits = [](f32x4 v) {
+        uint16_t e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = to_bits16(v[i], ST{});
+        i32x2 u;
+        __builtin_memcpy(&u, e, 8);
+        return u;
+    };
+    auto put = [&](int m, int n, i32x2 u) {   // columns n .. n + 3
+        uint16_t e[4];
+        __builtin_memcpy(e, &u, 8);
+        uint16_t *to = (uint16_t *)(C + m * pitch) + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (m < rows && n + i < cols) to[i] = e[i];
+    };
+    if constexpr (Loop::NI % 2 == 0) {
+        const int g = (threadIdx.x >> 4) & 3;
+        t.each_pair([&](int m, int n, f32x4 lo, f32x4 hi) {
+            const i32x2 a = bits(lo), b = bits(hi);
+            const int n32 = n - 4 * g;
+            if (wide && n32 + 32 <= cols) {
+                const i32x4 v = join_pair(a, b);
+                if (m < rows) *(i32x4 *)(C + m * pitch + (n32 + pair_column(g)) * 2) = v;
+            } else {
+                put(m, n, a);
+                put(m, n + 16, b);
+            }
+        });
+    } else {
+        t.each([&](int m, int n, f32x4 v) {
+            const i32x2 u = bits(v);
+            if (wide && n + 4 <= cols) {
+                if (m < rows) *(i32x2 *)(C + m * pitch + n * 2) = u;
+            } else {
+                put(m, n, u);
+            }
+        });
+    }
+}
+
 template <typename ST, typename Sh, bool DMA>
 __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_kernel(GroupedParams p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -103,24 +148,7 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_kernel(Grou
                           : TileSrc{Bg + n0 * p.b_pitch, p.b_pitch, cols, none ? 0 : p.K * 2};
     t.run(A, B, smem);
 
-    char *C = p.C + lo * p.c_pitch + n0 * 2;
-    const bool wide = ((p.c_pitch | (int64_t)(uintptr_t)C) & 7) == 0;
-    t.each([&](int m, int n, f32x4 v) {
-        if (m >= rows || n >= cols) return;
-        uint16_t e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = to_bits16(v[i], ST{});
-        uint16_t *to = (uint16_t *)(C + m * p.c_pitch) + n;
-        if (wide && n + 4 <= cols) {
-            i32x2 u;
-            __builtin_memcpy(&u, e, 8);
-            *(i32x2 *)to = u;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (n + i < cols) to[i] = e[i];
-        }
-    });
+    store_tile<ST>(t, p.C + lo * p.c_pitch + n0 * 2, p.c_pitch, rows, cols);
 }
 
 // dB: the rows of a group are the contraction, both operands "cols".  With
@@ -169,24 +197,8 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_grad_kernel
         });
         return;
     }
-    char *C = p.dB + (int64_t)g * p.db_group + k0 * p.db_pitch + n0 * 2;
-    const bool wide = ((p.db_pitch | (int64_t)(uintptr_t)C) & 7) == 0;
-    t.each([&](int m, int n, f32x4 v) {
-        if (m >= rows || n >= cols) return;
-        uint16_t e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = to_bits16(v[i], ST{});
-        uint16_t *to = (uint16_t *)(C + m * p.db_pitch) + n;
-        if (wide && n + 4 <= cols) {
-            i32x2 u;
-            __builtin_memcpy(&u, e, 8);
-            *(i32x2 *)to = u;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (n + i < cols) to[i] = e[i];
-        }
-    });
+    store_tile<ST>(t, p.dB + (int64_t)g * p.db_group + k0 * p.db_pitch + n0 * 2, p.db_pitch, rows,
+                   cols);
 }
 
 template <typename ST>

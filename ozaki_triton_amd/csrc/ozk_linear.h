@@ -86,11 +86,27 @@ hipError_t launch_quantize_w4(const QuantParams &p, int dtype, hipStream_t st);
 hipError_t launch_dequantize_w4(const QuantParams &p, int dtype, int scale_dtype, hipStream_t st);
 
 // Newton-Schulz orthogonalisation of batch matrices G [M, N]; inside, X is
-// [m, n] with m <= n (G transposed where M > N).
-struct OrthStep {            // factors of the products and of what is added, scales included
-    float a_acc;             // A = X X^T
-    float b_a, b_acc;        // B = b A + c A A
-    float x_x, x_acc;        // X' = a X + B X
+// [m, n] with m <= n (G transposed where M > N).  A plan is a list of products
+//   D = f_acc L R + f_y Y + f_i I
+// of matrices that are kept as slices, the last one into the result.
+enum OrthKind {
+    kOrthXX = 0,     // D [m, m] = X X^T
+    kOrthSym = 1,    // D [m, m] symmetric, L and R symmetric and commuting
+    kOrthX = 2,      // D [m, n], R and Y of X's size
+    kOrthLast = 3    // the same into the result
+};
+constexpr int kOrthSquares = 5;   // [m, m] buffers
+struct OrthOp {
+    int kind;
+    int L, R, Y, D;          // buffers: 0 .. 4 square, -1 and -2 X's two, -9 none
+    float f_acc, f_y, f_i;   // scales of the slices included
+};
+constexpr int kOrthMaxOps = 4 * 64;
+struct OrthPlan {
+    OrthOp op[kOrthMaxOps];
+    int ops;
+    int squares, xs;         // buffers used
+    float start_scale;       // of X's slices at the start, a power of two
 };
 struct OrthParams {
     const char *G;
@@ -98,14 +114,13 @@ struct OrthParams {
     int64_t batch, M, N;
     int64_t g_batch, g_row, o_batch, o_row;    // elements
     double eps;
-    float start_scale;                         // of X's slices at the start, a power of two
+    float start_scale;
     // workspace
     double *sums;                              // [batch, blocks] partial sums of squares
     int blocks;
-    char *X[2], *A, *B;                        // slices
+    char *X[2], *S[kOrthSquares];              // slices
 };
 int orth_blocks(int64_t batch, int64_t M, int64_t N);
-hipError_t launch_orth(const OrthParams &p, const OrthStep *steps, int count, int dtype,
-                       hipStream_t st);
+hipError_t launch_orth(const OrthParams &p, const OrthPlan &plan, int dtype, hipStream_t st);
 
 }  // namespace ozk

@@ -94,25 +94,37 @@ template <typename T> __global__ __launch_bounds__(256) void orth_start_kernel(O
     }
 }
 
-enum OrthKind { kOrthA = 0, kOrthB = 1, kOrthX = 2, kOrthLast = 3 };
-
 struct OrthGemm {
-    const char *L, *R, *Y;       // left and right operand, what is added (slices)
+    const char *L, *R, *Y;       // left and right operand, what is added or null
     char *D;
     int64_t m, n;                // of X
     int64_t l_batch, r_batch, y_batch, d_batch;   // bytes
     int64_t d_row;               // kOrthLast: elements
-    float f_y, f_acc;
+    float f_acc, f_y, f_i;
     int64_t tiles_m, tiles_n;
     uint32_t total;
     int flip;
 };
 
+// the largest r with r (r + 1) / 2 <= t
+OZK_DEV uint32_t triangle_row(uint32_t t) {
+    uint32_t r = (uint32_t)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((uint64_t)r * (r + 1) / 2 > t) --r;
+    while ((uint64_t)(r + 1) * (r + 2) / 2 <= t) ++r;
+    return (uint32_t)uniform((int)r);
+}
+
+OZK_DEV i32x2 pack_half(const _Float16 (&v)[4]) {
+    i32x2 u;
+    __builtin_memcpy(&u, v, 8);
+    return u;
+}
+
 template <typename T, int KIND, typename Sh>
 __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(OrthGemm p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int BM = Sh::BM, BN = Sh::BN;
-    constexpr bool kSym = KIND == kOrthA || KIND == kOrthB;
+    constexpr bool kSym = KIND == kOrthXX || KIND == kOrthSym;
     static_assert(!kSym || BM == BN, "symmetric products run on square tiles");
     const int64_t tile = xcd_tile(blockIdx.x, p.total);
     if (tile < 0) return;
@@ -121,11 +133,22 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
     const uint32_t b = (uint32_t)tile / each, in = (uint32_t)tile - b * each;
     uint32_t tm, tn;
     if (kSym) {
-        tm = (uint32_t)((sqrtf(8.f * (float)in + 1.f) - 1.f) * 0.5f);
-        while ((uint64_t)tm * (tm + 1) / 2 > in) --tm;
-        while ((uint64_t)(tm + 1) * (tm + 2) / 2 <= in) ++tm;
-        tm = (uint32_t)uniform((int)tm);
-        tn = in - tm * (tm + 1) / 2;
+        // on and below the diagonal, in blocks of 512 x 512 (row of blocks by row
+        // of blocks, inside one column by column): an XCD's workgroups share the
+        // rows of a block, not those of a whole row of tiles
+        constexpr uint32_t SB = 512 / BM;
+        const uint32_t r0 = triangle_row(in) / SB * SB, rest = in - r0 * (r0 + 1) / 2;
+        const uint32_t left = (uint32_t)p.tiles_m - r0, h = left < SB ? left : SB;
+        const uint32_t J = rest / (h * SB) * SB;
+        if (J < r0) {
+            const uint32_t t = rest - J * h;
+            tn = J + t / h;
+            tm = r0 + t - (t / h) * h;
+        } else {
+            const uint32_t t = rest - r0 * h, r = triangle_row(t);
+            tm = r0 + r;
+            tn = r0 + t - r * (r + 1) / 2;
+        }
     } else {
         // 8 tile rows at a time, column by column
         const uint32_t first = in / (uint32_t)p.tiles_n / 8 * 8;
@@ -135,8 +158,8 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
         tm = first + at - tn * high;
     }
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-    const int64_t lp = KIND == kOrthA ? slice_pitch(p.n) : slice_pitch(p.m);
-    const int64_t rp = KIND == kOrthB ? slice_pitch(p.m) : slice_pitch(p.n);
+    const int64_t lp = KIND == kOrthXX ? slice_pitch(p.n) : slice_pitch(p.m);
+    const int64_t rp = KIND == kOrthSym ? slice_pitch(p.m) : slice_pitch(p.n);
     const int64_t cols_all = kSym ? p.m : p.n;
     const int rows = (int)(p.m - m0 < BM ? p.m - m0 : BM);
     const int cols = (int)(cols_all - n0 < BN ? cols_all - n0 : BN);
@@ -148,54 +171,115 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
                                 : TileSrc{R + n0 * rp, rp, cols, rp};
     t.run(A, B, smem);
 
-    const int64_t dp = kSym ? slice_pitch(p.m) : slice_pitch(p.n);   // of D's slices
+    const int64_t dp = kSym ? slice_pitch(p.m) : slice_pitch(p.n);   // of D's and Y's slices
     const int cols_up = (cols + 31) / 32 * 32, rows_up = (rows + 31) / 32 * 32;   // with the zeros
-    const char *Y = p.Y + (int64_t)b * p.y_batch;
+    const char *Y = p.Y ? p.Y + (int64_t)b * p.y_batch : nullptr;
     char *D = p.D + (int64_t)b * p.d_batch;
-    t.each([&](int mi, int ni, f32x4 acc) {
-        if (ni >= cols_up) return;
+    const int g = (threadIdx.x >> 4) & 3, q = threadIdx.x & 3;
+    const bool diagonal = KIND == kOrthSym && tm == tn && p.f_i != 0.f;
+    // 32 columns at a time: a line of D's slices
+    t.each_pair([&](int mi, int ni, f32x4 lo, f32x4 hi) {
+        const int n32 = ni - 4 * g;
+        if (n32 >= cols_up) return;
         const int64_t m = m0 + mi, n = n0 + ni;
-        float v[4];
-        if constexpr (KIND == kOrthA) {
+        const int64_t line = m * dp + (n0 + n32) * 4;
+        float v[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[e] * p.f_acc;
-        } else {
-            _Float16 h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
-            if (mi < rows) {
-                const char *at = Y + m * dp + n / 32 * 128 + n % 32 * 2;
-                __builtin_memcpy(h, at, 8);
-                __builtin_memcpy(l, at + 64, 8);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = __builtin_fmaf(acc[e], p.f_acc, ((float)h[e] + (float)l[e]) * p.f_y);
+        for (int e = 0; e < 4; ++e) {
+            v[0][e] = lo[e] * p.f_acc;
+            v[1][e] = hi[e] * p.f_acc;
         }
-        if constexpr (KIND == kOrthLast) {
-            if (mi >= rows) return;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (ni + e < cols)
-                    orth_store<T>(D, p.flip ? (n + e) * p.d_row + m : m * p.d_row + n + e, v[e]);
-        } else {
-            _Float16 h[4], l[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                h[e] = (_Float16)v[e];
-                l[e] = (_Float16)(v[e] - (float)h[e]);
-            }
+        if (KIND != kOrthXX && Y) {
+            i32x4 y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
             if (mi < rows) {
-                char *at = D + m * dp + n / 32 * 128 + n % 32 * 2;
-                __builtin_memcpy(at, h, 8);
-                __builtin_memcpy(at + 64, l, 8);
+                y[0] = *(const i32x4 *)(Y + line + pair_column(g) * 2);
+                y[1] = *(const i32x4 *)(Y + line + pair_column(g) * 2 + 64);
             }
-            if (kSym && tm != tn && mi < rows_up) {
+            i32x2 h[2], l[2];
+            split_pair(y[0], h[0], h[1]);
+            split_pair(y[1], l[0], l[1]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                _Float16 hv[4], lv[4];
+                __builtin_memcpy(hv, &h[u], 8);
+                __builtin_memcpy(lv, &l[u], 8);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[u][e] += ((float)hv[e] + (float)lv[e]) * p.f_y;
+            }
+        }
+        if (diagonal)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (ni + e < cols) {
-                        char *at = D + (n + e) * dp + m / 32 * 128 + m % 32 * 2;
-                        *(_Float16 *)at = h[e];
-                        *(_Float16 *)(at + 64) = l[e];
+                    if (mi == ni + 16 * u + e && mi < rows) v[u][e] += p.f_i;
+        if constexpr (KIND == kOrthLast) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int c = ni + 16 * u;
+                if constexpr (sizeof(T) == 2) {
+                    uint16_t e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[i] = to_bits16(v[u][i], T{});
+                    i32x2 w;
+                    __builtin_memcpy(&w, e, 8);
+                    int64_t at = m * p.d_row + n0 + c;
+                    bool whole = mi < rows && c + 4 <= cols;
+                    if (p.flip) {
+                        // four rows of the result, four of its columns
+                        w = transpose_quad(w);
+                        __builtin_memcpy(e, &w, 8);
+                        at = (n0 + c + q) * p.d_row + m - q;
+                        whole = mi - q + 4 <= rows && c + q < cols;
                     }
+                    char *to = D + at * 2;
+                    if (whole && ((uintptr_t)to & 7) == 0) {
+                        *(i32x2 *)to = w;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (p.flip ? mi - q + i < rows && c + q < cols : mi < rows && c + i < cols)
+                                ((uint16_t *)to)[i] = e[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (mi < rows && c + i < cols)
+                            ((float *)D)[p.flip ? (n0 + c + i) * p.d_row + m
+                                                : m * p.d_row + n0 + c + i] = v[u][i];
+                }
+            }
+        } else {
+            i32x2 h[2], l[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                _Float16 hv[4], lv[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    hv[e] = (_Float16)v[u][e];
+                    lv[e] = (_Float16)(v[u][e] - (float)hv[e]);
+                }
+                h[u] = pack_half(hv);
+                l[u] = pack_half(lv);
+            }
+            const i32x4 hj = join_pair(h[0], h[1]), lj = join_pair(l[0], l[1]);
+            if (mi < rows) {
+                char *to = D + line + pair_column(g) * 2;
+                *(i32x4 *)to = hj;
+                *(i32x4 *)(to + 64) = lj;
+            }
+            if (kSym && tm != tn) {
+                // the mirrored tile: four lanes' values of a column, a row there
+                const int m4 = mi - q;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const i32x2 ht = transpose_quad(h[u]), lt = transpose_quad(l[u]);
+                    if (m4 < rows_up && ni + 16 * u + q < cols) {
+                        char *to = D + (n + 16 * u + q) * dp + (m0 + m4) / 32 * 128 + (m0 + m4) % 32 * 2;
+                        *(i32x2 *)to = ht;
+                        *(i32x2 *)(to + 64) = lt;
+                    }
+                }
             }
         }
     });
@@ -240,7 +324,7 @@ hipError_t orth_product(const OrthGemm &q, int64_t batch, hipStream_t st) {
 }
 
 template <typename T>
-hipError_t orth_run(const OrthParams &p, const OrthStep *steps, int count, hipStream_t st) {
+hipError_t orth_run(const OrthParams &p, const OrthPlan &plan, hipStream_t st) {
     const bool flip = p.M > p.N;
     const int64_t m = flip ? p.N : p.M, n = flip ? p.M : p.N;
     const int64_t xb = m * slice_pitch(n), ab = m * slice_pitch(m);
@@ -248,38 +332,29 @@ hipError_t orth_run(const OrthParams &p, const OrthStep *steps, int count, hipSt
     orth_start_kernel<T><<<dim3((uint32_t)((n + 31) / 32), (uint32_t)((m + 63) / 64),
                                 (uint32_t)p.batch), 256, 0, st>>>(p);
     hipError_t e = hipGetLastError();
-    OrthGemm q;
-    q.m = m;
-    q.n = n;
-    q.flip = flip;
-    q.d_row = p.o_row;
-    for (int i = 0; i < count && e == hipSuccess; ++i) {
-        const char *X = p.X[i & 1];
-        q.L = q.R = q.Y = X;
-        q.l_batch = q.r_batch = q.y_batch = xb;
-        q.D = p.A;
-        q.d_batch = ab;
-        q.f_y = 0.f;
-        q.f_acc = steps[i].a_acc;
-        e = orth_product<T, kOrthA>(q, p.batch, st);
-        if (e != hipSuccess) break;
-        q.L = q.R = q.Y = p.A;
-        q.l_batch = q.r_batch = q.y_batch = ab;
-        q.D = p.B;
-        q.f_y = steps[i].b_a;
-        q.f_acc = steps[i].b_acc;
-        e = orth_product<T, kOrthB>(q, p.batch, st);
-        if (e != hipSuccess) break;
-        q.L = p.B;
-        q.R = q.Y = X;
-        q.r_batch = q.y_batch = xb;
-        q.f_y = steps[i].x_x;
-        q.f_acc = steps[i].x_acc;
-        if (i + 1 < count) {
-            q.D = p.X[(i + 1) & 1];
-            q.d_batch = xb;
-            e = orth_product<T, kOrthX>(q, p.batch, st);
-        } else {
+    auto buffer = [&](int id, int64_t &bytes) -> char * {
+        bytes = id >= 0 ? ab : xb;
+        return id >= 0 ? p.S[id] : id >= -2 ? p.X[-1 - id] : nullptr;
+    };
+    for (int i = 0; i < plan.ops && e == hipSuccess; ++i) {
+        const OrthOp &op = plan.op[i];
+        OrthGemm q;
+        q.m = m;
+        q.n = n;
+        q.flip = flip;
+        q.d_row = p.o_row;
+        q.f_acc = op.f_acc;
+        q.f_y = op.f_y;
+        q.f_i = op.f_i;
+        q.L = buffer(op.L, q.l_batch);
+        q.R = buffer(op.R, q.r_batch);
+        q.Y = buffer(op.Y, q.y_batch);
+        q.D = buffer(op.D, q.d_batch);
+        switch (op.kind) {
+        case kOrthXX: e = orth_product<T, kOrthXX>(q, p.batch, st); break;
+        case kOrthSym: e = orth_product<T, kOrthSym>(q, p.batch, st); break;
+        case kOrthX: e = orth_product<T, kOrthX>(q, p.batch, st); break;
+        default:
             q.D = p.out;
             q.d_batch = p.o_batch * (int64_t)sizeof(T);
             e = orth_product<T, kOrthLast>(q, p.batch, st);
@@ -297,10 +372,9 @@ int orth_blocks(int64_t batch, int64_t M, int64_t N) {
     return (int)(b < 1 ? 1 : b);
 }
 
-hipError_t launch_orth(const OrthParams &p, const OrthStep *steps, int count, int dtype,
-                       hipStream_t st) {
-    if (dtype == 1) return orth_run<float>(p, steps, count, st);
-    return dtype == 2 ? orth_run<_Float16>(p, steps, count, st) : orth_run<__bf16>(p, steps, count, st);
+hipError_t launch_orth(const OrthParams &p, const OrthPlan &plan, int dtype, hipStream_t st) {
+    if (dtype == 1) return orth_run<float>(p, plan, st);
+    return dtype == 2 ? orth_run<_Float16>(p, plan, st) : orth_run<__bf16>(p, plan, st);
 }
 
 }  // namespace ozk
