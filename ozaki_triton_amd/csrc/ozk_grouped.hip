@@ -146,7 +146,7 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_kernel(Grou
     const char *Bg = p.B + (none ? 0 : seg - 1) * p.b_group;
     TileSrc B = Sh::BCOLS ? TileSrc{Bg + n0 * 2, p.b_pitch, cols * 2, none ? 0 : p.K}
                           : TileSrc{Bg + n0 * p.b_pitch, p.b_pitch, cols, none ? 0 : p.K * 2};
-    t.run(A, B, smem);
+    if (!t.run(A, B, smem)) return;
 
     store_tile<ST>(t, p.C + lo * p.c_pitch + n0 * 2, p.c_pitch, rows, cols);
 }
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_grad_kernel
     TileLoop<ST, Sh, DMA> t;
     const TileSrc A = {p.A + lo * p.a_pitch + k0 * 2, p.a_pitch, rows * 2, hi - lo};
     const TileSrc B = {p.D + lo * p.d_pitch + n0 * 2, p.d_pitch, cols * 2, hi - lo};
-    t.run(A, B, smem);
+    if (!t.run(A, B, smem)) return;
 
     if (p.splits > 1) {
         float *P = p.part + ((int64_t)s * p.G + g) * p.K * p.N + k0 * p.N + n0;
@@ -243,17 +243,20 @@ hipError_t grad_go(const GroupedGradParams &p, hipStream_t st) {
 // group is taken to leave half a tile row unused.  The largest tile reads the
 // least per product but wants two rounds of workgroups; smaller groups take
 // the tile that covers most groups whole (each tile row reads the group's
-// matrix again), with more stages in flight where a CU has one workgroup.
-// Measured (us, T x G x K x N, counts uneven, bf16; 256 x 256 / 128 x 128 of 8
-// waves and 4 stages / 64 x 128 of 2 stages / 64 x 64 of 4 / 32 x 64 of 4):
-//     32768 x 16 x 2048 x 4096   570 /  789 /  800 / 1068 / 1357
+// matrix again); where a CU has one workgroup at most, two groups of waves
+// share its stages.  Measured (us, T x G x K x N, counts uneven, bf16;
+// 256 x 256 / 128 x 128 of 4 stages / 64 x 128 / 64 x 64 in two groups / 32 x 64
+// in two groups of 4 stages):
+//     32768 x 16 x 2048 x 4096   552 /  789 /  800 / 1068 / 1357
 //     16384 x 32 x 1024 x 2048   101 /  128 /  112 /  161 /  203
-//     4096 x 8 x 1024 x 4096      69 /   72 /   58 /   85 /  104
-//     1999 x 7 x 1000 x 520       28 /   14 /   13 /   12 /   14
-//     512 x 8 x 1024 x 2048       32 /   16 /   17 /   15 /   14
-//     300 x 8 x 4096 x 4096       96 /   46 /   65 /   64 /   70
-//     200 x 32 x 1024 x 2048      30 /   29 /   23 /   27 /   26
-//     16 x 16 x 1024 x 2048       26 /   13 /   12 /   10 /    9
+//     4096 x 8 x 1024 x 4096      69 /   65 /   57 /   86 /  189
+//     1999 x 7 x 1000 x 520       28 /   14 /   13 /   11 /   19
+//     512 x 8 x 1024 x 2048       32 /   15 /   17 /   14 /   20
+//     300 x 8 x 4096 x 4096       96 /   46 /   67 /   71 /   71
+//     200 x 32 x 1024 x 2048      30 /   30 /   23 /   26 /   35
+//     2000 x 2 x 4096 x 256        - /   38 /   48 /   25 /   16
+//     4 x 4 x 4096 x 1024          - /   40 /   39 /   20 /   15
+//     16 x 16 x 1024 x 2048       26 /   13 /   12 /  8.4 /  7.7
 template <typename ST, bool BCOLS> hipError_t grouped_plan(const GroupedParams &p, hipStream_t st) {
     const bool pieces = (((uintptr_t)p.A | (uintptr_t)p.B | p.a_pitch | p.b_pitch | p.b_group |
                           p.K * 2 | (BCOLS ? p.N * 2 : 0)) & 15) == 0;
@@ -271,8 +274,9 @@ template <typename ST, bool BCOLS> hipError_t grouped_plan(const GroupedParams &
         return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 4, 4>, true>(p, st);
     if (tiles(64, 128) >= 256)
         return grouped_go<ST, TileShape<1, false, BCOLS, 64, 128, 1, 4, 2>, true>(p, st);
-    if (rows >= 8) return grouped_go<ST, TileShape<1, false, BCOLS, 64, 64, 2, 2, 4>, true>(p, st);
-    return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 4>, true>(p, st);
+    if (tiles(32, 64) <= 256)
+        return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 4, 2>, true>(p, st);
+    return grouped_go<ST, TileShape<1, false, BCOLS, 64, 64, 2, 2, 2, 2>, true>(p, st);
 }
 
 template <typename ST> hipError_t grad_plan(const GroupedGradParams &p, hipStream_t st) {

@@ -169,7 +169,7 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
     const TileSrc A = {L + m0 * lp, lp, rows, lp};
     const TileSrc B = Sh::BCOLS ? TileSrc{R + n0 * 4, rp, (int)(rp - n0 * 4 < BN * 4 ? rp - n0 * 4 : BN * 4), p.m}
                                 : TileSrc{R + n0 * rp, rp, cols, rp};
-    t.run(A, B, smem);
+    if (!t.run(A, B, smem)) return;
 
     const int64_t dp = kSym ? slice_pitch(p.m) : slice_pitch(p.n);   // of D's and Y's slices
     const int cols_up = (cols + 31) / 32 * 32, rows_up = (rows + 31) / 32 * 32;   // with the zeros
@@ -287,9 +287,9 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
 
 namespace {
 
-template <typename T, int KIND, int BM, int WM, int WN, int NST>
+template <typename T, int KIND, int BM, int WM, int WN, int NST, int KW = 1>
 hipError_t orth_gemm(OrthGemm q, int64_t batch, hipStream_t st) {
-    using Sh = TileShape<2, false, KIND >= kOrthX, BM, BM, WM, WN, NST>;
+    using Sh = TileShape<2, false, KIND >= kOrthX, BM, BM, WM, WN, NST, KW>;
     q.tiles_m = (q.m + BM - 1) / BM;
     q.tiles_n = ((KIND >= kOrthX ? q.n : q.m) + BM - 1) / BM;
     const int64_t tiles = batch * (KIND >= kOrthX ? q.tiles_m * q.tiles_n
@@ -310,17 +310,19 @@ hipError_t orth_product(const OrthGemm &q, int64_t batch, hipStream_t st) {
         const int64_t tm = (q.m + bm - 1) / bm, tn = (cols + bm - 1) / bm;
         return batch * (KIND >= kOrthX ? tm * tn : tm * (tm + 1) / 2);
     };
-    // the largest tile that still gives the CUs enough workgroups; where each has
-    // one at most, more stages in flight.  Measured (us, A = X X^T / B X of
-    // 2048 x 8192, then of 1024 x 1024, then of 8 matrices 256 x 512):
-    //     256 x 256                452 / 200    76 / 84    44 / 38
-    //     128 x 128                265 / 200    41 / 44    21 / 16
-    //     64 x 64, two stages      168 / 249    23 / 24    11 / 8.4
-    //     64 x 64, four stages     205 / 274    16 / 17    10 / 8.1
+    // The largest tile that still gives the CUs enough workgroups; below 256 x 256
+    // a CU has one at most, and two groups of waves share its stages.  Measured
+    // (us, X X^T / A A / B X of 2048 x 8192, then of 1024 x 1024, then of 8
+    // matrices 256 x 512):
+    //     256 x 256, 8 waves               424 / 129 / 175   75 / 82 / 71    44 / 36 / 38
+    //     128 x 128, 2 x 8 waves           140 /  45 / 182   26 / 30 / 24    17 / 14 / 11
+    //     128 x 128, 8 waves, 4 stages     166 /  51 / 221   27 / 31 / 28    17 / 14 / 14
+    //     64 x 64, 2 x 4 waves, 4 stages   177 /  57 / 338   13 / 13 / 15   8.8 / 7.2 / 7.6
+    //     64 x 64, 4 waves, 4 stages       199 /  59 / 315   15 / 16 / 18   9.8 / 7.4 / 8.1
+    //     64 x 64, 4 waves, 2 stages       161 /  49 / 236   22 / 23 / 25    11 / 7.5 / 8.4
     if (tiles(256) >= 192) return orth_gemm<T, KIND, 256, 2, 4, 2>(q, batch, st);
-    if (tiles(128) >= 256) return orth_gemm<T, KIND, 128, 2, 2, 2>(q, batch, st);
-    if (tiles(64) >= 384) return orth_gemm<T, KIND, 64, 2, 2, 2>(q, batch, st);
-    return orth_gemm<T, KIND, 64, 2, 2, 4>(q, batch, st);
+    if (tiles(128) >= 112) return orth_gemm<T, KIND, 128, 2, 4, 2, 2>(q, batch, st);
+    return orth_gemm<T, KIND, 64, 2, 2, 4, 2>(q, batch, st);
 }
 
 template <typename T>

@@ -64,11 +64,14 @@ struct TileSrc {
 
 constexpr uint32_t kTileOOB = 0x80000000u;   // past every buffer: the DMA writes zeros
 
-template <int S_, bool ACOLS_, bool BCOLS_, int BM_, int BN_, int WM_, int WN_, int NST_>
+// KW > 1: so many groups of WM x WN waves, group w takes every KW-th stage from
+// w on; the groups' sums are added in order at the end.
+template <int S_, bool ACOLS_, bool BCOLS_, int BM_, int BN_, int WM_, int WN_, int NST_,
+          int KW_ = 1>
 struct TileShape {
-    static constexpr int S = S_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, NST = NST_;
+    static constexpr int S = S_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, NST = NST_, KW = KW_;
     static constexpr bool ACOLS = ACOLS_, BCOLS = BCOLS_;
-    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES * KW;   // waves of a group
     static constexpr int KS = 64 / S;                 // elements of K per stage
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
     static constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
@@ -78,7 +81,8 @@ struct TileShape {
     static constexpr bool ONE = BM / 8 % LP == 0;
     static constexpr int LPA = ONE ? 0 : BM / 8 / WAVES;
     static_assert(ONE || (BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0), "windows per operand");
-    static constexpr int LDS_BYTES = NST * STAGE;
+    static constexpr int SLOT = KW * STAGE, JOIN = (KW - 1) * WAVES * MI * NI * 1024;
+    static constexpr int LDS_BYTES = NST * SLOT > JOIN ? NST * SLOT : JOIN;
     // waves per SIMD that the registers have to leave room for
     static constexpr int PER_SIMD = 2;
     static_assert(LP * WAVES * 1024 == STAGE, "windows split evenly over the waves");
@@ -177,9 +181,11 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
     static constexpr int S = Sh::S, LP = Sh::LP, MI = Sh::MI, NI = Sh::NI;
     f32x4 acc[MI][NI];
 
-    OZK_DEV void run(const TileSrc &A, const TileSrc &B, char *smem) {
+    // All waves; false in the waves whose sums another one has taken over.
+    OZK_DEV bool run(const TileSrc &A, const TileSrc &B, char *smem) {
         const int lane = threadIdx.x & 63;
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % Sh::WAVES;
+        const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / Sh::WAVES;
         const int wm = wave / Sh::WN, wn = wave % Sh::WN;
 #pragma unroll
         for (int i = 0; i < MI; ++i)
@@ -188,20 +194,29 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
 
         constexpr int ua = Sh::ACOLS ? Sh::KS : 128, ub = Sh::BCOLS ? Sh::KS : 128;
         const int nka = (int)((A.klen + ua - 1) / ua), nkb_b = (int)((B.klen + ub - 1) / ub);
-        const int nkb = nka < nkb_b ? nka : nkb_b;
+        const int nkb = ((nka < nkb_b ? nka : nkb_b) + Sh::KW - 1) / Sh::KW;   // of each group
 
         // the operands as this wave stages them, `base` that of the stage it is at
         struct Feed {
             const char *base;
             int64_t step;
             int whole, rest;   // whole stages, and what the one behind them has of K
-            // what stage kb has of K, as WindowAt counts it
-            OZK_DEV int left(int kb) const { return kb < whole ? 128 : rest; }
+            // what the group's stage kb has of K, as WindowAt counts it
+            OZK_DEV int left(int kb, int kw) const {
+                const int at = kb * Sh::KW + kw;
+                return at < whole ? 128 : at == whole ? rest : 0;
+            }
         };
-        const Feed fa = {A.base, Sh::ACOLS ? Sh::KS * A.pitch : 128, (int)(A.klen / ua),
-                         (int)(A.klen % ua)};
-        const Feed fb = {B.base, Sh::BCOLS ? Sh::KS * B.pitch : 128, (int)(B.klen / ub),
-                         (int)(B.klen % ub)};
+        Feed fa = {A.base, Sh::ACOLS ? Sh::KS * A.pitch : 128, (int)(A.klen / ua),
+                   (int)(A.klen % ua)};
+        Feed fb = {B.base, Sh::BCOLS ? Sh::KS * B.pitch : 128, (int)(B.klen / ub),
+                   (int)(B.klen % ub)};
+        if constexpr (Sh::KW > 1) {
+            fa.base += kw * fa.step;
+            fb.base += kw * fb.step;
+            fa.step *= Sh::KW;
+            fb.step *= Sh::KW;
+        }
         const bool onlyA = Sh::ONE && wave * LP < Sh::BM / 8;
         Feed feed[Sh::ONE ? 1 : 2];
         if constexpr (Sh::ONE) {
@@ -238,12 +253,12 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
         auto issue = [&](int kb, int q0, int q1) {
             if (kb >= nkb) return;
             if (q0 == 0 && kb > 0) advance();
-            const uint32_t dst = lds + (uint32_t)(kb % Sh::NST) * Sh::STAGE;
+            const uint32_t dst = lds + (uint32_t)(kb % Sh::NST) * Sh::SLOT + kw * Sh::STAGE;
 #pragma unroll
             for (int q = 0; q < LP; ++q) {
                 if (q < q0 || q >= q1) continue;
                 const Feed &f = feed[of(q)];
-                dma_piece(f.base, win[q].k < f.left(kb) ? win[q].off : kTileOOB, dst + slot_at[q]);
+                dma_piece(f.base, win[q].k < f.left(kb, kw) ? win[q].off : kTileOOB, dst + slot_at[q]);
             }
         };
         // the same through registers, for rows of any alignment
@@ -255,14 +270,14 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 const Feed &f = feed[of(q)];
                 const bool cols = Sh::ONE ? (onlyA ? Sh::ACOLS : Sh::BCOLS)
                                           : (of(q) == 0 ? Sh::ACOLS : Sh::BCOLS);
-                const int left = f.left(kb) - win[q].k;
+                const int left = f.left(kb, kw) - win[q].k;
                 int n = left > 0 ? win[q].n : 0;
                 if (!cols && left < n) n = left;
                 held[q] = load_piece(f.base + (n > 0 ? win[q].off : 0u), n);
             }
         };
         auto put = [&](int kb) {
-            char *dst = smem + (kb % Sh::NST) * Sh::STAGE + lane * 16;
+            char *dst = smem + (kb % Sh::NST) * Sh::SLOT + kw * Sh::STAGE + lane * 16;
 #pragma unroll
             for (int q = 0; q < LP; ++q) *(i32x4 *)(dst + slot_at[q]) = held[q];
         };
@@ -320,8 +335,8 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
         // ready(): stage kb + 1 has landed and every wave has read stage kb;
         // during(n): what else group n issues
         auto stage = [&](int kb, auto &&ready, auto &&during) {
-            const char *buf = smem + (kb % Sh::NST) * Sh::STAGE;
-            const char *next = smem + ((kb + 1) % Sh::NST) * Sh::STAGE;
+            const char *buf = smem + (kb % Sh::NST) * Sh::SLOT + kw * Sh::STAGE;
+            const char *next = smem + ((kb + 1) % Sh::NST) * Sh::SLOT + kw * Sh::STAGE;
             static_for_tile<G>([&](auto n_) {
                 constexpr int n = decltype(n_)::value, i = n % MI;
                 if constexpr (n == BG) ready();
@@ -368,7 +383,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 if (nkb >= Sh::NST) wait_vmcnt<(Sh::NST - 1) * LP>();
                 else wait_vmcnt<0>();
                 exec_barrier();
-                first(smem);
+                first(smem + kw * Sh::STAGE);
             }
             for (int kb = 0; kb < nkb; ++kb)
                 stage(
@@ -398,7 +413,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 put(0);
                 __syncthreads();
                 if (nkb > 1) fetch(1);
-                first(smem);
+                first(smem + kw * Sh::STAGE);
             }
             static_assert(DMA || Sh::NST == 2, "two slots");
             for (int kb = 0; kb < nkb; ++kb) {
@@ -413,6 +428,33 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                     [](auto) {});
             }
         }
+
+        if constexpr (Sh::KW > 1) {
+            // the groups' sums, added in order through the LDS
+            __syncthreads();
+            f32x4 *part = (f32x4 *)smem;
+            if (kw > 0)
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j)
+                        part[(((kw - 1) * Sh::WAVES + wave) * MI * NI + i * NI + j) * 64 + lane] =
+                            acc[i][j];
+            __syncthreads();
+            if (kw > 0) return false;
+#pragma unroll
+            for (int w = 0; w < Sh::KW - 1; ++w)
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) {
+                        const f32x4 v =
+                            part[((w * Sh::WAVES + wave) * MI * NI + i * NI + j) * 64 + lane];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] += v[e];
+                    }
+        }
+        return true;
     }
 
     // f(m, n, lo, hi): the four values lo of row m (of the tile), columns n ..
