@@ -270,16 +270,25 @@ int ozk_matmul_static(const void *A, const int64_t a_strides[3], const void *B,
  * strides of B; ozk_grouped_matmul_wgrad gives the one to B:
  *   dB[g] = A[rows of g]^T D[rows of g], D [T, N] the gradient of C; dB
  *   [G, K, N] with N contiguous, strides db_strides[2] of group and row, zeros
- *   for a group without rows.  Workspace: partial sums where few tiles share
- *   many rows, 0 bytes otherwise.
- * Rows longer than 2^22 elements apart return OZK_ERR_TOO_LARGE.
+ *   for a group without rows.
+ * Workspace (16-byte aligned): partial sums of dB where few tiles share many
+ * rows, which it needs, and copies of operands whose rows are no whole 16-byte
+ * pieces (size, distance or address) where they pay, without which it runs
+ * slower.  The queries look at the pointers' alignment only.
+ * Rows of 2^22 or more elements apart return OZK_ERR_TOO_LARGE.
  */
+int ozk_grouped_matmul_workspace_bytes(const void *A, int64_t a_stride, const void *B,
+                                       const int64_t b_strides[3], int64_t T, int64_t K, int64_t N,
+                                       int64_t G, size_t *bytes_out);
+
 int ozk_grouped_matmul(const void *A, int64_t a_stride, const void *B, const int64_t b_strides[3],
                        const void *offsets, int offset_bytes, int64_t T, int64_t K, int64_t N,
-                       int64_t G, int dtype, void *C, int64_t c_stride, void *stream);
+                       int64_t G, int dtype, void *C, int64_t c_stride, void *workspace,
+                       size_t workspace_bytes, void *stream);
 
-int ozk_grouped_matmul_wgrad_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t G,
-                                             size_t *bytes_out);
+int ozk_grouped_matmul_wgrad_workspace_bytes(const void *A, int64_t a_stride, const void *D,
+                                             int64_t d_stride, int64_t T, int64_t K, int64_t N,
+                                             int64_t G, size_t *bytes_out);
 
 int ozk_grouped_matmul_wgrad(const void *A, int64_t a_stride, const void *D, int64_t d_stride,
                              const void *offsets, int offset_bytes, int64_t T, int64_t K,

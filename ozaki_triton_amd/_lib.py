@@ -43,6 +43,7 @@ EXPORTED = (
     "ozk_matmul_static",
     "ozk_cross_gemm_pairs",
     "ozk_matmul_pairs",
+    "ozk_grouped_matmul_workspace_bytes",
     "ozk_grouped_matmul",
     "ozk_grouped_matmul_wgrad_workspace_bytes",
     "ozk_grouped_matmul_wgrad",
@@ -127,8 +128,10 @@ def load() -> ctypes.CDLL:
     L.ozk_matmul_pairs.restype = i32
     psz, pd = ctypes.POINTER(sz), ctypes.POINTER(ctypes.c_double)
     for name, args in (
-            ("ozk_grouped_matmul", [vp, i64, vp, p64, vp, i32, i64, i64, i64, i64, i32, vp, i64, vp]),
-            ("ozk_grouped_matmul_wgrad_workspace_bytes", [i64, i64, i64, i64, psz]),
+            ("ozk_grouped_matmul_workspace_bytes", [vp, i64, vp, p64, i64, i64, i64, i64, psz]),
+            ("ozk_grouped_matmul", [vp, i64, vp, p64, vp, i32, i64, i64, i64, i64, i32, vp, i64, vp,
+                                    sz, vp]),
+            ("ozk_grouped_matmul_wgrad_workspace_bytes", [vp, i64, vp, i64, i64, i64, i64, i64, psz]),
             ("ozk_grouped_matmul_wgrad", [vp, i64, vp, i64, vp, i32, i64, i64, i64, i64, i32, vp,
                                           p64, vp, sz, vp]),
             ("ozk_quantize_w4", [vp, i32, i64, i64, i64, i32, vp, i64, vp, i64, vp, i64, vp]),

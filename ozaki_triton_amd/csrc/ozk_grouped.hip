@@ -40,7 +40,6 @@ OZK_DEV Segment segment_at(const GroupedParams &p, int64_t s) {
 // The tile's values, rounded, to C [rows, cols]
 template <typename ST, typename Loop>
 OZK_DEV void store_tile(const Loop &t, char *C, int64_t pitch, int rows, int cols) {
-    const bool wide = ((pitch | (int64_t)(uintptr_t)C) & 15) == 0;
     auto bits = [](f32x4 v) {
         uint16_t e[4];
 #pragma unroll
@@ -62,9 +61,11 @@ OZK_DEV void store_tile(const Loop &t, char *C, int64_t pitch, int rows, int col
         t.each_pair([&](int m, int n, f32x4 lo, f32x4 hi) {
             const i32x2 a = bits(lo), b = bits(hi);
             const int n32 = n - 4 * g;
-            if (wide && n32 + 32 <= cols) {
+            if (n32 + 32 <= cols) {
                 const i32x4 v = join_pair(a, b);
-                if (m < rows) *(i32x4 *)(C + m * pitch + (n32 + pair_column(g)) * 2) = v;
+                // (rows of any alignment)
+                if (m < rows)
+                    __builtin_memcpy(C + m * pitch + (n32 + pair_column(g)) * 2, &v, 16);
             } else {
                 put(m, n, a);
                 put(m, n + 16, b);
@@ -73,8 +74,8 @@ OZK_DEV void store_tile(const Loop &t, char *C, int64_t pitch, int rows, int col
     } else {
         t.each([&](int m, int n, f32x4 v) {
             const i32x2 u = bits(v);
-            if (wide && n + 4 <= cols) {
-                if (m < rows) *(i32x2 *)(C + m * pitch + n * 2) = u;
+            if (n + 4 <= cols) {
+                if (m < rows) __builtin_memcpy(C + m * pitch + n * 2, &u, 8);
             } else {
                 put(m, n, u);
             }
@@ -142,10 +143,12 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_kernel(Grou
 
     TileLoop<ST, Sh, DMA> t;
     const bool none = seg == 0 || seg == p.G + 1;
-    TileSrc A = {p.A + lo * p.a_pitch, p.a_pitch, rows, none ? 0 : p.K * 2};
+    const int64_t ka = p.a_padded ? (p.K + 7) / 8 * 16 : p.K * 2;   // bytes of K
+    const int64_t kb = p.b_padded ? (p.K + 7) / 8 * 16 : p.K * 2;
+    TileSrc A = {p.A + lo * p.a_pitch, p.a_pitch, rows, none ? 0 : ka, p.A};
     const char *Bg = p.B + (none ? 0 : seg - 1) * p.b_group;
-    TileSrc B = Sh::BCOLS ? TileSrc{Bg + n0 * 2, p.b_pitch, cols * 2, none ? 0 : p.K}
-                          : TileSrc{Bg + n0 * p.b_pitch, p.b_pitch, cols, none ? 0 : p.K * 2};
+    TileSrc B = Sh::BCOLS ? TileSrc{Bg + n0 * 2, p.b_pitch, p.b_padded ? (cols + 7) / 8 * 16 : cols * 2, none ? 0 : p.K, p.B}
+                          : TileSrc{Bg + n0 * p.b_pitch, p.b_pitch, cols, none ? 0 : kb, p.B};
     if (!t.run(A, B, smem)) return;
 
     store_tile<ST>(t, p.C + lo * p.c_pitch + n0 * 2, p.c_pitch, rows, cols);
@@ -183,8 +186,10 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_grad_kernel
     const int cols = (int)(p.N - n0 < BN ? p.N - n0 : BN);
 
     TileLoop<ST, Sh, DMA> t;
-    const TileSrc A = {p.A + lo * p.a_pitch + k0 * 2, p.a_pitch, rows * 2, hi - lo};
-    const TileSrc B = {p.D + lo * p.d_pitch + n0 * 2, p.d_pitch, cols * 2, hi - lo};
+    const TileSrc A = {p.A + lo * p.a_pitch + k0 * 2, p.a_pitch,
+                       p.a_padded ? (rows + 7) / 8 * 16 : rows * 2, hi - lo, p.A};
+    const TileSrc B = {p.D + lo * p.d_pitch + n0 * 2, p.d_pitch,
+                       p.d_padded ? (cols + 7) / 8 * 16 : cols * 2, hi - lo, p.D};
     if (!t.run(A, B, smem)) return;
 
     if (p.splits > 1) {
@@ -213,7 +218,60 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedGradParams p) 
     }
 }
 
+// Rows copied to whole 16-byte pieces, zeros behind their end: [groups] blocks of
+// `rows` rows of `cols` 16-bit elements, one behind another in dst.
+struct PackJob {
+    const char *src;
+    char *dst;
+    int64_t group, pitch;    // bytes in src
+    uint32_t rows, all;      // of a group, of all groups
+    int cols, pieces;        // elements and 16-byte pieces of a row
+    uint32_t blocks, per;    // workgroups, and rows of each
+};
+__global__ __launch_bounds__(256) void grouped_pack_kernel(PackJob a, PackJob b) {
+    const bool second = blockIdx.x >= a.blocks;
+    const PackJob &j = second ? b : a;
+    const uint32_t r0 = (blockIdx.x - (second ? a.blocks : 0u)) * j.per;
+    const uint32_t left = j.all - r0, rows = left < j.per ? left : j.per;
+    const float rcp = 1.f / (float)j.pieces;
+    for (int i = threadIdx.x; i < (int)rows * j.pieces; i += 256) {
+        const int r = part_of(i, j.pieces, rcp), at = i - r * j.pieces;
+        const uint32_t row = r0 + r, g = row / j.rows;
+        const char *from = j.src + g * j.group + (int64_t)(row - g * j.rows) * j.pitch + at * 16;
+        *(i32x4 *)(j.dst + (int64_t)row * j.pieces * 16 + at * 16) =
+            load_piece(from, (j.cols - at * 8) * 2, j.src);
+    }
+}
+
 namespace {
+
+// rows that are whole aligned 16-byte pieces, which the LDS-DMA takes
+bool whole_pieces(const void *p, int64_t pitch, int64_t group, int64_t cols, bool padded) {
+    return (((uintptr_t)p | (uintptr_t)pitch | (uintptr_t)group) & 15) == 0 &&
+           (padded || cols % 8 == 0);
+}
+bool a_pieces(const GroupedParams &p) { return whole_pieces(p.A, p.a_pitch, 0, p.K, p.a_padded); }
+bool b_pieces(const GroupedParams &p) {
+    return whole_pieces(p.B, p.b_pitch, p.b_group, p.b_cols ? p.N : p.K, p.b_padded);
+}
+int64_t pieces_of(int64_t cols) { return (cols + 7) / 8; }
+size_t packed_bytes(int64_t rows, int64_t cols) { return (size_t)(rows * pieces_of(cols) * 16); }
+PackJob pack_job(const char *src, char *dst, int64_t groups, int64_t group, int64_t rows,
+                 int64_t pitch, int64_t cols) {
+    PackJob j = {src, dst, group, pitch, (uint32_t)rows, (uint32_t)(rows * groups), (int)cols,
+                 (int)pieces_of(cols), 0, 1};
+    while (j.per < 4096 && (int64_t)j.per * j.pieces < 1024) j.per *= 2;
+    j.blocks = (j.all + j.per - 1) / j.per;
+    return j;
+}
+hipError_t pack(const PackJob &a, const PackJob &b, hipStream_t st) {
+    grouped_pack_kernel<<<dim3(a.blocks + b.blocks), 256, 0, st>>>(a, b);
+    return hipGetLastError();
+}
+// rows and pieces that the pack kernel counts in 32 bits
+bool packable(int64_t rows, int64_t cols) {
+    return rows < (int64_t)1 << 30 && pieces_of(cols) < (int64_t)1 << 22;
+}
 
 template <typename ST, typename Sh, bool DMA>
 hipError_t grouped_go(const GroupedParams &p, hipStream_t st) {
@@ -258,8 +316,7 @@ hipError_t grad_go(const GroupedGradParams &p, hipStream_t st) {
 //     4 x 4 x 4096 x 1024          - /   40 /   39 /   20 /   15
 //     16 x 16 x 1024 x 2048       26 /   13 /   12 /  8.4 /  7.7
 template <typename ST, bool BCOLS> hipError_t grouped_plan(const GroupedParams &p, hipStream_t st) {
-    const bool pieces = (((uintptr_t)p.A | (uintptr_t)p.B | p.a_pitch | p.b_pitch | p.b_group |
-                          p.K * 2 | (BCOLS ? p.N * 2 : 0)) & 15) == 0;
+    const bool pieces = a_pieces(p) && b_pieces(p);
     const int64_t groups = p.G < 1 ? 1 : p.G < p.T ? p.G : p.T, rows = p.T / groups;
     auto tiles = [&](int64_t bm, int64_t bn) {
         return (p.T / bm + (groups + 1) / 2) * ((p.N + bn - 1) / bn);
@@ -280,8 +337,8 @@ template <typename ST, bool BCOLS> hipError_t grouped_plan(const GroupedParams &
 }
 
 template <typename ST> hipError_t grad_plan(const GroupedGradParams &p, hipStream_t st) {
-    const bool pieces = (((uintptr_t)p.A | (uintptr_t)p.D | p.a_pitch | p.d_pitch | p.K * 2 |
-                          p.N * 2) & 15) == 0;
+    const bool pieces = whole_pieces(p.A, p.a_pitch, 0, p.K, p.a_padded) &&
+                        whole_pieces(p.D, p.d_pitch, 0, p.N, p.d_padded);
     const int64_t large = ((p.K + 255) / 256) * ((p.N + 255) / 256) * p.G;
     hipError_t e;
     if (!pieces)
@@ -302,6 +359,66 @@ template <typename ST> hipError_t grad_plan(const GroupedGradParams &p, hipStrea
 hipError_t launch_grouped(const GroupedParams &p, int dtype, hipStream_t st) {
     if (dtype == 2) return p.b_cols ? grouped_plan<_Float16, true>(p, st) : grouped_plan<_Float16, false>(p, st);
     return p.b_cols ? grouped_plan<__bf16, true>(p, st) : grouped_plan<__bf16, false>(p, st);
+}
+
+// Rows that are no whole pieces go through registers, or are copied first
+// where that pays.  Through registers costs about 5e-15 s a product more (twice
+// that for B's rows along N, 2e-14 for dB), a copy 1e-12 s an element and 3e-6 s.
+// Measured (us, T x G x K x N, through registers / with the copy):
+//     8192 x 4 x 1001 x 1003       128 / 52      dB 321 / 72
+//     32768 x 16 x 1023 x 2047     479 / 275     dB 2201 / 366
+//     19944 x 5 x 220 x 103        30 (no copy)  dB 264 / 48
+PackedSizes plan_grouped_pack(const GroupedParams &p) {
+    const bool a = !a_pieces(p), b = p.G > 0 && !b_pieces(p);
+    const int64_t b_rows = p.b_cols ? p.K : p.N, b_len = p.b_cols ? p.N : p.K;
+    if ((!a && !b) || p.K == 0 || !packable(p.T, p.K) || !packable(p.G * b_rows, b_len))
+        return {0, 0};
+    const double products = (double)p.T * p.K * p.N;
+    const double cost = 1e-12 * ((a ? (double)p.T * p.K : 0) + (b ? (double)p.G * p.K * p.N : 0)) + 3e-6;
+    if ((b && p.b_cols ? 1e-14 : 5e-15) * products < cost) return {0, 0};
+    return {a ? packed_bytes(p.T, p.K) : 0, b ? packed_bytes(p.G * b_rows, b_len) : 0};
+}
+PackedSizes plan_grad_pack(const GroupedGradParams &p) {
+    const bool a = !whole_pieces(p.A, p.a_pitch, 0, p.K, p.a_padded);
+    const bool d = !whole_pieces(p.D, p.d_pitch, 0, p.N, p.d_padded);
+    if ((!a && !d) || p.T == 0 || !packable(p.T, p.K) || !packable(p.T, p.N)) return {0, 0};
+    const double cost = 1e-12 * p.T * ((a ? (double)p.K : 0) + (d ? (double)p.N : 0)) + 3e-6;
+    if (2e-14 * p.T * p.K * p.N < cost) return {0, 0};
+    return {a ? packed_bytes(p.T, p.K) : 0, d ? packed_bytes(p.T, p.N) : 0};
+}
+hipError_t pack_grouped(GroupedParams &p, const PackedSizes &n, char *ws, hipStream_t st) {
+    PackJob a = {}, b = {};
+    const int64_t b_rows = p.b_cols ? p.K : p.N, b_len = p.b_cols ? p.N : p.K;
+    if (n.a) {
+        a = pack_job(p.A, ws, 1, 0, p.T, p.a_pitch, p.K);
+        p.A = ws;
+        p.a_pitch = pieces_of(p.K) * 16;
+        p.a_padded = true;
+    }
+    if (n.b) {
+        b = pack_job(p.B, ws + n.a, p.G, p.b_group, b_rows, p.b_pitch, b_len);
+        p.B = ws + n.a;
+        p.b_pitch = pieces_of(b_len) * 16;
+        p.b_group = b_rows * p.b_pitch;
+        p.b_padded = true;
+    }
+    return pack(a, b, st);
+}
+hipError_t pack_grad(GroupedGradParams &p, const PackedSizes &n, char *ws, hipStream_t st) {
+    PackJob a = {}, b = {};
+    if (n.a) {
+        a = pack_job(p.A, ws, 1, 0, p.T, p.a_pitch, p.K);
+        p.A = ws;
+        p.a_pitch = pieces_of(p.K) * 16;
+        p.a_padded = true;
+    }
+    if (n.b) {
+        b = pack_job(p.D, ws + n.a, 1, 0, p.T, p.d_pitch, p.N);
+        p.D = ws + n.a;
+        p.d_pitch = pieces_of(p.N) * 16;
+        p.d_padded = true;
+    }
+    return pack(a, b, st);
 }
 
 int grouped_grad_splits(int64_t T, int64_t K, int64_t N, int64_t G) {

@@ -35,6 +35,7 @@ struct GroupedParams {
     int64_t T, K, N, G;
     int64_t a_pitch, b_group, b_pitch, c_pitch;
     int b_cols, offsets64;
+    bool a_padded, b_padded;   // rows go on with zeros up to a whole 16-byte piece
 };
 // dB[g, k, n] = sum over the rows t of group g of A[t, k] D[t, n]
 struct GroupedGradParams {
@@ -45,9 +46,21 @@ struct GroupedGradParams {
     int64_t T, K, N, G;
     int64_t a_pitch, d_pitch, db_group, db_pitch;
     int offsets64;
+    bool a_padded, d_padded;
     float *part;            // workspace: partial sums of the row ranges (splits > 1)
     int splits;
 };
+// Operands that are copied to whole 16-byte pieces first (packed): the bytes of
+// the copies, 0 for none.  plan_* say which; pack_* point the parameters at the
+// copies in `ws` and enqueue them.
+struct PackedSizes {
+    size_t a, b;
+    size_t total() const { return a + b; }
+};
+PackedSizes plan_grouped_pack(const GroupedParams &p);
+PackedSizes plan_grad_pack(const GroupedGradParams &p);
+hipError_t pack_grouped(GroupedParams &p, const PackedSizes &n, char *ws, hipStream_t st);
+hipError_t pack_grad(GroupedGradParams &p, const PackedSizes &n, char *ws, hipStream_t st);
 // dtype: 2 fp16, 3 bf16
 hipError_t launch_grouped(const GroupedParams &p, int dtype, hipStream_t st);
 hipError_t launch_grouped_grad(const GroupedGradParams &p, int dtype, hipStream_t st);

@@ -43,11 +43,6 @@ int stride_status(std::initializer_list<int64_t> v) {
     return st;
 }
 
-size_t wgrad_bytes(int64_t T, int64_t K, int64_t N, int64_t G) {
-    const int s = ozk::grouped_grad_splits(T, K, N, G);
-    return s > 1 ? (size_t)s * (size_t)(G * K * N) * 4 : 0;
-}
-
 // the largest power of two that keeps values up to `bound` within fp16, with
 // room for a factor of two
 double slice_scale(double bound) {
@@ -212,24 +207,18 @@ OrthLayout orth_most(int64_t batch, int64_t M, int64_t N, int steps) {
 
 extern "C" {
 
-int ozk_grouped_matmul(const void *A, int64_t a_stride, const void *B, const int64_t b_strides[3],
-                       const void *offsets, int offset_bytes, int64_t T, int64_t K, int64_t N,
-                       int64_t G, int dtype, void *C, int64_t c_stride, void *stream) {
-    if (!is_half(dtype) || (offset_bytes != 4 && offset_bytes != 8)) return OZK_ERR_DTYPE;
+static int grouped_params(ozk::GroupedParams &p, const void *A, int64_t a_stride, const void *B,
+                          const int64_t b_strides[3], int64_t T, int64_t K, int64_t N, int64_t G) {
     if (!b_strides) return OZK_ERR_NULL;
     if (!sizes_ok({T, K, N, G})) return OZK_ERR_SHAPE;
     if (b_strides[2] != 1 && b_strides[1] != 1) return OZK_ERR_SHAPE;
-    if (T == 0 || N == 0) return OZK_OK;
-    if (!C || !offsets || (K > 0 && (!A || (G > 0 && !B)))) return OZK_ERR_NULL;
     const bool cols = b_strides[2] == 1;
     const int64_t b_pitch = cols ? b_strides[1] : b_strides[2];
-    if (c_stride < 0 || b_strides[0] < 0) return OZK_ERR_SHAPE;
+    if (b_strides[0] < 0) return OZK_ERR_SHAPE;
     if (int st = stride_status({a_stride, b_pitch})) return st;
-    ozk::GroupedParams p;
+    p = {};
     p.A = (const char *)A;
     p.B = (const char *)B;
-    p.C = (char *)C;
-    p.offsets = offsets;
     p.T = T;
     p.K = K;
     p.N = N;
@@ -237,17 +226,72 @@ int ozk_grouped_matmul(const void *A, int64_t a_stride, const void *B, const int
     p.a_pitch = a_stride * 2;
     p.b_group = b_strides[0] * 2;
     p.b_pitch = b_pitch * 2;
-    p.c_pitch = c_stride * 2;
     p.b_cols = cols;
-    p.offsets64 = offset_bytes == 8;
-    return launched(ozk::launch_grouped(p, dtype, (hipStream_t)stream));
+    return OZK_OK;
 }
 
-int ozk_grouped_matmul_wgrad_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t G,
-                                             size_t *bytes_out) {
+int ozk_grouped_matmul_workspace_bytes(const void *A, int64_t a_stride, const void *B,
+                                       const int64_t b_strides[3], int64_t T, int64_t K, int64_t N,
+                                       int64_t G, size_t *bytes_out) {
     if (!bytes_out) return OZK_ERR_NULL;
+    ozk::GroupedParams p;
+    if (int st = grouped_params(p, A, a_stride, B, b_strides, T, K, N, G)) return st;
+    *bytes_out = ozk::plan_grouped_pack(p).total();
+    return OZK_OK;
+}
+
+int ozk_grouped_matmul(const void *A, int64_t a_stride, const void *B, const int64_t b_strides[3],
+                       const void *offsets, int offset_bytes, int64_t T, int64_t K, int64_t N,
+                       int64_t G, int dtype, void *C, int64_t c_stride, void *workspace,
+                       size_t workspace_bytes, void *stream) {
+    if (!is_half(dtype) || (offset_bytes != 4 && offset_bytes != 8)) return OZK_ERR_DTYPE;
+    ozk::GroupedParams p;
+    if (int st = grouped_params(p, A, a_stride, B, b_strides, T, K, N, G)) return st;
+    if (c_stride < 0) return OZK_ERR_SHAPE;
+    if (T == 0 || N == 0) return OZK_OK;
+    if (!C || !offsets || (K > 0 && (!A || (G > 0 && !B)))) return OZK_ERR_NULL;
+    p.C = (char *)C;
+    p.offsets = offsets;
+    p.c_pitch = c_stride * 2;
+    p.offsets64 = offset_bytes == 8;
+    const hipStream_t st = (hipStream_t)stream;
+    const ozk::PackedSizes n = ozk::plan_grouped_pack(p);
+    if (n.total() && workspace && workspace_bytes >= n.total()) {
+        if ((uintptr_t)workspace & 15) return OZK_ERR_WORKSPACE;
+        if (hipError_t e = ozk::pack_grouped(p, n, (char *)workspace, st); e != hipSuccess)
+            return launched(e);
+    }
+    return launched(ozk::launch_grouped(p, dtype, st));
+}
+
+static int grad_params(ozk::GroupedGradParams &p, const void *A, int64_t a_stride, const void *D,
+                       int64_t d_stride, int64_t T, int64_t K, int64_t N, int64_t G) {
     if (!sizes_ok({T, K, N, G})) return OZK_ERR_SHAPE;
-    *bytes_out = wgrad_bytes(T, K, N, G);
+    if (int st = stride_status({a_stride, d_stride})) return st;
+    p = {};
+    p.A = (const char *)A;
+    p.D = (const char *)D;
+    p.T = T;
+    p.K = K;
+    p.N = N;
+    p.G = G;
+    p.a_pitch = a_stride * 2;
+    p.d_pitch = d_stride * 2;
+    p.splits = ozk::grouped_grad_splits(T, K, N, G);
+    return OZK_OK;
+}
+// the partial sums, in whole 16 bytes, then the copies
+static size_t part_bytes(const ozk::GroupedGradParams &p) {
+    return p.splits > 1 ? (size_t)round_up((int64_t)p.splits * p.G * p.K * p.N * 4, 16) : 0;
+}
+
+int ozk_grouped_matmul_wgrad_workspace_bytes(const void *A, int64_t a_stride, const void *D,
+                                             int64_t d_stride, int64_t T, int64_t K, int64_t N,
+                                             int64_t G, size_t *bytes_out) {
+    if (!bytes_out) return OZK_ERR_NULL;
+    ozk::GroupedGradParams p;
+    if (int st = grad_params(p, A, a_stride, D, d_stride, T, K, N, G)) return st;
+    *bytes_out = part_bytes(p) + ozk::plan_grad_pack(p).total();
     return OZK_OK;
 }
 
@@ -258,31 +302,26 @@ int ozk_grouped_matmul_wgrad(const void *A, int64_t a_stride, const void *D, int
                              size_t workspace_bytes, void *stream) {
     if (!is_half(dtype) || (offset_bytes != 4 && offset_bytes != 8)) return OZK_ERR_DTYPE;
     if (!db_strides) return OZK_ERR_NULL;
-    if (!sizes_ok({T, K, N, G})) return OZK_ERR_SHAPE;
+    ozk::GroupedGradParams p;
+    if (int st = grad_params(p, A, a_stride, D, d_stride, T, K, N, G)) return st;
+    if (db_strides[0] < 0 || db_strides[1] < 0) return OZK_ERR_SHAPE;
     if (K == 0 || N == 0 || G == 0) return OZK_OK;
     if (!dB || !offsets || (T > 0 && (!A || !D))) return OZK_ERR_NULL;
-    if (db_strides[0] < 0 || db_strides[1] < 0) return OZK_ERR_SHAPE;
-    if (int st = stride_status({a_stride, d_stride})) return st;
-    const size_t need = wgrad_bytes(T, K, N, G);
-    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
-        return OZK_ERR_WORKSPACE;
-    ozk::GroupedGradParams p;
-    p.A = (const char *)A;
-    p.D = (const char *)D;
+    const size_t part = part_bytes(p);
+    if (part && (!workspace || workspace_bytes < part)) return OZK_ERR_WORKSPACE;
+    if (workspace && ((uintptr_t)workspace & 15)) return OZK_ERR_WORKSPACE;
     p.dB = (char *)dB;
     p.offsets = offsets;
-    p.T = T;
-    p.K = K;
-    p.N = N;
-    p.G = G;
-    p.a_pitch = a_stride * 2;
-    p.d_pitch = d_stride * 2;
     p.db_group = db_strides[0] * 2;
     p.db_pitch = db_strides[1] * 2;
     p.offsets64 = offset_bytes == 8;
     p.part = (float *)workspace;
-    p.splits = ozk::grouped_grad_splits(T, K, N, G);
-    return launched(ozk::launch_grouped_grad(p, dtype, (hipStream_t)stream));
+    const hipStream_t st = (hipStream_t)stream;
+    const ozk::PackedSizes n = ozk::plan_grad_pack(p);
+    if (n.total() && workspace && workspace_bytes >= part + n.total())
+        if (hipError_t e = ozk::pack_grad(p, n, (char *)workspace + part, st); e != hipSuccess)
+            return launched(e);
+    return launched(ozk::launch_grouped_grad(p, dtype, st));
 }
 
 static int w4_checks(int64_t N, int64_t K, int group, const void *packed, int64_t packed_stride,

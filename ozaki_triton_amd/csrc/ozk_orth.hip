@@ -166,9 +166,9 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
 
     TileLoop<_Float16, Sh, true> t;
     const char *L = p.L + (int64_t)b * p.l_batch, *R = p.R + (int64_t)b * p.r_batch;
-    const TileSrc A = {L + m0 * lp, lp, rows, lp};
-    const TileSrc B = Sh::BCOLS ? TileSrc{R + n0 * 4, rp, (int)(rp - n0 * 4 < BN * 4 ? rp - n0 * 4 : BN * 4), p.m}
-                                : TileSrc{R + n0 * rp, rp, cols, rp};
+    const TileSrc A = {L + m0 * lp, lp, rows, lp, L};
+    const TileSrc B = Sh::BCOLS ? TileSrc{R + n0 * 4, rp, (int)(rp - n0 * 4 < BN * 4 ? rp - n0 * 4 : BN * 4), p.m, R}
+                                : TileSrc{R + n0 * rp, rp, cols, rp, R};
     if (!t.run(A, B, smem)) return;
 
     const int64_t dp = kSym ? slice_pitch(p.m) : slice_pitch(p.n);   // of D's and Y's slices

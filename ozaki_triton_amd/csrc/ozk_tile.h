@@ -54,12 +54,17 @@ OZK_DEV uint16_t to_bits16(float v, __bf16) { return __builtin_bit_cast(uint16_t
 OZK_DEV float from_bits16(uint16_t v, _Float16) { return (float)__builtin_bit_cast(_Float16, v); }
 OZK_DEV float from_bits16(uint16_t v, __bf16) { return bf16_bits_to_f32(v); }
 
+// i / n for 0 <= i < 2^22, n a small part of it: (i + 1/2) / n is at least 1 / 2n
+// away from a whole number, the two roundings of rcp * (i + 1/2) less
+OZK_DEV int part_of(int i, int n, float rcp) { return (int)(((float)i + 0.5f) * rcp); }
+
 // An operand's part that a tile reads.
 struct TileSrc {
     const char *base;   // its first row at k = 0 ("cols": the first column, at row k = 0)
     int64_t pitch;      // bytes between rows
     int rows;           // "rows": rows there are; "cols": bytes of a row there are
     int64_t klen;       // "rows": bytes of K; "cols": rows
+    const char *first;  // the whole operand's first byte
 };
 
 constexpr uint32_t kTileOOB = 0x80000000u;   // past every buffer: the DMA writes zeros
@@ -153,19 +158,39 @@ OZK_DEV void dma_piece(const char *base, uint32_t off, uint32_t to) {
 #pragma clang diagnostic pop
 }
 
-// 16 bytes at an address of any alignment, of which the first `n` exist
-OZK_DEV i32x4 load_piece(const char *p, int n) {
+// 16 bytes built element by element, the last first: a rolled loop, since code
+// that is fetched and skipped costs short kernels more
+OZK_DEV void push16(i32x4 &v, uint32_t e) {
+    v.w = (int)__builtin_amdgcn_alignbit((uint32_t)v.w, (uint32_t)v.z, 16);
+    v.z = (int)__builtin_amdgcn_alignbit((uint32_t)v.z, (uint32_t)v.y, 16);
+    v.y = (int)__builtin_amdgcn_alignbit((uint32_t)v.y, (uint32_t)v.x, 16);
+    v.x = (int)(((uint32_t)v.x << 16) | e);
+}
+
+// 16 bytes from an address of any alignment on, of which the first `n` (even)
+// exist; `first`: the operand's first byte.  A piece with an end inside is read
+// up to that end, from what lies before it, and shifted down: its elements one
+// by one cost the edge tiles more than everything else (19944 x 220 x 103 in 5
+// groups, dB: 264 us).
+OZK_DEV i32x4 load_piece(const char *p, int n, const char *first) {
     i32x4 v = {0, 0, 0, 0};
     if (n >= 16) {
         __builtin_memcpy(&v, p, 16);
-    } else {
-        uint16_t e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            e[i] = 0;
-            if (2 * i < n) __builtin_memcpy(&e[i], p + 2 * i, 2);
+    } else if (n > 0) {
+        const int s = 16 - n;
+        if (p - first >= s) {
+            __builtin_memcpy(&v, p - s, 16);
+            if (s & 8) v = i32x4{v.z, v.w, 0, 0};
+            if (s & 4) v = i32x4{v.y, v.z, v.w, 0};
+            const uint32_t h = (uint32_t)(s & 2) * 8;
+            v = i32x4{(int)__builtin_amdgcn_alignbit((uint32_t)v.y, (uint32_t)v.x, h),
+                      (int)__builtin_amdgcn_alignbit((uint32_t)v.z, (uint32_t)v.y, h),
+                      (int)__builtin_amdgcn_alignbit((uint32_t)v.w, (uint32_t)v.z, h),
+                      (int)((uint32_t)v.w >> h)};
+        } else {
+#pragma unroll 1
+            for (int i = n / 2 - 1; i >= 0; --i) push16(v, ((const uint16_t *)p)[i]);
         }
-        __builtin_memcpy(&v, e, 16);
     }
     return v;
 }
@@ -198,7 +223,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
 
         // the operands as this wave stages them, `base` that of the stage it is at
         struct Feed {
-            const char *base;
+            const char *base, *first;
             int64_t step;
             int whole, rest;   // whole stages, and what the one behind them has of K
             // what the group's stage kb has of K, as WindowAt counts it
@@ -207,9 +232,9 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 return at < whole ? 128 : at == whole ? rest : 0;
             }
         };
-        Feed fa = {A.base, Sh::ACOLS ? Sh::KS * A.pitch : 128, (int)(A.klen / ua),
+        Feed fa = {A.base, A.first, Sh::ACOLS ? Sh::KS * A.pitch : 128, (int)(A.klen / ua),
                    (int)(A.klen % ua)};
-        Feed fb = {B.base, Sh::BCOLS ? Sh::KS * B.pitch : 128, (int)(B.klen / ub),
+        Feed fb = {B.base, B.first, Sh::BCOLS ? Sh::KS * B.pitch : 128, (int)(B.klen / ub),
                    (int)(B.klen % ub)};
         if constexpr (Sh::KW > 1) {
             fa.base += kw * fa.step;
@@ -273,7 +298,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 const int left = f.left(kb, kw) - win[q].k;
                 int n = left > 0 ? win[q].n : 0;
                 if (!cols && left < n) n = left;
-                held[q] = load_piece(f.base + (n > 0 ? win[q].off : 0u), n);
+                held[q] = load_piece(f.base + (n > 0 ? win[q].off : 0u), n, f.first);
             }
         };
         auto put = [&](int kb) {

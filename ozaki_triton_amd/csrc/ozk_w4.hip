@@ -61,14 +61,6 @@ OZK_DEV void transpose_words(uint32_t (&r)[4]) {
     swap16(r[2], r[3]);
 }
 
-// 16 bytes built element by element, the last first: a rolled loop, since code
-// that is fetched and skipped costs these short kernels more than it would
-OZK_DEV void push16(i32x4 &v, uint32_t e) {
-    v.w = (int)__builtin_amdgcn_alignbit((uint32_t)v.w, (uint32_t)v.z, 16);
-    v.z = (int)__builtin_amdgcn_alignbit((uint32_t)v.z, (uint32_t)v.y, 16);
-    v.y = (int)__builtin_amdgcn_alignbit((uint32_t)v.y, (uint32_t)v.x, 16);
-    v.x = (int)(((uint32_t)v.x << 16) | e);
-}
 OZK_DEV void push32(i32x4 &lo, i32x4 &hi, int e) {
     hi = i32x4{lo.w, hi.x, hi.y, hi.z};
     lo = i32x4{e, lo.x, lo.y, lo.z};
@@ -111,10 +103,6 @@ struct SPiece {
         return float2{f, p.zeros ? 16.f + (float)q : 24.f};
     }
 };
-
-// i / n for 0 <= i < 2^22, n a small part of it: (i + 1/2) / n is at least 1 / 2n
-// away from a whole number, the two roundings of rcp * (i + 1/2) less
-OZK_DEV int part_of(int i, int n, float rcp) { return (int)(((float)i + 0.5f) * rcp); }
 
 // the sum over 4, 8 or 16 consecutive lanes, in each of them
 template <int CTRL> OZK_DEV float dpp_add(float v) {

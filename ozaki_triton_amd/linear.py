@@ -62,9 +62,16 @@ def _call(name: str, dev: torch.device, *args) -> None:
 
 
 @functools.lru_cache(maxsize=1024)
+def _i64(*vals):
+    return _lib.i64arr(vals)
+
+
+@functools.lru_cache(maxsize=1024)
 def _bytes(name: str, *args) -> int:
-    """Workspace query `name`: it depends on nothing but its arguments."""
+    """Workspace query `name`: it depends on nothing but its arguments (of a pointer
+    its alignment, which is passed in its place; strides come as a tuple)."""
     n = ctypes.c_size_t(0)
+    args = [_i64(*a) if isinstance(a, tuple) else a for a in args]
     _lib.check(name, getattr(_lib.load(), name)(*args, ctypes.byref(n)))
     return n.value
 
@@ -76,11 +83,6 @@ def _workspace(nbytes: int, dev: torch.device):
         return None, None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     return ws, ws.data_ptr()
-
-
-@functools.lru_cache(maxsize=1024)
-def _i64(*vals):
-    return _lib.i64arr(vals)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -123,9 +125,12 @@ def _grouped_forward(A, B, offsets):
         offsets = offsets.contiguous()
     dtype, dev = A.dtype, A.device
     C = torch.empty((T, N), dtype=dtype, device=dev)
-    _call("ozk_grouped_matmul", dev, A.data_ptr(), A.stride(0), B.data_ptr(), _i64(*sb),
-          offsets.data_ptr(), offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype],
-          C.data_ptr(), N)
+    ap, bp, sa = A.data_ptr(), B.data_ptr(), A.stride(0)
+    n = _bytes("ozk_grouped_matmul_workspace_bytes", ap & 15, sa, bp & 15, sb, T, K, N, G)
+    ws, wsp = _workspace(n, dev)
+    _call("ozk_grouped_matmul", dev, ap, sa, bp, _i64(*sb), offsets.data_ptr(), offsets.element_size(), T,
+          K, N, G, _TORCH_TO_OZK[dtype], C.data_ptr(), N, wsp, n)
+    del ws
     return C
 
 
@@ -137,10 +142,10 @@ def _grouped_wgrad(A, D, offsets, G):
         offsets = offsets.contiguous()
     dtype, dev = A.dtype, A.device
     dB = torch.empty((G, K, N), dtype=dtype, device=dev)
-    n = _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", T, K, N, G)
+    ap, dp, sa, sd = A.data_ptr(), D.data_ptr(), A.stride(0), D.stride(0)
+    n = _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", ap & 15, sa, dp & 15, sd, T, K, N, G)
     ws, wsp = _workspace(n, dev)
-    _call("ozk_grouped_matmul_wgrad", dev, A.data_ptr(), A.stride(0), D.data_ptr(), D.stride(0),
-          offsets.data_ptr(), offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype],
+    _call("ozk_grouped_matmul_wgrad", dev, ap, sa, dp, sd, offsets.data_ptr(), offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype],
           dB.data_ptr(), _i64(K * N, N), wsp, n)
     del ws
     return dB

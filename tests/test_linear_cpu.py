@@ -91,7 +91,7 @@ def test_c_calls_check_before_they_launch():
     L = _lib.load()
     g = lambda **k: L.ozk_grouped_matmul(*{**dict(  # noqa: E731
         A=_p(), a=8, B=_p(), bs=_b(24, 3, 1), off=_p(), ob=4, T=4, K=8, N=3, G=2,
-        d=_lib.OZK_BF16, C=_p(), c=3, st=None), **k}.values())
+        d=_lib.OZK_BF16, C=_p(), c=3, ws=None, n=0, st=None), **k}.values())
     assert g(d=_lib.OZK_F32) == _lib.OZK_ERR_DTYPE
     assert g(ob=2) == _lib.OZK_ERR_DTYPE
     assert g(bs=None) == g(C=None) == g(off=None) == g(A=None) == g(B=None) == _lib.OZK_ERR_NULL
@@ -135,10 +135,18 @@ def _bytes(fn, *args):
 
 def test_workspace_sizes():
     # many tiles, or few rows: no partial sums; one tile under many rows: some
-    assert _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", 16384, 2048, 1024, 32) == 0
-    assert _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", 64, 64, 64, 1) == 0
-    assert _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", 1 << 15, 64, 64, 1) % (64 * 64 * 4) == 0
-    assert _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", 1 << 15, 64, 64, 1) > 0
+    assert _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", 0, 2048, 0, 1024, 16384, 2048, 1024, 32) == 0
+    assert _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", 0, 64, 0, 64, 64, 64, 64, 1) == 0
+    assert _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", 0, 64, 0, 64, 1 << 15, 64, 64, 1) % (64 * 64 * 4) == 0
+    assert _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", 0, 64, 0, 64, 1 << 15, 64, 64, 1) > 0
+    # rows that are no whole 16-byte pieces, by size, distance or address: copies
+    # where there is enough to multiply
+    w = lambda a, sa, T, K, N: _bytes("ozk_grouped_matmul_workspace_bytes", a, sa, 0,  # noqa: E731
+                                      _b(K * N, N, 1), T, K, N, 4)
+    assert w(0, 1024, 8192, 1024, 1024) == w(0, 1001, 64, 1001, 1024) == 0
+    assert w(0, 1001, 8192, 1001, 1024) == w(2, 1008, 8192, 1001, 1024) == 8192 * 1008 * 2
+    assert w(2, 1024, 8192, 1024, 1024) == w(0, 1025, 8192, 1024, 1024) == 8192 * 1024 * 2
+    assert w(0, 1001, 8192, 1001, 1003) == 8192 * 1008 * 2 + 4 * 1001 * 1008 * 2
     assert _bytes("ozk_matmul_w4_workspace_bytes", _lib.OZK_BF16, 1, 0, 64, 32) == 0
     assert _bytes("ozk_matmul_w4_workspace_bytes", _lib.OZK_BF16, 1, 64, 1 << 14, 128) % (64 * 4) == 0
     # X twice and two square matrices, 4 bytes an element, columns up to whole 32
