@@ -362,28 +362,38 @@ hipError_t launch_grouped(const GroupedParams &p, int dtype, hipStream_t st) {
 }
 
 // Rows that are no whole pieces go through registers, or are copied first
-// where that pays.  Through registers costs about 5e-15 s a product more (twice
-// that for B's rows along N, 2e-14 for dB), a copy 1e-12 s an element and 3e-6 s.
-// Measured (us, T x G x K x N, through registers / with the copy):
-//     8192 x 4 x 1001 x 1003       128 / 52      dB 321 / 72
-//     32768 x 16 x 1023 x 2047     479 / 275     dB 2201 / 366
-//     19944 x 5 x 220 x 103        30 (no copy)  dB 264 / 48
+// where that pays: a copy costs 1e-12 s an element and 5e-6 s, the way through
+// registers so much more a stage of a tile, 1.1e-6 s (2.5e-6 where B's rows run
+// along N; a quarter of it in the small tiles of few rows; 3e-6 for dB), and again
+// for every so many tiles.  Measured (us, T x G x K x N, B along N, with the copy /
+// through registers):
+//     8192 x 4 x 1001 x 1003       53 /  86     dB  70 /  224
+//     32768 x 16 x 1023 x 2047    256 / 335     dB 440 / 1131
+//     2000 x 2 x 4097 x 257        41 / 231     dB  46 /   49
+//     948 x 13 x 1344 x 2259       52 /  92     dB  62 /   64
+//     4030 x 28 x 1920 x 2121     190 / 168     dB 169 /  177
+//     1000 x 64 x 1025 x 1025      76 /  35     dB 101 /   90
+//     16 x 16 x 1025 x 2049        34 /  20     dB  56 /   46
 PackedSizes plan_grouped_pack(const GroupedParams &p) {
     const bool a = !a_pieces(p), b = p.G > 0 && !b_pieces(p);
     const int64_t b_rows = p.b_cols ? p.K : p.N, b_len = p.b_cols ? p.N : p.K;
-    if ((!a && !b) || p.K == 0 || !packable(p.T, p.K) || !packable(p.G * b_rows, b_len))
+    if ((!a && !b) || p.T == 0 || p.K == 0 || p.N == 0 || !packable(p.T, p.K) || !packable(p.G * b_rows, b_len))
         return {0, 0};
-    const double products = (double)p.T * p.K * p.N;
-    const double cost = 1e-12 * ((a ? (double)p.T * p.K : 0) + (b ? (double)p.G * p.K * p.N : 0)) + 3e-6;
-    if ((b && p.b_cols ? 1e-14 : 5e-15) * products < cost) return {0, 0};
+    const double cost = 1e-12 * ((a ? (double)p.T * p.K : 0) + (b ? (double)p.G * p.K * p.N : 0)) + 5e-6;
+    const int64_t groups = p.G < 1 ? 1 : p.G < p.T ? p.G : p.T;
+    const double tiles = ((double)p.T / 128 + groups / 2) * ((double)p.N / 128 + 1) / 1536;
+    const double stage = (b && p.b_cols ? 2.5e-6 : 1.1e-6) * (p.T / groups >= 48 ? 1 : 0.25) *
+                         (tiles > 1 ? tiles : 1);
+    if (stage * ((p.K + 63) / 64) < cost) return {0, 0};
     return {a ? packed_bytes(p.T, p.K) : 0, b ? packed_bytes(p.G * b_rows, b_len) : 0};
 }
 PackedSizes plan_grad_pack(const GroupedGradParams &p) {
     const bool a = !whole_pieces(p.A, p.a_pitch, 0, p.K, p.a_padded);
     const bool d = !whole_pieces(p.D, p.d_pitch, 0, p.N, p.d_padded);
-    if ((!a && !d) || p.T == 0 || !packable(p.T, p.K) || !packable(p.T, p.N)) return {0, 0};
-    const double cost = 1e-12 * p.T * ((a ? (double)p.K : 0) + (d ? (double)p.N : 0)) + 3e-6;
-    if (2e-14 * p.T * p.K * p.N < cost) return {0, 0};
+    if ((!a && !d) || p.T == 0 || p.K == 0 || p.N == 0 || p.G == 0 || !packable(p.T, p.K) || !packable(p.T, p.N)) return {0, 0};
+    const double cost = 1e-12 * p.T * ((a ? (double)p.K : 0) + (d ? (double)p.N : 0)) + 5e-6;
+    const double tiles = ((double)p.K / 128 + 1) * ((double)p.N / 128 + 1) * p.G / 1024;
+    if (3e-6 * (tiles > 1 ? tiles : 1) * p.T / (64.0 * p.G * p.splits) < cost) return {0, 0};
     return {a ? packed_bytes(p.T, p.K) : 0, d ? packed_bytes(p.T, p.N) : 0};
 }
 hipError_t pack_grouped(GroupedParams &p, const PackedSizes &n, char *ws, hipStream_t st) {

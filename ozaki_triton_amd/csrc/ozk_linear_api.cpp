@@ -22,8 +22,9 @@ int launched(hipError_t e) {
                                                : OZK_ERR_LAUNCH;
 }
 
-// the tile kernels step through up to 256 rows with 32-bit offsets
-constexpr int64_t kMaxStride = (int64_t)1 << 22;
+// the tile kernels step through up to 256 rows with 31-bit byte offsets: of two
+// bytes an element, and of four in the slices of an orthogonalisation
+constexpr int64_t kMaxStride = (int64_t)1 << 22, kMaxOrth = (int64_t)1 << 20;
 // no size negative, the product of all within 60 bits (so are byte offsets)
 bool sizes_ok(std::initializer_list<int64_t> v) {
     double all = 1.0;
@@ -391,6 +392,7 @@ int ozk_matmul_w4_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K, in
     if (!is_float(dtype)) return OZK_ERR_DTYPE;
     if (!sizes_ok({M, N, K}) || (group != 32 && group != 64 && group != 128)) return OZK_ERR_SHAPE;
     *bytes_out = 0;
+    if (K >= (int64_t)1 << 30) return OZK_ERR_TOO_LARGE;
     if (M == 0 || N == 0) return OZK_OK;
     ozk::W4Params p = {};
     p.M = M;
@@ -409,6 +411,7 @@ int ozk_matmul_w4(const void *x, int dtype, int64_t x_stride, const void *packed
                   void *stream) {
     if (!is_float(dtype) || (scale_dtype != dtype && scale_dtype != OZK_F32)) return OZK_ERR_DTYPE;
     if (!sizes_ok({M, N, K}) || K == 0) return OZK_ERR_SHAPE;
+    if (K >= (int64_t)1 << 30) return OZK_ERR_TOO_LARGE;
     if (int st = w4_checks(N, K, group, packed, packed_stride, scales, s_stride, zeros, z_stride))
         return st;
     if (M == 0 || N == 0) return OZK_OK;
@@ -444,7 +447,7 @@ int ozk_orthogonalize_workspace_bytes(int64_t batch, int64_t M, int64_t N, int s
                                       size_t *bytes_out) {
     if (!bytes_out) return OZK_ERR_NULL;
     if (!sizes_ok({batch, M, N}) || steps < 1) return OZK_ERR_SHAPE;
-    if (M >= kMaxStride || N >= kMaxStride || batch > 65535) return OZK_ERR_TOO_LARGE;
+    if (M >= kMaxOrth || N >= kMaxOrth || batch > 65535) return OZK_ERR_TOO_LARGE;
     *bytes_out = batch && M && N ? orth_most(batch, M, N, steps).total : 0;
     return OZK_OK;
 }
@@ -455,7 +458,7 @@ int ozk_orthogonalize(const void *G, int dtype, int64_t batch, int64_t M, int64_
                       size_t workspace_bytes, void *stream) {
     if (!is_float(dtype)) return OZK_ERR_DTYPE;
     if (!sizes_ok({batch, M, N}) || steps < 1 || steps > 64) return OZK_ERR_SHAPE;
-    if (M >= kMaxStride || N >= kMaxStride || batch > 65535) return OZK_ERR_TOO_LARGE;
+    if (M >= kMaxOrth || N >= kMaxOrth || batch > 65535) return OZK_ERR_TOO_LARGE;
     if (!coefficients || !g_strides || !o_strides) return OZK_ERR_NULL;
     if (!batch || !M || !N) return OZK_OK;
     if (!G || !out) return OZK_ERR_NULL;
