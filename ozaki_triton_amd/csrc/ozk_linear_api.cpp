@@ -106,10 +106,11 @@ struct OrthBounds {
 // 2048 x 8192: 411 us for a step by itself, 200 for one of these).  What it costs
 // is accuracy: an error of 2^-22 in A (its slices) is amplified by P^2 a step
 // and by P's slope at the end, and j is as large as keeps that worst case within
-// half a unit of the result's type (fp32: 2^-16, what the steps in fp32 are off
-// in theirs).  Seen on random and on ill-conditioned (1e4) matrices, with the
-// coefficients 3.4445, -4.775, 2.0315: j = 2 no different from 1, j = 3 2e-5, j =
-// 4 7e-5, against bounds of 1.4e-5, 1.6e-4 and 1.9e-3.
+// half a unit of a 16-bit result's rounding; for fp32 results every step runs by
+// itself (4 steps of 1.5, -0.5, 0 at 65 x 400 were 4.3e-7 off together, 8e-8 in
+// plain fp32).  Seen on random and on ill-conditioned (1e4) matrices, with the
+// coefficients 3.4445, -4.775, 2.0315: j = 2 1.8e-6, as j = 1, j = 3 2e-5, j = 4
+// 7e-5, against bounds of 1.4e-5, 1.6e-4 and 1.9e-3.
 void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int steps, int dtype) {
     double bound[65];
     bound[0] = 1.0;
@@ -119,8 +120,8 @@ void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int 
         return OrthBounds(co[3 * i], co[3 * i + 1], co[3 * i + 2], bound[i] * bound[i]);
     };
     int j = 1;
-    if (n >= 3 * m) {
-        const double limit = dtype == OZK_BF16 ? 0x1p-9 : dtype == OZK_F16 ? 0x1p-12 : 0x1p-16;
+    if (n >= 3 * m && dtype != OZK_F32) {
+        const double limit = dtype == OZK_BF16 ? 0x1p-9 : 0x1p-12;
         double gain = 0x1p-22;
         while (j < steps) {
             gain *= at(steps - 1 - j).p * at(steps - 1 - j).p;

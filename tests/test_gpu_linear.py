@@ -87,6 +87,41 @@ def test_grouped(dtype, bt, counts, K, N, spare):
     _check_grouped(A, B.mT if bt else B.mT.contiguous(), D, _offsets(counts))
 
 
+@pytest.mark.parametrize("counts, K, N", [
+    ([1500, 900], 1001, 1003), ([300, 200, 100], 513, 515), ([900], 4097, 257),
+    ([64], 2049, 2047), ([5000, 3000], 220, 103), ([2500], 1344, 1001)])
+def test_grouped_copied_operands(counts, K, N):
+    """Sizes whose rows are copied to whole 16-byte pieces first, at aligned and
+    misaligned addresses, by both layouts of B; without the copies' workspace the
+    same products go through registers."""
+    offsets = _offsets(counts)
+    A, D, B = _randn(1, sum(counts), K), _randn(3, sum(counts), N), _randn(2, len(counts), K, N)
+    _check_grouped(A, B, D, offsets)
+    _check_grouped(A, B.mT.contiguous().mT, D, offsets)
+    buffer = torch.empty(A.numel() + 3, dtype=BF, device="cuda")
+    A2 = buffer[3:].view(A.shape).copy_(A)
+    assert A2.data_ptr() % 16 == 6
+    assert torch.equal(ozk.grouped_matmul(A2, B, offsets), ozk.grouped_matmul(A, B, offsets))
+    lib, C = ozk.ozaki._lib, torch.empty(sum(counts), N, dtype=BF, device="cuda")
+    lib.check("ozk_grouped_matmul", lib.load().ozk_grouped_matmul(
+        A.data_ptr(), K, B.data_ptr(), lib.i64arr((K * N, N, 1)), offsets.data_ptr(), 4, A.shape[0],
+        K, N, len(counts), lib.OZK_BF16, C.data_ptr(), N, None, 0,
+        torch.cuda.current_stream().cuda_stream))
+    _close(C, *_grouped(A, B, offsets.tolist()), K, BF)
+
+
+@pytest.mark.parametrize("counts, K, N", [
+    ([600] * 4, 256, 8192),       # the largest tile
+    ([40] * 8, 2048, 2048),       # 128 x 128, four stages
+    ([700, 500], 4096, 256),      # two groups of waves on a tile's stages
+    ([3, 0, 2], 4096, 1024), ([70, 90], 520, 520)])
+def test_grouped_tiles(counts, K, N):
+    offsets, rows = _offsets(counts), sum(counts)
+    for bt in (False, True):
+        B = _randn(2, len(counts), N, K)
+        _check_grouped(_randn(1, rows, K), B.mT if bt else B.mT.contiguous(), _randn(3, rows, N), offsets)
+
+
 def test_grouped_offsets_inside_the_rows():
     """int64 offsets that start after row 0: the rows before and after get zeros."""
     A, B, D = _randn(1, 90, 64), _randn(2, 3, 64, 72), _randn(3, 90, 72)
@@ -461,6 +496,33 @@ def test_orthogonalize(dtype, shape):
 ])
 def test_orthogonalize_steps(steps, coefficients):
     _check_orth(_randn(2, 96, 160, dtype=F32), steps, coefficients)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("shape, steps, coefficients", [
+    ((64, 200), 5, COEFFICIENTS), ((300, 64), 6, COEFFICIENTS), ((3, 40, 130), 2, COEFFICIENTS),
+    ((100, 1000), 8, (1.875, -1.25, 0.375)), ((65, 400), 4, (1.5, -0.5, 0.0)),
+    ((33, 100), 3, [(3.4445, -4.7750, 2.0315), (2.5, -3.0, 1.5), (1.875, -1.25, 0.375)])])
+def test_orthogonalize_long(dtype, shape, steps, coefficients):
+    """Matrices three times longer than high and more: the last steps run on the
+    square matrices alone, as many as the dtype's precision bears."""
+    _check_orth(_randn(7, *shape, dtype=dtype), steps, coefficients)
+
+
+def test_orthogonalize_long_of_any_condition():
+    """Singular values over four decades, and a matrix of rank 3."""
+    g = _gen(8)
+    u, v = (torch.linalg.qr(torch.randn(n, 48, generator=g, device="cuda"))[0] for n in (48, 200))
+    G = u @ torch.diag(torch.logspace(0, -4, 48, device="cuda")) @ v.T
+    low = _randn(5, 40, 3, dtype=F32) @ _randn(6, 3, 160, dtype=F32)
+    for dtype in (BF, F16):
+        # the values that bfloat16 has of G are other ones: compare on those
+        for m in (G, low):
+            x = m.to(dtype)
+            got, want = ozk.orthogonalize(x).double(), _steps(x.cpu().double(), [COEFFICIENTS] * 5, 1e-7, torch.float64)
+            off = float((got.cpu() - want).norm() / want.norm())
+            # half a unit for the rounding, half a unit for the steps
+            assert off <= 2 * ROUND[dtype], (dtype, off)
 
 
 @pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e25])
