@@ -20,9 +20,10 @@ import functools
 import torch
 
 from . import _lib
-from .ozaki import _TORCH_TO_OZK, _require_gpu, _stream
+from .ozaki import _RAW_STREAM, _TORCH_TO_OZK, _require_gpu, _stream
 
 _HALF = (torch.float16, torch.bfloat16)
+_OFFSETS = (torch.int32, torch.int64)
 _FLOAT = (torch.float32, torch.float16, torch.bfloat16)
 _MAX_STRIDE = 1 << 22      # the kernels' limit on the distance of two rows
 
@@ -49,11 +50,17 @@ def _on_one_gpu(a: torch.Tensor, *others) -> None:
     _require_gpu(a, *(t for t in others if t is not None))
 
 
+_FUNCTIONS: dict = {}
+
+
 def _call(name: str, dev: torch.device, *args) -> None:
     """Library call `name` on dev's current stream, its last argument."""
-    fn = getattr(_lib.load(), name)
-    if dev.index == _current_device():
-        st = fn(*args, _stream(dev))
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_lib.load(), name)
+    idx = dev.index
+    if _RAW_STREAM is not None and idx == _current_device():
+        st = fn(*args, _RAW_STREAM(idx))
     else:
         with torch.cuda.device(dev):
             st = fn(*args, _stream(dev))
@@ -97,39 +104,47 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 # ============================================================
 
 def _grouped_checks(A, B, offsets):
+    a, b, dev = A.shape, B.shape, A.device
+    if (len(a) == 2 and len(b) == 3 and a[1] == b[1] and A.dtype in _HALF and B.dtype == A.dtype
+            and offsets.shape == (b[0] + 1,) and offsets.dtype in _OFFSETS and dev.type == "cuda"
+            and B.device == dev and offsets.device == dev):
+        return
+    # one of these says what is wrong
     assert A.dim() == 2, f"A must be [rows, K], got {tuple(A.shape)}"
     assert B.dim() == 3, f"B must be [groups, K, N], got {tuple(B.shape)}"
     assert A.shape[1] == B.shape[1], f"contraction dim mismatch: A K={A.shape[1]}, B K={B.shape[1]}"
     assert A.dtype == B.dtype, f"A/B dtype mismatch: {A.dtype} vs {B.dtype}"
-    _offset_checks(offsets, B.shape[0])
+    assert offsets.dim() == 1 and offsets.shape[0] == B.shape[0] + 1, \
+        f"offsets must be [groups + 1] = [{B.shape[0] + 1}], got {tuple(offsets.shape)}"
+    if offsets.dtype not in _OFFSETS:
+        raise NotImplementedError(f"offsets must be int32 or int64, got {offsets.dtype}")
     _on_one_gpu(A, B, offsets)
     _require_dtype("grouped_matmul", A.dtype, _HALF)
-
-
-def _offset_checks(offsets, G):
-    assert offsets.dim() == 1 and offsets.shape[0] == G + 1, \
-        f"offsets must be [groups + 1] = [{G + 1}], got {tuple(offsets.shape)}"
-    if offsets.dtype not in (torch.int32, torch.int64):
-        raise NotImplementedError(f"offsets must be int32 or int64, got {offsets.dtype}")
 
 
 def _grouped_forward(A, B, offsets):
     T, K = A.shape
     G, _, N = B.shape
-    A = _rows(A)
-    sb = B.stride()
+    dtype, dev = A.dtype, A.device
+    sa, sb = A.stride(), B.stride()
+    if sa[1] != 1 or sa[0] >= _MAX_STRIDE:
+        A = _rows(A)
+        sa = A.stride()
     if not ((sb[2] == 1 and sb[1] < _MAX_STRIDE) or (sb[1] == 1 and sb[2] < _MAX_STRIDE)):
         B = B.contiguous()
         sb = B.stride()
     if offsets.stride(0) != 1:
         offsets = offsets.contiguous()
-    dtype, dev = A.dtype, A.device
-    C = torch.empty((T, N), dtype=dtype, device=dev)
-    ap, bp, sa = A.data_ptr(), B.data_ptr(), A.stride(0)
-    n = _bytes("ozk_grouped_matmul_workspace_bytes", ap & 15, sa, bp & 15, sb, T, K, N, G)
-    ws, wsp = _workspace(n, dev)
-    _call("ozk_grouped_matmul", dev, ap, sa, bp, _i64(*sb), offsets.data_ptr(), offsets.element_size(), T,
-          K, N, G, _TORCH_TO_OZK[dtype], C.data_ptr(), N, wsp, n)
+    C = A.new_empty((T, N))
+    ap, bp = A.data_ptr(), B.data_ptr()
+    ws = wsp = None
+    n = 0
+    # whole 16-byte pieces need no workspace: most calls spare the query
+    if (ap | bp | (sa[0] | sb[0] | sb[1] * sb[2] | K | N) * 2) & 15:
+        n = _bytes("ozk_grouped_matmul_workspace_bytes", ap & 15, sa[0], bp & 15, sb, T, K, N, G)
+        ws, wsp = _workspace(n, dev)
+    _call("ozk_grouped_matmul", dev, ap, sa[0], bp, _i64(*sb), offsets.data_ptr(),
+          offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype], C.data_ptr(), N, wsp, n)
     del ws
     return C
 
@@ -141,12 +156,13 @@ def _grouped_wgrad(A, D, offsets, G):
     if offsets.stride(0) != 1:
         offsets = offsets.contiguous()
     dtype, dev = A.dtype, A.device
-    dB = torch.empty((G, K, N), dtype=dtype, device=dev)
+    dB = A.new_empty((G, K, N))
     ap, dp, sa, sd = A.data_ptr(), D.data_ptr(), A.stride(0), D.stride(0)
     n = _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", ap & 15, sa, dp & 15, sd, T, K, N, G)
     ws, wsp = _workspace(n, dev)
-    _call("ozk_grouped_matmul_wgrad", dev, ap, sa, dp, sd, offsets.data_ptr(), offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype],
-          dB.data_ptr(), _i64(K * N, N), wsp, n)
+    _call("ozk_grouped_matmul_wgrad", dev, ap, sa, dp, sd, offsets.data_ptr(),
+          offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype], dB.data_ptr(),
+          _i64(K * N, N), wsp, n)
     del ws
     return dB
 
@@ -189,7 +205,8 @@ def grouped_matmul_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
                             offsets: torch.Tensor):
     """The gradients (dA, dB) of grouped_matmul(A, B, offsets) for dC (rows, N):
     dA[t] = dC[t] @ B[g]^T, zeros in the rows of no group; dB[g] = A[rows of g]^T
-    @ dC[rows of g], zeros for a group without rows.  Both have A's dtype."""
+    @ dC[rows of g], zeros for a group without rows.  Both have A's dtype; they are
+    not differentiable themselves."""
     _grouped_checks(A, B, offsets)
     assert dC.shape == (A.shape[0], B.shape[2]), \
         f"dC must be {(A.shape[0], B.shape[2])}, got {tuple(dC.shape)}"
@@ -219,7 +236,7 @@ def _w4_checks(packed, scales, zeros, group_size, K):
         f"packed must be a 2-d uint8 tensor, got {packed.dtype} {tuple(packed.shape)}"
     assert packed.shape[1] >= (K + 31) // 32 * 16, \
         f"packed has {packed.shape[1]} bytes a row, K={K} needs {(K + 31) // 32 * 16}"
-    want = (packed.shape[0], -(-K // group_size))
+    want = (packed.shape[0], (K + group_size - 1) // group_size)
     assert scales.shape == want, f"scales must be {want}, got {tuple(scales.shape)}"
     assert zeros is None or (zeros.shape == want and zeros.dtype == torch.uint8), \
         f"zeros must be {want} uint8, got {zeros.dtype} {tuple(zeros.shape)}"
@@ -259,7 +276,7 @@ def quantize_w4(W: torch.Tensor, group_size: int = 128, *, zeros: bool = False):
     W = W if W.stride(1) == 1 or K == 1 else W.contiguous()
     dev = W.device
     packed = torch.empty((N, (K + 31) // 32 * 16), dtype=torch.uint8, device=dev)
-    scales = torch.empty((N, groups), dtype=W.dtype, device=dev)
+    scales = W.new_empty((N, groups))
     z = torch.empty((N, groups), dtype=torch.uint8, device=dev) if zeros else None
     _call("ozk_quantize_w4", dev, W.data_ptr(), _TORCH_TO_OZK[W.dtype], N, K, W.stride(0),
           group_size, packed.data_ptr(), packed.shape[1], scales.data_ptr(), groups,
@@ -303,20 +320,19 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
         with an infinity or NaN gives a row of NaN.
     """
     assert x.dim() >= 1 and x.shape[-1] >= 1, f"x must be [..., K], got {tuple(x.shape)}"
-    K = x.shape[-1]
+    K, dtype, dev = x.shape[-1], x.dtype, x.device
     _w4_checks(packed, scales, zeros, group_size, K)
-    assert scales.dtype in (x.dtype, torch.float32), \
-        f"scales must be {x.dtype} or float32, got {scales.dtype}"
+    assert scales.dtype == dtype or scales.dtype == torch.float32, \
+        f"scales must be {dtype} or float32, got {scales.dtype}"
     _on_one_gpu(x, packed, scales, zeros)
-    dtype = x.dtype
     _require_dtype("matmul_w4", dtype, _FLOAT)
     _no_grad("matmul_w4", x, scales)
     packed, scales, zeros = _w4_operands(packed, scales, zeros)
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     if x2.stride(1) != 1 and K != 1:
         x2 = x2.contiguous()
-    M, N, dev = x2.shape[0], packed.shape[0], x.device
-    y = torch.empty((M, N), dtype=dtype, device=dev)
+    M, N = x2.shape[0], packed.shape[0]
+    y = x2.new_empty((M, N))
     code = _TORCH_TO_OZK[dtype]
     n = _bytes("ozk_matmul_w4_workspace_bytes", code, M, N, K, group_size)
     ws, wsp = _workspace(n, dev)
