@@ -154,6 +154,66 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_kernel(Grou
     store_tile<ST>(t, p.C + lo * p.c_pitch + n0 * 2, p.c_pitch, rows, cols);
 }
 
+// Which of its `all` work items of which group a workgroup of the dB kernel
+// takes.  Groups about as long as their mean: an XCD has groups of its own, whose
+// rows its L2 then reads once.  A group of more than twice the mean: every group
+// over all XCDs, the longest first, so that no XCD and no workgroup is left with
+// them at the end (four classes of length are enough: the order in full took
+// longer than it saved).  More than 64 groups: over all XCDs in their order.
+// Measured (us, T x G x K x N; a group to an XCD / spread / spread and ordered):
+//     16384 x 32 x 2048 x 1024, uneven   135 / 119 / 102
+//     32768 x 16 x 2048 x 4096, uneven  1325 / 539 / 531
+//     16384 x 32 x 2048 x 1024, even      88 /  95 / 100
+struct GradItem {
+    int64_t lo, hi;   // the group's rows
+    int g, item;      // g < 0: none
+};
+OZK_DEV GradItem grad_item(const GroupedGradParams &p, uint32_t all) {
+    const uint32_t slots = (all + 7) / 8;
+    uint32_t r = blockIdx.x / 8 / slots;   // the place of its group in their order
+    const uint32_t i = blockIdx.x / 8 - r * slots, x = (blockIdx.x + r) % 8;
+    const uint32_t from = (uint32_t)((uint64_t)all * x / 8);
+    const bool none = i >= (uint32_t)((uint64_t)all * (x + 1) / 8) - from;
+    GradItem at = {0, 0, none ? -1 : (int)r, (int)(from + i)};
+    if (p.G > 64) {
+        if (none) return at;
+        at.lo = uniform(offset_at(p.offsets, p.offsets64, r, p.T));
+        at.hi = uniform(offset_at(p.offsets, p.offsets64, r + 1, p.T));
+        return at;
+    }
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0, hi = 0;
+    if (lane < p.G) {
+        lo = offset_at(p.offsets, p.offsets64, lane, p.T);
+        hi = offset_at(p.offsets, p.offsets64, lane + 1, p.T);
+    }
+    const int64_t n = hi - lo;
+    const uint64_t there = p.G == 64 ? ~0ull : ((uint64_t)1 << p.G) - 1;
+    const uint64_t over2 = __ballot(n > 2 * p.share);
+    if (over2) {
+        if (none) return at;
+        const uint64_t over4 = __ballot(n > 4 * p.share), over1 = __ballot(n > p.share);
+        const uint64_t cls[4] = {over4, over2 & ~over4, over1 & ~over2, there & ~over1};
+        uint32_t before = 0, rank = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (cls[c] >> lane & 1)
+                rank = before + (uint32_t)__popcll(cls[c] & (((uint64_t)1 << lane) - 1));
+            before += (uint32_t)__popcll(cls[c]);
+        }
+        r = (uint32_t)__ffsll((unsigned long long)__ballot(lane < p.G && rank == r)) - 1;
+    } else {
+        const int64_t tile = xcd_tile(blockIdx.x, all * (uint32_t)p.G);
+        if (tile < 0) return GradItem{0, 0, -1, 0};
+        r = (uint32_t)tile / all;
+        at.item = (int)((uint32_t)tile - r * all);
+    }
+    at.g = uniform((int)r);
+    at.lo = uniform(__shfl(lo, at.g));
+    at.hi = uniform(__shfl(hi, at.g));
+    return at;
+}
+
 // dB: the rows of a group are the contraction, both operands "cols".  With
 // splits > 1 workgroup s of a tile sums the s-th part of the group's rows into
 // the workspace, and grouped_join_kernel adds the parts in order.
@@ -164,15 +224,15 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_grad_kernel
     const uint32_t tiles_k = (uint32_t)((p.K + BM - 1) / BM);
     const uint32_t tiles_n = (uint32_t)((p.N + BN - 1) / BN);
     const uint32_t each = tiles_k * tiles_n;
-    const int64_t tile = xcd_tile(blockIdx.x, each * (uint32_t)p.G * (uint32_t)p.splits);
-    if (tile < 0) return;
-    const uint32_t gs = (uint32_t)tile / each, in = (uint32_t)tile - gs * each;
-    const uint32_t g = gs / (uint32_t)p.splits, s = gs - g * (uint32_t)p.splits;
-    const uint32_t tk = in / tiles_n, tn = in - tk * tiles_n;
-
-    int64_t lo = uniform(offset_at(p.offsets, p.offsets64, g, p.T));
-    int64_t hi = uniform(offset_at(p.offsets, p.offsets64, g + 1, p.T));
-    if (hi < lo) hi = lo;
+    const GradItem at = grad_item(p, each * (uint32_t)p.splits);
+    if (at.g < 0) return;
+    const int64_t g = at.g;
+    const uint32_t s = (uint32_t)at.item / each, in = (uint32_t)at.item - s * each;
+    // squares of tiles about as large as what an XCD has of a group
+    const uint32_t h = p.block, first = in / tiles_n / h * h;
+    const uint32_t high = tiles_k - first < h ? tiles_k - first : h, ahead = in - first * tiles_n;
+    const uint32_t tn = ahead / high, tk = first + ahead - tn * high;
+    int64_t lo = at.lo, hi = at.hi < at.lo ? at.lo : at.hi;
     if (p.splits > 1) {
         // whole stages each
         const int64_t stages = (hi - lo + Sh::KS - 1) / Sh::KS;
@@ -287,13 +347,17 @@ hipError_t grouped_go(const GroupedParams &p, hipStream_t st) {
 
 template <typename ST, typename Sh, bool DMA>
 hipError_t grad_go(const GroupedGradParams &p, hipStream_t st) {
-    const int64_t tiles = ((p.K + Sh::BM - 1) / Sh::BM) * ((p.N + Sh::BN - 1) / Sh::BN) * p.G *
-                          p.splits;
-    if (tiles >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
+    const int64_t each = ((p.K + Sh::BM - 1) / Sh::BM) * ((p.N + Sh::BN - 1) / Sh::BN);
+    const int64_t slots = (each * p.splits + 7) / 8;
+    if (slots >= (int64_t)1 << 28 || slots * p.G >= (int64_t)1 << 28)
+        return hipErrorInvalidConfiguration;
     if (hipError_t e = allow_lds<&grouped_grad_kernel<ST, Sh, DMA>>(Sh::LDS_BYTES);
         e != hipSuccess)
         return e;
-    grouped_grad_kernel<ST, Sh, DMA><<<dim3((uint32_t)((tiles + 7) / 8 * 8)), Sh::THREADS, Sh::LDS_BYTES, st>>>(p);
+    GroupedGradParams q = p;
+    q.share = p.T / p.G;
+    for (q.block = 1; q.block < 8 && 4 * q.block * q.block <= slots;) q.block *= 2;
+    grouped_grad_kernel<ST, Sh, DMA><<<dim3((uint32_t)(slots * 8 * p.G)), Sh::THREADS, Sh::LDS_BYTES, st>>>(q);
     return hipGetLastError();
 }
 

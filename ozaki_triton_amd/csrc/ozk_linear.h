@@ -49,6 +49,9 @@ struct GroupedGradParams {
     bool a_padded, d_padded;
     float *part;            // workspace: partial sums of the row ranges (splits > 1)
     int splits;
+    // set by the launch
+    int64_t share;      // rows of a group on average
+    uint32_t block;     // tiles on a side of the squares they are taken in
 };
 // Operands that are copied to whole 16-byte pieces first (packed): the bytes of
 // the copies, 0 for none.  plan_* say which; pack_* point the parameters at the

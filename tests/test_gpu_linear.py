@@ -122,6 +122,22 @@ def test_grouped_tiles(counts, K, N):
         _check_grouped(_randn(1, rows, K), B.mT if bt else B.mT.contiguous(), _randn(3, rows, N), offsets)
 
 
+@pytest.mark.parametrize("counts, K, N", [
+    ([1] * 30 + [90, 500, 60, 200], 520, 264),     # every class of length
+    ([0] * 63 + [300], 136, 72), ([300] + [0] * 62 + [7], 512, 320), ([3] * 64 + [400], 136, 200),
+    ([10, 900, 10, 10], 2048, 2048), ([200] * 4, 2048, 2056), ([90, 110, 100], 1304, 1112),
+    ([0, 5000, 0, 30], 64, 64)])
+def test_grouped_gradient_of_uneven_groups(counts, K, N):
+    """Every tile of dB is written once, whatever the order of the groups: by length
+    where they differ, their own where not or where they are many."""
+    A, D, offsets = _randn(1, sum(counts), K), _randn(3, sum(counts), N), _offsets(counts)
+    B = torch.zeros(len(counts), K, N, dtype=BF, device="cuda")
+    stale = torch.full((len(counts), K, N), math.nan, dtype=BF, device="cuda")
+    del stale    # the memory that dB is likely to get
+    _, dB = ozk.grouped_matmul_backward(D, A, B, offsets)
+    _close(dB, *_wgrad(A, D, offsets.tolist()), max(counts) + 16, BF)
+
+
 def test_grouped_offsets_inside_the_rows():
     """int64 offsets that start after row 0: the rows before and after get zeros."""
     A, B, D = _randn(1, 90, 64), _randn(2, 3, 64, 72), _randn(3, 90, 72)
