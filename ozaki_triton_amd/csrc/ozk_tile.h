@@ -140,21 +140,21 @@ template <int S, bool COLS, int BX> OZK_DEV WindowAt window_at(const TileSrc &s,
 }
 
 // One LDS-DMA instruction: 16 bytes per lane from `base` + off to LDS byte `to`
-// + 16 * lane; zeros where off is past the 2 GiB behind base.  Written in
+// + PLUS + 16 * lane; zeros where off is past the 2 GiB behind base.  Written in
 // assembly because behind the builtin the compiler waits for every DMA on its
 // way before a ds_read_b64_tr_b16 (measured: 1028 us against 815 without the
 // read-ahead below, 32768 x 2048 x 4096).  It has no register result; its LDS
 // writes are waited for by wait_vmcnt and a barrier like the builtin's.
-OZK_DEV void dma_piece(const char *base, uint32_t off, uint32_t to) {
+template <int PLUS> OZK_DEV void dma_piece(const char *base, uint32_t off, uint32_t to) {
     const uint64_t at = (uint64_t)(uintptr_t)base;
     const i32x4 desc = {uniform((int)(uint32_t)at), uniform((int)(uint32_t)(at >> 32)), 0x7FFFFFFF,
                         0x00020000};
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"   // m0 holds nothing else in these kernels
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
-                 : "s"(uniform((int)to)), "v"(off), "s"(desc)
-                 : "memory", "m0");
+                 : "s"(uniform((int)to)), "v"(off), "s"(desc), "n"(PLUS)
+                 : "memory", "m0", "scc");
 #pragma clang diagnostic pop
 }
 
@@ -226,16 +226,18 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
             const char *base, *first;
             int64_t step;
             int whole, rest;   // whole stages, and what the one behind them has of K
+            int slot;          // its first window's place in a stage
             // what the group's stage kb has of K, as WindowAt counts it
             OZK_DEV int left(int kb, int kw) const {
                 const int at = kb * Sh::KW + kw;
                 return at < whole ? 128 : at == whole ? rest : 0;
             }
         };
+        constexpr int LPB = LP - Sh::LPA;
         Feed fa = {A.base, A.first, Sh::ACOLS ? Sh::KS * A.pitch : 128, (int)(A.klen / ua),
-                   (int)(A.klen % ua)};
+                   (int)(A.klen % ua), wave * (Sh::ONE ? LP : Sh::LPA) * 1024};
         Feed fb = {B.base, B.first, Sh::BCOLS ? Sh::KS * B.pitch : 128, (int)(B.klen / ub),
-                   (int)(B.klen % ub)};
+                   (int)(B.klen % ub), (Sh::ONE ? wave * LP : Sh::BM / 8 + wave * LPB) * 1024};
         if constexpr (Sh::KW > 1) {
             fa.base += kw * fa.step;
             fb.base += kw * fb.step;
@@ -251,21 +253,18 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
             feed[1] = fb;
         }
         constexpr auto of = [](int q) { return Sh::ONE || q < Sh::LPA ? 0 : 1; };   // window q's feed
+        // and its place among the feed's
+        constexpr auto nth = [](int q) { return Sh::ONE || q < Sh::LPA ? q : q - Sh::LPA; };
         WindowAt win[LP];
-        int slot_at[LP];   // its place in a stage
 #pragma unroll
         for (int q = 0; q < LP; ++q) {
             if constexpr (Sh::ONE) {
                 const int w = wave * LP + q;
                 win[q] = onlyA ? window_at<S, Sh::ACOLS, Sh::BM>(A, w, lane)
                                : window_at<S, Sh::BCOLS, Sh::BN>(B, w - Sh::BM / 8, lane);
-                slot_at[q] = w * 1024;
             } else {
-                constexpr int LPB = LP - Sh::LPA;
-                const int w = of(q) == 0 ? wave * Sh::LPA + q : wave * LPB + q - Sh::LPA;
-                win[q] = of(q) == 0 ? window_at<S, Sh::ACOLS, Sh::BM>(A, w, lane)
-                                    : window_at<S, Sh::BCOLS, Sh::BN>(B, w, lane);
-                slot_at[q] = (of(q) == 0 ? w : Sh::BM / 8 + w) * 1024;
+                win[q] = of(q) == 0 ? window_at<S, Sh::ACOLS, Sh::BM>(A, wave * Sh::LPA + nth(q), lane)
+                                    : window_at<S, Sh::BCOLS, Sh::BN>(B, wave * LPB + nth(q), lane);
             }
         }
         auto advance = [&] {
@@ -273,18 +272,30 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
             for (Feed &f : feed) f.base += f.step;
         };
 
-        // windows q0 .. q1 of stage kb, if there is one; stages come in order
-        const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
-        auto issue = [&](int kb, int q0, int q1) {
-            if (kb >= nkb) return;
-            if (q0 == 0 && kb > 0) advance();
-            const uint32_t dst = lds + (uint32_t)(kb % Sh::NST) * Sh::SLOT + kw * Sh::STAGE;
+        // Stage kb, which is the next one: the last whole one is followed by one
+        // whose windows are cut, and then by empty ones (of a group of waves)
+        auto begin = [&](int kb) {
+            if (kb > 0) advance();
 #pragma unroll
-            for (int q = 0; q < LP; ++q) {
-                if (q < q0 || q >= q1) continue;
-                const Feed &f = feed[of(q)];
-                dma_piece(f.base, win[q].k < f.left(kb, kw) ? win[q].off : kTileOOB, dst + slot_at[q]);
+            for (int f = 0; f < (Sh::ONE ? 1 : 2); ++f) {
+                const int left = feed[f].left(kb, kw);
+                if (left < 128)
+#pragma unroll
+                    for (int q = 0; q < LP; ++q)
+                        if (of(q) == f && win[q].k >= left) win[q].off = kTileOOB;
             }
+        };
+        // and windows Q0 .. Q1 of it
+        const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem +
+                             kw * Sh::STAGE;
+        auto issue = [&](int kb, auto q0_, auto q1_) {
+            constexpr int Q0 = decltype(q0_)::value, Q1 = decltype(q1_)::value;
+            const uint32_t dst = lds + (uint32_t)kb % Sh::NST * Sh::SLOT;
+            static_for_tile<Q1 - Q0>([&](auto q_) {
+                constexpr int q = Q0 + decltype(q_)::value;
+                const Feed &f = feed[of(q)];
+                dma_piece<nth(q) * 1024>(f.base, win[q].off, dst + (uint32_t)f.slot);
+            });
         };
         // the same through registers, for rows of any alignment
         i32x4 held[DMA ? 1 : LP];
@@ -302,9 +313,9 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
             }
         };
         auto put = [&](int kb) {
-            char *dst = smem + (kb % Sh::NST) * Sh::SLOT + kw * Sh::STAGE + lane * 16;
+            char *dst = smem + ((uint32_t)kb % Sh::NST) * Sh::SLOT + kw * Sh::STAGE + lane * 16;
 #pragma unroll
-            for (int q = 0; q < LP; ++q) *(i32x4 *)(dst + slot_at[q]) = held[q];
+            for (int q = 0; q < LP; ++q) *(i32x4 *)(dst + feed[of(q)].slot + nth(q) * 1024) = held[q];
         };
 
         const int g = lane >> 4, i16 = lane & 15;
@@ -360,8 +371,8 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
         // ready(): stage kb + 1 has landed and every wave has read stage kb;
         // during(n): what else group n issues
         auto stage = [&](int kb, auto &&ready, auto &&during) {
-            const char *buf = smem + (kb % Sh::NST) * Sh::SLOT + kw * Sh::STAGE;
-            const char *next = smem + ((kb + 1) % Sh::NST) * Sh::SLOT + kw * Sh::STAGE;
+            const char *buf = smem + ((uint32_t)kb % Sh::NST) * Sh::SLOT + kw * Sh::STAGE;
+            const char *next = smem + ((uint32_t)(kb + 1) % Sh::NST) * Sh::SLOT + kw * Sh::STAGE;
             static_for_tile<G>([&](auto n_) {
                 constexpr int n = decltype(n_)::value, i = n % MI;
                 if constexpr (n == BG) ready();
@@ -400,38 +411,60 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
         };
 
         if constexpr (DMA) {
-            constexpr int NOW = LP < 2 ? LP : 2;   // windows issued right after the barrier
+            // NOW windows are issued right after the barrier, the others during the
+            // next groups
+            constexpr int NOW = LP < 2 ? LP : 2, NST = Sh::NST;
+            static_assert((NST - 1) * LP < 64, "vmcnt");
+            constexpr std::integral_constant<int, 0> Q0;
+            constexpr std::integral_constant<int, NOW> QN;
+            constexpr std::integral_constant<int, LP> QE;
 #pragma unroll
-            for (int s = 0; s < Sh::NST; ++s) issue(s, 0, LP);
+            for (int s = 0; s < NST; ++s) {
+                if (s >= nkb) continue;
+                begin(s);
+                if (s < NST - 1) issue(s, Q0, QE);
+                else issue(s, Q0, QN);
+            }
             if (nkb > 0) {
                 // the first has landed; few stages: all have
-                if (nkb >= Sh::NST) wait_vmcnt<(Sh::NST - 1) * LP>();
+                if (nkb >= NST) wait_vmcnt<(NST - 2) * LP + NOW>();
                 else wait_vmcnt<0>();
                 exec_barrier();
                 first(smem + kw * Sh::STAGE);
             }
-            for (int kb = 0; kb < nkb; ++kb)
+            // all: stages kb + NST - 1 and kb + NST exist
+            auto one = [&](int kb, auto all_) {
+                constexpr bool all = decltype(all_)::value;
                 stage(
                     kb,
                     [&] {
                         // kb + 1 has landed; the last stages, on their way for a
                         // while, all have
-                        if (kb + Sh::NST <= nkb) wait_vmcnt<(Sh::NST - 2) * LP>();
+                        if (all || kb + NST <= nkb) wait_vmcnt<(NST - 2) * LP>();
                         else wait_vmcnt<0>();
-                        static_assert((Sh::NST - 1) * LP < 64, "vmcnt");
                         __builtin_amdgcn_s_waitcnt(0xC07F);   // this wave's reads of the slot
                         exec_barrier();
-                        issue(kb + Sh::NST, 0, NOW);
+                        if (all || kb + NST < nkb) {
+                            begin(kb + NST);
+                            issue(kb + NST, Q0, QN);
+                        }
                     },
                     [&](auto n_) {
                         // the rest of the stage begun behind the last barrier
                         constexpr int n = decltype(n_)::value;
                         constexpr int groups = BG > 1 ? BG : 1;
                         constexpr int per = (LP - NOW + groups - 1) / groups;
-                        if constexpr (n < BG && NOW + n * per < LP)
-                            if (kb > 0) issue(kb - 1 + Sh::NST, NOW + n * per,
-                                              NOW + (n + 1) * per < LP ? NOW + (n + 1) * per : LP);
+                        if constexpr (n < BG && NOW + n * per < LP) {
+                            constexpr int to = NOW + (n + 1) * per < LP ? NOW + (n + 1) * per : LP;
+                            if (all || kb + NST - 1 < nkb)
+                                issue(kb + NST - 1, std::integral_constant<int, NOW + n * per>{},
+                                      std::integral_constant<int, to>{});
+                        }
                     });
+            };
+            int kb = 0;
+            for (; kb < nkb - NST; ++kb) one(kb, std::true_type{});
+            for (; kb < nkb; ++kb) one(kb, std::false_type{});
         } else {
             if (nkb > 0) {
                 fetch(0);
