@@ -95,6 +95,8 @@ struct OrthBounds {
     }
 };
 
+bool chain_pays(int64_t m, int64_t n) { return n >= 2 * m; }   // see plan_orth
+
 // The products of an orthogonalisation (X [m, n], m <= n).
 //
 // One step by itself is A = X X^T, B = b A + c A A, X' = a X + B X, one
@@ -102,8 +104,9 @@ struct OrthBounds {
 // between: with P = a I + b A + c A A, X' = P X and so A' = P A P, and all of
 // these are polynomials in A, symmetric and commuting.  Then A = X X^T and Q X
 // are paid once, Q the product of the P's, and a step is P, P A, (P A) P and P Q,
-// four symmetric products of [m, m]: less where n is at least 3 m (measured,
-// 2048 x 8192: 411 us for a step by itself, 200 for one of these).  What it costs
+// four symmetric products of [m, m]: less where n is at least 2 m (measured, a
+// step by itself / one of these, 2048 x 8192: 323 / 145 us, 2048 x 4096: 193 /
+// 145, 2048 x 2048: 120 / 145).  What it costs
 // is accuracy: an error of 2^-22 in A (its slices) is amplified by P^2 a step
 // and by P's slope at the end, and j is as large as keeps that worst case within
 // half a unit of a 16-bit result's rounding; for fp32 results every step runs by
@@ -120,7 +123,7 @@ void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int 
         return OrthBounds(co[3 * i], co[3 * i + 1], co[3 * i + 2], bound[i] * bound[i]);
     };
     int j = 1;
-    if (n >= 3 * m && dtype != OZK_F32) {
+    if (chain_pays(m, n) && dtype != OZK_F32) {
         const double limit = dtype == OZK_BF16 ? 0x1p-9 : 0x1p-12;
         double gain = 0x1p-22;
         while (j < steps) {
@@ -202,7 +205,7 @@ struct OrthLayout {
 OrthLayout orth_most(int64_t batch, int64_t M, int64_t N, int steps) {
     const int64_t m = M < N ? M : N, n = M < N ? N : M;
     return OrthLayout(batch, M, N, steps > 1 ? 2 : 1,
-                      steps > 1 && n >= 3 * m ? ozk::kOrthSquares : 2);
+                      steps > 1 && chain_pays(m, n) ? ozk::kOrthSquares : 2);
 }
 
 }  // namespace
@@ -470,6 +473,7 @@ int ozk_orthogonalize(const void *G, int dtype, int64_t batch, int64_t M, int64_
         return OZK_ERR_WORKSPACE;
     ozk::OrthPlan plan;
     plan_orth(plan, M < N ? M : N, M < N ? N : M, coefficients, steps, dtype);
+    if (at.sums + plan.xs * at.x + plan.squares * at.a > at.total) return OZK_ERR_WORKSPACE;
     ozk::OrthParams p;
     p.G = (const char *)G;
     p.out = (char *)out;

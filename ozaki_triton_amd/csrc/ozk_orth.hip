@@ -305,23 +305,37 @@ hipError_t orth_gemm(OrthGemm q, int64_t batch, hipStream_t st) {
 
 template <typename T, int KIND>
 hipError_t orth_product(const OrthGemm &q, int64_t batch, hipStream_t st) {
-    const int64_t cols = KIND >= kOrthX ? q.n : q.m;
-    auto tiles = [&](int64_t bm) {
-        const int64_t tm = (q.m + bm - 1) / bm, tn = (cols + bm - 1) / bm;
-        return batch * (KIND >= kOrthX ? tm * tn : tm * (tm + 1) / 2);
+    // A CU has one workgroup, whatever the tile: the tile is the one whose rounds of
+    // workgroups over the 256 CUs take the shortest.  A round takes (us, K in 1024s,
+    // fitted to what follows; R by rows / by columns):
+    //     256 x 256, 8 waves               31 + 46 K / 31 + 60 K
+    //     128 x 128, 2 x 8 waves           16 + 15 K / 12 + 18 K
+    //     96 x 96, 2 x 6 waves, 3 stages   11 + 12 K /  4 + 15 K (never the shortest)
+    //     64 x 64, 2 x 4 waves, 4 stages    7 +  5 K /  3 +  7 K
+    // Measured (us, X X^T / A A / B X of 2048 x 8192, then of 1400 x 2000, of two
+    // 1024 x 4096, of 8 matrices 512 x 1024, of 8 256 x 512):
+    //     256   424 / 129 / 165     - /  - /  -     - /  - /  -     - /  - /  -    44 /  36 /  38
+    //     128   141 /  46 / 195     - /  - / 33    72 / 34 / 59    25 / 19 / 19    17 /  14 /  11
+    //     96    109 /  35 / 275    26 / 22 / 44    47 / 19 / 77    18 / 14 / 33     - /   - /   -
+    //     64    155 /  52 / 280    20 / 18 / 41    53 / 22 / 82    20 / 16 / 29   8.8 / 7.2 / 7.6
+    // (A A of 2048 in tiles of 96 with two stages: 41 us, in one group of waves 38)
+    constexpr bool cols = KIND >= kOrthX;
+    const double k = (double)(KIND == kOrthXX ? q.n : q.m) / 1024;
+    auto time = [&](int64_t bm, double fixed, double slope) {
+        const int64_t tm = (q.m + bm - 1) / bm, tn = ((cols ? q.n : q.m) + bm - 1) / bm;
+        const int64_t tiles = batch * (cols ? tm * tn : tm * (tm + 1) / 2);
+        return (double)((tiles + 255) / 256) * (fixed + slope * k);
     };
-    // The largest tile that still gives the CUs enough workgroups; below 256 x 256
-    // a CU has one at most, and two groups of waves share its stages.  Measured
-    // (us, X X^T / A A / B X of 2048 x 8192, then of 1024 x 1024, then of 8
-    // matrices 256 x 512):
-    //     256 x 256, 8 waves               424 / 129 / 175   75 / 82 / 71    44 / 36 / 38
-    //     128 x 128, 2 x 8 waves           140 /  45 / 182   26 / 30 / 24    17 / 14 / 11
-    //     128 x 128, 8 waves, 4 stages     166 /  51 / 221   27 / 31 / 28    17 / 14 / 14
-    //     64 x 64, 2 x 4 waves, 4 stages   177 /  57 / 338   13 / 13 / 15   8.8 / 7.2 / 7.6
-    //     64 x 64, 4 waves, 4 stages       199 /  59 / 315   15 / 16 / 18   9.8 / 7.4 / 8.1
-    //     64 x 64, 4 waves, 2 stages       161 /  49 / 236   22 / 23 / 25    11 / 7.5 / 8.4
-    if (tiles(256) >= 192) return orth_gemm<T, KIND, 256, 2, 4, 2>(q, batch, st);
-    if (tiles(128) >= 112) return orth_gemm<T, KIND, 128, 2, 4, 2, 2>(q, batch, st);
+    const double t256 = cols ? time(256, 31, 60) : time(256, 31, 46);
+    const double t128 = cols ? time(128, 12, 18) : time(128, 16, 15);
+    const double t64 = cols ? time(64, 3, 7) : time(64, 7, 5);
+    if constexpr (!cols) {
+        const double t96 = time(96, 11, 12);
+        if (t96 < t256 && t96 < t128 && t96 < t64)
+            return orth_gemm<T, KIND, 96, 2, 3, 3, 2>(q, batch, st);
+    }
+    if (t256 <= t128 && t256 <= t64) return orth_gemm<T, KIND, 256, 2, 4, 2>(q, batch, st);
+    if (t128 <= t64) return orth_gemm<T, KIND, 128, 2, 4, 2, 2>(q, batch, st);
     return orth_gemm<T, KIND, 64, 2, 2, 4, 2>(q, batch, st);
 }
 

@@ -102,6 +102,7 @@ template <int S, int BX> struct ColsRow { static constexpr int RB = BX * 2 * S; 
 // transposing read touch (k = 0..3 and 8..11 and so on) fall into 8 different
 // bank groups
 template <int RB> OZK_DEV int cols_swz(int k) {
+    static_assert((RB & (RB - 1)) == 0, "the XOR leaves a chunk in its row");
     if constexpr (RB >= 256) return (k & 3) | ((k >> 1) & 4);
     else if constexpr (RB == 128) return ((k >> 1) & 1) | ((k >> 2) & 2);
     else return (k >> 3) & 1;
@@ -344,12 +345,12 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
         // / MI, block n % MI) with B's.  S = 1: a step is one K step, B's fragments
         // of the step.  S = 2: step 0 is slice h of A with both slices of B, step 1
         // slice l of A with slice h of B.  A's fragments are read two groups ahead
-        // into a ring of 4; behind the last read of a stage, two groups before its
+        // into a ring of RA; behind the last read of a stage, two groups before its
         // end, comes the barrier that hands the slot back and the next stage over,
         // so the next stage's first reads run under the last MFMAs.
-        constexpr int G = 2 * MI, BG = G - 2;
-        static_assert(G % 4 == 0, "the ring goes on from stage to stage");
-        i32x4 a[4], b[2][NI], bn[NI];
+        constexpr int G = 2 * MI, BG = G - 2, RA = G % 4 == 0 ? 4 : 3;
+        static_assert(G % RA == 0, "the ring goes on from stage to stage");
+        i32x4 a[RA], b[2][NI], bn[NI];
         auto readA = [&](const char *buf, int n, auto n_) {
             constexpr int N_ = decltype(n_)::value;   // ring place
             a[N_] = frag(buf, std::integral_constant<bool, Sh::ACOLS>{},
@@ -377,7 +378,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                 constexpr int n = decltype(n_)::value, i = n % MI;
                 if constexpr (n == BG) ready();
                 if constexpr (n + 2 < G) {
-                    readA(buf, n + 2, std::integral_constant<int, (n + 2) % 4>{});
+                    readA(buf, n + 2, std::integral_constant<int, (n + 2) % RA>{});
                     if constexpr (S == 1 && n < MI) {
                         constexpr int on = MI < BG ? MI : BG, per = (NI + on - 1) / on;
 #pragma unroll
@@ -386,7 +387,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                     }
                 } else {
                     // the next stage's first fragments
-                    readA(next, n + 2 - G, std::integral_constant<int, (n + 2) % 4>{});
+                    readA(next, n + 2 - G, std::integral_constant<int, (n + 2) % RA>{});
 #pragma unroll
                     for (int j = 0; j < NI; ++j)
                         if (j * 2 / NI == n - BG) {
@@ -395,7 +396,7 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
                         }
                 }
                 during(n_);
-                constexpr int r = n % 4;
+                constexpr int r = n % RA;
 #pragma unroll
                 for (int j = 0; j < NI; ++j)
                     acc[i][j] = mfma16(b[S == 1 ? n / MI : 0][j], a[r], acc[i][j], ST{});

@@ -580,6 +580,20 @@ def test_orthogonalize_large_tiles():
     _check_orth(_randn(1, 40, 200, 232, dtype=F32), 2)
 
 
+@pytest.mark.parametrize("shape, steps", [((2000, 2100), 2), ((4100, 4100), 1), ((16, 333, 700), 3),
+                                          ((700, 1500), 4)])
+def test_orthogonalize_every_square_tile(shape, steps):
+    """Symmetric products in tiles of 96 and 256, with ragged edges, and a chain of
+    products on a matrix twice as long as high."""
+    G = _randn(1, *shape, dtype=BF)
+    got = ozk.orthogonalize(G, steps)
+    for g, y in zip(G.view(-1, *shape[-2:]), got.view(-1, *shape[-2:])):
+        want = _steps(g.double(), [COEFFICIENTS] * steps, 1e-7, torch.float64)
+        plain = _steps(g.float(), [COEFFICIENTS] * steps, 1e-7, F32)
+        off = lambda t: float((t.double() - want).norm() / want.norm())  # noqa: E731
+        assert off(y) <= 4 * max(off(plain), 2.0 ** -24) + ROUND[BF]
+
+
 def test_orthogonalize_in_a_graph():
     G = _randn(1, 2, 100, 160)
     graph = torch.cuda.CUDAGraph()

@@ -154,3 +154,16 @@ def test_workspace_sizes():
     two = _bytes("ozk_orthogonalize_workspace_bytes", 1, 64, 100, 2)
     assert two - one == 64 * 128 * 4 and one >= 64 * 128 * 4 + 2 * 64 * 64 * 4
     assert _bytes("ozk_orthogonalize_workspace_bytes", 1, 100, 64, 2) == two
+
+
+@pytest.mark.parametrize("m, n, squares", [(64, 127, 2), (64, 128, 5), (64, 150, 5), (64, 192, 5),
+                                           (700, 1399, 2), (700, 1400, 5), (700, 1500, 5), (1, 1, 2)])
+def test_orthogonalize_workspace_holds_the_chain(m, n, squares):
+    """From twice as long as high on the last steps run on the square matrix alone,
+    which takes three more of them."""
+    up = lambda v: -(-v // 32) * 32  # noqa: E731
+    for batch in (1, 3):
+        want = batch * (2 * m * up(n) + squares * m * up(m)) * 4
+        for shape in ((m, n), (n, m)):   # and the partial sums of the norm
+            got = _bytes("ozk_orthogonalize_workspace_bytes", batch, *shape, 5)
+            assert want < got <= want + 64 * 1024
