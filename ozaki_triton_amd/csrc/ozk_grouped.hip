@@ -362,23 +362,31 @@ hipError_t grad_go(const GroupedGradParams &p, hipStream_t st) {
 }
 
 // Tiles for T rows in G groups, the counts themselves being on the device: a
-// group is taken to leave half a tile row unused.  The largest tile reads the
-// least per product but wants two rounds of workgroups; smaller groups take
-// the tile that covers most groups whole (each tile row reads the group's
-// matrix again); where a CU has one workgroup at most, two groups of waves
-// share its stages.  Measured (us, T x G x K x N, counts uneven, bf16;
-// 256 x 256 / 128 x 128 of 4 stages / 64 x 128 / 64 x 64 in two groups / 32 x 64
-// in two groups of 4 stages):
-//     32768 x 16 x 2048 x 4096   552 /  789 /  800 / 1068 / 1357
-//     16384 x 32 x 1024 x 2048   101 /  128 /  112 /  161 /  203
-//     4096 x 8 x 1024 x 4096      69 /   65 /   57 /   86 /  189
-//     1999 x 7 x 1000 x 520       28 /   14 /   13 /   11 /   19
-//     512 x 8 x 1024 x 2048       32 /   15 /   17 /   14 /   20
-//     300 x 8 x 4096 x 4096       96 /   46 /   67 /   71 /   71
-//     200 x 32 x 1024 x 2048      30 /   30 /   23 /   26 /   35
-//     2000 x 2 x 4096 x 256        - /   38 /   48 /   25 /   16
-//     4 x 4 x 4096 x 1024          - /   40 /   39 /   20 /   15
-//     16 x 16 x 1024 x 2048       26 /   13 /   12 /  8.4 /  7.7
+// group is taken to leave half a tile row unused.  Where the rows fill tiles of
+// 64 x 128 at least once over, the tile is the one of the shortest time, rounds of
+// workgroups (256 CUs, with 2 and 3 workgroups of the small tiles each) by a
+// round's time, which is (us, K in 1024s)
+//     256 x 256          3 + 27 K        192 x 256          5 + 21 K
+//     128 x 128          1 + 18.5 K      64 x 128           5 + 13 K
+// Measured (us, T x G x K x N, bf16, counts uneven; 256 x 256 / 192 x 256 /
+// 128 x 128 / 64 x 128):
+//     32768 x 16 x 2048 x 4096   533 / 609 / 672 / 732
+//     16384 x 32 x 1024 x 2048    88 /  97 /  90 / 101
+//     8192 x 8 x 1024 x 2048      58 /  53 /  53 /  55
+//     4096 x 8 x 1024 x 4096      55 /  52 /  51 /  55
+//     4096 x 4 x 2048 x 2048      50 /  44 /  57 /  55
+//     2000 x 4 x 1024 x 4096      30 /  27 /  33 /  31
+// Smaller groups take the tile that covers most groups whole (each tile row reads
+// the group's matrix again); where a CU has one workgroup at most, two groups of
+// waves share its stages.  Measured (us; 128 x 128 of 4 stages / 64 x 128 / 64 x 64
+// in two groups / 32 x 64 in two groups of 4 stages):
+//     1999 x 7 x 1000 x 520       14 /  13 /  11 /  19
+//     512 x 8 x 1024 x 2048       15 /  17 /  14 /  20
+//     300 x 8 x 4096 x 4096       46 /  67 /  71 /  71
+//     200 x 32 x 1024 x 2048      30 /  23 /  26 /  35
+//     2000 x 2 x 4096 x 256       38 /  48 /  25 /  16
+//     4 x 4 x 4096 x 1024         40 /  39 /  20 /  15
+//     16 x 16 x 1024 x 2048       13 /  12 / 8.4 / 7.7
 template <typename ST, bool BCOLS> hipError_t grouped_plan(const GroupedParams &p, hipStream_t st) {
     const bool pieces = a_pieces(p) && b_pieces(p);
     const int64_t groups = p.G < 1 ? 1 : p.G < p.T ? p.G : p.T, rows = p.T / groups;
@@ -389,26 +397,47 @@ template <typename ST, bool BCOLS> hipError_t grouped_plan(const GroupedParams &
         if (rows >= 48) return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 2, 2>, false>(p, st);
         return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 2>, false>(p, st);
     }
-    if (rows >= 192 && tiles(256, 256) >= 512)
-        return grouped_go<ST, TileShape<1, false, BCOLS, 256, 256, 2, 4, 2>, true>(p, st);
     if (rows > 24 && rows <= 128 && p.K * p.N >= (int64_t)1 << 22 && tiles(128, 128) >= 128)
         return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 4, 4>, true>(p, st);
-    if (tiles(64, 128) >= 256)
+    if (tiles(64, 128) >= 256) {
+        const double k = (double)p.K / 1024;
+        auto time = [&](int64_t bm, int64_t bn, int64_t at_once, double fixed, double slope) {
+            return (double)((tiles(bm, bn) + at_once - 1) / at_once) * (fixed + slope * k);
+        };
+        const double t256 = time(256, 256, 256, 3, 27), t192 = time(192, 256, 256, 5, 21);
+        const double t128 = time(128, 128, 512, 1, 18.5), t64 = time(64, 128, 768, 5, 13);
+        if (t256 <= t192 && t256 <= t128 && t256 <= t64)
+            return grouped_go<ST, TileShape<1, false, BCOLS, 256, 256, 2, 4, 2>, true>(p, st);
+        if (t192 <= t128 && t192 <= t64)
+            return grouped_go<ST, TileShape<1, false, BCOLS, 192, 256, 2, 4, 2>, true>(p, st);
+        if (t128 <= t64)
+            return grouped_go<ST, TileShape<1, false, BCOLS, 128, 128, 2, 4, 2>, true>(p, st);
         return grouped_go<ST, TileShape<1, false, BCOLS, 64, 128, 1, 4, 2>, true>(p, st);
+    }
     if (tiles(32, 64) <= 256)
         return grouped_go<ST, TileShape<1, false, BCOLS, 32, 64, 1, 4, 4, 2>, true>(p, st);
     return grouped_go<ST, TileShape<1, false, BCOLS, 64, 64, 2, 2, 2, 2>, true>(p, st);
 }
 
+// The same for dB, whose row ranges (splits) are planned for 64 x 128.  Measured
+// (us; 256 x 256 / 128 x 128 / 64 x 128):
+//     16384 x 32 x 2048 x 1024    91 /  98 / 113
+//     8192 x 64 x 1024 x 1024     53 /  55 /  59
+//     3000 x 6 x 2048 x 1024      32 /  24 /  37
+//     4096 x 4 x 1024 x 2048      43 /  33 /  46
+//     1999 x 7 x 1000 x 520       25 /  13 /  12
 template <typename ST> hipError_t grad_plan(const GroupedGradParams &p, hipStream_t st) {
     const bool pieces = whole_pieces(p.A, p.a_pitch, 0, p.K, p.a_padded) &&
                         whole_pieces(p.D, p.d_pitch, 0, p.N, p.d_padded);
     const int64_t large = ((p.K + 255) / 256) * ((p.N + 255) / 256) * p.G;
+    const int64_t medium = ((p.K + 127) / 128) * ((p.N + 127) / 128) * p.G;
     hipError_t e;
     if (!pieces)
         e = grad_go<ST, TileShape<1, true, true, 128, 128, 2, 2, 2>, false>(p, st);
-    else if (large >= 192)
+    else if (large >= 512)
         e = grad_go<ST, TileShape<1, true, true, 256, 256, 2, 4, 2>, true>(p, st);
+    else if (medium >= 384)
+        e = grad_go<ST, TileShape<1, true, true, 128, 128, 2, 4, 2>, true>(p, st);
     else
         e = grad_go<ST, TileShape<1, true, true, 64, 128, 1, 4, 2>, true>(p, st);
     if (e != hipSuccess || p.splits == 1) return e;

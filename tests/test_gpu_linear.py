@@ -111,7 +111,8 @@ def test_grouped_copied_operands(counts, K, N):
 
 
 @pytest.mark.parametrize("counts, K, N", [
-    ([600] * 4, 256, 8192),       # the largest tile
+    ([600] * 4, 256, 8192), ([900, 1300, 1000], 192, 16384),   # the largest tiles
+    ([1000, 500, 500], 1024, 4096), ([300, 700], 2048, 2048), ([1000, 3000], 264, 2056),
     ([40] * 8, 2048, 2048),       # 128 x 128, four stages
     ([700, 500], 4096, 256),      # two groups of waves on a tile's stages
     ([3, 0, 2], 4096, 1024), ([70, 90], 520, 520)])
@@ -125,7 +126,8 @@ def test_grouped_tiles(counts, K, N):
 @pytest.mark.parametrize("counts, K, N", [
     ([1] * 30 + [90, 500, 60, 200], 520, 264),     # every class of length
     ([0] * 63 + [300], 136, 72), ([300] + [0] * 62 + [7], 512, 320), ([3] * 64 + [400], 136, 200),
-    ([10, 900, 10, 10], 2048, 2048), ([200] * 4, 2048, 2056), ([90, 110, 100], 1304, 1112),
+    ([10, 900, 10, 10], 2048, 2048), ([200] * 4, 2048, 2056), ([20, 900] * 4, 2048, 2048),
+    ([40] * 8, 2048, 2048), ([300, 100, 80], 1288, 2056), ([90, 110, 100], 1304, 1112),
     ([0, 5000, 0, 30], 64, 64)])
 def test_grouped_gradient_of_uneven_groups(counts, K, N):
     """Every tile of dB is written once, whatever the order of the groups: by length
