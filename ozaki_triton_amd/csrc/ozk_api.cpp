@@ -140,7 +140,7 @@ const char *ozk_strerror(int status) {
     }
 }
 
-int ozk_version(void) { return 300; }   // 0.3.0: the *_pairs calls
+int ozk_version(void) { return 400; }   // 0.4.0: the products for linear layers
 
 int ozk_device_status(int clear, int *status_out, void *stream) {
     if (!status_out) return OZK_ERR_NULL;

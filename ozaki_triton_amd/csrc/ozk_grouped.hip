@@ -147,7 +147,8 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void grouped_kernel(Grou
     const int64_t kb = p.b_padded ? (p.K + 7) / 8 * 16 : p.K * 2;
     TileSrc A = {p.A + lo * p.a_pitch, p.a_pitch, rows, none ? 0 : ka, p.A};
     const char *Bg = p.B + (none ? 0 : seg - 1) * p.b_group;
-    TileSrc B = Sh::BCOLS ? TileSrc{Bg + n0 * 2, p.b_pitch, p.b_padded ? (cols + 7) / 8 * 16 : cols * 2, none ? 0 : p.K, p.B}
+    const int row = p.b_padded ? (cols + 7) / 8 * 16 : cols * 2;   // bytes, B along N
+    TileSrc B = Sh::BCOLS ? TileSrc{Bg + n0 * 2, p.b_pitch, row, none ? 0 : p.K, p.B}
                           : TileSrc{Bg + n0 * p.b_pitch, p.b_pitch, cols, none ? 0 : kb, p.B};
     if (!t.run(A, B, smem)) return;
 
@@ -470,7 +471,8 @@ hipError_t launch_grouped(const GroupedParams &p, int dtype, hipStream_t st) {
 PackedSizes plan_grouped_pack(const GroupedParams &p) {
     const bool a = !a_pieces(p), b = p.G > 0 && !b_pieces(p);
     const int64_t b_rows = p.b_cols ? p.K : p.N, b_len = p.b_cols ? p.N : p.K;
-    if ((!a && !b) || p.T == 0 || p.K == 0 || p.N == 0 || !packable(p.T, p.K) || !packable(p.G * b_rows, b_len))
+    if ((!a && !b) || p.T == 0 || p.K == 0 || p.N == 0 || !packable(p.T, p.K) ||
+        !packable(p.G * b_rows, b_len))
         return {0, 0};
     const double cost = 1e-12 * ((a ? (double)p.T * p.K : 0) + (b ? (double)p.G * p.K * p.N : 0)) + 5e-6;
     const int64_t groups = p.G < 1 ? 1 : p.G < p.T ? p.G : p.T;
@@ -483,7 +485,9 @@ PackedSizes plan_grouped_pack(const GroupedParams &p) {
 PackedSizes plan_grad_pack(const GroupedGradParams &p) {
     const bool a = !whole_pieces(p.A, p.a_pitch, 0, p.K, p.a_padded);
     const bool d = !whole_pieces(p.D, p.d_pitch, 0, p.N, p.d_padded);
-    if ((!a && !d) || p.T == 0 || p.K == 0 || p.N == 0 || p.G == 0 || !packable(p.T, p.K) || !packable(p.T, p.N)) return {0, 0};
+    if ((!a && !d) || p.T == 0 || p.K == 0 || p.N == 0 || p.G == 0 || !packable(p.T, p.K) ||
+        !packable(p.T, p.N))
+        return {0, 0};
     const double cost = 1e-12 * p.T * ((a ? (double)p.K : 0) + (d ? (double)p.N : 0)) + 5e-6;
     const double tiles = ((double)p.K / 128 + 1) * ((double)p.N / 128 + 1) * p.G / 1024;
     if (3e-6 * (tiles > 1 ? tiles : 1) * p.T / (64.0 * p.G * p.splits) < cost) return {0, 0};

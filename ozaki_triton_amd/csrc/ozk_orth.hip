@@ -41,16 +41,44 @@ OZK_DEV double block_sum(double v) {   // of 256 lanes, in every lane
     return part[0] + part[1] + part[2] + part[3];
 }
 
+// 16 bytes of a row
+template <typename T> struct OrthPiece {
+    static constexpr int E = 16 / (int)sizeof(T);
+    i32x4 raw;
+    OZK_DEV float at(int e) const {
+        if constexpr (sizeof(T) == 4) return __int_as_float(raw[e]);
+        else return from_bits16((uint16_t)((uint32_t)raw[e / 2] >> (16 * (e & 1))), T{});
+    }
+};
+template <typename T> OZK_DEV bool orth_wide(const OrthParams &p, const char *G) {
+    return (((uintptr_t)G | (uintptr_t)(p.g_row * (int64_t)sizeof(T))) & 15) == 0;
+}
+
 // Sums of squares, in fp64 (no overflow, whatever the gradient's scale), of
-// the rows blockIdx.x, + blocks, .. of matrix blockIdx.y
+// the rows blockIdx.x, + blocks, .. of matrix blockIdx.y.  Bound by its loads,
+// 16 bytes a lane where the rows allow (2048 x 8192 bf16: 9 us, 19 one by one)
 template <typename T> __global__ __launch_bounds__(256) void orth_norm_kernel(OrthParams p) {
     const char *G = p.G + (int64_t)blockIdx.y * p.g_batch * (int64_t)sizeof(T);
     double sum = 0.0;
-    for (int64_t r = blockIdx.x; r < p.M; r += p.blocks)
-        for (int64_t c = threadIdx.x; c < p.N; c += 256) {
-            const double v = orth_load<T>(G, r * p.g_row + c);
+    constexpr int E = OrthPiece<T>::E;
+    const int64_t whole = orth_wide<T>(p, G) ? p.N / E : 0;   // pieces of a row
+    for (int64_t r = blockIdx.x; r < p.M; r += p.blocks) {
+        const char *row = G + r * p.g_row * (int64_t)sizeof(T);
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < whole; i += 256) {
+            OrthPiece<T> x;
+            x.raw = *(const i32x4 *)(row + i * 16);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const double v = x.at(e);
+                sum += v * v;
+            }
+        }
+        for (int64_t c = whole * E + threadIdx.x; c < p.N; c += 256) {
+            const double v = orth_load<T>(row, c);
             sum += v * v;
         }
+    }
     sum = block_sum(sum);
     if (threadIdx.x == 0) p.sums[(int64_t)blockIdx.y * p.blocks + blockIdx.x] = sum;
 }
@@ -62,29 +90,70 @@ OZK_DEV void put_slices(char *at, float v) {
     *(_Float16 *)(at + 64) = l;
 }
 
-// X0's slices, 32 columns x 64 rows of X a workgroup, transposed through the
-// LDS where M > N
+// X0's slices, 32 columns x 64 rows of X a workgroup: 8 columns a lane where G's
+// rows are X's and allow wide loads (2048 x 8192 bf16: 25 us, 38 one by one),
+// else through the LDS, which transposes them where M > N.  G is on its way while
+// the partial sums are added.
 template <typename T> __global__ __launch_bounds__(256) void orth_start_kernel(OrthParams p) {
     const bool flip = p.M > p.N;
     const int64_t m = flip ? p.N : p.M, n = flip ? p.M : p.N;
     const int64_t b = blockIdx.z, r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 32;
+    const char *G = p.G + b * p.g_batch * (int64_t)sizeof(T);
+    char *X = p.X[0] + b * m * slice_pitch(n);
+    const bool wide = !flip && orth_wide<T>(p, G) && c0 + 32 <= n;
+
+    __shared__ float tile[64][33];
+    float v[8];
+    if (wide) {
+        const int64_t row = r0 + threadIdx.x / 4;
+        constexpr int E = OrthPiece<T>::E;
+        OrthPiece<T> x[8 / E] = {};
+        if (row < m)
+#pragma unroll
+            for (int i = 0; i < 8 / E; ++i)
+                x[i].raw = *(const i32x4 *)(G + (row * p.g_row + c0 + threadIdx.x % 4 * 8 + i * E) *
+                                                    (int64_t)sizeof(T));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = x[e / E].at(e % E);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            // consecutive lanes along G's rows
+            const int r = flip ? threadIdx.x % 64 : threadIdx.x / 32 + 8 * q;
+            const int c = flip ? threadIdx.x / 64 + 4 * q : threadIdx.x % 32;
+            const int64_t row = r0 + r, col = c0 + c;
+            v[q] = 0.f;
+            if (row < m && col < n) v[q] = orth_load<T>(G, flip ? col * p.g_row + row : row * p.g_row + col);
+        }
+    }
     double sum = 0.0;
     for (int i = threadIdx.x; i < p.blocks; i += 256) sum += p.sums[b * p.blocks + i];
     const double f = (double)p.start_scale / (sqrt(block_sum(sum)) + p.eps);
-    const char *G = p.G + b * p.g_batch * (int64_t)sizeof(T);
-    char *X = p.X[0] + b * m * slice_pitch(n);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = (float)((double)v[q] * f);
 
-    __shared__ float tile[64][33];
+    if (wide) {
+        const int64_t row = r0 + threadIdx.x / 4;
+        if (row >= m) return;
+        _Float16 h[8], l[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            h[e] = (_Float16)v[e];
+            l[e] = (_Float16)(v[e] - (float)h[e]);
+        }
+        i32x4 u[2];
+        __builtin_memcpy(&u[0], h, 16);
+        __builtin_memcpy(&u[1], l, 16);
+        char *to = X + row * slice_pitch(n) + c0 * 4 + threadIdx.x % 4 * 16;
+        *(i32x4 *)to = u[0];
+        *(i32x4 *)(to + 64) = u[1];
+        return;
+    }
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-        // consecutive lanes along G's rows
         const int r = flip ? threadIdx.x % 64 : threadIdx.x / 32 + 8 * q;
         const int c = flip ? threadIdx.x / 64 + 4 * q : threadIdx.x % 32;
-        const int64_t row = r0 + r, col = c0 + c;
-        float v = 0.f;
-        if (row < m && col < n)
-            v = (float)((double)orth_load<T>(G, flip ? col * p.g_row + row : row * p.g_row + col) * f);
-        tile[r][c] = v;
+        tile[r][c] = v[q];
     }
     __syncthreads();
 #pragma unroll
@@ -167,7 +236,8 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
     TileLoop<_Float16, Sh, true> t;
     const char *L = p.L + (int64_t)b * p.l_batch, *R = p.R + (int64_t)b * p.r_batch;
     const TileSrc A = {L + m0 * lp, lp, rows, lp, L};
-    const TileSrc B = Sh::BCOLS ? TileSrc{R + n0 * 4, rp, (int)(rp - n0 * 4 < BN * 4 ? rp - n0 * 4 : BN * 4), p.m, R}
+    const int row = (int)(rp - n0 * 4 < BN * 4 ? rp - n0 * 4 : BN * 4);
+    const TileSrc B = Sh::BCOLS ? TileSrc{R + n0 * 4, rp, row, p.m, R}
                                 : TileSrc{R + n0 * rp, rp, cols, rp, R};
     if (!t.run(A, B, smem)) return;
 
@@ -381,8 +451,10 @@ hipError_t orth_run(const OrthParams &p, const OrthPlan &plan, hipStream_t st) {
 
 }  // namespace
 
+// Partial sums of a matrix; each workgroup of the next kernel adds all of them
+// (2048 x 8192 bf16: with 2048 of them it takes 32 us, with 512 25)
 int orth_blocks(int64_t batch, int64_t M, int64_t N) {
-    int64_t b = 2048 / (batch > 0 ? batch : 1);
+    int64_t b = 512 / (batch > 0 ? batch : 1);
     if (b > M) b = M;
     if (b > M * N / 1024) b = M * N / 1024;
     return (int)(b < 1 ? 1 : b);
