@@ -145,14 +145,18 @@ template <int S, bool COLS, int BX> OZK_DEV WindowAt window_at(const TileSrc &s,
 // assembly because behind the builtin the compiler waits for every DMA on its
 // way before a ds_read_b64_tr_b16 (measured: 1028 us against 815 without the
 // read-ahead below, 32768 x 2048 x 4096).  It has no register result; its LDS
-// writes are waited for by wait_vmcnt and a barrier like the builtin's.
+// writes are waited for by wait_vmcnt and a barrier like the builtin's.  Nor
+// does the compiler see that it reads the descriptor: a vector-memory
+// instruction may do so from five wait states after a vector instruction wrote
+// it on, and a v_readfirstlane can stand right before this block, so the five
+// are in it: the addition, which m0 needs too, and the s_nop.
 template <int PLUS> OZK_DEV void dma_piece(const char *base, uint32_t off, uint32_t to) {
     const uint64_t at = (uint64_t)(uintptr_t)base;
     const i32x4 desc = {uniform((int)(uint32_t)at), uniform((int)(uint32_t)(at >> 32)), 0x7FFFFFFF,
                         0x00020000};
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"   // m0 holds nothing else in these kernels
-    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(uniform((int)to)), "v"(off), "s"(desc), "n"(PLUS)
                  : "memory", "m0", "scc");
@@ -244,6 +248,11 @@ template <typename ST, typename Sh, bool DMA> struct TileLoop {
             fb.base += kw * fb.step;
             fa.step *= Sh::KW;
             fb.step *= Sh::KW;
+        }
+        // in scalar registers from here on, not moved there for every window
+        for (Feed *f : {&fa, &fb}) {
+            f->base = (const char *)uniform((int64_t)(uintptr_t)f->base);
+            f->step = uniform(f->step);
         }
         const bool onlyA = Sh::ONE && wave * LP < Sh::BM / 8;
         Feed feed[Sh::ONE ? 1 : 2];
