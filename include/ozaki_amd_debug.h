@@ -108,6 +108,17 @@ int ozk_debug_matmul_workspace(int dtype, int64_t batch, int64_t M, int64_t N, i
                                const int64_t a_strides[3], const int64_t b_strides[3],
                                int num_splits, int slice_dtype, size_t have, size_t *bytes_out);
 
+/*
+ * The products that ozk_orthogonalize would run for matrices of m x n (or
+ * n x m), m <= n, in order: *ops of them, at most 256.  Of each five of
+ * buffers[], kind, L, R, Y, D, and three of factors[], f, f_y, f_i: D = f L R +
+ * f_y Y + f_i I (kind 0: R transposed) of the slices as they are, D rounded to
+ * slices but for kind 3, the result.  Buffers 0 to 4 are square, -1 and -2 of
+ * X's size, -9 none; -1 starts as G / (|G| + eps) times *start_scale.
+ */
+int ozk_debug_orth_plan(int64_t m, int64_t n, const double *coefficients, int steps, int dtype,
+                        int *buffers, float *factors, float *start_scale, int *ops);
+
 #ifdef __cplusplus
 }
 #endif

@@ -67,6 +67,7 @@ EXPORTED_DEBUG = (
     "ozk_debug_gemm_kernel_out",
     "ozk_debug_split_kernel",
     "ozk_debug_matmul_workspace",
+    "ozk_debug_orth_plan",
 )
 
 _lib = None
@@ -144,6 +145,9 @@ def load() -> ctypes.CDLL:
                                    vp, sz, vp])):
         fn = getattr(L, name)
         fn.argtypes, fn.restype = args, i32
+    pi, pf = ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_float)
+    L.ozk_debug_orth_plan.argtypes = [i64, i64, pd, i32, i32, pi, pf, pf, pi]
+    L.ozk_debug_orth_plan.restype = i32
     cp = ctypes.c_char_p
     L.ozk_debug_force_gemm_kernel.argtypes = [cp]
     L.ozk_debug_force_gemm_kernel.restype = i32

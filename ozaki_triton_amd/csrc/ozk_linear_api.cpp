@@ -7,6 +7,7 @@
 #include <initializer_list>
 
 #include "../../include/ozaki_amd.h"
+#include "../../include/ozaki_amd_debug.h"
 #include "ozk_linear.h"
 
 namespace {
@@ -67,6 +68,8 @@ struct OrthBounds {
     double p;     // of P: |a + b t + c t^2|
     double w;     // of P A: the same times t
     double slope; // |b + 2 c t|
+    double gain;  // of an error in X: |a + b t + c t^2|, or |a + 3 b t + 5 c t^2| along s
+    OrthBounds() = default;
     OrthBounds(double a, double b_, double c, double top) {
         auto poly = [&](double t) { return a + b_ * t + c * t * t; };
         // where (a + b t + c t^2) t^k turns: k a + (k + 1) b t + (k + 2) c t^2 = 0
@@ -92,6 +95,45 @@ struct OrthBounds {
         n = turns(1, t);
         w = largest([&](double u) { return poly(u) * u; }, top, t, n);
         slope = largest([&](double u) { return b_ + 2 * c * u; }, top, t, 0);
+        t[0] = c != 0 ? -3 * b_ / (10 * c) : 0;
+        gain = largest([&](double u) { return a + 3 * b_ * u + 5 * c * u * u; }, top, t, 1);
+        if (p > gain) gain = p;
+    }
+};
+
+// Worst-case error of a result, to first order, from what the slices round:
+// 2^-22 of a matrix' bound, each time one is made.
+struct OrthErrors {
+    static constexpr double e = 0x1p-22;
+    const OrthBounds *at;
+    const double *bound;   // of X before each step
+    // Steps by themselves: an error d in X leaves a step as gain d, and the step
+    // adds what the slices of A, B and the new X round.
+    double own(int steps) const {
+        double d = e;
+        for (int i = 0; i < steps; ++i) {
+            const double top = bound[i] * bound[i];
+            d = at[i].gain * d + bound[i] * e * (at[i].slope * top + at[i].b) + e * bound[i + 1];
+        }
+        return d;
+    }
+    // The last j steps on A alone: with W = P A and A' = W P errors go from A to
+    // P by P's slope, from both to W and A', and from every P to Q.
+    double chain(int steps, int j) const {
+        const int from = steps - j;
+        double d = own(from), dA = e * bound[from] * bound[from], dP = 0, q = 1, dQ = 0;
+        for (int i = from; i < steps; ++i) {
+            d *= at[i].gain;
+            if (i > from) {
+                const OrthBounds &k = at[i - 1];
+                const double dW = k.p * dA + bound[i - 1] * bound[i - 1] * dP + e * k.w;
+                dA = k.p * dW + k.w * dP + e * bound[i] * bound[i];
+            }
+            dP = at[i].slope * dA + e * at[i].p;
+            dQ = at[i].p * dQ + q * dP + (i > from ? e * q * at[i].p : 0);
+            q *= at[i].p;
+        }
+        return d + dQ * bound[from];
     }
 };
 
@@ -107,30 +149,25 @@ bool chain_pays(int64_t m, int64_t n) { return n >= 2 * m; }   // see plan_orth
 // four symmetric products of [m, m]: less where n is at least 2 m (measured, a
 // step by itself / one of these, 2048 x 8192: 323 / 145 us, 2048 x 4096: 193 /
 // 145, 2048 x 2048: 120 / 145).  What it costs
-// is accuracy: an error of 2^-22 in A (its slices) is amplified by P^2 a step
-// and by P's slope at the end, and j is as large as keeps that worst case within
-// half a unit of a 16-bit result's rounding; for fp32 results every step runs by
-// itself (4 steps of 1.5, -0.5, 0 at 65 x 400 were 4.3e-7 off together, 8e-8 in
-// plain fp32).  Seen on random and on ill-conditioned (1e4) matrices, with the
-// coefficients 3.4445, -4.775, 2.0315: j = 2 1.8e-6, as j = 1, j = 3 2e-5, j = 4
-// 7e-5, against bounds of 1.4e-5, 1.6e-4 and 1.9e-3.
+// is accuracy: A's rounding is amplified by P^2 a step and by P's slope into
+// every P.  So j is the most whose worst case (OrthErrors) is within 1.5 times that
+// of the steps by themselves, and the result is as near as theirs.  With the
+// coefficients 3.4445, -4.775, 2.0315 that is 2 of 5 steps; error before the last
+// rounding on matrices of 64 x 200 with singular values over four decades, for j =
+// 1 .. 5: 3.7e-6, 3.7e-6, 6.4e-6, 3.7e-5, 7.7e-5 (plain fp32 4.6e-6).  For fp32
+// results every step runs by itself: products more of 22 bits show there (4 steps
+// of 1.5, -0.5, 0: 1.0e-7, with j = 2 1.6e-7).
 void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int steps, int dtype) {
-    double bound[65];
-    bound[0] = 1.0;
-    for (int i = 0; i < steps; ++i)
-        bound[i + 1] = OrthBounds(co[3 * i], co[3 * i + 1], co[3 * i + 2], bound[i] * bound[i]).x;
-    auto at = [&](int i) {
-        return OrthBounds(co[3 * i], co[3 * i + 1], co[3 * i + 2], bound[i] * bound[i]);
-    };
+    double bound[65] = {1.0};
+    OrthBounds at[64];
+    for (int i = 0; i < steps; ++i) {
+        at[i] = OrthBounds(co[3 * i], co[3 * i + 1], co[3 * i + 2], bound[i] * bound[i]);
+        bound[i + 1] = at[i].x;
+    }
     int j = 1;
     if (chain_pays(m, n) && dtype != OZK_F32) {
-        const double limit = dtype == OZK_BF16 ? 0x1p-9 : 0x1p-12;
-        double gain = 0x1p-22;
-        while (j < steps) {
-            gain *= at(steps - 1 - j).p * at(steps - 1 - j).p;
-            if (!(gain * at(steps - 1).slope <= limit)) break;
-            ++j;
-        }
+        const OrthErrors err = {at, bound};
+        while (j < steps && err.chain(steps, j + 1) <= 1.5 * err.own(steps)) ++j;
     }
     auto push = [&](int kind, int L, int R, int Y, int D, double f_acc, double f_y, double f_i) {
         plan.op[plan.ops++] = {kind, L, R, Y, D, (float)f_acc, (float)f_y, (float)f_i};
@@ -146,7 +183,7 @@ void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int 
     for (int i = 0; i < own; ++i) {
         const double a = co[3 * i], b = co[3 * i + 1], c = co[3 * i + 2];
         const bool last = i + 1 == steps;
-        const double sa = slice_scale(bound[i] * bound[i]), sb = slice_scale(at(i).b);
+        const double sa = slice_scale(bound[i] * bound[i]), sb = slice_scale(at[i].b);
         const double next = last ? 1.0 : slice_scale(bound[i + 1]);
         push(ozk::kOrthXX, x, x, none, 0, sa / (sx * sx), 0, 0);
         push(ozk::kOrthSym, 0, 0, 0, 1, c * sb / (sa * sa), b * sb / sa, 0);
@@ -162,12 +199,12 @@ void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int 
     for (int i = own; i < steps; ++i) {
         const double a = co[3 * i], b = co[3 * i + 1], c = co[3 * i + 2];
         if (i > own) {
-            const double sw = slice_scale(at(i - 1).w), na = slice_scale(bound[i] * bound[i]);
+            const double sw = slice_scale(at[i - 1].w), na = slice_scale(bound[i] * bound[i]);
             push(ozk::kOrthSym, P, 0, none, 2, sw / (sp * sa), 0, 0);
             push(ozk::kOrthSym, 2, P, none, 0, na / (sw * sp), 0, 0);
             sa = na;
         }
-        const OrthBounds k = at(i);
+        const OrthBounds &k = at[i];
         sp = slice_scale(k.p);
         all *= k.p;
         P = Q == 1 ? 3 : 1;
@@ -493,6 +530,23 @@ int ozk_orthogonalize(const void *G, int dtype, int64_t batch, int64_t M, int64_
     p.X[1] = p.X[0] + (plan.xs > 1 ? at.x : 0);
     for (int i = 0; i < ozk::kOrthSquares; ++i) p.S[i] = p.X[1] + at.x + i * at.a;
     return launched(ozk::launch_orth(p, plan, dtype, (hipStream_t)stream));
+}
+
+int ozk_debug_orth_plan(int64_t m, int64_t n, const double *coefficients, int steps, int dtype,
+                        int *buffers, float *factors, float *start_scale, int *ops) {
+    if (!coefficients || !buffers || !factors || !start_scale || !ops) return OZK_ERR_NULL;
+    if (!is_float(dtype)) return OZK_ERR_DTYPE;
+    if (m > n || steps < 1 || steps > 64) return OZK_ERR_SHAPE;
+    ozk::OrthPlan plan;
+    plan_orth(plan, m, n, coefficients, steps, dtype);
+    for (int i = 0; i < plan.ops; ++i) {
+        const ozk::OrthOp &op = plan.op[i];
+        for (int b : {op.kind, op.L, op.R, op.Y, op.D}) *buffers++ = b;
+        for (float f : {op.f_acc, op.f_y, op.f_i}) *factors++ = f;
+    }
+    *start_scale = plan.start_scale;
+    *ops = plan.ops;
+    return OZK_OK;
 }
 
 }  // extern "C"
