@@ -128,7 +128,8 @@ template <typename T> __global__ __launch_bounds__(256) void orth_start_kernel(O
     }
     double sum = 0.0;
     for (int i = threadIdx.x; i < p.blocks; i += 256) sum += p.sums[b * p.blocks + i];
-    const double f = (double)p.start_scale / (sqrt(block_sum(sum)) + p.eps);
+    const double norm = sqrt(block_sum(sum)) + p.eps;
+    const double f = norm == 0.0 ? 0.0 : (double)p.start_scale / norm;   // zero stays zero
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = (float)((double)v[q] * f);
 

@@ -37,3 +37,15 @@ def test_orthogonalize_long_rounds_like_fp32(triples, dtype):
         moved = lambda y: int((y.cpu() != want).sum())  # noqa: E731
         got, allowed = moved(ozk.orthogonalize(G, len(triples), triples)), 4 * moved(plain)
         assert got <= allowed + 5 * math.sqrt(allowed) + 5, (got, allowed)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+def test_orthogonalize_zero_matrix_without_eps(dtype):
+    """A zero matrix stays zero, also where nothing is added to its norm of 0."""
+    G = torch.randn(3, 40, 50, generator=_gen(1), device="cuda").to(dtype)
+    G[1] = 0
+    for g in (G, G.mT):
+        X = ozk.orthogonalize(g, eps=0.0)
+        assert not X[1].any()
+        assert all(torch.equal(X[i], ozk.orthogonalize(g[i], eps=0.0)) for i in (0, 2))
+        assert torch.isfinite(X).all()
