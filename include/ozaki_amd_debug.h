@@ -114,7 +114,11 @@ int ozk_debug_matmul_workspace(int dtype, int64_t batch, int64_t M, int64_t N, i
  * buffers[], kind, L, R, Y, D, and three of factors[], f, f_y, f_i: D = f L R +
  * f_y Y + f_i I (kind 0: R transposed) of the slices as they are, D rounded to
  * slices but for kind 3, the result.  Buffers 0 to 4 are square, -1 and -2 of
- * X's size, -9 none; -1 starts as G / (|G| + eps) times *start_scale.
+ * X's size, -9 none; -1 starts as G / (|G| + eps) times *start_scale.  Where the
+ * scales are measured there are kinds 4 and 5: D is rounded to slices of D / |D|
+ * times *start_scale, and |D| is then |B| (4) or |X| (5, 1 at the start); f of kind
+ * 4 is times |X|^4 and f_y times |X|^2, f of kinds 5 and 3 times |B| |X| and f_y
+ * times |X|.
  */
 int ozk_debug_orth_plan(int64_t m, int64_t n, const double *coefficients, int steps, int dtype,
                         int *buffers, float *factors, float *start_scale, int *ops);

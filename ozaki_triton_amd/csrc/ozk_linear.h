@@ -109,13 +109,17 @@ enum OrthKind {
     kOrthXX = 0,     // D [m, m] = X X^T
     kOrthSym = 1,    // D [m, m] symmetric, L and R symmetric and commuting
     kOrthX = 2,      // D [m, n], R and Y of X's size
-    kOrthLast = 3    // the same into the result
+    kOrthLast = 3,   // the same into the result
+    // where the scales are measured (OrthPlan): through fp32 values, their norm and
+    // slices of them over it
+    kOrthNewB = 4,   // D [m, m], of A
+    kOrthNewX = 5    // D [m, n], of B and X
 };
 constexpr int kOrthSquares = 5;   // [m, m] buffers
 struct OrthOp {
     int kind;
     int L, R, Y, D;          // buffers: 0 .. 4 square, -1 and -2 X's two, -9 none
-    float f_acc, f_y, f_i;   // scales of the slices included
+    float f_acc, f_y, f_i;   // scales of the slices included (not the measured ones)
 };
 constexpr int kOrthMaxOps = 4 * 64;
 struct OrthPlan {
@@ -123,6 +127,7 @@ struct OrthPlan {
     int ops;
     int squares, xs;         // buffers used
     float start_scale;       // of X's slices at the start, a power of two
+    bool measured;           // slices of X / |X|, of A / |X|^2 and of B / |B|, norms on the GPU
 };
 struct OrthParams {
     const char *G;
@@ -134,6 +139,7 @@ struct OrthParams {
     // workspace
     double *sums;                              // [batch, blocks] partial sums of squares
     int blocks;
+    double *norms;                             // [2, batch], |X| and |B| where measured, else null
     char *X[2], *S[kOrthSquares];              // slices
 };
 int orth_blocks(int64_t batch, int64_t M, int64_t N);

@@ -137,6 +137,10 @@ struct OrthErrors {
     }
 };
 
+// The slices' scales come from the bounds where each is within this: values of
+// order 1 then keep 22 bits (2^-25 of 2^14 / 2^10) in sums of up to 2^13 of them.
+constexpr double kOrthTight = 1024;
+
 bool chain_pays(int64_t m, int64_t n) { return n >= 2 * m; }   // see plan_orth
 
 // The products of an orthogonalisation (X [m, n], m <= n).
@@ -157,6 +161,13 @@ bool chain_pays(int64_t m, int64_t n) { return n >= 2 * m; }   // see plan_orth
 // 1 .. 5: 3.7e-6, 3.7e-6, 6.4e-6, 3.7e-5, 7.7e-5 (plain fp32 4.6e-6).  For fp32
 // results every step runs by itself: products more of 22 bits show there (4 steps
 // of 1.5, -0.5, 0: 1.0e-7, with j = 2 1.6e-7).
+//
+// The bounds are over whole intervals, each step's over all that the one before
+// may give, and can grow far past every value (published triples from 8.29, -23.6,
+// 17.3 to 1.875, -1.25, 0.375: to 1e89 in seven steps that take all of [0, 1] to
+// within 2; slices on that scale are zeros).  Where a bound is past kOrthTight, every
+// step runs by itself on scales that are measured: A of X / |X| has entries within
+// 1, and B and the next X are written as fp32 values first (two launches more each).
 void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int steps, int dtype) {
     double bound[65] = {1.0};
     OrthBounds at[64];
@@ -164,10 +175,16 @@ void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int 
         at[i] = OrthBounds(co[3 * i], co[3 * i + 1], co[3 * i + 2], bound[i] * bound[i]);
         bound[i + 1] = at[i].x;
     }
+    plan.measured = false;
+    for (int i = 0; i < steps; ++i)
+        if (!(bound[i] * bound[i] <= kOrthTight && at[i].b <= kOrthTight)) plan.measured = true;
     int j = 1;
-    if (chain_pays(m, n) && dtype != OZK_F32) {
+    if (chain_pays(m, n) && dtype != OZK_F32 && !plan.measured) {
         const OrthErrors err = {at, bound};
-        while (j < steps && err.chain(steps, j + 1) <= 1.5 * err.own(steps)) ++j;
+        double q = at[steps - 1].p;
+        while (j < steps && (q *= at[steps - 1 - j].p) <= kOrthTight &&
+               err.chain(steps, j + 1) <= 1.5 * err.own(steps))
+            ++j;
     }
     auto push = [&](int kind, int L, int R, int Y, int D, double f_acc, double f_y, double f_i) {
         plan.op[plan.ops++] = {kind, L, R, Y, D, (float)f_acc, (float)f_y, (float)f_i};
@@ -178,6 +195,18 @@ void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int 
     plan.xs = steps - j > 0 ? 2 : 1;
     double sx = slice_scale(1.0);
     plan.start_scale = (float)sx;
+    if (plan.measured) {
+        for (int i = 0; i < steps; ++i) {
+            const double a = co[3 * i], b = co[3 * i + 1], c = co[3 * i + 2];
+            const bool last = i + 1 == steps;
+            push(ozk::kOrthXX, -1, -1, none, 0, 1 / sx, 0, 0);
+            push(ozk::kOrthNewB, 0, 0, 0, 0, c / (sx * sx), b / sx, 0);
+            push(last ? ozk::kOrthLast : ozk::kOrthNewX, 0, -1, -1, last ? none : -1,
+                 1 / (sx * sx), a / sx, 0);
+        }
+        plan.squares = 2;                         // and one for B's fp32 values
+        return;
+    }
     int x = -1;                                   // X's buffer
     const int own = j > 1 ? steps - j : steps;    // steps by themselves
     for (int i = 0; i < own; ++i) {
@@ -223,15 +252,16 @@ void plan_orth(ozk::OrthPlan &plan, int64_t m, int64_t n, const double *co, int 
     push(ozk::kOrthLast, Q, x, none, none, 1.0 / (sq * sx), 0, 0);
 }
 
-// workspace of an orthogonalisation, in order: the partial sums, X (twice where
-// steps run by themselves), the square matrices.  The size covers every plan.
+// workspace of an orthogonalisation, in order: the partial sums and the norms of
+// X and B, X (twice where steps run by themselves), the square matrices.  The size covers every plan.
 struct OrthLayout {
-    size_t sums, x, a, total;
+    size_t norms, sums, x, a, total;
     int blocks;
     OrthLayout(int64_t batch, int64_t M, int64_t N, int xs, int squares) {
         const int64_t m = M < N ? M : N, n = M < N ? N : M;
         blocks = ozk::orth_blocks(batch, M, N);
-        sums = (size_t)round_up(batch * blocks * 8, 256);
+        norms = (size_t)(batch * blocks * 8);
+        sums = (size_t)round_up((int64_t)norms + 2 * batch * 8, 256);
         x = (size_t)(batch * m * ((n + 31) / 32 * 128));
         a = (size_t)(batch * m * ((m + 31) / 32 * 128));
         total = sums + xs * x + squares * a;
@@ -525,6 +555,7 @@ int ozk_orthogonalize(const void *G, int dtype, int64_t batch, int64_t M, int64_
     char *ws = (char *)workspace;
     p.sums = (double *)ws;
     p.blocks = at.blocks;
+    p.norms = plan.measured ? (double *)(ws + at.norms) : nullptr;
     p.start_scale = plan.start_scale;
     p.X[0] = ws + at.sums;
     p.X[1] = p.X[0] + (plan.xs > 1 ? at.x : 0);

@@ -10,7 +10,9 @@
 // result is 2.2e-6 off, as with fp32 products; with one fp16 slice 1.8e-3,
 // with bf16 matrices 2.3e-2.  The scales come from the host, which bounds the
 // singular values of X, A and B step by step from the coefficients, so no
-// entry leaves fp16's range.
+// entry leaves fp16's range.  Where these bounds grow far past what a matrix does,
+// its entries would keep few bits, or none: there B and X are written as fp32
+// values, and their slices are those of B / |B|_F and X / |X|_F.
 //
 // A and B are symmetric: only tiles on and below the diagonal are computed,
 // each stored twice.
@@ -94,7 +96,9 @@ OZK_DEV void put_slices(char *at, float v) {
 // rows are X's and allow wide loads (2048 x 8192 bf16: 25 us, 38 one by one),
 // else through the LDS, which transposes them where M > N.  G is on its way while
 // the partial sums are added.
-template <typename T> __global__ __launch_bounds__(256) void orth_start_kernel(OrthParams p) {
+// norm_out: takes the norm, or with `first` a 1 (X0's own, whose norm is 1).
+template <typename T>
+__global__ __launch_bounds__(256) void orth_start_kernel(OrthParams p, double *norm_out, bool first) {
     const bool flip = p.M > p.N;
     const int64_t m = flip ? p.N : p.M, n = flip ? p.M : p.N;
     const int64_t b = blockIdx.z, r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 32;
@@ -128,7 +132,9 @@ template <typename T> __global__ __launch_bounds__(256) void orth_start_kernel(O
     }
     double sum = 0.0;
     for (int i = threadIdx.x; i < p.blocks; i += 256) sum += p.sums[b * p.blocks + i];
-    const double norm = sqrt(block_sum(sum)) + p.eps;
+    const double root = sqrt(block_sum(sum)), norm = root + p.eps;
+    if (norm_out && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+        norm_out[b] = first ? 1.0 : root;
     const double f = norm == 0.0 ? 0.0 : (double)p.start_scale / norm;   // zero stays zero
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = (float)((double)v[q] * f);
@@ -171,6 +177,7 @@ struct OrthGemm {
     int64_t l_batch, r_batch, y_batch, d_batch;   // bytes
     int64_t d_row;               // kOrthLast: elements
     float f_acc, f_y, f_i;
+    const double *norm_x, *norm_b;   // kOrthLast: the slices' measured scales, or null
     int64_t tiles_m, tiles_n;
     uint32_t total;
     int flip;
@@ -248,6 +255,17 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
     char *D = p.D + (int64_t)b * p.d_batch;
     const int g = (threadIdx.x >> 4) & 3, q = threadIdx.x & 3;
     const bool diagonal = KIND == kOrthSym && tm == tn && p.f_i != 0.f;
+    float f_acc = p.f_acc, f_y = p.f_y;
+    if (KIND == kOrthLast && p.norm_x) {
+        const double x = p.norm_x[b];
+        if (p.norm_b) {        // of B and X, and of X
+            f_acc = (float)(f_acc * p.norm_b[b] * x);
+            f_y = (float)(f_y * x);
+        } else {               // of A twice, and of A
+            f_acc = (float)(f_acc * x * x * x * x);
+            f_y = (float)(f_y * x * x);
+        }
+    }
     // 32 columns at a time: a line of D's slices
     t.each_pair([&](int mi, int ni, f32x4 lo, f32x4 hi) {
         const int n32 = ni - 4 * g;
@@ -257,8 +275,8 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
         float v[2][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[0][e] = lo[e] * p.f_acc;
-            v[1][e] = hi[e] * p.f_acc;
+            v[0][e] = lo[e] * f_acc;
+            v[1][e] = hi[e] * f_acc;
         }
         if (KIND != kOrthXX && Y) {
             i32x4 y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -275,7 +293,7 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void orth_gemm_kernel(Or
                 __builtin_memcpy(hv, &h[u], 8);
                 __builtin_memcpy(lv, &l[u], 8);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[u][e] += ((float)hv[e] + (float)lv[e]) * p.f_y;
+                for (int e = 0; e < 4; ++e) v[u][e] += ((float)hv[e] + (float)lv[e]) * f_y;
             }
         }
         if (diagonal)
@@ -410,15 +428,45 @@ hipError_t orth_product(const OrthGemm &q, int64_t batch, hipStream_t st) {
     return orth_gemm<T, KIND, 64, 2, 2, 4, 2>(q, batch, st);
 }
 
+// p.G's slices over its norm into p.X[0]
+template <typename T>
+hipError_t orth_slices(const OrthParams &p, double *norm_out, bool first, hipStream_t st) {
+    const int64_t m = p.M > p.N ? p.N : p.M, n = p.M > p.N ? p.M : p.N;
+    orth_norm_kernel<T><<<dim3((uint32_t)p.blocks, (uint32_t)p.batch), 256, 0, st>>>(p);
+    orth_start_kernel<T><<<dim3((uint32_t)((n + 31) / 32), (uint32_t)((m + 63) / 64),
+                                (uint32_t)p.batch), 256, 0, st>>>(p, norm_out, first);
+    return hipGetLastError();
+}
+
+// A product into `fp32` [m, n], and from there its slices over its norm, which
+// goes to norm_out, into `to`.  (The partial sums have room: orth_blocks grows
+// with either side.)
+hipError_t orth_measured(const OrthParams &p, OrthGemm q, char *fp32, char *to, double *norm_out,
+                         hipStream_t st) {
+    q.flip = 0;
+    q.D = fp32;
+    q.d_batch = q.m * slice_pitch(q.n);
+    q.d_row = slice_pitch(q.n) / 4;
+    if (hipError_t e = orth_product<float, kOrthLast>(q, p.batch, st); e != hipSuccess) return e;
+    OrthParams s = p;
+    s.G = fp32;
+    s.M = q.m;
+    s.N = q.n;
+    s.g_batch = q.d_batch / 4;
+    s.g_row = q.d_row;
+    s.eps = 0;
+    s.blocks = orth_blocks(p.batch, q.m, q.n);
+    s.X[0] = to;
+    return orth_slices<float>(s, norm_out, false, st);
+}
+
 template <typename T>
 hipError_t orth_run(const OrthParams &p, const OrthPlan &plan, hipStream_t st) {
     const bool flip = p.M > p.N;
     const int64_t m = flip ? p.N : p.M, n = flip ? p.M : p.N;
     const int64_t xb = m * slice_pitch(n), ab = m * slice_pitch(m);
-    orth_norm_kernel<T><<<dim3((uint32_t)p.blocks, (uint32_t)p.batch), 256, 0, st>>>(p);
-    orth_start_kernel<T><<<dim3((uint32_t)((n + 31) / 32), (uint32_t)((m + 63) / 64),
-                                (uint32_t)p.batch), 256, 0, st>>>(p);
-    hipError_t e = hipGetLastError();
+    double *norm_x = p.norms, *norm_b = p.norms ? p.norms + p.batch : nullptr;
+    hipError_t e = orth_slices<T>(p, norm_x, true, st);
     auto buffer = [&](int id, int64_t &bytes) -> char * {
         bytes = id >= 0 ? ab : xb;
         return id >= 0 ? p.S[id] : id >= -2 ? p.X[-1 - id] : nullptr;
@@ -433,6 +481,8 @@ hipError_t orth_run(const OrthParams &p, const OrthPlan &plan, hipStream_t st) {
         q.f_acc = op.f_acc;
         q.f_y = op.f_y;
         q.f_i = op.f_i;
+        q.norm_x = norm_x;
+        q.norm_b = norm_b;
         q.L = buffer(op.L, q.l_batch);
         q.R = buffer(op.R, q.r_batch);
         q.Y = buffer(op.Y, q.y_batch);
@@ -441,6 +491,12 @@ hipError_t orth_run(const OrthParams &p, const OrthPlan &plan, hipStream_t st) {
         case kOrthXX: e = orth_product<T, kOrthXX>(q, p.batch, st); break;
         case kOrthSym: e = orth_product<T, kOrthSym>(q, p.batch, st); break;
         case kOrthX: e = orth_product<T, kOrthX>(q, p.batch, st); break;
+        case kOrthNewB:
+            q.n = m;
+            q.norm_b = nullptr;
+            e = orth_measured(p, q, p.S[1], q.D, norm_b, st);
+            break;
+        case kOrthNewX: e = orth_measured(p, q, p.X[1], q.D, norm_x, st); break;
         default:
             q.D = p.out;
             q.d_batch = p.o_batch * (int64_t)sizeof(T);

@@ -5,7 +5,8 @@ import math
 
 import pytest
 import torch
-from test_gpu_linear import BF, COEFFICIENTS, F16, F32, _gen, _steps
+from test_gpu_linear import BF, COEFFICIENTS, F16, F32, ROUND, _check_orth, _gen, _randn, _steps
+from test_orthogonalize_plan import OVERSHOOTING, STANDARD
 
 import ozaki_triton_amd as ozk
 
@@ -37,6 +38,53 @@ def test_orthogonalize_long_rounds_like_fp32(triples, dtype):
         moved = lambda y: int((y.cpu() != want).sum())  # noqa: E731
         got, allowed = moved(ozk.orthogonalize(G, len(triples), triples)), 4 * moved(plain)
         assert got <= allowed + 5 * math.sqrt(allowed) + 5, (got, allowed)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("triples", [OVERSHOOTING, [(40.0, -30.0, 10.0)] * 2, [(9.0, 2e3, -3e3)],
+                                     [STANDARD, (1e-3, 0.0, 0.0), (900.0, -4e8, 0.0)]])
+def test_orthogonalize_bounds_that_no_matrix_reaches(triples, dtype):
+    """Schedules whose bound on the singular values grows far past the matrices' own."""
+    for shape in ((64, 200), (96, 160), (160, 96), (256, 512), (3, 65, 40), (2, 3, 40, 24), (700, 1100)):
+        G = _randn(1, *shape, dtype=dtype)
+        want = _steps(G.cpu().double(), triples, 1e-7, torch.float64)
+        if bool((want.abs() < torch.finfo(dtype).max).all()):
+            _check_orth(G, len(triples), triples)
+            continue
+        # entries past the type's range become infinities, the others are held to the same
+        got = ozk.orthogonalize(G, len(triples), triples).cpu()
+        inside = want.abs() < torch.finfo(dtype).max * 0.999
+        assert bool((got == want.to(dtype))[want.abs() > torch.finfo(dtype).max * 1.001].all())
+        off = lambda y: float((y.double() - want)[inside].norm() / want[inside].norm())  # noqa: E731
+        plain = _steps(G.cpu().float(), triples, 1e-7, F32)
+        assert off(got) <= 4 * max(off(plain), 2.0 ** -24) + ROUND[dtype]
+
+
+def test_orthogonalize_measured_scales_are_each_matrix_own():
+    """Matrices of a batch beside a zero one, one with a NaN and one of rank 1 (all of
+    its norm in one value) are what they are alone; a schedule that diverges gives no
+    finite value."""
+    G = _randn(1, 5, 64, 80, dtype=F32)
+    G[1], G[2, 3, 4], G[4] = 0, math.nan, _randn(2, 64, 1, dtype=F32) * _randn(3, 80, dtype=F32)
+    X = ozk.orthogonalize(G, 7, OVERSHOOTING)
+    assert not X[1].any() and X[2].isnan().all()
+    for i in (0, 3, 4):
+        assert torch.equal(X[i], _check_orth(G[i], 7, OVERSHOOTING)) and torch.isfinite(X[i]).all()
+    assert not torch.isfinite(ozk.orthogonalize(G[0], 6, (40.0, -30.0, 10.0))).any()
+
+
+def test_orthogonalize_measured_scales_in_a_graph():
+    G = _randn(1, 2, 100, 160)
+    graph = torch.cuda.CUDAGraph()
+    ozk.orthogonalize(G, 7, OVERSHOOTING)
+    with torch.cuda.graph(graph):
+        got = ozk.orthogonalize(G, 7, OVERSHOOTING)
+    for n in range(3):
+        G.copy_(_randn(2 + n, 2, 100, 160))
+        want = ozk.orthogonalize(G, 7, OVERSHOOTING)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF, F16])
