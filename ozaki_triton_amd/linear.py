@@ -92,11 +92,28 @@ def _workspace(nbytes: int, dev: torch.device):
     return ws, ws.data_ptr()
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t with its last dim contiguous and its rows as far apart as the kernels take."""
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-2) < _MAX_STRIDE:
-        return t
-    return t.contiguous()
+def _rows(t: torch.Tensor):
+    """t [rows, columns] with its columns contiguous, and its rows' distance, which
+    the kernels take up to a limit.  (Strides of dims of size 1 mean nothing, to
+    contiguous() either: one row of a longer tensor keeps the distance of its rows.)"""
+    if t.shape[0] <= 1 and (t.stride(1) == 1 or t.shape[1] <= 1):
+        return t, 0
+    if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) < _MAX_STRIDE:
+        return t, t.stride(0)
+    return t.contiguous(), t.shape[1]
+
+
+def _matrices(t: torch.Tensor):
+    """t [groups, K, N] with K or N contiguous, and its strides, one of K and N 1 and
+    the other within the kernels' limit.  Strides of dims of size 1 as in _rows."""
+    (G, K, N), (s_g, s_k, s_n) = t.shape, t.stride()
+    if G <= 1:
+        s_g = 0
+    if (s_n == 1 or N == 1) and (s_k < _MAX_STRIDE or K <= 1):
+        return t, (s_g, s_k if K > 1 else 0, 1)
+    if (s_k == 1 or K == 1) and (s_n < _MAX_STRIDE or N <= 1):
+        return t, (s_g, 1, s_n if N > 1 else 0)
+    return t.contiguous(), (K * N, N, 1)
 
 
 # ============================================================
@@ -127,12 +144,11 @@ def _grouped_forward(A, B, offsets):
     G, _, N = B.shape
     dtype, dev = A.dtype, A.device
     sa, sb = A.stride(), B.stride()
-    if sa[1] != 1 or sa[0] >= _MAX_STRIDE:
-        A = _rows(A)
-        sa = A.stride()
+    pitch = sa[0]
+    if sa[1] != 1 or pitch >= _MAX_STRIDE:
+        A, pitch = _rows(A)
     if not ((sb[2] == 1 and sb[1] < _MAX_STRIDE) or (sb[1] == 1 and sb[2] < _MAX_STRIDE)):
-        B = B.contiguous()
-        sb = B.stride()
+        B, sb = _matrices(B)
     if offsets.stride(0) != 1:
         offsets = offsets.contiguous()
     C = A.new_empty((T, N))
@@ -140,10 +156,10 @@ def _grouped_forward(A, B, offsets):
     ws = wsp = None
     n = 0
     # whole 16-byte pieces need no workspace: most calls spare the query
-    if (ap | bp | (sa[0] | sb[0] | sb[1] * sb[2] | K | N) * 2) & 15:
-        n = _bytes("ozk_grouped_matmul_workspace_bytes", ap & 15, sa[0], bp & 15, sb, T, K, N, G)
+    if (ap | bp | (pitch | sb[0] | sb[1] * sb[2] | K | N) * 2) & 15:
+        n = _bytes("ozk_grouped_matmul_workspace_bytes", ap & 15, pitch, bp & 15, sb, T, K, N, G)
         ws, wsp = _workspace(n, dev)
-    _call("ozk_grouped_matmul", dev, ap, sa[0], bp, _i64(*sb), offsets.data_ptr(),
+    _call("ozk_grouped_matmul", dev, ap, pitch, bp, _i64(*sb), offsets.data_ptr(),
           offsets.element_size(), T, K, N, G, _TORCH_TO_OZK[dtype], C.data_ptr(), N, wsp, n)
     del ws
     return C
@@ -152,12 +168,12 @@ def _grouped_forward(A, B, offsets):
 def _grouped_wgrad(A, D, offsets, G):
     T, K = A.shape
     N = D.shape[1]
-    A, D = _rows(A), _rows(D)
+    (A, sa), (D, sd) = _rows(A), _rows(D)
     if offsets.stride(0) != 1:
         offsets = offsets.contiguous()
     dtype, dev = A.dtype, A.device
     dB = A.new_empty((G, K, N))
-    ap, dp, sa, sd = A.data_ptr(), D.data_ptr(), A.stride(0), D.stride(0)
+    ap, dp = A.data_ptr(), D.data_ptr()
     n = _bytes("ozk_grouped_matmul_wgrad_workspace_bytes", ap & 15, sa, dp & 15, sd, T, K, N, G)
     ws, wsp = _workspace(n, dev)
     _call("ozk_grouped_matmul_wgrad", dev, ap, sa, dp, sd, offsets.data_ptr(),

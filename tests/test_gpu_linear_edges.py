@@ -5,7 +5,8 @@ import math
 
 import pytest
 import torch
-from test_gpu_linear import BF, COEFFICIENTS, F16, F32, ROUND, _check_orth, _gen, _randn, _steps
+from test_gpu_linear import (BF, COEFFICIENTS, F16, F32, ROUND, _check_grouped, _check_orth, _gen,
+                             _offsets, _randn, _steps)
 from test_orthogonalize_plan import OVERSHOOTING, STANDARD
 
 import ozaki_triton_amd as ozk
@@ -97,3 +98,26 @@ def test_orthogonalize_zero_matrix_without_eps(dtype):
         assert not X[1].any()
         assert all(torch.equal(X[i], ozk.orthogonalize(g[i], eps=0.0)) for i in (0, 2))
         assert torch.isfinite(X).all()
+
+
+# ---------------------------------------------------------------------------
+# grouped products
+# ---------------------------------------------------------------------------
+
+def test_grouped_single_rows_of_longer_tensors():
+    """The last token of one sequence, a matrix with one row or one column: their strides
+    are those of what they were cut from, past the kernels' limit."""
+    h, d = _randn(1, 1, 2048, 4096), _randn(2, 1, 40000, 136)
+    last, grad, B = h[:, -1], d[:, -1], _randn(3, 1, 4096, 136)
+    assert last.stride(0) >= 1 << 22 and grad.stride(0) >= 1 << 22 and last.is_contiguous()
+    offsets = _offsets([1])
+    _check_grouped(last, B, grad, offsets)
+    far = torch.zeros(1, 8, (1 << 22) + 24, dtype=BF, device="cuda")
+    far[:, :, :64] = _randn(4, 1, 8, 64)
+    A, D, offsets = _randn(5, 50, 8), _randn(6, 50, 64), _offsets([40])
+    _check_grouped(A[:, 3:4], far[:, 3:4, :64], D, offsets)                   # K = 1
+    _check_grouped(D, far[:, 3:4, :64].mT, A[:, 3:4], offsets)                # N = 1
+    _check_grouped(A, far[:, :, 5:6], D[:, 5:6], offsets)
+    _check_grouped(A[:, 3:4], far[:, 3:4, 5:6], D[:, 5:6], offsets)           # both
+    one = far[0, 3, 5].expand(1, 1, 1).as_strided((1, 1, 1), (7, 7, 7))
+    _check_grouped(A[:, 3:4], one, D[:, 5:6], offsets)

@@ -167,3 +167,28 @@ def test_orthogonalize_workspace_holds_the_chain(m, n, squares):
         for shape in ((m, n), (n, m)):   # and the partial sums of the norm
             got = _bytes("ozk_orthogonalize_workspace_bytes", batch, *shape, 5)
             assert want < got <= want + 64 * 1024
+
+
+def test_strides_of_single_rows_mean_nothing():
+    """A dim of size 1 keeps the stride of the tensor it was cut from, contiguous() leaves
+    it, and the kernels have a limit."""
+    from ozaki_triton_amd.linear import _MAX_STRIDE, _matrices, _rows
+    far = _MAX_STRIDE + 8
+    strided = lambda size, stride: torch.empty(1, dtype=BF).as_strided(  # noqa: E731
+        size, stride) if 0 in size or all(n == 1 for n in size) else \
+        torch.empty(sum((n - 1) * s for n, s in zip(size, stride)) + 1, dtype=BF).as_strided(size, stride)
+    for t in (strided((1, 64), (far, 1)), strided((1, 1), (far, far)), strided((0, 64), (far, 1)),
+              strided((3, 1), (2, far)), strided((1, 8), (far, 3)), strided((3, 8), (far, 1))):
+        r, pitch = _rows(t)
+        assert r.shape == t.shape and pitch < _MAX_STRIDE
+        assert r.shape[1] <= 1 or r.stride(1) == 1
+        assert r.shape[0] <= 1 or pitch == r.stride(0)
+    for size, stride in (((1, 1, 64), (far, far, 1)), ((1, 1, 1), (far, far, far)), ((1, 1, 1), (7, 7, 7)),
+                         ((1, 8, 1), (far, 1, far)), ((1, 8, 1), (far, 2, far)), ((1, 8, 1), (far, far, 1)),
+                         ((1, 1, 8), (far, far, 3)), ((2, 1, 8), (far, far, 1)), ((1, 4, 3), (far, 3, 1)),
+                         ((1, 4, 3), (far, 1, 4)), ((2, 4, 3), (2, 6, 2)), ((0, 4, 3), (far, far, far))):
+        t = strided(size, stride)
+        b, (s_g, s_k, s_n) = _matrices(t)
+        assert b.shape == t.shape and 1 in (s_k, s_n) and max(s_k, s_n) < _MAX_STRIDE
+        for dim, s in enumerate((s_g, s_k, s_n)):
+            assert b.shape[dim] <= 1 or b.numel() == 0 or s == b.stride(dim), (size, stride)
