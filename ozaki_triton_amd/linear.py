@@ -387,14 +387,14 @@ def orthogonalize(G: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750
     _on_one_gpu(G)
     _require_dtype("orthogonalize", G.dtype, _FLOAT)
     _no_grad("orthogonalize", G)
+    if G.numel() == 0:
+        return torch.empty_like(G, memory_format=torch.contiguous_format)
     M, N = G.shape[-2:]
     G3 = G if G.dim() == 3 else G.reshape(-1, M, N)
     if G3.stride(2) != 1 and N != 1:
         G3 = G3.contiguous()
     B, dev = G3.shape[0], G.device
     out = torch.empty((B, M, N), dtype=G.dtype, device=dev)
-    if out.numel() == 0:
-        return out.view(G.shape)
     n = _bytes("ozk_orthogonalize_workspace_bytes", B, M, N, steps)
     ws, wsp = _workspace(n, dev)
     flat = (ctypes.c_double * (3 * steps))(*[float(v) for t in triples for v in t])

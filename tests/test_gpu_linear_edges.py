@@ -100,6 +100,13 @@ def test_orthogonalize_zero_matrix_without_eps(dtype):
         assert torch.isfinite(X).all()
 
 
+@pytest.mark.parametrize("shape", [(0, 48), (48, 0), (0, 0), (2, 3, 0, 5), (2, 0, 4, 5), (0, 4, 5), (3, 4, 0)])
+def test_orthogonalize_empty(shape):
+    G = torch.zeros(shape, dtype=BF, device="cuda")
+    X = ozk.orthogonalize(G)
+    assert X.shape == shape and X.dtype == BF and X.data_ptr() == 0
+
+
 # ---------------------------------------------------------------------------
 # grouped products
 # ---------------------------------------------------------------------------
