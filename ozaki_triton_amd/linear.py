@@ -18,6 +18,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ozaki import _RAW_STREAM, _TORCH_TO_OZK, _require_gpu, _stream
@@ -48,6 +49,14 @@ def _on_one_gpu(a: torch.Tensor, *others) -> None:
         else:
             return
     _require_gpu(a, *(t for t in others if t is not None))
+
+
+def _no_tangent(name: str, *tensors) -> None:
+    """Forward-mode derivatives would be lost without a word: there are none here."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative: call it on primal tensors")
 
 
 _FUNCTIONS: dict = {}
@@ -209,9 +218,10 @@ def grouped_matmul(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor) -> t
                  offsets[groups] on belong to no group.
     Returns:
         C: (rows, N), dtype of A, summed in float32 and rounded once; zeros in the
-        rows of no group.  Differentiable in A and B.
+        rows of no group.  Differentiable in A and B (reverse mode, once).
     """
     _grouped_checks(A, B, offsets)
+    _no_tangent("grouped_matmul", A, B)
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad):
         return _GroupedMatmul.apply(A, B, offsets)
     return _grouped_forward(A, B, offsets)
@@ -228,6 +238,7 @@ def grouped_matmul_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
         f"dC must be {(A.shape[0], B.shape[2])}, got {tuple(dC.shape)}"
     assert dC.dtype == A.dtype, f"dC/A dtype mismatch: {dC.dtype} vs {A.dtype}"
     _on_one_gpu(dC, A)
+    _no_tangent("grouped_matmul_backward", dC, A, B)
     return _grouped_forward(dC, B.mT, offsets), _grouped_wgrad(A, dC, offsets, B.shape[0])
 
 
@@ -244,6 +255,7 @@ def _no_grad(name: str, *tensors) -> None:
             if t.requires_grad:
                 raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or on "
                                    "detached tensors")
+    _no_tangent(name, *tensors)
 
 
 def _w4_checks(packed, scales, zeros, group_size, K):

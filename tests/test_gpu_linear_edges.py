@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 from test_gpu_linear import (BF, COEFFICIENTS, F16, F32, ROUND, _check_grouped, _check_orth, _gen,
                              _offsets, _randn, _steps)
 from test_orthogonalize_plan import OVERSHOOTING, STANDARD
@@ -128,3 +129,23 @@ def test_grouped_single_rows_of_longer_tensors():
     _check_grouped(A[:, 3:4], far[:, 3:4, 5:6], D[:, 5:6], offsets)           # both
     one = far[0, 3, 5].expand(1, 1, 1).as_strided((1, 1, 1), (7, 7, 7))
     _check_grouped(A[:, 3:4], one, D[:, 5:6], offsets)
+
+
+def test_forward_mode_is_refused():
+    """A tangent is not dropped: none of the operators has a forward-mode derivative."""
+    A, B, D, offsets = _randn(1, 6, 32), _randn(2, 1, 32, 40), _randn(3, 6, 40), _offsets([6])
+    weights, G = ozk.quantize_w4(_randn(4, 40, 32), 32), _randn(5, 8, 16)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ozk.grouped_matmul(dual(A), B, offsets),
+                     lambda: ozk.grouped_matmul(A, dual(B), offsets),
+                     lambda: ozk.grouped_matmul_backward(dual(D), A, B, offsets),
+                     lambda: ozk.matmul_w4(dual(A), *weights, group_size=32),
+                     lambda: ozk.quantize_w4(dual(B[0].T), 32),
+                     lambda: ozk.orthogonalize(dual(G))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert torch.equal(ozk.grouped_matmul(A, B, offsets), ozk.grouped_matmul(A, B, offsets))
+    assert ozk.orthogonalize(G).shape == G.shape
