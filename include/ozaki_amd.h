@@ -298,8 +298,8 @@ int ozk_grouped_matmul_wgrad(const void *A, int64_t a_stride, const void *D, int
 
 /*
  * 4-bit weights: W[n, k] = (q[n, k] - z[n, k / group]) s[n, k / group].
- *   packed  [N] rows of packed_stride bytes, 16-byte aligned, at least K / 2
- *           rounded up to whole 16 bytes: q of 0 .. 15, k even in the low half
+ *   packed  [N] rows of K / 2 bytes, rounded up to whole 16 bytes, packed_stride
+ *           bytes apart, 16-byte aligned: q of 0 .. 15, k even in the low half
  *           of byte k / 2
  *   scales  [N, ceil(K / group)], rows s_stride apart
  *   zeros   the same of uint8 (0 .. 15), or NULL: z = 8

@@ -460,6 +460,9 @@ template <int CTRL> OZK_DEV void dpp_range(float &lo, float &hi) {
     hi = fmaxf(hi, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(hi), CTRL, 0xF, 0xF, true)));
 }
 
+// bytes of a packed row: those up to its distance are not the format's
+__host__ __device__ inline int64_t packed_bytes_of(int64_t K) { return (K + 31) / 32 * 16; }
+
 // 8 weights a lane: a group is 4, 8 or 16 lanes, a wave 512 weights of a row.
 // The divisions and roundings bound it (8192 x 8192 bf16: 64 us with v / s and
 // rint per weight), so a group divides once, y = fl(1 / s), and each quotient is
@@ -467,7 +470,8 @@ template <int CTRL> OZK_DEV void dpp_range(float &lo, float &hi) {
 // 1990: one correction of a quotient within a unit does where y is fl(1 / s));
 // adding 1.5 2^23 rounds it to a whole number, ties to even.
 template <typename T> __global__ __launch_bounds__(256) void quantize_w4_kernel(QuantParams p) {
-    const uint32_t per_row = (uint32_t)((p.p_pitch * 2 + 511) / 512);
+    const int64_t row_bytes = packed_bytes_of(p.K);
+    const uint32_t per_row = (uint32_t)((row_bytes * 2 + 511) / 512);
     const uint32_t part = blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int64_t n = part / per_row, k = (int64_t)(part - (uint32_t)n * per_row) * 512 + lane * 8;
@@ -524,7 +528,7 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_w4_kernel(
         store_value<T>(p.scales, n * p.s_pitch + g, s);
         if (p.zeros) p.zeros[n * p.z_pitch + g] = (uint8_t)(int)z;
     }
-    if (k / 2 < p.p_pitch) *(uint32_t *)(p.packed + n * p.p_pitch + k / 2) = word;
+    if (k / 2 < row_bytes) *(uint32_t *)(p.packed + n * p.p_pitch + k / 2) = word;
 }
 
 // 8 weights a lane, a wave 512 of a row; bound by its stores (8192 x 8192 bf16: 27 us, 6.3
@@ -662,7 +666,7 @@ hipError_t launch_w4(const W4Params &p, int dtype, hipStream_t st) {
 }
 
 hipError_t launch_quantize_w4(const QuantParams &p, int dtype, hipStream_t st) {
-    const int64_t parts = p.N * ((p.p_pitch * 2 + 511) / 512);
+    const int64_t parts = p.N * ((packed_bytes_of(p.K) * 2 + 511) / 512);
     const int64_t blocks = (parts + 3) / 4;
     if (parts >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
     auto *k = dtype == 1   ? quantize_w4_kernel<float>

@@ -149,3 +149,28 @@ def test_forward_mode_is_refused():
                 call()
         assert torch.equal(ozk.grouped_matmul(A, B, offsets), ozk.grouped_matmul(A, B, offsets))
     assert ozk.orthogonalize(G).shape == G.shape
+
+
+# ---------------------------------------------------------------------------
+# 4-bit weights
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("N, K, group", [(5, 33, 32), (3, 64, 64), (4, 1000, 128), (2, 513, 32)])
+def test_quantize_leaves_what_lies_between_its_rows(N, K, group):
+    """Packed rows, scales and zero points inside wider buffers (the C call): the bytes
+    between the rows, and those behind the last one, stay."""
+    lib, W = ozk.ozaki._lib, _randn(1, N, K, dtype=F32)
+    groups, width, stride, apart = -(-K // group), -(-K // 32) * 16, -(-K // 32) * 16 + 48, -(-K // group) + 3
+    packed = torch.full((N * stride + 512,), 0xA5, dtype=torch.uint8, device="cuda")
+    scales = torch.full((N * apart + 64,), -7.0, device="cuda")
+    zeros = torch.full((N * apart + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    lib.check("ozk_quantize_w4", lib.load().ozk_quantize_w4(
+        W.data_ptr(), lib.OZK_F32, N, K, K, group, packed.data_ptr(), stride, scales.data_ptr(), apart,
+        zeros.data_ptr(), apart, torch.cuda.current_stream().cuda_stream))
+    want = ozk.quantize_w4(W, group, zeros=True)
+    for got, columns, distance, w, other in ((packed, width, stride, want[0], 0xA5),
+                                             (scales, groups, apart, want[1], -7.0),
+                                             (zeros, groups, apart, want[2], 0xA5)):
+        rows = got[:N * distance].view(N, distance)
+        assert torch.equal(rows[:, :columns], w)
+        assert bool((rows[:, columns:] == other).all()) and bool((got[N * distance:] == other).all())
