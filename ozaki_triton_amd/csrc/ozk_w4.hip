@@ -14,6 +14,11 @@
 // against 3e-7 at K = 2048).  (A row of x with an
 // infinity gives NaN: the two sums cancel.)
 //
+// Both sums are up to 31 times the sum of |x|, so where x has fp32's exponents
+// they and all that follows are kept times 2^-12 until the result is stored:
+// 128 of 31 times the largest float then stay within it, and no finite x gives
+// NaN.  (Values of x below 2^-100 or so lose their last bits instead.)
+//
 // Few rows of x make this a read of the weights: they go straight from memory
 // to registers, 16 bytes (32 weights) of a row per lane, several loads ahead;
 // x waits in the LDS.
@@ -27,18 +32,22 @@ template <> struct W4Type<_Float16> { using M = _Float16; static constexpr int S
 template <> struct W4Type<__bf16> { using M = __bf16; static constexpr int SL = 1; };
 template <> struct W4Type<float> { using M = __bf16; static constexpr int SL = 3; };
 
-// the 8 weights of a word as 16 + q: element order 0, 4, 1, 5, 2, 6, 3, 7
+// what the sums are kept times
+template <typename M> constexpr float kW4Down = std::is_same<M, __bf16>::value ? 0x1p-12f : 1.f;
+
+// the 8 weights of a word as 16 + q, times kW4Down: element order 0, 4, 1, 5, 2, 6,
+// 3, 7
 OZK_DEV i32x4 unpack_w4(uint32_t w, _Float16) {   // q << 6 beside fp16's 16.0
     return i32x4{(int)(((w << 6) & 0x03C003C0u) | 0x4C004C00u),
                  (int)(((w << 2) & 0x03C003C0u) | 0x4C004C00u),
                  (int)(((w >> 2) & 0x03C003C0u) | 0x4C004C00u),
                  (int)(((w >> 6) & 0x03C003C0u) | 0x4C004C00u)};
 }
-OZK_DEV i32x4 unpack_w4(uint32_t w, __bf16) {     // q << 3 beside bf16's 16.0
-    return i32x4{(int)(((w << 3) & 0x00780078u) | 0x41804180u),
-                 (int)(((w >> 1) & 0x00780078u) | 0x41804180u),
-                 (int)(((w >> 5) & 0x00780078u) | 0x41804180u),
-                 (int)(((w >> 9) & 0x00780078u) | 0x41804180u)};
+OZK_DEV i32x4 unpack_w4(uint32_t w, __bf16) {     // q << 3 beside bf16's 2^-8
+    return i32x4{(int)(((w << 3) & 0x00780078u) | 0x3B803B80u),
+                 (int)(((w >> 1) & 0x00780078u) | 0x3B803B80u),
+                 (int)(((w >> 5) & 0x00780078u) | 0x3B803B80u),
+                 (int)(((w >> 9) & 0x00780078u) | 0x3B803B80u)};
 }
 
 // Lane group j's word i against lane group i's word j: lane group g held 32
@@ -238,7 +247,7 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_kernel(W4Params p) {
                 __builtin_memcpy(&u, o, 16);
                 if (i < all) *(i32x4 *)(smem + row * pitch + at * 16) = u;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum[0] += v[e];
+                for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(v[e], kW4Down<MT>, sum[0]);
             } else {
                 // 8, 8 and 8 bits of the 24: a slice is the upper half of what is left
 #pragma unroll
@@ -254,8 +263,8 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_kernel(W4Params p) {
                         const float h = __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
                         if (s + 1 < SL) v[e] -= h;
                         if (s == 0) {
-                            sum[0] += h;
-                            sum[AC - 1] += v[e];
+                            sum[0] = __builtin_fmaf(h, kW4Down<MT>, sum[0]);
+                            sum[AC - 1] = __builtin_fmaf(v[e], kW4Down<MT>, sum[AC - 1]);
                         }
                     }
                 }
@@ -411,9 +420,9 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_kernel(W4Params p) {
             for (int e = 0; e < 4; ++e) {
                 const int row = 16 * t + 4 * g + e;
                 if (row >= rows) continue;
-                const float v = acc[r][t][e];
+                const float v = acc[r][t][e] * (1.f / kW4Down<MT>);
                 if (p.splits > 1) {
-                    p.part[((int64_t)blockIdx.z * p.M + m0 + row) * p.N + n] = v;
+                    p.part[((int64_t)blockIdx.z * p.M + m0 + row) * p.N + n] = acc[r][t][e];
                 } else if constexpr (sizeof(XT) == 4) {
                     ((float *)p.y)[(m0 + row) * p.y_pitch + n] = v;
                 } else {
@@ -429,6 +438,7 @@ template <typename XT> __global__ __launch_bounds__(256) void w4_join_kernel(W4P
          i += (int64_t)gridDim.x * 256) {
         float v = 0.f;
         for (int s = 0; s < p.splits; ++s) v += p.part[s * all + i];
+        v *= 1.f / kW4Down<typename W4Type<XT>::M>;
         const int64_t m = i / p.N, n = i - m * p.N;
         if constexpr (sizeof(XT) == 4) ((float *)p.y)[m * p.y_pitch + n] = v;
         else ((uint16_t *)p.y)[m * p.y_pitch + n] = to_bits16(v, XT{});

@@ -6,8 +6,8 @@ import math
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
-from test_gpu_linear import (BF, COEFFICIENTS, F16, F32, ROUND, _check_grouped, _check_orth, _gen,
-                             _offsets, _randn, _steps)
+from test_gpu_linear import (BF, COEFFICIENTS, F16, F32, ROUND, _check_grouped, _check_orth, _check_w4, _gen,
+                             _offsets, _random_w4, _randn, _steps)
 from test_orthogonalize_plan import OVERSHOOTING, STANDARD
 
 import ozaki_triton_amd as ozk
@@ -174,3 +174,21 @@ def test_quantize_leaves_what_lies_between_its_rows(N, K, group):
         rows = got[:N * distance].view(N, distance)
         assert torch.equal(rows[:, :columns], w)
         assert bool((rows[:, columns:] == other).all()) and bool((got[N * distance:] == other).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M, N, K", [(1, 200, 512), (3, 9000, 256), (20, 300, 1024), (40, 300, 640), (2, 64, 16384)])
+def test_w4_activations_up_to_the_largest(dtype, group, M, N, K):
+    """Finite x gives finite y where y itself is: the two sums that are subtracted are up to
+    31 times sum |x|, past fp32's range here.  Powers of two change nothing else."""
+    packed, scales, z = _random_w4(2, N, K, group, dtype, True)
+    scales = (scales.float() / 64).to(dtype)
+    x = _randn(1, M, K, dtype=dtype)
+    y = ozk.matmul_w4(x, packed, scales, z, group_size=group)
+    for power in (123, 60, -60):
+        big = ozk.matmul_w4((x.double() * 2.0 ** power).to(dtype), packed, scales, z, group_size=group)
+        assert torch.equal(big.double(), y.double() * 2.0 ** power)
+    x[:, ::7] = 3.3e38
+    x[:, 1::7] = -3.3e38
+    _check_w4(x, packed, (scales.double() / 2 ** 7).to(dtype), z, group)
