@@ -192,3 +192,22 @@ def test_w4_activations_up_to_the_largest(dtype, group, M, N, K):
     x[:, ::7] = 3.3e38
     x[:, 1::7] = -3.3e38
     _check_w4(x, packed, (scales.double() / 2 ** 7).to(dtype), z, group)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M, N, K", [
+    (1, 4096, 1024), (5, 1000, 2047), (16, 512, 4096),         # one block of 16 columns a workgroup
+    (2, 8208, 1024), (4, 9001, 515),                           # few rows, many columns
+    (6, 4112, 1000), (17, 300, 2048), (32, 9000, 640),         # many of both
+    (33, 260, 1024), (65, 130, 2048), (150, 300, 700),
+    (1, 64, 16384), (3, 100, 8191), (20, 70, 16384)])          # K in ranges
+def test_w4_full_precision_activations_in_every_shape(M, N, K, group, zeros):
+    """fp32 x at fp32's accuracy: within four times the error of a plain fp32 product (x cut to
+    16 bits is 30 times as far off, to 8 bits 8000 times)."""
+    x, (p, s, z) = _randn(1, M, K, dtype=F32), _random_w4(2, N, K, group, F32, zeros)
+    W = ozk.dequantize_w4(p, s, z, group_size=group, K=K)
+    want = x.cpu().double() @ W.cpu().double().T
+    off = lambda y: float((y.cpu().double() - want).norm() / want.norm())  # noqa: E731
+    plain = off(x.cpu() @ W.cpu().T)
+    assert off(ozk.matmul_w4(x, p, s, z, group_size=group)) <= 4 * max(plain, 2.0 ** -24)
