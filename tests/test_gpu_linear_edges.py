@@ -7,7 +7,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fw
 from test_gpu_linear import (BF, COEFFICIENTS, F16, F32, ROUND, _check_grouped, _check_orth, _check_w4, _gen,
-                             _offsets, _random_w4, _randn, _steps)
+                             _offsets, _random_w4, _randn, _steps, _unpack)
 from test_orthogonalize_plan import OVERSHOOTING, STANDARD
 
 import ozaki_triton_amd as ozk
@@ -211,3 +211,68 @@ def test_w4_full_precision_activations_in_every_shape(M, N, K, group, zeros):
     off = lambda y: float((y.cpu().double() - want).norm() / want.norm())  # noqa: E731
     plain = off(x.cpu() @ W.cpu().T)
     assert off(ozk.matmul_w4(x, p, s, z, group_size=group)) <= 4 * max(plain, 2.0 ** -24)
+
+
+def _format(W, group, zeros):
+    """q, s and z of the format by its definition, in fp32 as stated."""
+    N, K = W.shape
+    w = torch.nn.functional.pad(W.cpu().float(), (0, -K % group)).view(N, -1, group)
+    lo, hi = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+    s = (((hi - lo) * (1 / 15)) if zeros else torch.maximum(hi, -lo) * (1 / 7)).to(W.dtype).float()
+    over = lambda a, b: torch.where(b > 0, torch.round(a / b), torch.zeros_like(a))  # noqa: E731
+    z = over(-lo, s).clamp(0, 15) if zeros else torch.full_like(s, 8)
+    q = (over(w, s[..., None].expand_as(w)) + z[..., None]).clamp(0, 15)
+    return q.view(N, -1)[:, :K].long(), s, z
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantize_is_the_format_to_the_last_value(dtype, zeros, group):
+    """q and z equal the definition's, at ties of a power-of-two scale (k + 1/2 steps, to the
+    even one), at quotients beside them, and on random weights of any size."""
+    g = _gen(9)
+    ties = torch.randint(-14, 15, (64, 4 * group), generator=g, device="cuda").float() / 2
+    if zeros:
+        ties = ties.clamp(-7, 7)
+        ties[:, ::group], ties[:, 1::group] = -7.5, 7.5         # s = 1, z = 7.5 to even
+        ties[32:, ::group], ties[32:, 1::group] = -4.5, 10.5
+    else:
+        ties[:, ::group] = 7.0                                  # s = 1
+    ties = ties * 2.0 ** torch.randint(-8, 8, (64, 1), generator=g, device="cuda")
+    beside = ties * (1 + torch.finfo(dtype).eps * torch.randint(-1, 2, ties.shape, generator=g, device="cuda"))
+    sizes = 10.0 ** torch.linspace(-4, 4 if dtype == F16 else 30, 64, device="cuda")[:, None]
+    for W in (ties, beside, _randn(1, 64, 4 * group, dtype=F32) * sizes, _randn(2, 7, 3 * group + 5, dtype=F32),
+              _randn(3, 64, group, dtype=F32).abs(), -_randn(4, 64, group, dtype=F32).abs()):
+        W = W.to(dtype)
+        q, s, z = _format(W, group, zeros)
+        packed, scales, got_z = ozk.quantize_w4(W, group, zeros=zeros)
+        assert torch.equal(scales.cpu().float(), s)
+        assert not zeros or torch.equal(got_z.cpu().float(), z)
+        assert torch.equal(_unpack(packed, W.shape[1]), q)
+    # (the first weights do hold ties)
+    steps = ties.to(dtype).cpu().float().view(64, 4, group) / _format(ties.to(dtype), group, zeros)[1][..., None]
+    assert int((steps % 1 == 0.5).sum()) > 1000
+
+
+def test_w4_packed_rows_past_4_gib():
+    """Rows whose first byte lies past 2^32."""
+    N, K = (1 << 16) + 5, 1 << 17
+    packed = torch.zeros(N, K // 2, dtype=torch.uint8, device="cuda")
+    rows = torch.tensor([0, 1, 4, 1 << 16, N - 4, N - 1], device="cuda")   # 1, 4: where 32 bits would read
+    p, s, z = _random_w4(2, 6, K, 128, BF, True)
+    packed[rows] = p
+    scales = torch.ones(N, K // 128, dtype=BF, device="cuda")
+    zeros = torch.zeros(N, K // 128, dtype=torch.uint8, device="cuda")
+    scales[rows], zeros[rows] = s, z
+    for M in (2, 20):
+        _check_w4(_randn(1, M, K), packed, scales, zeros, 128, rows.cpu())
+    W = ozk.dequantize_w4(packed[-6:], scales[-6:], zeros[-6:])
+    assert torch.equal(W[2], ozk.dequantize_w4(p[4:5], s[4:5], z[4:5])[0])
+    assert torch.equal(W[5], ozk.dequantize_w4(p[5:], s[5:], z[5:])[0])
+    # the whole of it back to weights and to 4 bits again
+    back = ozk.dequantize_w4(packed, scales, zeros)
+    assert torch.equal(back[rows], ozk.dequantize_w4(p, s, z))
+    again, s2, z2 = ozk.quantize_w4(back, zeros=True)
+    for got, want in zip((again[rows], s2[rows], z2[rows]), ozk.quantize_w4(back[rows], zeros=True)):
+        assert torch.equal(got, want)
