@@ -329,9 +329,10 @@ hipError_t pack(const PackJob &a, const PackJob &b, hipStream_t st) {
     grouped_pack_kernel<<<dim3(a.blocks + b.blocks), 256, 0, st>>>(a, b);
     return hipGetLastError();
 }
-// rows and pieces that the pack kernel counts in 32 bits
+// rows that the pack kernel counts in 32 bits, and copies of them no further apart
+// than the tiles step (2^22 elements: overlapping rows can be longer than that)
 bool packable(int64_t rows, int64_t cols) {
-    return rows < (int64_t)1 << 30 && pieces_of(cols) < (int64_t)1 << 22;
+    return rows < (int64_t)1 << 30 && pieces_of(cols) < (int64_t)1 << 19;
 }
 
 template <typename ST, typename Sh, bool DMA>

@@ -131,6 +131,20 @@ def test_grouped_single_rows_of_longer_tensors():
     _check_grouped(A[:, 3:4], one, D[:, 5:6], offsets)
 
 
+@pytest.mark.parametrize("rows, N", [(2, 64), (64, 3)])
+def test_grouped_rows_longer_than_their_distance_may_be(rows, N):
+    """One row (column) for all, of more elements than rows may be apart, and no whole 16-byte
+    pieces: 64 copies of it on rows of their own end past the tiles' 31-bit offsets."""
+    K, offsets = (1 << 24) + 500001, _offsets([rows])
+    whole = lambda seed, *s: torch.randint(-2, 3, s, generator=_gen(seed), device="cuda",  # noqa: E731
+                                           dtype=torch.int8).to(BF)
+    a, b = whole(1, 1, K), whole(2, 1, 1, K).mT
+    want = (a.double() @ b[0].double()).to(BF)          # every sum is a whole number, and exact
+    assert bool(want.any()) and 63 * 2 * K > 1 << 31
+    C = ozk.grouped_matmul(a.expand(rows, K), b.expand(1, K, N), offsets)
+    assert torch.equal(C, want.expand(rows, N))
+
+
 def test_forward_mode_is_refused():
     """A tangent is not dropped: none of the operators has a forward-mode derivative."""
     A, B, D, offsets = _randn(1, 6, 32), _randn(2, 1, 32, 40), _randn(3, 6, 40), _offsets([6])
