@@ -323,6 +323,7 @@ def dequantize_w4(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tenso
     dtype = scales.dtype if dtype is None else dtype
     _on_one_gpu(packed, scales, zeros)
     _require_dtype("dequantize_w4", dtype, _FLOAT)
+    _no_grad("dequantize_w4", scales)
     assert scales.dtype in (dtype, torch.float32), \
         f"scales must be {dtype} or float32, got {scales.dtype}"
     packed, scales, zeros = _w4_operands(packed, scales, zeros)

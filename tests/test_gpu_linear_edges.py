@@ -290,3 +290,14 @@ def test_w4_packed_rows_past_4_gib():
     again, s2, z2 = ozk.quantize_w4(back, zeros=True)
     for got, want in zip((again[rows], s2[rows], z2[rows]), ozk.quantize_w4(back[rows], zeros=True)):
         assert torch.equal(got, want)
+
+
+def test_dequantize_has_no_gradient():
+    """Scales that want a gradient are refused, as by matmul_w4."""
+    p, s, z = _random_w4(2, 30, 64, 32, BF, True)
+    want = ozk.dequantize_w4(p, s, z, group_size=32)
+    s.requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ozk.dequantize_w4(p, s, z, group_size=32)
+    with torch.no_grad():
+        assert torch.equal(ozk.dequantize_w4(p, s, z, group_size=32), want)
