@@ -270,9 +270,11 @@ def _w4_checks(packed, scales, zeros, group_size, K):
         f"zeros must be {want} uint8, got {zeros.dtype} {tuple(zeros.shape)}"
 
 
-def _w4_operands(packed, scales, zeros):
-    """The three as the kernels read them: rows contiguous, packed ones 16-byte aligned."""
-    if packed.stride(1) != 1 or packed.stride(0) % 16 or packed.data_ptr() % 16:
+def _w4_operands(packed, scales, zeros, K):
+    """The three as the kernels read them: rows contiguous, packed ones 16-byte aligned
+    and no closer than they are long."""
+    if (packed.stride(1) != 1 or packed.stride(0) % 16 or packed.data_ptr() % 16
+            or packed.stride(0) < (K + 31) // 32 * 16):
         if packed.shape[1] % 16:
             packed = torch.nn.functional.pad(packed, (0, -packed.shape[1] % 16))
         packed = packed.clone(memory_format=torch.contiguous_format)
@@ -326,7 +328,7 @@ def dequantize_w4(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tenso
     _no_grad("dequantize_w4", scales)
     assert scales.dtype in (dtype, torch.float32), \
         f"scales must be {dtype} or float32, got {scales.dtype}"
-    packed, scales, zeros = _w4_operands(packed, scales, zeros)
+    packed, scales, zeros = _w4_operands(packed, scales, zeros, K)
     N, dev = packed.shape[0], packed.device
     W = torch.empty((N, K), dtype=dtype, device=dev)
     _call("ozk_dequantize_w4", dev, packed.data_ptr(), packed.stride(0), scales.data_ptr(),
@@ -356,7 +358,7 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     _on_one_gpu(x, packed, scales, zeros)
     _require_dtype("matmul_w4", dtype, _FLOAT)
     _no_grad("matmul_w4", x, scales)
-    packed, scales, zeros = _w4_operands(packed, scales, zeros)
+    packed, scales, zeros = _w4_operands(packed, scales, zeros, K)
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     if x2.stride(1) != 1 and K != 1:
         x2 = x2.contiguous()

@@ -301,3 +301,18 @@ def test_dequantize_has_no_gradient():
         ozk.dequantize_w4(p, s, z, group_size=32)
     with torch.no_grad():
         assert torch.equal(ozk.dequantize_w4(p, s, z, group_size=32), want)
+
+
+def test_w4_rows_that_overlap():
+    """One packed row, scale and zero point for all rows of W, and rows that overlap."""
+    x, (p, s, z) = _randn(1, 3, 96), _random_w4(2, 1, 96, 32, BF, True)
+    one = ozk.matmul_w4(x, p, s, z, group_size=32)
+    wide = [t.expand(20, -1) for t in (p, s, z)]
+    assert torch.equal(ozk.matmul_w4(x, *wide, group_size=32), one.expand(3, 20))
+    assert torch.equal(ozk.dequantize_w4(*wide, group_size=32), ozk.dequantize_w4(p, s, z, group_size=32).expand(20, 96))
+    p, s, z = _random_w4(3, 4, 32, 32, BF, True)
+    windows = p.flatten().as_strided((2, 48), (16, 1))
+    for n in range(2):
+        got = ozk.matmul_w4(x, windows, s[:2].expand(2, 3), z[:2].expand(2, 3), group_size=32)[:, n]
+        assert torch.equal(got, ozk.matmul_w4(x, windows[n:n + 1].clone(), s[n:n + 1].expand(1, 3),
+                                              z[n:n + 1].expand(1, 3), group_size=32)[:, 0])
