@@ -612,14 +612,22 @@ int lds_of(const W4Params &p, const W4Shape &s, int slices) {
 
 template <typename XT, int I, int GPC> hipError_t w4_start(const W4Params &p, hipStream_t st) {
     constexpr W4Shape s = kW4Shapes[I];
-    const dim3 grid((uint32_t)((p.N + 16 * s.rt * s.wn - 1) / (16 * s.rt * s.wn)),
-                    (uint32_t)((p.M + 16 * s.tt - 1) / (16 * s.tt)), (uint32_t)p.splits);
-    if (grid.y > 65535) return hipErrorInvalidConfiguration;
     const int lds = lds_of(p, s, W4Type<XT>::SL);
     if (hipError_t e = allow_lds<&w4_kernel<XT, s.wn, s.wk, s.rt, s.tt, GPC>>(lds); e != hipSuccess)
         return e;
-    w4_kernel<XT, s.wn, s.wk, s.rt, s.tt, GPC><<<grid, 64 * s.wn * s.wk, lds, st>>>(p);
-    return hipGetLastError();
+    // a launch counts 65535 blocks of rows (so many fill the GPU without K ranges)
+    constexpr int64_t rows = 65535 * 16 * s.tt;
+    for (int64_t m = 0; m < p.M; m += rows) {
+        W4Params q = p;
+        q.x += m * p.x_pitch * (int64_t)sizeof(XT);
+        q.y += m * p.y_pitch * (int64_t)sizeof(XT);
+        q.M = p.M - m < rows ? p.M - m : rows;
+        const dim3 grid((uint32_t)((p.N + 16 * s.rt * s.wn - 1) / (16 * s.rt * s.wn)),
+                        (uint32_t)((q.M + 16 * s.tt - 1) / (16 * s.tt)), (uint32_t)p.splits);
+        w4_kernel<XT, s.wn, s.wk, s.rt, s.tt, GPC><<<grid, 64 * s.wn * s.wk, lds, st>>>(q);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 template <typename XT, int I> hipError_t w4_go(const W4Params &p, hipStream_t st) {

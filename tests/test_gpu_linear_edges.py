@@ -316,3 +316,13 @@ def test_w4_rows_that_overlap():
         got = ozk.matmul_w4(x, windows, s[:2].expand(2, 3), z[:2].expand(2, 3), group_size=32)[:, n]
         assert torch.equal(got, ozk.matmul_w4(x, windows[n:n + 1].clone(), s[n:n + 1].expand(1, 3),
                                               z[n:n + 1].expand(1, 3), group_size=32)[:, 0])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_w4_more_rows_than_a_launch_counts(dtype):
+    """65535 blocks of 64 rows (fp32: of 32) and some more."""
+    M, (p, s, z) = 65535 * (32 if dtype == F32 else 64) + 70, _random_w4(2, 5, 32, 32, dtype, True)
+    x = _randn(1, M, 33, dtype=dtype)[:, 1:]
+    y = ozk.matmul_w4(x, p, s, z, group_size=32)
+    for rows in (slice(0, 100), slice(M // 2, M // 2 + 100), slice(M - 200, M)):
+        assert torch.equal(y[rows], ozk.matmul_w4(x[rows], p, s, z, group_size=32))
