@@ -27,6 +27,7 @@ _HALF = (torch.float16, torch.bfloat16)
 _OFFSETS = (torch.int32, torch.int64)
 _FLOAT = (torch.float32, torch.float16, torch.bfloat16)
 _MAX_STRIDE = 1 << 22      # the kernels' limit on the distance of two rows
+_MAX_BATCH = 65535         # matrices that one orthogonalisation takes
 
 
 def _require_dtype(name: str, dtype: torch.dtype, allowed) -> None:
@@ -409,6 +410,8 @@ def orthogonalize(G: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750
     if G3.stride(2) != 1 and N != 1:
         G3 = G3.contiguous()
     B, dev = G3.shape[0], G.device
+    if B > _MAX_BATCH:
+        return torch.cat([orthogonalize(g, steps, triples, eps) for g in G3.split(_MAX_BATCH)]).view(G.shape)
     out = torch.empty((B, M, N), dtype=G.dtype, device=dev)
     n = _bytes("ozk_orthogonalize_workspace_bytes", B, M, N, steps)
     ws, wsp = _workspace(n, dev)

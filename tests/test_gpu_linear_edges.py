@@ -108,6 +108,14 @@ def test_orthogonalize_empty(shape):
     assert X.shape == shape and X.dtype == BF and X.data_ptr() == 0
 
 
+def test_orthogonalize_more_matrices_than_a_launch_counts():
+    G = _randn(1, 2, 33000, 3, 5, dtype=F32)
+    X = ozk.orthogonalize(G)
+    assert X.shape == G.shape
+    for b, n in ((0, 0), (1, 32534), (1, 32535), (1, 32999)):     # 65535 = 33000 + 32535
+        assert torch.equal(X[b, n], ozk.orthogonalize(G[b, n]))
+
+
 # ---------------------------------------------------------------------------
 # grouped products
 # ---------------------------------------------------------------------------
