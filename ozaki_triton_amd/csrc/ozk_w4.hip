@@ -447,8 +447,9 @@ template <typename XT> __global__ __launch_bounds__(256) void w4_join_kernel(W4P
 
 // ---------------------------------------------------------------------------
 // The format.  Symmetric: s = fl(max |w| fl(1 / 7)), z = 8; with zero points: s =
-// fl((max(w, 0) - min(w, 0)) fl(1 / 15)), z = rint(-min(w, 0) / s).  q = rint(w / s)
-// + z within 0 .. 15; a group of zeros has s = 0 and q = z.  NaN counts as 0.
+// fl((max(w, 0) - min(w, 0)) fl(1 / 15)) (the two multiplied first where their
+// difference is past fp32), z = rint(-min(w, 0) / s).  q = rint(w / s) + z within 0
+// .. 15; a group of zeros has s = 0 and q = z.  NaN counts as 0.
 // ---------------------------------------------------------------------------
 template <typename T> OZK_DEV float load_value(const char *p, int64_t i) {
     if constexpr (sizeof(T) == 4) return ((const float *)p)[i];
@@ -502,7 +503,9 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_w4_kernel(
     if (p.group == 128) dpp_range<0x140>(lo, hi);      // the other eight of 16
     float s, z = 8.f;
     if (p.zeros) {
-        s = rounded<T>((hi - lo) * (1.f / 15.f));
+        const float range = hi - lo;
+        s = rounded<T>(__builtin_isinf(range) ? hi * (1.f / 15.f) - lo * (1.f / 15.f)
+                                              : range * (1.f / 15.f));
         z = s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
     } else {
         s = rounded<T>(fmaxf(hi, -lo) * (1.f / 7.f));

@@ -277,6 +277,20 @@ def test_quantize_is_the_format_to_the_last_value(dtype, zeros, group):
     assert int((steps % 1 == 0.5).sum()) > 1000
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantize_ranges_past_the_largest_float(dtype):
+    """Weights of both signs near the type's largest: their range is past it, their scale
+    is not.  Each comes back within half a step (and a whole one at the ends)."""
+    W = (_randn(1, 6, 96, dtype=F32) / 5).clamp(-1, 1)
+    W[:, ::32], W[:, 1::32] = 1, -0.8
+    W = (W * 3e38).to(dtype)
+    packed, scales, z = ozk.quantize_w4(W, 32, zeros=True)
+    step = scales.cpu().double().repeat_interleave(32, 1)
+    assert bool(((step > 3.5e37) & (step < 3.7e37)).all()) and bool((z == 7).all())      # 1.8 / 15, 0.8 / 0.12
+    off = (ozk.dequantize_w4(packed, scales, z, group_size=32).cpu().double() - W.cpu().double()).abs()
+    assert bool((off <= step * 1.01).all()) and float((off <= step * 0.51).double().mean()) > 0.9
+
+
 def test_w4_packed_rows_past_4_gib():
     """Rows whose first byte lies past 2^32."""
     N, K = (1 << 16) + 5, 1 << 17
