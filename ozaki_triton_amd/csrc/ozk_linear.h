@@ -95,7 +95,7 @@ struct QuantParams {
     uint8_t *packed;
     char *scales;             // W's type
     uint8_t *zeros;           // null: symmetric, zero point 8
-    int64_t N, K, w_pitch, p_pitch, groups, s_pitch, z_pitch;
+    int64_t N, K, w_pitch, p_pitch, s_pitch, z_pitch;
     int group;
 };
 hipError_t launch_quantize_w4(const QuantParams &p, int dtype, hipStream_t st);

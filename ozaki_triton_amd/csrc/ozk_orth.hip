@@ -24,15 +24,6 @@ namespace ozk {
 // bytes of a slice row of n columns: 64 of h and 64 of l for every 32 columns
 __host__ __device__ inline int64_t slice_pitch(int64_t n) { return (n + 31) / 32 * 128; }
 
-template <typename T> OZK_DEV float orth_load(const char *p, int64_t i) {
-    if constexpr (sizeof(T) == 4) return ((const float *)p)[i];
-    else return from_bits16(((const uint16_t *)p)[i], T{});
-}
-template <typename T> OZK_DEV void orth_store(char *p, int64_t i, float v) {
-    if constexpr (sizeof(T) == 4) ((float *)p)[i] = v;
-    else ((uint16_t *)p)[i] = to_bits16(v, T{});
-}
-
 OZK_DEV double block_sum(double v) {   // of 256 lanes, in every lane
     __shared__ double part[4];
 #pragma unroll
@@ -77,7 +68,7 @@ template <typename T> __global__ __launch_bounds__(256) void orth_norm_kernel(Or
             }
         }
         for (int64_t c = whole * E + threadIdx.x; c < p.N; c += 256) {
-            const double v = orth_load<T>(row, c);
+            const double v = load_value<T>(row, c);
             sum += v * v;
         }
     }
@@ -127,7 +118,7 @@ __global__ __launch_bounds__(256) void orth_start_kernel(OrthParams p, double *n
             const int c = flip ? threadIdx.x / 64 + 4 * q : threadIdx.x % 32;
             const int64_t row = r0 + r, col = c0 + c;
             v[q] = 0.f;
-            if (row < m && col < n) v[q] = orth_load<T>(G, flip ? col * p.g_row + row : row * p.g_row + col);
+            if (row < m && col < n) v[q] = load_value<T>(G, flip ? col * p.g_row + row : row * p.g_row + col);
         }
     }
     double sum = 0.0;

@@ -54,6 +54,16 @@ OZK_DEV uint16_t to_bits16(float v, __bf16) { return __builtin_bit_cast(uint16_t
 OZK_DEV float from_bits16(uint16_t v, _Float16) { return (float)__builtin_bit_cast(_Float16, v); }
 OZK_DEV float from_bits16(uint16_t v, __bf16) { return bf16_bits_to_f32(v); }
 
+// element i of fp32 or 16-bit values as fp32, and back
+template <typename T> OZK_DEV float load_value(const char *p, int64_t i) {
+    if constexpr (sizeof(T) == 4) return ((const float *)p)[i];
+    else return from_bits16(((const uint16_t *)p)[i], T{});
+}
+template <typename T> OZK_DEV void store_value(char *p, int64_t i, float v) {
+    if constexpr (sizeof(T) == 4) ((float *)p)[i] = v;
+    else ((uint16_t *)p)[i] = to_bits16(v, T{});
+}
+
 // i / n for 0 <= i < 2^22, n a small part of it: (i + 1/2) / n is at least 1 / 2n
 // away from a whole number, the two roundings of rcp * (i + 1/2) less
 OZK_DEV int part_of(int i, int n, float rcp) { return (int)(((float)i + 0.5f) * rcp); }

@@ -451,14 +451,6 @@ template <typename XT> __global__ __launch_bounds__(256) void w4_join_kernel(W4P
 // difference is past fp32), z = rint(-min(w, 0) / s).  q = rint(w / s) + z within 0
 // .. 15; a group of zeros has s = 0 and q = z.  NaN counts as 0.
 // ---------------------------------------------------------------------------
-template <typename T> OZK_DEV float load_value(const char *p, int64_t i) {
-    if constexpr (sizeof(T) == 4) return ((const float *)p)[i];
-    else return from_bits16(((const uint16_t *)p)[i], T{});
-}
-template <typename T> OZK_DEV void store_value(char *p, int64_t i, float v) {
-    if constexpr (sizeof(T) == 4) ((float *)p)[i] = v;
-    else ((uint16_t *)p)[i] = to_bits16(v, T{});
-}
 template <typename T> OZK_DEV float rounded(float v) {
     if constexpr (sizeof(T) == 4) return v;
     else return from_bits16(to_bits16(v, T{}), T{});
