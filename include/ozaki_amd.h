@@ -340,7 +340,11 @@ int ozk_matmul_w4(const void *x, int dtype, int64_t x_stride, const void *packed
  *           strides of batch and row
  *   coefficients  host memory, 3 * steps
  * The products are fp32-grade: two fp16 slices of each matrix, three of the
- * four slice pairs, sums in fp32.
+ * four slice pairs, sums in fp32.  For 16-bit results and sides of 1 to 2 or
+ * more the last steps may run on A alone, where their worst case is that of steps
+ * by themselves.  The slices' scales follow the coefficients; those under which
+ * singular values may grow past about 30 have them measured instead.  A zero
+ * matrix stays zero, one with an infinity or NaN becomes NaN.
  */
 int ozk_orthogonalize_workspace_bytes(int64_t batch, int64_t M, int64_t N, int steps,
                                       size_t *bytes_out);

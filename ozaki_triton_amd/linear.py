@@ -349,7 +349,7 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
         packed, scales, zeros: quantize_w4's; scales in x's dtype or float32
     Returns:
         y: (..., N), dtype of x, summed in float32 and rounded once.  A row of x
-        with an infinity or NaN gives a row of NaN.
+        with an infinity or NaN gives a row of NaN; finite ones do not.
     """
     assert x.dim() >= 1 and x.shape[-1] >= 1, f"x must be [..., K], got {tuple(x.shape)}"
     K, dtype, dev = x.shape[-1], x.dtype, x.device
@@ -391,8 +391,8 @@ def orthogonalize(G: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750
         coefficients: (a, b, c) of every step, or a sequence of ``steps`` such triples
     Returns:
         X: the shape and dtype of G.  Products are fp32-grade (two fp16 slices, sums
-        in fp32), whatever G's dtype.  A zero matrix stays zero; one with an
-        infinity or NaN becomes NaN.
+        in fp32), whatever G's dtype and the coefficients.  A zero matrix stays
+        zero; one with an infinity or NaN becomes NaN.
     """
     assert G.dim() >= 2, f"G must be [..., M, N], got {tuple(G.shape)}"
     assert 1 <= steps <= 64, f"steps must be 1 .. 64, got {steps}"
