@@ -354,6 +354,104 @@ int ozk_orthogonalize(const void *G, int dtype, int64_t batch, int64_t M, int64_
                       double eps, void *out, const int64_t o_strides[2], void *workspace,
                       size_t workspace_bytes, void *stream);
 
+/*
+ * The product of a linear layer with its epilogue, in training and serving:
+ *   z = x W^T + bias,  y = act(z) + residual
+ *   x [M, K], rows x_stride apart; W [N, K], strides w_strides, K or N contiguous;
+ *   bias [N] or NULL; residual [M, N] or NULL, rows r_stride apart; y [M, N]; all
+ *   of dtype OZK_F16 or OZK_BF16, sums and epilogue in fp32, rounded once.
+ *   z  NULL, or [M, N] of that dtype, rows of N: what act is applied to, rounded,
+ *      for the backward call (a z that underflows keeps its sign).
+ * act: z; max(z, 0); z Phi(z) of the normal distribution; z (1 + tanh(sqrt(2 / pi)
+ * (z + 0.044715 z^3))) / 2; z / (1 + e^-z).
+ * Workspace (16-byte aligned): partial sums of K ranges, which it needs, and copies
+ * of operands whose rows are no whole 16-byte pieces, without which it runs slower.
+ *
+ * ozk_linear_backward: for dy [M, N], with dz = dy act'(z) rounded to dtype,
+ *   dx = dz W [M, K], dW = dz^T x [N, K], db = sum of the unrounded dz over the
+ *   rows [N]; each where its pointer is given.  z as above; not read without act.
+ * Its workspace is 256-byte aligned; `want` of the query: 1 dx, 2 dW, 4 db.
+ * Rows of 2^22 or more elements apart return OZK_ERR_TOO_LARGE.
+ */
+#define OZK_ACT_NONE 0
+#define OZK_ACT_RELU 1
+#define OZK_ACT_GELU 2
+#define OZK_ACT_GELU_TANH 3
+#define OZK_ACT_SILU 4
+
+int ozk_linear_workspace_bytes(const void *x, int64_t x_stride, const void *W,
+                               const int64_t w_strides[2], int64_t M, int64_t N, int64_t K,
+                               size_t *bytes_out);
+
+int ozk_linear(const void *x, int64_t x_stride, const void *W, const int64_t w_strides[2],
+               const void *bias, const void *residual, int64_t r_stride, int activation, int64_t M,
+               int64_t N, int64_t K, int dtype, void *y, int64_t y_stride, void *z, void *workspace,
+               size_t workspace_bytes, void *stream);
+
+int ozk_linear_backward_workspace_bytes(const void *dy, int64_t dy_stride, const void *x,
+                                        int64_t x_stride, const void *W, const int64_t w_strides[2],
+                                        int activation, int64_t M, int64_t N, int64_t K, int want,
+                                        size_t *bytes_out);
+
+int ozk_linear_backward(const void *dy, int64_t dy_stride, const void *z, const void *x,
+                        int64_t x_stride, const void *W, const int64_t w_strides[2],
+                        int activation, int64_t M, int64_t N, int64_t K, int dtype, void *dx,
+                        int64_t dx_stride, void *dW, int64_t dw_stride, void *db, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/*
+ * The router of a layer of experts: T tokens, E experts (OZK_MAX_EXPERTS at most),
+ * k of them to a token, p = softmax(logits).
+ *   logits   [T, E] of OZK_F32, OZK_F16 or OZK_BF16, rows l_stride apart
+ *   mask     [T] of bytes, 0: the token is left out; NULL: none is
+ *   experts  [T, k]: those of the greatest logits, the greatest first, of equal ones
+ *            (0 and -0 are) the lowest index, NaN above all; E for a masked token
+ *   weights  [T, k]: their p, with normalize over the sum of the k; 0 if masked
+ *   order    [T k]: the slots t k + j sorted by expert, in their order within one,
+ *            the masked ones last;  place [T, k]: the slots' places in it
+ *   offsets  [E + 1]: where each expert's slots begin (ozk_grouped_matmul's), the
+ *            last the number of all;  counts [E]: how many there are
+ *   loss     E sum_e f_e P_e with f_e = counts[e] / (n k) and P_e the mean of p[t, e],
+ *            over the n tokens that are not masked; 0 if there is none
+ * T k is under 2^31.  ozk_route_backward gives the logits' gradient for those of the
+ * weights [T, k] and of the loss (each may be NULL), the counts taken as constants;
+ * dlogits [T, E] of the logits' type, zeros for masked tokens.
+ */
+#define OZK_MAX_EXPERTS 1024
+
+int ozk_route_workspace_bytes(int64_t T, int64_t E, int64_t k, size_t *bytes_out);
+
+int ozk_route(const void *logits, int dtype, int64_t l_stride, const void *mask, int64_t T, int64_t E,
+              int64_t k, int normalize, int32_t *experts, float *weights, int32_t *order,
+              int32_t *place, int32_t *offsets, int32_t *counts, float *loss, void *workspace,
+              size_t workspace_bytes, void *stream);
+
+int ozk_route_backward(const void *logits, int dtype, int64_t l_stride, const void *mask, int64_t T,
+                       int64_t E, int64_t k, int normalize, const int32_t *experts,
+                       const float *weights, const int32_t *counts, const float *dweights,
+                       const float *dloss, void *dlogits, void *stream);
+
+/*
+ * The norm of many tensors taken as one vector, and their scaling to a norm of at
+ * most max_norm: out = g min(1, max_norm / norm).
+ *   grads, outs, counts, dtypes  host arrays of `tensors` addresses, element counts
+ *            and types (OZK_F32, OZK_F16 or OZK_BF16, mixed as they come); each
+ *            tensor contiguous.  outs[i] may be grads[i]; no other overlap of an out
+ *            with any tensor (OZK_ERR_SHAPE).
+ *   norm     one float on the device; the sum of squares is taken in 64 bits, in
+ *            the same order every time
+ * With a norm of infinity everything finite becomes 0, with NaN everything NaN.
+ */
+int ozk_gradient_norm_workspace_bytes(int64_t tensors, size_t *bytes_out);
+
+int ozk_gradient_norm(const void *const *grads, const int64_t *counts, const int *dtypes,
+                      int64_t tensors, float *norm, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
+int ozk_clip_gradients(const void *const *grads, void *const *outs, const int64_t *counts,
+                       const int *dtypes, int64_t tensors, double max_norm, float *norm,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

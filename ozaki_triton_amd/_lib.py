@@ -27,6 +27,8 @@ OZK_ERR_TOO_LARGE = -10
 OZK_STATIC_SCRATCH_BYTES = 64 << 20
 OZK_MAX_SPLITS = 8
 OZK_PAIRS_ALL, OZK_PAIRS_TRIANGULAR = 0, 1
+OZK_ACT_NONE, OZK_ACT_RELU, OZK_ACT_GELU, OZK_ACT_GELU_TANH, OZK_ACT_SILU = 0, 1, 2, 3, 4
+OZK_MAX_EXPERTS = 1024
 
 # every symbol include/ozaki_amd.h declares
 EXPORTED = (
@@ -53,6 +55,16 @@ EXPORTED = (
     "ozk_matmul_w4",
     "ozk_orthogonalize_workspace_bytes",
     "ozk_orthogonalize",
+    "ozk_linear_workspace_bytes",
+    "ozk_linear",
+    "ozk_linear_backward_workspace_bytes",
+    "ozk_linear_backward",
+    "ozk_route_workspace_bytes",
+    "ozk_route",
+    "ozk_route_backward",
+    "ozk_gradient_norm_workspace_bytes",
+    "ozk_gradient_norm",
+    "ozk_clip_gradients",
 )
 
 # the test hooks of include/ozaki_amd_debug.h
@@ -142,7 +154,21 @@ def load() -> ctypes.CDLL:
                                i64, vp, sz, vp]),
             ("ozk_orthogonalize_workspace_bytes", [i64, i64, i64, i32, psz]),
             ("ozk_orthogonalize", [vp, i32, i64, i64, i64, p64, pd, i32, ctypes.c_double, vp, p64,
-                                   vp, sz, vp])):
+                                   vp, sz, vp]),
+            ("ozk_linear_workspace_bytes", [vp, i64, vp, p64, i64, i64, i64, psz]),
+            ("ozk_linear", [vp, i64, vp, p64, vp, vp, i64, i32, i64, i64, i64, i32, vp, i64, vp, vp,
+                            sz, vp]),
+            ("ozk_linear_backward_workspace_bytes", [vp, i64, vp, i64, vp, p64, i32, i64, i64, i64,
+                                                     i32, psz]),
+            ("ozk_linear_backward", [vp, i64, vp, vp, i64, vp, p64, i32, i64, i64, i64, i32, vp, i64,
+                                     vp, i64, vp, vp, sz, vp]),
+            ("ozk_route_workspace_bytes", [i64, i64, i64, psz]),
+            ("ozk_route", [vp, i32, i64, vp, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, sz,
+                           vp]),
+            ("ozk_route_backward", [vp, i32, i64, vp, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp]),
+            ("ozk_gradient_norm_workspace_bytes", [i64, psz]),
+            ("ozk_gradient_norm", [vp, vp, vp, i64, vp, vp, sz, vp]),
+            ("ozk_clip_gradients", [vp, vp, vp, vp, i64, ctypes.c_double, vp, vp, sz, vp])):
         fn = getattr(L, name)
         fn.argtypes, fn.restype = args, i32
     pi, pf = ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_float)

@@ -1,0 +1,192 @@
+// ozk_clip.hip -- the norm of many tensors taken as one vector, and their scaling
+// to a norm of at most max_norm.
+//
+// norm = sqrt(sum of squares), in 64 bits from each element on: the square of an
+// fp32 or bf16 value can be past fp32's range in both directions, and sums of 1e9
+// elements would lose their last ones in 32 bits.  The sum is that of fixed parts
+// in a fixed order (no atomics): the same bits every time.
+//
+// Tensors are cut into pieces of one size, which the workgroups take in turn; a
+// launch carries its tensors' addresses in its arguments (so a captured graph
+// keeps them), kClipTensors at most.  Bound by memory: every element read once
+// for the norm, read and written once more for the scaling.
+#include "../../include/ozaki_amd.h"
+#include "ozk_train.h"
+#include "ozk_tile.h"
+
+namespace ozk {
+
+// The tensor that holds piece i (the last whose first piece is not past it):
+// every lane compares two of them
+OZK_DEV int tensor_of(const ClipParams &p, uint32_t i) {
+    const int lane = threadIdx.x & 63;
+    const bool a = lane < p.count && p.t[lane].first <= i;
+    const bool b = lane + 64 < p.count && p.t[lane + 64 < kClipTensors ? lane + 64 : 0].first <= i;
+    return __popcll(__ballot(a)) + __popcll(__ballot(b)) - 1;
+}
+struct Piece {
+    const char *in;
+    char *out;
+    int n, dtype;   // elements
+};
+OZK_DEV Piece piece_of(const ClipParams &p, uint32_t i) {
+    const ClipTensor &t = p.t[uniform(tensor_of(p, i))];
+    const int64_t at = (int64_t)(i - t.first) * p.size, left = t.n - at;
+    const int64_t byte = at * (t.dtype == OZK_F32 ? 4 : 2);
+    return {t.in + byte, t.out + byte, (int)(left < p.size ? left : p.size), t.dtype};
+}
+
+template <typename T> OZK_DEV void values(i32x4 v, float (&f)[16 / sizeof(T)]) {
+    if constexpr (sizeof(T) == 4) {
+        __builtin_memcpy(f, &v, 16);
+    } else {
+        uint16_t e[8];
+        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = from_bits16(e[i], T{});
+    }
+}
+
+// Both of a workgroup's 256 lanes: whole 16-byte parts, four at a time, then the
+// elements behind the last.  f(whole part index) and so on are the callers'.
+constexpr int kAtOnce = 4;
+
+template <typename T> OZK_DEV double piece_squares(const Piece &c) {
+    constexpr int V = 16 / sizeof(T);
+    const int parts = c.n / V;
+    double s[4] = {};
+    auto add = [&](i32x4 v) {
+        float f[V];
+        values<T>(v, f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i & 3] = fma((double)f[i], (double)f[i], s[i & 3]);
+    };
+    int i = threadIdx.x;
+    for (; i + (kAtOnce - 1) * 256 < parts; i += kAtOnce * 256) {
+        i32x4 v[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) __builtin_memcpy(&v[u], c.in + (int64_t)(i + u * 256) * 16, 16);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) add(v[u]);
+    }
+    for (; i < parts; i += 256) {
+        i32x4 v;
+        __builtin_memcpy(&v, c.in + (int64_t)i * 16, 16);
+        add(v);
+    }
+    if ((int)threadIdx.x < c.n - parts * V) {
+        const double x = (double)load_value<T>(c.in, parts * V + threadIdx.x);
+        s[0] = fma(x, x, s[0]);
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// the 256 lanes' values, in a fixed order, in every lane
+OZK_DEV double sum256(double v) {
+    __shared__ double part[4];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__global__ __launch_bounds__(256) void square_sums_kernel(ClipParams p) {
+    double s = 0.0;
+    for (uint32_t i = blockIdx.x; i < p.pieces; i += gridDim.x) {
+        const Piece c = piece_of(p, i);
+        s += c.dtype == OZK_F32   ? piece_squares<float>(c)
+             : c.dtype == OZK_F16 ? piece_squares<_Float16>(c)
+                                  : piece_squares<__bf16>(c);
+    }
+    s = sum256(s);
+    if (threadIdx.x == 0) p.part[p.part0 + blockIdx.x] = s;
+}
+
+// the norm of all partial sums, in every lane of a workgroup
+OZK_DEV double norm_of(const ClipParams &p) {
+    double s = 0.0;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < p.parts; i += 256) s += p.part[i];
+    return sqrt(sum256(s));
+}
+
+__global__ __launch_bounds__(256) void norm_kernel(ClipParams p) {
+    const double norm = norm_of(p);
+    if (threadIdx.x == 0) *p.norm = (float)norm;
+}
+
+template <typename T> OZK_DEV void piece_scale(const Piece &c, double by) {
+    constexpr int V = 16 / sizeof(T);
+    const int parts = c.n / V;
+    // fp32: the product in 64 bits, rounded once; 16 bits: in 32 bits, whose
+    // rounding is 2^-13 of theirs, the factor a whole float above 2^-126
+    auto scaled = [&](i32x4 v) {
+        float f[V];
+        values<T>(v, f);
+        i32x4 r;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = (float)((double)f[i] * by);
+            __builtin_memcpy(&r, f, 16);
+        } else {
+            uint16_t e[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) e[i] = to_bits16(f[i] * (float)by, T{});
+            __builtin_memcpy(&r, e, 16);
+        }
+        return r;
+    };
+    int i = threadIdx.x;
+    for (; i + (kAtOnce - 1) * 256 < parts; i += kAtOnce * 256) {
+        i32x4 v[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) __builtin_memcpy(&v[u], c.in + (int64_t)(i + u * 256) * 16, 16);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const i32x4 r = scaled(v[u]);
+            __builtin_memcpy(c.out + (int64_t)(i + u * 256) * 16, &r, 16);
+        }
+    }
+    for (; i < parts; i += 256) {
+        i32x4 v;
+        __builtin_memcpy(&v, c.in + (int64_t)i * 16, 16);
+        v = scaled(v);
+        __builtin_memcpy(c.out + (int64_t)i * 16, &v, 16);
+    }
+    if ((int)threadIdx.x < c.n - parts * V) {
+        const int64_t at = parts * V + threadIdx.x;
+        store_value<T>(c.out, at, (float)((double)load_value<T>(c.in, at) * by));
+    }
+}
+
+__global__ __launch_bounds__(256) void scale_kernel(ClipParams p) {
+    const double norm = norm_of(p);
+    if (p.norm && blockIdx.x == 0 && threadIdx.x == 0) *p.norm = (float)norm;
+    // NaN makes everything NaN
+    const double by = norm <= p.max_norm ? 1.0 : p.max_norm / norm;
+    // the last pieces first: the memory-side cache holds what the norm's pass read last
+    for (uint32_t j = blockIdx.x; j < p.pieces; j += gridDim.x) {
+        const Piece c = piece_of(p, p.pieces - 1 - j);
+        if (by == 1.0 && c.in == c.out) continue;
+        if (c.dtype == OZK_F32) piece_scale<float>(c, by);
+        else if (c.dtype == OZK_F16) piece_scale<_Float16>(c, by);
+        else piece_scale<__bf16>(c, by);
+    }
+}
+
+hipError_t launch_square_sums(const ClipParams &p, uint32_t grid, hipStream_t st) {
+    square_sums_kernel<<<dim3(grid), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+hipError_t launch_norm(const ClipParams &p, hipStream_t st) {
+    norm_kernel<<<dim3(1), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+hipError_t launch_scale(const ClipParams &p, uint32_t grid, hipStream_t st) {
+    scale_kernel<<<dim3(grid), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+}  // namespace ozk

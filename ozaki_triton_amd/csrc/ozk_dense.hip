@@ -1,0 +1,568 @@
+// ozk_dense.hip -- the product of a linear layer, y = act(x W^T + b) + r, and
+// what its gradients need beside products.
+//
+// Three kernels compute the sums: tiles on the matrix cores (ozk_tile.h) with
+// the epilogue in them, the same with K cut into ranges whose fp32 sums a second
+// launch joins, and one for a few rows, which is bound by reading W.
+#include "../../include/ozaki_amd.h"
+#include "ozk_train.h"
+#include "ozk_tile.h"
+
+namespace ozk {
+
+// ---------------------------------------------------------------------------
+// Activations.  Results are rounded to 8 or 11 bits: exp2 and the reciprocal of
+// the hardware (1 ulp) and the rounding of exp2's argument, |z| 2^-24 relative,
+// stay far below that.
+// ---------------------------------------------------------------------------
+constexpr float kLog2e = 1.44269504f, kGelu2 = 1.59576912f /* 2 sqrt(2 / pi) */, kGelu3 = 0.044715f;
+
+OZK_DEV float sigmoid(float z) {   // 1 / (1 + e^-z)
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * z));
+}
+// Phi(-a) of the normal distribution for a >= 0, and e^(-a a / 2): their ratio is
+// smooth, a polynomial in t = 1 / (1 + 0.3 a) fitted to it over 0 .. 14 (beyond,
+// e^(-a a / 2) is below every result): relative error 2.2e-6 in fp32.  The
+// coefficients are a weighted least-squares fit to 0.5 erfcx(a / sqrt 2).
+OZK_DEV float normal_tail(float a, float &e) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));
+    float q = -0.08459325134754181f;
+    q = fmaf(q, t, 0.24057289958000183f);
+    q = fmaf(q, t, -0.048644598573446274f);
+    q = fmaf(q, t, 0.1647646278142929f);
+    q = fmaf(q, t, 0.1067044585943222f);
+    q = fmaf(q, t, 0.12127471715211868f);
+    q = fmaf(q, t, -7.979064685059711e-05f);
+    e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * a * a);
+    return q * e;
+}
+OZK_DEV float normal_below(float z, float &e) {   // Phi(z)
+    const float tail = normal_tail(fabsf(z), e);
+    return z < 0.f ? tail : 1.f - tail;
+}
+template <int ACT> OZK_DEV float activation(float z) {
+    if constexpr (ACT == OZK_ACT_RELU) return z < 0.f ? 0.f : z;   // NaN stays
+    if constexpr (ACT == OZK_ACT_SILU) return z * sigmoid(z);
+    if constexpr (ACT == OZK_ACT_GELU_TANH)
+        return z * sigmoid(kGelu2 * fmaf(kGelu3 * z * z, z, z));   // (1 + tanh u) / 2 = sigmoid(2u)
+    if constexpr (ACT == OZK_ACT_GELU) {
+        float e;
+        return z * normal_below(z, e);
+    }
+    return z;
+}
+// its derivative; past |z| = 1e4 that of the limit, which the formulas would
+// multiply out of infinities
+template <int ACT> OZK_DEV float derivative(float z) {
+    if constexpr (ACT == OZK_ACT_RELU) return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;   // NaN stays
+    z = z > 1e4f ? 1e4f : z < -1e4f ? -1e4f : z;
+    if constexpr (ACT == OZK_ACT_SILU) {
+        const float s = sigmoid(z);
+        return s * fmaf(z, sigmoid(-z), 1.f);
+    }
+    if constexpr (ACT == OZK_ACT_GELU_TANH) {
+        const float zz = kGelu3 * z * z, u = kGelu2 * fmaf(zz, z, z);
+        const float s = sigmoid(u);
+        return s * fmaf(z * sigmoid(-u), kGelu2 * fmaf(3.f, zz, 1.f), 1.f);
+    }
+    if constexpr (ACT == OZK_ACT_GELU) {
+        float e;
+        const float below = normal_below(z, e);
+        return fmaf(z * 0.398942280f, e, below);
+    }
+    return 1.f;
+}
+template <typename F> OZK_DEV void with_act(int act, F &&f) {
+    switch (act) {
+    case OZK_ACT_RELU: f(std::integral_constant<int, OZK_ACT_RELU>{}); break;
+    case OZK_ACT_GELU: f(std::integral_constant<int, OZK_ACT_GELU>{}); break;
+    case OZK_ACT_GELU_TANH: f(std::integral_constant<int, OZK_ACT_GELU_TANH>{}); break;
+    case OZK_ACT_SILU: f(std::integral_constant<int, OZK_ACT_SILU>{}); break;
+    default: break;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 8 consecutive 16-bit values of a row, of which `n` exist
+// ---------------------------------------------------------------------------
+OZK_DEV i32x4 load8(const char *p, int n) {
+    i32x4 v = {0, 0, 0, 0};
+    if (n >= 8) {
+        __builtin_memcpy(&v, p, 16);   // of any alignment
+    } else {
+#pragma unroll 1
+        for (int i = n - 1; i >= 0; --i) push16(v, ((const uint16_t *)p)[i]);
+    }
+    return v;
+}
+OZK_DEV void store8(char *p, int n, i32x4 v) {
+    if (n >= 8) {
+        __builtin_memcpy(p, &v, 16);
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            ((uint16_t *)p)[i] = (uint16_t)v.x;
+            v = i32x4{(int)__builtin_amdgcn_alignbit((uint32_t)v.y, (uint32_t)v.x, 16),
+                      (int)__builtin_amdgcn_alignbit((uint32_t)v.z, (uint32_t)v.y, 16),
+                      (int)__builtin_amdgcn_alignbit((uint32_t)v.w, (uint32_t)v.z, 16),
+                      (int)((uint32_t)v.w >> 16)};
+        }
+    }
+}
+template <typename ST> OZK_DEV void unpack8(i32x4 v, float (&f)[8]) {
+    uint16_t e[8];
+    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = from_bits16(e[i], ST{});
+}
+template <typename ST> OZK_DEV i32x4 pack8(const float (&f)[8]) {
+    uint16_t e[8];
+    i32x4 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = to_bits16(f[i], ST{});
+    __builtin_memcpy(&v, e, 16);
+    return v;
+}
+
+// The epilogue of 8 sums of row m from column n on, `left` columns to N
+template <typename ST>
+OZK_DEV void finish8(const DenseParams &p, float (&v)[8], const float (&bias)[8], i32x4 res,
+                     int64_t m, int64_t n, int left) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += bias[i];
+    if (p.Z) {
+        // z is kept in 16 bits for the backward pass: act' moves by at most 0.32 2^-9
+        // (bf16) with it, as much as dy's own rounding.  A z that underflows keeps its
+        // side of 0, on which relu's derivative depends.
+        uint16_t e[8];
+        i32x4 z;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            e[i] = to_bits16(v[i], ST{});
+            if ((e[i] & 0x7FFF) == 0 && v[i] != 0.f) e[i] |= 1;
+        }
+        __builtin_memcpy(&z, e, 16);
+        store8(p.Z + (m * p.N + n) * 2, left, z);
+    }
+    with_act(p.act, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = activation<decltype(act)::value>(v[i]);
+    });
+    if (p.res) {
+        float r[8];
+        unpack8<ST>(res, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += r[i];
+    }
+    store8(p.C + m * p.c_pitch + n * 2, left, pack8<ST>(v));
+}
+template <typename ST>
+OZK_DEV void bias_at(const DenseParams &p, int64_t n, int left, float (&bias)[8]) {
+    unpack8<ST>(p.bias && left > 0 ? load8(p.bias + n * 2, left) : i32x4{0, 0, 0, 0}, bias);
+}
+template <typename ST>
+OZK_DEV i32x4 res_at(const DenseParams &p, int64_t m, int64_t n, int left) {
+    return p.res ? load8(p.res + m * p.r_pitch + n * 2, left) : i32x4{0, 0, 0, 0};
+}
+
+// A wave's part of a tile through the LDS, so that a lane has 8 columns of a row:
+// the epilogue's code is there once, not once per accumulator (128 values a lane
+// in the largest tile), its columns' bias stays in registers, and residual, Z and
+// C are read and written in whole lines.
+template <typename ST, typename Sh, typename Loop>
+OZK_DEV void finish_tile(const Loop &t, const DenseParams &p, char *smem, int64_t m0, int64_t n0) {
+    constexpr int MI = Sh::MI, NI = Sh::NI, CHUNKS = NI * 4;   // 16-byte pieces of an LDS row
+    constexpr int ROOM = Sh::LDS_BYTES / Sh::WAVES / (NI * 1024);
+    constexpr auto most = [](int room) {
+        int c = MI < room ? MI : room;
+        while (MI % c) --c;
+        return c;
+    };
+    constexpr int CI = most(ROOM);          // blocks of 16 rows at a time
+    constexpr int LANES = NI * 2, RPI = 64 / LANES;   // lanes of a row, rows of a wave's step
+    static_assert(ROOM >= 1 && (NI == 1 || NI == 2 || NI == 4), "");
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    m0 += wave / Sh::WN * MI * 16;
+    n0 += wave % Sh::WN * NI * 16 + lane % LANES * 8;
+    const int64_t over = p.N - n0;
+    const int left = over < 8 ? (int)(over < 0 ? 0 : over) : 8;
+    float bias[8];
+    bias_at<ST>(p, n0, left, bias);
+    f32x4 *buf = (f32x4 *)(smem + wave * CI * NI * 1024);
+    // 16-byte pieces XORed with the row: neither the writes (16 rows of one column)
+    // nor the reads (8 lanes to 256 bytes) meet in a bank
+    auto at = [&](int row, int chunk) {
+        const int x = NI == 4 ? row & 15 : NI == 2 ? (row >> 1) & 7 : (row >> 2) & 3;
+        return row * CHUNKS + (chunk ^ x);
+    };
+    auto settle = [] {   // LDS writes of the other lanes before reads, and back
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+#pragma unroll
+    for (int c = 0; c < MI / CI; ++c) {
+        if (c) settle();
+#pragma unroll
+        for (int i = 0; i < CI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                buf[at(i * 16 + (lane & 15), j * 4 + g)] = t.acc[c * CI + i][j];
+        settle();
+#pragma unroll 2
+        for (int r = 0; r < CI * 16; r += RPI) {
+            const int row = r + lane / LANES;
+            const int64_t m = m0 + c * CI * 16 + row;
+            const f32x4 lo = buf[at(row, lane % LANES * 2)], hi = buf[at(row, lane % LANES * 2 + 1)];
+            if (m < p.M && left > 0) {
+                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                finish8<ST>(p, v, bias, res_at<ST>(p, m, n0, left), m, n0, left);
+            }
+        }
+    }
+}
+
+template <typename ST, typename Sh, bool DMA>
+__global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void dense_kernel(DenseParams p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int BM = Sh::BM, BN = Sh::BN;
+    const uint32_t tiles_m = (uint32_t)((p.M + BM - 1) / BM), tiles_n = (uint32_t)((p.N + BN - 1) / BN);
+    const uint32_t each = tiles_m * tiles_n;
+    const int64_t tile = xcd_tile(blockIdx.x, each * (uint32_t)p.splits);
+    if (tile < 0) return;
+    // 8 tile rows at a time, column by column: the workgroups of an XCD share a
+    // square block of both operands in its L2
+    const uint32_t s = (uint32_t)tile / each, in = (uint32_t)tile - s * each;
+    const uint32_t first = in / tiles_n / 8 * 8;
+    const uint32_t high = tiles_m - first < 8 ? tiles_m - first : 8, ahead = in - first * tiles_n;
+    const uint32_t tn = ahead / high, tm = first + ahead - tn * high;
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int rows = (int)(p.M - m0 < BM ? p.M - m0 : BM);
+    const int cols = (int)(p.N - n0 < BN ? p.N - n0 : BN);
+    // the s-th range of K, whole stages each
+    int64_t k0 = 0, k1 = p.K;
+    if (p.splits > 1) {
+        const int64_t stages = (p.K + Sh::KS - 1) / Sh::KS;
+        const int64_t per = (stages + p.splits - 1) / p.splits * Sh::KS;
+        k0 = per * s < p.K ? per * s : p.K;
+        k1 = p.K - k0 < per ? p.K : k0 + per;
+    }
+    auto bytes = [](int64_t n, bool padded) { return padded ? (n + 7) / 8 * 16 : n * 2; };
+    auto source = [&](const char *base, int64_t pitch, bool cols_, bool padded, int64_t at, int n) {
+        return cols_ ? TileSrc{base + k0 * pitch + at * 2, pitch, (int)bytes(n, padded), k1 - k0, base}
+                     : TileSrc{base + at * pitch + k0 * 2, pitch, n, bytes(k1 - k0, padded), base};
+    };
+    TileLoop<ST, Sh, DMA> t;
+    const TileSrc A = source(p.A, p.a_pitch, Sh::ACOLS, p.a_padded, m0, rows);
+    const TileSrc B = source(p.B, p.b_pitch, Sh::BCOLS, p.b_padded, n0, cols);
+    const bool mine = t.run(A, B, smem);
+    if (p.splits > 1) {
+        if (!mine) return;
+        float *P = p.part + (int64_t)s * p.M * p.N + m0 * p.N + n0;
+        t.each([&](int m, int n, f32x4 v) {
+            if (m >= rows) return;
+            if (n + 4 <= cols) {
+                __builtin_memcpy(P + (int64_t)m * p.N + n, &v, 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < cols) P[(int64_t)m * p.N + n + i] = v[i];
+            }
+        });
+        return;
+    }
+    if constexpr (Sh::ACOLS) {   // a weight's gradient: nothing but the sums
+        if (mine) store_tile<ST>(t, p.C + m0 * p.c_pitch + n0 * 2, p.c_pitch, rows, cols);
+    } else {
+        __syncthreads();         // every wave has read its last stage
+        if (mine) finish_tile<ST, Sh>(t, p, smem, m0, n0);
+    }
+}
+
+// The K ranges' sums, added in order, and the epilogue: 8 columns a lane
+template <typename ST>
+__global__ __launch_bounds__(256) void dense_join_kernel(DenseParams p) {
+    const int64_t pieces = (p.N + 7) / 8, all = p.M * pieces, each = p.M * p.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / pieces, n = (i - m * pieces) * 8;
+        const int left = p.N - n < 8 ? (int)(p.N - n) : 8;
+        float v[8] = {}, bias[8];
+        const float *P = p.part + m * p.N + n;
+        for (int s = 0; s < p.splits; ++s, P += each) {
+            if (left == 8) {
+                f32x4 lo, hi;
+                __builtin_memcpy(&lo, P, 16);
+                __builtin_memcpy(&hi, P + 4, 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] += lo[e];
+                    v[e + 4] += hi[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < left) v[e] += P[e];
+            }
+        }
+        bias_at<ST>(p, n, left, bias);
+        finish8<ST>(p, v, bias, res_at<ST>(p, m, n, left), m, n, left);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// A few rows: bound by reading W once.  A workgroup has NT blocks of 16 rows of W
+// (columns of C) and all of x; its waves take 64 elements of K in turn, and their
+// sums are added in the LDS in order.  Operands go from memory into the matrix
+// cores' registers: a lane reads 32 consecutive bytes of a row, the four lanes of
+// a row a whole line.  The order along K is that of the lanes' bytes, the same for
+// both operands.
+// ---------------------------------------------------------------------------
+template <typename ST, int MT, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(DenseParams p) {
+    __shared__ __attribute__((aligned(16))) f32x4 join[WAVES][MT * NT][64];
+    const int lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t n0 = (int64_t)blockIdx.x * NT * 16;
+    // rows past the last read the last one, and are not stored
+    const char *W[NT], *X[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t n = n0 + j * 16 + i16;
+        W[j] = p.B + (n < p.N ? n : p.N - 1) * p.b_pitch + g * 32;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t m = i * 16 + i16;
+        X[i] = p.A + (m < p.M ? m : p.M - 1) * p.a_pitch + g * 32;
+    }
+    f32x4 acc[MT][NT] = {};
+    const int64_t bytes = p.K * 2;
+    auto piece = [&](const char *row, const char *first, int64_t at, bool whole) -> i32x4 {
+        i32x4 v;
+        if (whole) {
+            __builtin_memcpy(&v, row + at, 16);
+            return v;
+        }
+        const int64_t n = bytes - at - g * 32;
+        return load_piece(row + (n > 0 ? at : 0), n < 16 ? (int)(n < 0 ? 0 : n) : 16, first);
+    };
+    // U steps, 128 bytes of K each: all loads, then the products
+    auto steps = [&](int64_t at, auto u_, auto whole_) {
+        constexpr int U = decltype(u_)::value;
+        constexpr bool whole = decltype(whole_)::value;
+        i32x4 w[U][NT][2], x[U][MT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int64_t k = at + u * WAVES * 128 + 16 * h;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) w[u][j][h] = piece(W[j], p.B, k, whole);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) x[u][i][h] = piece(X[i], p.A, k, whole);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        acc[i][j] = mfma16(w[u][j][h], x[u][i][h], acc[i][j], ST{});
+    };
+    using std::integral_constant;
+    constexpr int U = MT + NT <= 3 ? 4 : 2;
+    int64_t at = (int64_t)wave * 128;
+    for (; at + (U - 1) * WAVES * 128 + 128 <= bytes; at += U * WAVES * 128)
+        steps(at, integral_constant<int, U>{}, std::true_type{});
+    for (; at + 128 <= bytes; at += WAVES * 128)
+        steps(at, integral_constant<int, 1>{}, std::true_type{});
+    if (at < bytes) steps(at, integral_constant<int, 1>{}, std::false_type{});
+
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) join[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    // a lane has 4 columns of a row: two of them make the 8 of the epilogue
+    for (int o = threadIdx.x; o < MT * NT * 32; o += 64 * WAVES) {
+        const int b = o / 32, row = o % 32 / 2, half = o % 2;
+        float v[8] = {};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const f32x4 s = join[w][b][(half * 2 + q) * 16 + row];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[q * 4 + e] += s[e];
+            }
+        const int64_t m = b / NT * 16 + row, n = n0 + b % NT * 16 + half * 8;
+        const int left = p.N - n < 8 ? (int)(p.N - n) : 8;
+        if (m < p.M && left > 0) {
+            float bias[8];
+            bias_at<ST>(p, n, left, bias);
+            finish8<ST>(p, v, bias, res_at<ST>(p, m, n, left), m, n, left);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// dz = dy act'(z), rounded to 16 bits as the matrix cores take it, and its column
+// sums (of the unrounded values) over the rows of a workgroup: 32 lanes with 8
+// columns each, 8 rows at a time.  Bound by memory: 6 bytes an element.
+// ---------------------------------------------------------------------------
+template <typename ST> __global__ __launch_bounds__(256) void dense_grad_kernel(DenseGradParams p) {
+    __shared__ float join[8][256];
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x % 32 * 8;
+    const int64_t m0 = (int64_t)blockIdx.y * p.rows;
+    const int64_t m1 = p.M - m0 < p.rows ? p.M : m0 + p.rows;
+    const int left = p.N - n < 8 ? (int)(p.N - n < 0 ? 0 : p.N - n) : 8;
+    float sum[8] = {};
+    if (left > 0) {
+        with_act(p.act, [&](auto act_) {
+            constexpr int ACT = decltype(act_)::value;
+#pragma unroll 2
+            for (int64_t m = m0 + threadIdx.x / 32; m < m1; m += 8) {
+                float d[8], z[8];
+                unpack8<ST>(load8(p.dy + m * p.dy_pitch + n * 2, left), d);
+                unpack8<ST>(load8(p.z + (m * p.N + n) * 2, left), z);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    d[i] *= i < left ? derivative<ACT>(z[i]) : 0.f;
+                    sum[i] += d[i];
+                }
+                if (p.dz) {
+                    const i32x4 v = pack8<ST>(d);
+                    __builtin_memcpy(p.dz + m * p.dz_pitch + n * 2, &v, 16);   // zeros behind N
+                }
+            }
+        });
+        if (p.act == OZK_ACT_NONE)
+#pragma unroll 2
+            for (int64_t m = m0 + threadIdx.x / 32; m < m1; m += 8) {
+                float d[8];
+                unpack8<ST>(load8(p.dy + m * p.dy_pitch + n * 2, left), d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] += d[i];
+            }
+    }
+    if (!p.sums) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) join[threadIdx.x / 32][threadIdx.x % 32 * 8 + i] = sum[i];
+    __syncthreads();
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c < p.N) {
+        float v = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v += join[r][threadIdx.x];
+        p.sums[(int64_t)blockIdx.y * p.N + c] = v;
+    }
+}
+// db: the workgroups' sums, added in 64 bits
+template <typename ST> __global__ __launch_bounds__(256) void dense_bias_kernel(DenseGradParams p) {
+    __shared__ double join[4][64];
+    const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x % 64;
+    const int64_t blocks = (p.M + p.rows - 1) / p.rows;
+    double v = 0.0;
+    if (c < p.N)
+#pragma unroll 4
+        for (int64_t b = threadIdx.x / 64; b < blocks; b += 4) v += (double)p.sums[b * p.N + c];
+    join[threadIdx.x / 64][threadIdx.x % 64] = v;
+    __syncthreads();
+    if (threadIdx.x < 64 && c < p.N) {
+        const int i = threadIdx.x;
+        store_value<ST>(p.db, c, (float)(join[0][i] + join[1][i] + join[2][i] + join[3][i]));
+    }
+}
+
+bool dense_few(const DenseParams &p) { return !p.a_cols && !p.b_cols && p.M <= 64; }
+
+namespace {
+
+bool whole_pieces(const void *p, int64_t pitch, int64_t cols, bool padded) {
+    return (((uintptr_t)p | (uintptr_t)pitch) & 15) == 0 && (padded || cols % 8 == 0);
+}
+bool pieces(const DenseParams &p) {
+    return whole_pieces(p.A, p.a_pitch, p.a_cols ? p.M : p.K, p.a_padded) &&
+           whole_pieces(p.B, p.b_pitch, p.b_cols ? p.N : p.K, p.b_padded);
+}
+int64_t tiles(const DenseParams &p, int64_t bm, int64_t bn) {
+    return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);
+}
+
+template <typename ST, typename Sh, bool DMA>
+hipError_t dense_go(const DenseParams &p, hipStream_t st) {
+    const int64_t all = tiles(p, Sh::BM, Sh::BN) * p.splits;
+    if (all >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
+    if (hipError_t e = allow_lds<&dense_kernel<ST, Sh, DMA>>(Sh::LDS_BYTES); e != hipSuccess) return e;
+    dense_kernel<ST, Sh, DMA><<<dim3((uint32_t)((all + 7) / 8 * 8)), Sh::THREADS, Sh::LDS_BYTES, st>>>(p);
+    return hipGetLastError();
+}
+template <typename ST, int MT, int NT> hipError_t few_go(const DenseParams &p, hipStream_t st) {
+    const int64_t blocks = (p.N + NT * 16 - 1) / (NT * 16);
+    if (blocks >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
+    dense_few_kernel<ST, MT, NT, 8><<<dim3((uint32_t)blocks), 512, 0, st>>>(p);
+    return hipGetLastError();
+}
+template <typename ST> hipError_t few_plan(const DenseParams &p, hipStream_t st) {
+    if (p.M <= 16) return few_go<ST, 1, 1>(p, st);
+    if (p.M <= 32) return few_go<ST, 2, 1>(p, st);
+    return few_go<ST, 4, 1>(p, st);
+}
+
+template <typename ST, bool AC, bool BC> hipError_t tile_plan(const DenseParams &p, hipStream_t st) {
+    if (!pieces(p)) return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 2, 2>, false>(p, st);
+    if (tiles(p, 256, 256) >= 256)
+        return dense_go<ST, TileShape<1, AC, BC, 256, 256, 2, 4, 2>, true>(p, st);
+    if (tiles(p, 128, 128) * p.splits >= 192)
+        return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 4, 2>, true>(p, st);
+    return dense_go<ST, TileShape<1, AC, BC, 64, 64, 2, 2, 2, 2>, true>(p, st);
+}
+template <typename ST> hipError_t dense_plan(const DenseParams &p, hipStream_t st) {
+    if (dense_few(p)) return few_plan<ST>(p, st);
+    hipError_t e = p.a_cols ? tile_plan<ST, true, true>(p, st)
+                 : p.b_cols ? tile_plan<ST, false, true>(p, st)
+                            : tile_plan<ST, false, false>(p, st);
+    if (e != hipSuccess || p.splits == 1) return e;
+    const int64_t blocks = (p.M * ((p.N + 7) / 8) + 255) / 256;
+    dense_join_kernel<ST><<<dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int dense_splits(const DenseParams &p) {
+    if (dense_few(p) || p.M == 0 || p.N == 0) return 1;
+    const int64_t n = tiles(p, 64, 64), stages = (p.K + 63) / 64;
+    int s = 1;
+    while (s < 16 && n * s < 256 && stages / (2 * s) >= 8) s *= 2;
+    return s;
+}
+
+hipError_t launch_dense(const DenseParams &p, int dtype, hipStream_t st) {
+    return dtype == OZK_F16 ? dense_plan<_Float16>(p, st) : dense_plan<__bf16>(p, st);
+}
+
+int64_t dense_grad_rows(int64_t M, int64_t N) {
+    // 128 rows, or so many that there are about 1024 workgroups
+    const int64_t across = (N + 255) / 256;
+    int64_t rows = 128;
+    while (rows > 8 && ((M + rows - 1) / rows) * across < 512) rows /= 2;
+    while ((M + rows - 1) / rows >= 32768) rows *= 2;
+    return rows;
+}
+hipError_t launch_dense_grad(const DenseGradParams &p, int dtype, hipStream_t st) {
+    const dim3 grid((uint32_t)((p.N + 255) / 256), (uint32_t)((p.M + p.rows - 1) / p.rows));
+    if (dtype == OZK_F16) dense_grad_kernel<_Float16><<<grid, 256, 0, st>>>(p);
+    else dense_grad_kernel<__bf16><<<grid, 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+hipError_t launch_dense_bias(const DenseGradParams &p, int dtype, hipStream_t st) {
+    const dim3 grid((uint32_t)((p.N + 63) / 64));
+    if (dtype == OZK_F16) dense_bias_kernel<_Float16><<<grid, 256, 0, st>>>(p);
+    else dense_bias_kernel<__bf16><<<grid, 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+}  // namespace ozk

@@ -1,0 +1,543 @@
+// ozk_route.hip -- the router of a layer of experts.
+//
+//   p = softmax(l) over the E experts; a token goes to the k experts of its
+//   greatest logits, of equal ones to those of the lowest index; their weights
+//   are their p, or with `normalize` their p over the sum of the k.
+//   counts[e] = tokens that chose e; offsets: their running sum, the groups of the
+//   grouped products; order: the slots t k + j sorted by expert, in their own
+//   order within one; place: the slots' places there.
+//   loss = E sum_e f_e P_e with f_e = counts[e] / (n k), P_e the mean of p[t, e],
+//   over the n tokens that are not masked out.  Masked ones have expert E, weight 0
+//   and the places behind the last group.
+//
+// Three launches: rows (softmax, choice, counts of each workgroup's tokens and
+// the slots' places among them), scan (the counts of the workgroups before) and
+// place (slots to their places); few tokens need one workgroup and one launch.
+// The sums over tokens are those of fixed parts in a fixed order, no atomics but
+// whole-number counts.
+//
+// A token takes GL lanes with V consecutive logits each, so that several share a
+// wave; the k choices are k rounds of a maximum over keys (the logits' bits in
+// the order of their values, NaN greatest) in lane exchanges.
+#include "../../include/ozaki_amd.h"
+#include "ozk_train.h"
+#include "ozk_tile.h"
+
+namespace ozk {
+
+// lane exchanges over groups of GL lanes: f(own, other's) of pairs that cover the group
+template <int GL, typename T, typename F> OZK_DEV T over_group(T v, F &&f) {
+    static_assert(sizeof(T) == 4, "");
+    auto dpp = [](T x, auto ctrl_) {
+        constexpr int ctrl = decltype(ctrl_)::value;
+        return __builtin_bit_cast(
+            T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), ctrl, 0xF, 0xF, true));
+    };
+    if constexpr (GL >= 2) v = f(v, dpp(v, std::integral_constant<int, 0xB1>{}));    // quad 1 0 3 2
+    if constexpr (GL >= 4) v = f(v, dpp(v, std::integral_constant<int, 0x4E>{}));    // quad 2 3 0 1
+    if constexpr (GL >= 8) v = f(v, dpp(v, std::integral_constant<int, 0x141>{}));   // mirror of 8
+    if constexpr (GL >= 16) v = f(v, dpp(v, std::integral_constant<int, 0x140>{}));  // mirror of 16
+    if constexpr (GL >= 32) {
+        const auto x = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v),
+                                                        __builtin_bit_cast(uint32_t, v), false, false);
+        v = f(__builtin_bit_cast(T, (uint32_t)x[0]), __builtin_bit_cast(T, (uint32_t)x[1]));
+    }
+    if constexpr (GL >= 64) {
+        const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                                        __builtin_bit_cast(uint32_t, v), false, false);
+        v = f(__builtin_bit_cast(T, (uint32_t)x[0]), __builtin_bit_cast(T, (uint32_t)x[1]));
+    }
+    return v;
+}
+template <int GL> OZK_DEV uint32_t group_max(uint32_t v) {
+    return over_group<GL>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+template <int GL> OZK_DEV uint32_t group_min(uint32_t v) {
+    return over_group<GL>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+template <int GL> OZK_DEV float group_sum(float v) {
+    return over_group<GL>(v, [](float a, float b) { return a + b; });
+}
+
+// Whole numbers in the order of the values: -0 as 0, NaN above all; 0 is below
+// every logit's.
+OZK_DEV uint32_t key_of(float x) {
+    if (x != x) return 0xFFFFFFFFu;
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+OZK_DEV float value_of(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+}
+
+// A token's V logits of a lane, from expert e0 on; -inf behind the last expert
+template <typename T, int V>
+OZK_DEV void logits_at(const char *row, int e0, int E, bool there, float (&l)[V]) {
+    if (there && e0 + V <= E) {
+        T t[V];
+        __builtin_memcpy(t, row + (int64_t)e0 * sizeof(T), V * sizeof(T));
+#pragma unroll
+        for (int v = 0; v < V; ++v) l[v] = (float)t[v];
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            l[v] = there && e0 + v < E ? load_value<T>(row, e0 + v) : -__builtin_inff();
+    }
+}
+
+constexpr int kRouteWaves = 16;   // of a workgroup
+
+// LDS of a workgroup: its slots' experts, those of each wave, sums
+struct RouteLds {
+    uint32_t *wave_hist;   // [waves][E + 1]
+    float *psum;           // [waves][E]
+    float *top;            // [per]: the greatest logit
+    float *scale;          // [per]: 1 over the sum that the weights are divided by
+    float *value;          // [per k]: the chosen logits
+    uint16_t *expert;      // [per k]
+    OZK_DEV RouteLds(char *at, int E, int64_t per, int k) {
+        wave_hist = (uint32_t *)at;
+        psum = (float *)(wave_hist + kRouteWaves * (E + 1));
+        top = psum + kRouteWaves * E;
+        scale = top + per;
+        value = scale + per;
+        expert = (uint16_t *)(value + per * k);
+    }
+    static size_t bytes(int E, int64_t per, int k) {
+        return 4 * (size_t)(kRouteWaves * (2 * E + 1)) + 8 * (size_t)per + 6 * (size_t)(per * k);
+    }
+};
+
+// Prefix sums over E values by the workgroup: v is that of index threadIdx.x (E
+// is at most the 1024 lanes); the sum of those before.
+OZK_DEV uint32_t before_in_block(uint32_t v, uint32_t *parts) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t s = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t u = __shfl_up(s, d);
+        if (lane >= d) s += u;
+    }
+    __syncthreads();
+    if (lane == 63) parts[wave] = s;
+    __syncthreads();
+    uint32_t before = s - v;
+    for (int w = 0; w < wave; ++w) before += parts[w];
+    return before;
+}
+
+// offsets, counts and the loss, by one workgroup; total and P: of expert threadIdx.x
+OZK_DEV void finish_counts(const RouteParams &p, uint32_t total, double P, uint32_t before,
+                           uint32_t *parts) {
+    const int e = threadIdx.x, lane = threadIdx.x & 63;
+    if (e < p.E) {
+        p.counts[e] = (int32_t)total;
+        p.offsets[e] = (int32_t)before;
+        if (e == p.E - 1) p.offsets[p.E] = (int32_t)(before + total);
+    }
+    // sum over e of counts P
+    double s = e < p.E ? (double)total * P : 0.0;
+    double n = e < p.E ? (double)total : 0.0;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        s += __shfl_xor(s, d);
+        n += __shfl_xor(n, d);
+    }
+    double *sums = (double *)parts;   // [2][waves]
+    __syncthreads();
+    if (lane == 0) {
+        sums[threadIdx.x >> 6] = s;
+        sums[kRouteWaves + (threadIdx.x >> 6)] = n;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = n = 0.0;
+        for (int w = 0; w < kRouteWaves; ++w) {
+            s += sums[w];
+            n += sums[kRouteWaves + w];
+        }
+        // n: slots, k to a token
+        const double tokens = n / p.k;
+        *p.loss = n > 0.0 ? (float)(p.E * s / (n * tokens)) : 0.f;
+    }
+}
+
+template <typename T, int GL, int V, bool ONE>
+__global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteParams p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ __attribute__((aligned(16))) uint32_t parts[4 * kRouteWaves];
+    const RouteLds lds(smem, p.E, p.per, p.k);
+    constexpr int TPW = 64 / GL;   // tokens of a wave at a time
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int in = lane % GL, e0 = in * V;
+    const int64_t t0 = (int64_t)blockIdx.x * p.per;
+    const int tokens = (int)(p.T - t0 < p.per ? p.T - t0 : p.per);
+    for (int i = threadIdx.x; i < kRouteWaves * (p.E + 1); i += 64 * kRouteWaves) lds.wave_hist[i] = 0;
+
+    float psum[V] = {};
+    for (int r = wave * TPW; r < tokens; r += kRouteWaves * TPW) {
+        const int t = r + lane / GL;
+        const bool there = t < tokens;
+        const bool valid = there && (!p.mask || p.mask[t0 + t]);
+        float l[V];
+        logits_at<T, V>(p.logits + (t0 + t) * p.pitch * (int64_t)sizeof(T), e0, p.E, valid, l);
+        uint32_t key[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = e0 + v < p.E ? key_of(l[v]) : 0u;
+        float top = 0.f, chosen = 0.f;
+        for (int j = 0; j < p.k; ++j) {
+            uint32_t best = key[0];
+#pragma unroll
+            for (int v = 1; v < V; ++v) best = key[v] > best ? key[v] : best;
+            best = group_max<GL>(best);
+            uint32_t at = 0xFFFFu;
+#pragma unroll
+            for (int v = V - 1; v >= 0; --v) at = key[v] == best ? (uint32_t)(e0 + v) : at;
+            at = group_min<GL>(at);
+#pragma unroll
+            for (int v = 0; v < V; ++v) key[v] = (uint32_t)(e0 + v) == at ? 0u : key[v];
+            const float x = value_of(best);
+            if (j == 0) top = x;
+            chosen += expf(x - top);
+            if (in == 0 && there) {
+                lds.value[t * p.k + j] = x;
+                lds.expert[t * p.k + j] = (uint16_t)(valid ? at : (uint32_t)p.E);
+            }
+        }
+        float q[V], sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            q[v] = e0 + v < p.E ? expf(l[v] - top) : 0.f;
+            sum += q[v];
+        }
+        sum = group_sum<GL>(sum);
+        if (in == 0 && there) {
+            lds.top[t] = top;
+            lds.scale[t] = p.normalize ? chosen : sum;
+        }
+        if (valid) {
+            const float by = 1.f / sum;
+#pragma unroll
+            for (int v = 0; v < V; ++v) psum[v] += q[v] * by;
+        }
+    }
+    // the wave's sums of p: the lanes that hold the same experts
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float s = psum[v];
+        for (int d = GL; d < 64; d <<= 1) s += __shfl_xor(s, d);
+        if (lane < GL && e0 + v < p.E) lds.psum[wave * p.E + e0 + v] = s;
+    }
+    __syncthreads();
+
+    // each wave a range of the slots, in order: weights, and how often each expert
+    const int slots = tokens * p.k;
+    const int range = (slots + kRouteWaves * 64 - 1) / (kRouteWaves * 64) * 64;
+    const int lo = wave * range, hi = lo + range < slots ? lo + range : slots;
+    uint32_t *hist = lds.wave_hist + wave * (p.E + 1);
+    const int64_t s0 = t0 * p.k;
+    for (int i = lo + lane; i < hi; i += 64) {
+        const int t = (int)((uint32_t)i / (uint32_t)p.k), e = lds.expert[i];
+        atomicAdd(&hist[e], 1u);
+        p.experts[s0 + i] = e;
+        p.weights[s0 + i] = e == p.E ? 0.f : expf(lds.value[i] - lds.top[t]) / lds.scale[t];
+    }
+    __syncthreads();
+    // over the waves, in order; the workgroup's counts and sums
+    uint32_t total = 0;
+    double P = 0.0;
+    if ((int)threadIdx.x <= p.E) {
+        const int e = threadIdx.x;
+#pragma unroll
+        for (int w = 0; w < kRouteWaves; ++w) {
+            uint32_t *h = &lds.wave_hist[w * (p.E + 1) + e];
+            const uint32_t n = *h;
+            *h = total;
+            total += n;
+        }
+        if (e < p.E) {
+#pragma unroll
+            for (int w = 0; w < kRouteWaves; ++w) P += (double)lds.psum[w * p.E + e];
+            if constexpr (!ONE) {
+                p.hist[(int64_t)blockIdx.x * p.E + e] = total;
+                p.psum[(int64_t)blockIdx.x * p.E + e] = (float)P;
+            }
+        }
+    }
+    if (p.E == 64 * kRouteWaves) {   // the masked ones' column has no lane of its own
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t n = 0;
+            for (int w = 0; w < kRouteWaves; ++w) {
+                uint32_t *h = &lds.wave_hist[w * (p.E + 1) + p.E];
+                const uint32_t m = *h;
+                *h = n;
+                n += m;
+            }
+        }
+    }
+    if constexpr (ONE) {
+        __shared__ uint32_t last;   // where the groups end
+        const uint32_t before = before_in_block((int)threadIdx.x < p.E ? total : 0u, parts);
+        if ((int)threadIdx.x == p.E - 1) last = before + total;
+        finish_counts(p, total, P, before, parts);
+        __syncthreads();
+        if ((int)threadIdx.x < p.E)
+#pragma unroll
+            for (int w = 0; w < kRouteWaves; ++w) lds.wave_hist[w * (p.E + 1) + threadIdx.x] += before;
+        if (threadIdx.x < kRouteWaves) lds.wave_hist[threadIdx.x * (p.E + 1) + p.E] += last;
+    }
+    __syncthreads();
+    // the slots' places: those of the same expert before the range, then before it in it
+    const int bits = 32 - __builtin_clz(p.E);
+    for (int i0 = lo; i0 < hi; i0 += 64) {
+        const int i = i0 + lane;
+        const bool there = i < hi;
+        const uint32_t e = there ? lds.expert[i] : 0xFFFFu;
+        uint64_t same = __ballot(there);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t set = __ballot(e >> b & 1);
+            same &= e >> b & 1 ? set : ~set;
+        }
+        if (there) {
+            const uint32_t rank = (uint32_t)__popcll(same & (((uint64_t)1 << lane) - 1));
+            const uint32_t at = hist[e] + rank;
+            p.place[s0 + i] = (int32_t)at;
+            if constexpr (ONE) p.order[at] = (int32_t)i;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (rank == 0) hist[e] = at + (uint32_t)__popcll(same);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// One workgroup to 16 experts: hist[b, e] becomes the slots of e in the workgroups
+// before b; the totals go to counts, the sums of p to psum's first row.
+__global__ __launch_bounds__(1024) void route_scan_kernel(RouteParams p) {
+    __shared__ uint32_t sums[64][17];
+    __shared__ double ps[64][17];
+    const int e = blockIdx.x * 16 + threadIdx.x % 16, part = threadIdx.x / 16;
+    const int each = (p.blocks + 63) / 64, lo = part * each;
+    const int hi = lo + each < p.blocks ? lo + each : p.blocks;
+    uint32_t n = 0;
+    double P = 0.0;
+    if (e < p.E)
+        for (int b = lo; b < hi; ++b) {
+            n += p.hist[(int64_t)b * p.E + e];
+            P += (double)p.psum[(int64_t)b * p.E + e];
+        }
+    sums[part][threadIdx.x % 16] = n;
+    ps[part][threadIdx.x % 16] = P;
+    __syncthreads();
+    uint32_t before = 0;
+    for (int q = 0; q < part; ++q) before += sums[q][threadIdx.x % 16];
+    if (e < p.E) {
+        for (int b = lo; b < hi; ++b) {
+            uint32_t *h = &p.hist[(int64_t)b * p.E + e];
+            const uint32_t m = *h;
+            *h = before;
+            before += m;
+        }
+        if (part == 63) {
+            p.counts[e] = (int32_t)before;
+            P = 0.0;
+            for (int q = 0; q < 64; ++q) P += ps[q][threadIdx.x % 16];
+            p.psum[e] = (float)P;
+        }
+    }
+}
+
+__global__ __launch_bounds__(1024) void route_place_kernel(RouteParams p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ __attribute__((aligned(16))) uint32_t parts[4 * kRouteWaves];
+    uint32_t *start = (uint32_t *)smem;   // [E + 1]
+    const int e = threadIdx.x;
+    const uint32_t total = e < p.E ? (uint32_t)p.counts[e] : 0u;
+    const uint32_t before = before_in_block(total, parts);
+    if (blockIdx.x == 0) finish_counts(p, total, e < p.E ? (double)p.psum[e] : 0.0, before, parts);
+    if (e < p.E) {
+        start[e] = before + p.hist[(int64_t)blockIdx.x * p.E + e];
+        if (e == p.E - 1) {
+            // behind the last group, and the masked slots of the workgroups before: all
+            // of their slots less those of the experts
+            start[p.E] = before + total;
+        }
+    }
+    __syncthreads();
+    const int64_t t0 = (int64_t)blockIdx.x * p.per, s0 = t0 * p.k;
+    const int tokens = (int)(p.T - t0 < p.per ? p.T - t0 : p.per), slots = tokens * p.k;
+    if (p.mask) {
+        // the workgroups' slots before this one that have an expert
+        uint32_t n = e < p.E ? p.hist[(int64_t)blockIdx.x * p.E + e] : 0u;
+        const uint32_t upto = before_in_block(n, parts) + n;
+        __syncthreads();
+        if (e == 64 * kRouteWaves - 1) start[p.E] += (uint32_t)s0 - upto;
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < slots; i += 1024) {
+        const uint32_t at = start[p.experts[s0 + i]] + (uint32_t)p.place[s0 + i];
+        p.place[s0 + i] = (int32_t)at;
+        p.order[at] = (int32_t)(s0 + i);
+    }
+}
+
+// The logits' gradient.  With q = softmax(l), c_e the counts and n the tokens:
+//   dl = q (g - sum q g), g_e = dloss E c_e / (n k n), and
+//   normalised weights (a softmax over the chosen): dl at them += w (dw - sum w dw)
+//   others (q at the chosen): g at them += dw
+template <typename T, int GL, int V>
+__global__ __launch_bounds__(256) void route_grad_kernel(RouteGradParams p) {
+    constexpr int TPW = 64 / GL;
+    const int lane = threadIdx.x & 63, in = lane % GL, e0 = in * V;
+    float g0[V] = {};
+    if (p.dloss) {
+        uint32_t c[V], sum = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            c[v] = e0 + v < p.E ? (uint32_t)p.counts[e0 + v] : 0u;
+            sum += c[v];
+        }
+        sum = over_group<GL>(sum, [](uint32_t a, uint32_t b) { return a + b; });
+        const double n = (double)sum / p.k;
+        const double by = sum ? (double)*p.dloss * p.E / ((double)sum * n) : 0.0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) g0[v] = (float)(by * (double)c[v]);
+    }
+    const int64_t step = (int64_t)gridDim.x * 4 * TPW;
+    for (int64_t r = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * TPW; r < p.T; r += step) {
+        const int64_t t = r + lane / GL;
+        const bool there = t < p.T, valid = there && (!p.mask || p.mask[t]);
+        float l[V], g[V], d[V] = {};
+        logits_at<T, V>(p.logits + t * p.pitch * (int64_t)sizeof(T), e0, p.E, valid, l);
+        float top = l[0];
+        bool nan = l[0] != l[0];
+#pragma unroll
+        for (int v = 1; v < V; ++v) {
+            top = l[v] > top ? l[v] : top;
+            nan |= l[v] != l[v];
+        }
+        // (max as whole numbers orders by value, too; NaN is carried by the sums)
+        top = over_group<GL>(nan ? __builtin_inff() : top, [](float a, float b) { return a > b ? a : b; });
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            l[v] = e0 + v < p.E ? expf(l[v] - top) : 0.f;
+            sum += l[v];
+            g[v] = g0[v];
+        }
+        sum = group_sum<GL>(sum);
+        const float by = 1.f / sum;
+        if (p.dw && valid) {
+            const int64_t s = t * p.k;
+            float mean = 0.f;
+            if (p.normalize)
+                for (int j = 0; j < p.k; ++j) mean = fmaf(p.weights[s + j], p.dw[s + j], mean);
+            for (int j = 0; j < p.k; ++j) {
+                const int e = p.experts[s + j];
+                const float dw = p.dw[s + j];
+                const float add = p.normalize ? p.weights[s + j] * (dw - mean) : dw;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (p.normalize) d[v] += e == e0 + v ? add : 0.f;
+                    else g[v] += e == e0 + v ? add : 0.f;
+                }
+            }
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            l[v] *= by;
+            dot = fmaf(l[v], e0 + v < p.E ? g[v] : 0.f, dot);
+        }
+        dot = group_sum<GL>(dot);
+        if (!there) continue;
+#pragma unroll
+        for (int v = 0; v < V; ++v) d[v] = valid ? fmaf(l[v], g[v] - dot, d[v]) : 0.f;
+        char *out = p.dlogits + t * p.E * (int64_t)sizeof(T);
+        if (e0 + V <= p.E) {
+            T o[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] = (T)d[v];
+            __builtin_memcpy(out + (int64_t)e0 * sizeof(T), o, V * sizeof(T));
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (e0 + v < p.E) store_value<T>(out, e0 + v, d[v]);
+        }
+    }
+}
+
+namespace {
+
+// lanes of a token and values of a lane, by E
+template <typename F> hipError_t with_shape(int E, F &&f) {
+    using std::integral_constant;
+#define OZK_ROUTE(GL, V) return f(integral_constant<int, GL>{}, integral_constant<int, V>{})
+    if (E <= 8) OZK_ROUTE(2, 4);
+    if (E <= 16) OZK_ROUTE(4, 4);
+    if (E <= 32) OZK_ROUTE(8, 4);
+    if (E <= 64) OZK_ROUTE(16, 4);
+    if (E <= 128) OZK_ROUTE(32, 4);
+    if (E <= 256) OZK_ROUTE(64, 4);
+    if (E <= 512) OZK_ROUTE(64, 8);
+    OZK_ROUTE(64, 16);
+#undef OZK_ROUTE
+}
+int lanes_of(int E) { return E <= 8 ? 2 : E <= 16 ? 4 : E <= 32 ? 8 : E <= 64 ? 16 : E <= 128 ? 32 : 64; }
+
+template <typename T> hipError_t route_go(const RouteParams &p, hipStream_t st) {
+    return with_shape(p.E, [&](auto gl, auto v) {
+        constexpr int GL = decltype(gl)::value, V = decltype(v)::value;
+        const size_t lds = RouteLds::bytes(p.E, p.per, p.k);
+        if (p.blocks == 1) {
+            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, true>>((int)lds); e != hipSuccess)
+                return e;
+            route_rows_kernel<T, GL, V, true><<<1, 64 * kRouteWaves, lds, st>>>(p);
+        } else {
+            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, false>>((int)lds); e != hipSuccess)
+                return e;
+            route_rows_kernel<T, GL, V, false><<<(uint32_t)p.blocks, 64 * kRouteWaves, lds, st>>>(p);
+        }
+        return hipGetLastError();
+    });
+}
+template <typename T> hipError_t route_grad_go(const RouteGradParams &p, hipStream_t st) {
+    return with_shape(p.E, [&](auto gl, auto v) {
+        constexpr int GL = decltype(gl)::value, V = decltype(v)::value;
+        const int64_t blocks = (p.T + 4 * (64 / GL) - 1) / (4 * (64 / GL));
+        route_grad_kernel<T, GL, V><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(p);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace
+
+void plan_route(RouteParams &p) {
+    // a workgroup's tokens: one step of its waves, more where that makes more
+    // than 256 of them, as many as its LDS holds
+    const int64_t step = (int64_t)kRouteWaves * 64 / lanes_of(p.E);
+    int64_t per = step, most = (150 * 1024 - (int64_t)RouteLds::bytes(p.E, 0, 0)) / (8 + 6 * p.k);
+    while (per < most / 2 && (p.T + per - 1) / per > 256) per *= 2;
+    if (per > most) per = most;
+    p.per = per;
+    p.blocks = p.T > per ? (int)((p.T + per - 1) / per) : 1;
+}
+
+hipError_t launch_route(const RouteParams &p, int dtype, hipStream_t st) {
+    hipError_t e = dtype == OZK_F32   ? route_go<float>(p, st)
+                   : dtype == OZK_F16 ? route_go<_Float16>(p, st)
+                                      : route_go<__bf16>(p, st);
+    if (e != hipSuccess || p.blocks == 1) return e;
+    route_scan_kernel<<<(uint32_t)((p.E + 15) / 16), 1024, 0, st>>>(p);
+    if (e = hipGetLastError(); e != hipSuccess) return e;
+    route_place_kernel<<<(uint32_t)p.blocks, 1024, 4 * (p.E + 1), st>>>(p);
+    return hipGetLastError();
+}
+hipError_t launch_route_grad(const RouteGradParams &p, int dtype, hipStream_t st) {
+    return dtype == OZK_F32   ? route_grad_go<float>(p, st)
+           : dtype == OZK_F16 ? route_grad_go<_Float16>(p, st)
+                              : route_grad_go<__bf16>(p, st);
+}
+
+}  // namespace ozk

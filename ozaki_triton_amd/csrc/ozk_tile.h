@@ -1,6 +1,6 @@
 // ozk_tile.h -- one C tile of a 16-bit matrix product on the matrix cores, for
-// the grouped products (ozk_grouped.hip) and the orthogonalisation
-// (ozk_orth.hip).
+// the grouped products (ozk_grouped.hip), the dense ones (ozk_dense.hip) and the
+// orthogonalisation (ozk_orth.hip).
 //
 //   C[m, n] = sum_k A[m, k] B[n, k], accumulated in fp32
 //
@@ -607,6 +607,52 @@ OZK_DEV int64_t xcd_tile(uint32_t block, uint32_t total) {
     const uint32_t per = (total + 7) / 8, i = block / 8;
     const uint32_t t = (block % 8) * per + i;
     return i < per && t < total ? (int64_t)t : -1;
+}
+
+// The tile's values, rounded, to C [rows, cols]
+template <typename ST, typename Loop>
+OZK_DEV void store_tile(const Loop &t, char *C, int64_t pitch, int rows, int cols) {
+    auto bits = [](f32x4 v) {
+        uint16_t e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = to_bits16(v[i], ST{});
+        i32x2 u;
+        __builtin_memcpy(&u, e, 8);
+        return u;
+    };
+    auto put = [&](int m, int n, i32x2 u) {   // columns n .. n + 3
+        uint16_t e[4];
+        __builtin_memcpy(e, &u, 8);
+        uint16_t *to = (uint16_t *)(C + m * pitch) + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (m < rows && n + i < cols) to[i] = e[i];
+    };
+    if constexpr (Loop::NI % 2 == 0) {
+        const int g = (threadIdx.x >> 4) & 3;
+        t.each_pair([&](int m, int n, f32x4 lo, f32x4 hi) {
+            const i32x2 a = bits(lo), b = bits(hi);
+            const int n32 = n - 4 * g;
+            if (n32 + 32 <= cols) {
+                const i32x4 v = join_pair(a, b);
+                // (rows of any alignment)
+                if (m < rows)
+                    __builtin_memcpy(C + m * pitch + (n32 + pair_column(g)) * 2, &v, 16);
+            } else {
+                put(m, n, a);
+                put(m, n + 16, b);
+            }
+        });
+    } else {
+        t.each([&](int m, int n, f32x4 v) {
+            const i32x2 u = bits(v);
+            if (n + 4 <= cols) {
+                if (m < rows) __builtin_memcpy(C + m * pitch + n * 2, &u, 8);
+            } else {
+                put(m, n, u);
+            }
+        });
+    }
 }
 
 }  // namespace ozk

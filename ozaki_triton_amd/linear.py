@@ -5,7 +5,9 @@ reference):
   expert's matrix; differentiable, ``grouped_matmul_backward`` on its own;
 * ``quantize_w4`` / ``dequantize_w4`` / ``matmul_w4``: weights of 4 bits in groups
   with scales, and their product with a few rows of activations;
-* ``orthogonalize(G)``: the Newton-Schulz orthogonalisation of an update.
+* ``orthogonalize(G)``: the Newton-Schulz orthogonalisation of an update;
+* ``fused_linear(x, W, bias, activation=, residual=)``: the dense product with its
+  epilogue, differentiable.
 
 All arithmetic runs in the HIP kernels of libozaki_amd.so (C ABI:
 include/ozaki_amd.h), on the tensors' device and its current stream; nothing
@@ -16,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 
 import torch
 from torch.autograd import forward_ad
@@ -420,3 +423,139 @@ def orthogonalize(G: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750
           _i64(*G3.stride()[:2]), flat, steps, float(eps), out.data_ptr(), _i64(M * N, N), wsp, n)
     del ws
     return out.view(G.shape)
+
+
+# ============================================================
+# dense products with an epilogue
+# ============================================================
+
+_ACTIVATIONS = {None: _lib.OZK_ACT_NONE, "relu": _lib.OZK_ACT_RELU, "gelu": _lib.OZK_ACT_GELU,
+                "gelu_tanh": _lib.OZK_ACT_GELU_TANH, "silu": _lib.OZK_ACT_SILU}
+
+
+def _linear_checks(x, W, bias, activation, residual):
+    assert x.dim() >= 1 and W.dim() == 2 and x.shape[-1] == W.shape[1], \
+        f"x must be [..., K] and W [N, K], got {tuple(x.shape)} and {tuple(W.shape)}"
+    assert activation in _ACTIVATIONS, \
+        f"activation must be one of {', '.join(map(repr, _ACTIVATIONS))}, got {activation!r}"
+    N, dtype = W.shape[0], x.dtype
+    assert W.dtype == dtype, f"x/W dtype mismatch: {dtype} vs {W.dtype}"
+    assert bias is None or (bias.shape == (N,) and bias.dtype == dtype), \
+        f"bias must be {(N,)} {dtype}, got {tuple(bias.shape)} {bias.dtype}"
+    want = (*x.shape[:-1], N)
+    assert residual is None or (residual.shape == want and residual.dtype == dtype), \
+        f"residual must be {want} {dtype}, got {tuple(residual.shape)} {residual.dtype}"
+    _on_one_gpu(x, W, bias, residual)
+    _require_dtype("fused_linear", dtype, _HALF)
+
+
+def _weight(W):
+    """W [N, K] with K or N contiguous, and its strides, the contiguous one 1."""
+    (N, K), (s_n, s_k) = W.shape, W.stride()
+    if (s_k == 1 or K <= 1) and (s_n < _MAX_STRIDE or N <= 1):
+        return W, (s_n if N > 1 else 0, 1)
+    if (s_n == 1 or N <= 1) and s_k < _MAX_STRIDE:
+        return W, (1, s_k)
+    return W.contiguous(), (K, 1)
+
+
+def _linear_forward(x, W, bias, residual, act, want_z):
+    """y for x [M, K], and where wanted what act is applied to."""
+    M, K = x.shape
+    N, dtype, dev = W.shape[0], x.dtype, x.device
+    x, sx = _rows(x)
+    W, sw = _weight(W)
+    if bias is not None and bias.stride(0) != 1:
+        bias = bias.contiguous()
+    rp = sr = 0
+    if residual is not None:
+        residual, sr = _rows(residual)
+        rp = residual.data_ptr()
+    y = x.new_empty((M, N))
+    z = x.new_empty((M, N)) if want_z else None
+    xp, wp = x.data_ptr(), W.data_ptr()
+    n = _bytes("ozk_linear_workspace_bytes", xp & 15, sx, wp & 15, sw, M, N, K)
+    ws, wsp = _workspace(n, dev)
+    _call("ozk_linear", dev, xp, sx, wp, _i64(*sw), None if bias is None else bias.data_ptr(),
+          rp or None, sr, act, M, N, K, _TORCH_TO_OZK[dtype], y.data_ptr(), N,
+          z.data_ptr() if want_z else None, wsp, n)
+    del ws
+    return y, z
+
+
+def _linear_backward(dy, z, x, W, act, want):
+    """The gradients (dx, dW, db) that `want`, three truth values, asks for; x or W
+    may be None where only the other's is wanted."""
+    M, N = dy.shape
+    K = (x if W is None else W).shape[1] if x is not None or W is not None else 0
+    dev, dtype = dy.device, dy.dtype
+    dy, sy = _rows(dy)
+    (x, sx) = _rows(x) if x is not None else (None, 0)
+    (W, sw) = _weight(W) if W is not None else (None, (0, 1))
+    dx = dy.new_empty((M, K)) if want[0] else None
+    dW = dy.new_empty((N, K)) if want[1] else None
+    db = dy.new_empty((N,)) if want[2] else None
+    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+    align = lambda t: 0 if t is None else t.data_ptr() & 15   # noqa: E731
+    mask = want[0] | want[1] << 1 | want[2] << 2
+    n = _bytes("ozk_linear_backward_workspace_bytes", align(dy), sy, align(x), sx, align(W), sw, act,
+               M, N, K, mask)
+    ws, wsp = _workspace(n, dev)
+    _call("ozk_linear_backward", dev, ptr(dy), sy, ptr(z), ptr(x), sx, ptr(W), _i64(*sw), act, M, N,
+          K, _TORCH_TO_OZK[dtype], ptr(dx), K, ptr(dW), K, ptr(db), wsp, n)
+    del ws
+    return dx, dW, db
+
+
+class _FusedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, W, bias, residual, act):
+        need = ctx.needs_input_grad
+        y, z = _linear_forward(x, W, bias, residual, act, act != 0 and any(need[:3]))
+        ctx.save_for_backward(x if need[1] else None, W if need[0] else None, z)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, W, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grads = (None, None, None)
+        if any(need[:3]):
+            grads = _linear_backward(dy, z, x, W, ctx.act, need[:3])
+        return (*grads, dy if need[3] else None, None)
+
+
+def fused_linear(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor | None = None, *,
+                 activation: str | None = None,
+                 residual: torch.Tensor | None = None) -> torch.Tensor:
+    """y = activation(x @ W^T + bias) + residual in one pass over the operands.
+
+    Args:
+        x: (..., K) float16 / bfloat16, from one token to long batches
+        W: (N, K), dtype of x; a transposed view (N contiguous) is read in place
+        bias: (N,), dtype of x
+        activation: None, "relu", "gelu" (z Phi(z)), "gelu_tanh" or "silu"
+        residual: (..., N), dtype of x, added after the activation
+    Returns:
+        y: (..., N), dtype of x; sums and epilogue in float32, rounded once.
+        Differentiable in x, W, bias and residual (reverse mode, once): the backward
+        pass keeps x W^T + bias in x's dtype where there is an activation, and the
+        gradient to it is rounded to that dtype.
+    """
+    _linear_checks(x, W, bias, activation, residual)
+    _no_tangent("fused_linear", x, W, bias, residual)
+    act = _ACTIVATIONS[activation]
+    shape = x.shape
+    if len(shape) != 2:
+        M = math.prod(shape[:-1])
+        x = x.reshape(M, shape[-1])
+        residual = None if residual is None else residual.reshape(M, W.shape[0])
+    if torch.is_grad_enabled() and (
+            x.requires_grad or W.requires_grad or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad)):
+        y = _FusedLinear.apply(x, W, bias, residual, act)
+    else:
+        y, _ = _linear_forward(x, W, bias, residual, act, False)
+    return y if len(shape) == 2 else y.view(*shape[:-1], W.shape[0])

@@ -1,0 +1,375 @@
+"""fused_linear and its gradients against the formula in 64 bits.
+
+u = 2^-24 is half a step of fp32, h half a step of the dtype, both relative.  A sum
+of n products in fp32, in any order, is off by at most n u times the sum of their
+sizes; activations by their slope (at most 1.13) times that and 2^-18 |z| of their
+own (exp2's argument, the fitted tail); each rounding to the dtype by h."""
+import math
+
+import pytest
+import torch
+
+import ozaki_triton_amd as ozk
+
+pytestmark = pytest.mark.gpu
+
+BF, F16 = torch.bfloat16, torch.float16
+U = 2.0 ** -24
+ACTS = (None, "relu", "gelu", "gelu_tanh", "silu")
+
+
+def _act(z, act):
+    """act(z) and its derivative in 64 bits."""
+    if act is None:
+        return z, torch.ones_like(z)
+    if act == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    if act == "gelu":
+        below = 0.5 * torch.erfc(z * -math.sqrt(0.5))   # (1 + erf loses the lower tail)
+        return z * below, below + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    t = torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+    slope = math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z * z)
+    return 0.5 * z * (1 + t), 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * slope
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2, torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+
+
+def _inputs(M, N, K, dtype, seed=0, wt=False, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x, W, b, res = scale * r(M, K), r(N, K) / math.sqrt(max(K, 1)), r(N), r(M, N)
+    x, W, b, res, dy = (t.to(dtype) for t in (x, W, b, res, r(M, N)))
+    return x, W.mT.contiguous().mT if wt else W, b, res, dy
+
+
+def _check(y, x, W, b, res, act):
+    K, (h, least) = x.shape[-1], _half(x.dtype)
+    xd, Wd = x.double(), W.double().mT.contiguous()
+    z, size = xd @ Wd, xd.abs() @ Wd.abs()
+    if b is not None:
+        z, size = z + b.double(), size + b.double().abs()
+    want, _ = _act(z, act)
+    tol = 1.13 * (K + 4) * U * size + 2 ** -18 * z.abs()
+    if res is not None:
+        want = want + res.double()
+    tol = tol + (h + 2 * U) * (want.abs() + tol) + least
+    if res is not None:
+        tol = tol + U * res.double().abs()
+    off = (y.double() - want).abs()
+    assert y.shape == want.shape and y.dtype == x.dtype
+    assert bool((off <= tol).all()), float((off / tol).max())
+
+
+SHAPES = [
+    (1, 4096, 4096), (1, 1, 1), (1, 17, 100), (3, 1000, 2047), (16, 64, 512), (17, 250, 129), (31, 96, 8),
+    (33, 512, 1000), (64, 40, 4100), (65, 128, 256), (100, 1, 72), (128, 256, 4096), (200, 72, 2056),
+    (257, 300, 64), (500, 1030, 200), (1999, 520, 1000), (1024, 2048, 1024), (4096, 4100, 136),
+    (700, 333, 1001), (90, 90, 4097), (2300, 8, 3000), (70, 2000, 7)]
+
+
+@pytest.mark.parametrize("M, N, K", SHAPES)
+@pytest.mark.parametrize("wt", [False, True])
+def test_products(gpu, M, N, K, wt):
+    for dtype in (BF, F16):
+        x, W, b, res, _ = _inputs(M, N, K, dtype, seed=M + N, wt=wt)
+        _check(ozk.fused_linear(x, W), x, W, None, None, None)
+        act = ACTS[(M + N + K) % 5]
+        y = ozk.fused_linear(x, W, b, activation=act, residual=res)
+        _check(y, x, W, b, res, act)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M, N, K", [(2, 300, 64), (150, 200, 96), (130, 64, 8192), (8192, 2050, 64)])
+def test_epilogues(gpu, M, N, K, act):
+    for dtype in (BF, F16):
+        x, W, b, res, _ = _inputs(M, N, K, dtype, seed=1, scale=3.0)
+        for bias in (None, b):
+            for residual in (None, res):
+                y = ozk.fused_linear(x, W, bias, activation=act, residual=residual)
+                _check(y, x, W, bias, residual, act)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_over_their_range(gpu, act):
+    """x W^T = x where W is one column of 1: the activation alone, at every value."""
+    for dtype in (BF, F16):
+        bits = torch.arange(-32768, 32768, dtype=torch.int32, device="cuda").to(torch.int16)
+        x = bits.view(dtype)
+        x = x[torch.isfinite(x)][:, None].contiguous()
+        one = torch.ones(1, 1, dtype=dtype, device="cuda")
+        h, least = _half(dtype)
+        for rows in (x, x[:50], x[-50:]):
+            y = ozk.fused_linear(rows, one, activation=act).double()
+            z = rows.double()
+            want = z.clamp(min=0) if act == "relu" else _act(z, act)[0]
+            if act == "gelu_tanh":     # tanh + 1 loses what is far below 0, in 64 bits from -8 on
+                u = 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+                want = z * torch.sigmoid(u)
+            # relative, down to the values whose exponential the hardware flushes to 0
+            tol = (h + 2 ** -16) * want.abs() + least + 2 ** -126 * z.abs().clamp(min=1)
+            assert bool(((y - want).abs() <= tol).all()), (act, dtype, float(((y - want).abs() / tol).max()))
+
+
+def test_infinities_and_nan(gpu):
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[1.0], [inf], [-inf], [nan]], device="cuda", dtype=BF)
+    for M in (4, 200):
+        rows = x if M == 4 else x.repeat(50, 1)
+        one = torch.ones(1, 1, dtype=BF, device="cuda")
+        for act in ACTS:
+            y = ozk.fused_linear(rows, one, activation=act)[:4, 0].float()
+            assert y[1] == inf and y[3] != y[3]
+            assert y[2] == (-inf if act is None else 0.0) or (act in ("gelu", "gelu_tanh", "silu") and y[2] != y[2])
+        # a row's infinity stays in its row
+        a, W, b, _, _ = _inputs(M, 100, 72, BF)
+        clean = ozk.fused_linear(a, W, b, activation="gelu")
+        a[1, 3] = nan
+        y = ozk.fused_linear(a, W, b, activation="gelu")
+        assert bool(torch.isnan(y[1]).all())
+        keep = torch.arange(M, device="cuda") != 1
+        assert torch.equal(y[keep], clean[keep])
+
+
+@pytest.mark.parametrize("M, N, K", [(5, 70, 300), (64, 33, 65), (300, 200, 136), (260, 515, 520), (100, 64, 2048)])
+def test_whole_numbers_are_exact(gpu, M, N, K):
+    """Small whole numbers: every sum is exact, so is every gradient, in any order."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    draw = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g, device="cuda").to(F16)  # noqa: E731
+    keep = (torch.rand(M, K, generator=g, device="cuda") < 0.2).to(F16)
+    x, W, b = draw(-2, 3, M, K) * keep, draw(-1, 2, N, K), draw(-3, 4, N)
+    res, dy = draw(-5, 6, M, N), draw(-1, 2, M, N)
+    for wt in (False, True):
+        leaves = [t.clone().requires_grad_() for t in (x, W.mT.contiguous().mT if wt else W, b, res)]
+        y = ozk.fused_linear(leaves[0], leaves[1], leaves[2], activation="relu", residual=leaves[3])
+        grads = torch.autograd.grad(y, leaves, dy)
+        z = x.double() @ W.double().mT.contiguous() + b.double()
+        dz = dy.double() * (z > 0)
+        assert torch.equal(y.double(), z.clamp(min=0) + res.double())
+        for got, want in zip(grads, (dz @ W.double(), dz.mT.contiguous() @ x.double(), dz.sum(0), dy.double())):
+            assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("M, N, K", [(1, 100, 64), (16, 333, 200), (40, 512, 1000), (300, 72, 2056), (1999, 520, 1000),
+                                     (1024, 1024, 512), (129, 1001, 130), (3000, 136, 72), (90, 2, 3)])
+@pytest.mark.parametrize("act", ACTS)
+def test_gradients(gpu, M, N, K, act):
+    for dtype in (BF, F16):
+        x, W, b, res, dy = _inputs(M, N, K, dtype, seed=K, wt=(M + N) % 2 == 1)
+        leaves = [t.requires_grad_() for t in (x, W, b, res)]
+        y = ozk.fused_linear(x, W, b, activation=act, residual=res)
+        dx, dW, db, dres = torch.autograd.grad(y, leaves, dy)
+        x, W, b, res = (t.detach() for t in leaves)
+        _check(y.detach(), x, W, b, res, act)
+        assert torch.equal(dres, dy)
+        h, least = _half(dtype)
+        z = x.double() @ W.double().mT.contiguous() + b.double()
+        dz = dy.double() * _act(z, act)[1]
+        if act == "relu":
+            # next to 0 either side is right: leave those rows and columns out
+            near = z.abs() < (K + 4) * U * (x.double().abs() @ W.double().mT.contiguous().abs() + b.double().abs())
+        else:
+            near = torch.zeros_like(z, dtype=torch.bool)
+        # z to h |z| moves the derivative by at most 0.8 of that; dz to h
+        zero = 0.0 if act in (None, "relu") else 1.0
+        e = dy.double().abs() * zero * (0.8 * (h * z.abs() + least + (K + 4) * U * 4) + 2 ** -17)
+        e = e + (h * dz.abs() + least if act is not None else 0.0)
+        Wa, xa = W.double().abs(), x.double().abs()
+        size = dz.abs() + e
+        for got, want, tol, skip in (
+                (dx, dz @ W.double(), e @ Wa + (N + 2) * U * (size @ Wa), near.any(1)[:, None]),
+                (dW, dz.mT.contiguous() @ x.double(), e.mT.contiguous() @ xa + (M + 2) * U * (size.mT.contiguous() @ xa),
+                 near.any(0)[:, None]),
+                (db, dz.sum(0), e.sum(0) + (M + 2) * U * size.sum(0), near.any(0))):
+            tol = tol + (h + U) * (want.abs() + tol) + least
+            off = (got.double() - want).abs()
+            assert got.shape == want.shape and got.dtype == dtype
+            assert bool(((off <= tol) | skip).all()), float((off / tol).max())
+            # the roundings are as good as independent: far below their worst case together
+            if act != "relu" and want.numel() > 1000:
+                assert float((got.double() - want).norm()) <= 2 * h * float(want.norm())
+
+
+def test_gradients_against_differences(gpu):
+    """d/dt of <y(x + t dx), dy>, with y in 64 bits from the formula, not from its derivative."""
+    M, N, K = 70, 90, 64
+    for act in ACTS[2:]:
+        x, W, b, _, dy = _inputs(M, N, K, F16, seed=5)
+        leaves = [t.requires_grad_() for t in (x, W, b)]
+        grads = torch.autograd.grad(ozk.fused_linear(x, W, b, activation=act), leaves, dy)
+        vals = [t.detach().double() for t in leaves]
+        g = torch.Generator(device="cuda").manual_seed(7)
+        for i in range(3):
+            d = torch.randn(vals[i].shape, generator=g, device="cuda", dtype=torch.float64)
+
+            def at(t):
+                v = [w + t * d if j == i else w for j, w in enumerate(vals)]
+                return float((_act(v[0] @ v[1].mT.contiguous() + v[2], act)[0] * dy.double()).sum())
+            slope = (at(1e-4) - at(-1e-4)) / 2e-4
+            got = float((grads[i].double() * d).sum())
+            # each of n gradients is off by about h times itself, with signs as they fall
+            tol = 16 * 2.0 ** -11 * float((grads[i].double() * d).norm()) + 1e-6 * abs(slope)
+            assert abs(got - slope) <= tol, (act, i, got, slope)
+
+
+def test_only_what_is_wanted(gpu):
+    x, W, b, res, dy = _inputs(150, 96, 72, BF)
+    whole = None
+    for need in ((1, 1, 1, 1), (1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (0, 1, 1, 0)):
+        for act in (None, "silu"):
+            ts = [t.clone().requires_grad_(bool(n)) for t, n in zip((x, W, b, res), need)]
+            y = ozk.fused_linear(ts[0], ts[1], ts[2], activation=act, residual=ts[3])
+            y.backward(dy)
+            if all(need):
+                whole = {**(whole or {}), act: [t.grad for t in ts]}
+            for t, n, want in zip(ts, need, whole[act]):
+                assert (t.grad is None) == (not n) and (not n or torch.equal(t.grad, want))
+    with torch.no_grad():
+        assert not ozk.fused_linear(x.clone().requires_grad_(), W).requires_grad
+
+
+def test_layouts(gpu):
+    """Rows with gaps, views, expanded and misaligned operands give the bits of copies."""
+    base = torch.randn(400, 600, device="cuda").to(BF)
+    flat = torch.randn(200 * 136 + 1, device="cuda").to(BF)
+    b = torch.randn(400, device="cuda").to(BF)[::2]
+    for M in (10, 200):
+        xs = [base[:M, 8:144], base[:M, 3:139], base[:M, ::2][:, :136], base[:136, :M].mT,
+              flat[1:1 + M * 136].view(M, 136), base[:1, :136].expand(M, 136)]
+        Ws = [base[200:400, 16:152], base[200:400, 1:137], base[:136, 100:300].mT, base[:136, 101:301].mT,
+              base[:272:2, ::3][:, :200].mT, base[:1, :136].expand(200, 136)]
+        r = base[:M, 7:207]
+        for x in xs:
+            for W in Ws:
+                y = ozk.fused_linear(x, W, b, activation="gelu", residual=r)
+                _check(y, x, W, b, r, "gelu")
+    # any number of dims
+    x = base[:60, :136].reshape(3, 4, 5, 136)
+    r = base[:60, :200].reshape(3, 4, 5, 200)
+    y = ozk.fused_linear(x, Ws[0], b, residual=r)
+    assert torch.equal(y.view(60, 200), ozk.fused_linear(x.reshape(60, 136), Ws[0], b, residual=r.reshape(60, 200)))
+    assert ozk.fused_linear(x[0, 0, 0], Ws[0]).shape == (200,)
+    # a gradient that comes expanded or with gaps
+    for act in (None, "silu"):
+        t = base[:100, :136].clone().requires_grad_()
+        W = Ws[0].clone().requires_grad_()
+        ozk.fused_linear(t, W, activation=act).sum().backward()
+        ones = torch.ones(100, 200, device="cuda", dtype=BF)
+        got = torch.autograd.grad(ozk.fused_linear(t, W, activation=act), (t, W), ones)
+        assert torch.equal(t.grad, got[0]) and torch.equal(W.grad, got[1])
+        dy = base[:100, 11:211]
+        for a, c in zip(torch.autograd.grad(ozk.fused_linear(t, W, activation=act), (t, W), dy),
+                        torch.autograd.grad(ozk.fused_linear(t, W, activation=act), (t, W), dy.contiguous())):
+            assert float((a.double() - c.double()).norm()) <= 2.0 ** -8 * float(c.double().norm())
+
+
+def test_empty(gpu):
+    for M, N, K in ((0, 5, 7), (4, 0, 7), (4, 5, 0), (100, 5, 0), (0, 0, 0)):
+        x, W, b, res, dy = _inputs(M, N, K, BF)
+        leaves = [t.requires_grad_() for t in (x, W, b, res)]
+        y = ozk.fused_linear(x, W, b, activation="gelu", residual=res)
+        grads = torch.autograd.grad(y, leaves, dy)
+        z = b.detach().double().expand(M, N)
+        assert y.shape == (M, N)
+        if M and N:
+            want = _act(z, "gelu")[0] + res.detach().double()
+            assert float((y.detach().double() - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max()) + 1e-5
+        assert [g.shape for g in grads] == [t.shape for t in leaves]
+        if K == 0 and M and N:
+            want = (dy.double() * _act(z, "gelu")[1]).sum(0)
+            assert float((grads[2].double() - want).abs().max()) <= 2.0 ** -6 * float(want.abs().max())
+        elif M == 0:
+            assert not grads[1].any() and not grads[2].any()
+        elif N == 0:
+            assert not grads[0].any()
+    x = torch.zeros(2, 0, 8, device="cuda", dtype=BF)
+    assert ozk.fused_linear(x, torch.zeros(3, 8, device="cuda", dtype=BF)).shape == (2, 0, 3)
+
+
+def test_relu_keeps_its_side(gpu):
+    """Sums too small for the dtype have a derivative of 1 above 0 and of 0 below."""
+    tiny = torch.full((80, 64), 2.0 ** -20, device="cuda", dtype=F16)
+    for sign in (1.0, -1.0):
+        W = torch.full((40, 64), sign * 2.0 ** -20, device="cuda", dtype=F16)
+        x = tiny.clone().requires_grad_()
+        b = torch.zeros(40, device="cuda", dtype=F16).requires_grad_()
+        ozk.fused_linear(x, W, b, activation="relu").backward(torch.ones(80, 40, device="cuda", dtype=F16))
+        assert bool((b.grad == (80 if sign > 0 else 0)).all())
+
+
+def test_large_rows(gpu):
+    """Rows that lie 2^22 elements and more apart are copied, those closer are read in place;
+    byte offsets past 2^32."""
+    flat = torch.randn((1 << 31) // 2 + 4096, device="cuda", dtype=BF)
+    for M, pitch in ((300, 1 << 21), (250, (1 << 22) + 8), (40, (1 << 22) + 8)):
+        x = flat.as_strided((M, 64), (pitch, 1))
+        W = torch.randn(80, 64, device="cuda").to(BF)
+        _check(ozk.fused_linear(x, W), x.contiguous(), W, None, None, None)
+        _check(ozk.fused_linear(W, x), W, x.contiguous(), None, None, None)
+
+
+def test_same_bits_every_time_and_on_any_stream(gpu):
+    x, W, b, res, dy = _inputs(520, 300, 2048, BF)
+    leaves = [t.requires_grad_() for t in (x, W, b)]
+
+    def step():
+        y = ozk.fused_linear(x, W, b, activation="gelu", residual=res)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    first = step()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    results = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            results.append(step())
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(a, c) for a, c in zip(r, first))
+
+
+def test_captured(gpu):
+    """A captured step of forward and backward, replayed on new values between eager calls."""
+    x, W, b, res, dy = _inputs(200, 130, 264, BF)
+    leaves = [t.requires_grad_() for t in (x, W, b)]
+
+    def step():
+        y = ozk.fused_linear(x, W, b, activation="silu", residual=res)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(4):
+        with torch.no_grad():
+            for t, n in zip((x, W, b, res, dy), _inputs(200, 130, 264, BF, seed=seed)):
+                t.copy_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, c in zip(got, step()):
+            assert torch.equal(a, c)
+
+
+def test_refusals_on_the_gpu(gpu):
+    x, W = torch.zeros(2, 8, device="cuda"), torch.zeros(3, 8, device="cuda")
+    with pytest.raises(NotImplementedError):
+        ozk.fused_linear(x, W)
+    with pytest.raises(RuntimeError):
+        ozk.fused_linear(x.to(BF), W.to(BF), torch.zeros(3, dtype=BF))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.to(BF), x.to(BF))
+        with pytest.raises(RuntimeError):
+            ozk.fused_linear(dual, W.to(BF))
+    t = x.to(BF).requires_grad_()
+    g, = torch.autograd.grad(ozk.fused_linear(t, W.to(BF)).sum(), t, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
