@@ -29,7 +29,7 @@ SOURCES = ["ozk_gemm_i8.hip", "ozk_gemm_f16.hip", "ozk_gemm_bf16.hip", "ozk_gemm
            "ozk_split_i8.hip", "ozk_split_f16.hip", "ozk_split_bf16.hip", "ozk_split_f32.hip",
            "ozk_split.hip", "ozk_api.cpp", "ozk_gemm.hip",
            "ozk_grouped.hip", "ozk_w4.hip", "ozk_orth.hip", "ozk_linear_api.cpp",
-           "ozk_dense.hip", "ozk_route.hip", "ozk_clip.hip", "ozk_train_api.cpp"]
+           "ozk_route.hip", "ozk_clip.hip", "ozk_train_api.cpp"]
 
 COMMON_FLAGS = [
     f"--offload-arch={ARCH}",

@@ -1,9 +1,12 @@
-// ozk_dense.hip -- the product of a linear layer, y = act(x W^T + b) + r, and
-// what its gradients need beside products.
+// ozk_dense.h -- the product of a linear layer, y = act(x W^T + b) + r, and
+// what its gradients need beside products.  Part of the unit of the grouped
+// products (ozk_grouped.hip), whose tiles and copies it shares.
 //
 // Three kernels compute the sums: tiles on the matrix cores (ozk_tile.h) with
 // the epilogue in them, the same with K cut into ranges whose fp32 sums a second
 // launch joins, and one for a few rows, which is bound by reading W.
+#pragma once
+
 #include "../../include/ozaki_amd.h"
 #include "ozk_train.h"
 #include "ozk_tile.h"
@@ -480,12 +483,9 @@ bool dense_few(const DenseParams &p) { return !p.a_cols && !p.b_cols && p.M <= 6
 
 namespace {
 
-bool whole_pieces(const void *p, int64_t pitch, int64_t cols, bool padded) {
-    return (((uintptr_t)p | (uintptr_t)pitch) & 15) == 0 && (padded || cols % 8 == 0);
-}
 bool pieces(const DenseParams &p) {
-    return whole_pieces(p.A, p.a_pitch, p.a_cols ? p.M : p.K, p.a_padded) &&
-           whole_pieces(p.B, p.b_pitch, p.b_cols ? p.N : p.K, p.b_padded);
+    return whole_pieces(p.A, p.a_pitch, 0, p.a_cols ? p.M : p.K, p.a_padded) &&
+           whole_pieces(p.B, p.b_pitch, 0, p.b_cols ? p.N : p.K, p.b_padded);
 }
 int64_t tiles(const DenseParams &p, int64_t bm, int64_t bn) {
     return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);

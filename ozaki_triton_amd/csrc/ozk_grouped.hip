@@ -496,3 +496,5 @@ hipError_t launch_grouped_grad(const GroupedGradParams &p, int dtype, hipStream_
 }
 
 }  // namespace ozk
+
+#include "ozk_dense.h"

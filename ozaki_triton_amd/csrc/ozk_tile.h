@@ -1,5 +1,5 @@
 // ozk_tile.h -- one C tile of a 16-bit matrix product on the matrix cores, for
-// the grouped products (ozk_grouped.hip), the dense ones (ozk_dense.hip) and the
+// the grouped products (ozk_grouped.hip), the dense ones (ozk_dense.h) and the
 // orthogonalisation (ozk_orth.hip).
 //
 //   C[m, n] = sum_k A[m, k] B[n, k], accumulated in fp32

@@ -1,6 +1,6 @@
 // ozk_train.h -- parameter blocks and launchers of what stands around a model's
 // linear layers in training and serving: the dense product with its epilogue
-// (ozk_dense.hip), the router (ozk_route.hip), gradient norms and clipping
+// (ozk_dense.h), the router (ozk_route.hip), gradient norms and clipping
 // (ozk_clip.hip); shared between their C entry points (ozk_train_api.cpp) and
 // their kernels.
 #pragma once
