@@ -135,16 +135,17 @@ OZK_DEV void finish8(const DenseParams &p, float (&v)[8], const float (&bias)[8]
     for (int i = 0; i < 8; ++i) v[i] += bias[i];
     if (p.Z) {
         // z is kept in 16 bits for the backward pass: act' moves by at most 0.32 2^-9
-        // (bf16) with it, as much as dy's own rounding.  A z that underflows keeps its
-        // side of 0, on which relu's derivative depends.
-        uint16_t e[8];
-        i32x4 z;
+        // (bf16) with it, as much as dy's own rounding.  Where relu's side depends on
+        // it, a z that underflows keeps its own.
+        i32x4 z = pack8<ST>(v);
+        if (p.act == OZK_ACT_RELU) {
+            uint16_t e[8];
+            __builtin_memcpy(e, &z, 16);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            e[i] = to_bits16(v[i], ST{});
-            if ((e[i] & 0x7FFF) == 0 && v[i] != 0.f) e[i] |= 1;
+            for (int i = 0; i < 8; ++i)
+                if ((e[i] & 0x7FFF) == 0 && v[i] != 0.f) e[i] |= 1;
+            __builtin_memcpy(&z, e, 16);
         }
-        __builtin_memcpy(&z, e, 16);
         store8(p.Z + (m * p.N + n) * 2, left, z);
     }
     with_act(p.act, [&](auto act) {
@@ -183,7 +184,7 @@ OZK_DEV void finish_tile(const Loop &t, const DenseParams &p, char *smem, int64_
     };
     constexpr int CI = most(ROOM);          // blocks of 16 rows at a time
     constexpr int LANES = NI * 2, RPI = 64 / LANES;   // lanes of a row, rows of a wave's step
-    static_assert(ROOM >= 1 && (NI == 1 || NI == 2 || NI == 4), "");
+    static_assert(ROOM >= 1 && (NI == 1 || NI == 2 || NI == 4) && CI * 16 >= RPI, "");
     const int lane = threadIdx.x & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     m0 += wave / Sh::WN * MI * 16;
@@ -313,99 +314,82 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// A few rows: bound by reading W once.  A workgroup has NT blocks of 16 rows of W
-// (columns of C) and all of x; its waves take 64 elements of K in turn, and their
-// sums are added in the LDS in order.  Operands go from memory into the matrix
-// cores' registers: a lane reads 32 consecutive bytes of a row, the four lanes of
-// a row a whole line.  The order along K is that of the lanes' bytes, the same for
-// both operands.
+// Up to 16 rows: bound by reading W once.  A wave takes a range of K; operands go
+// from memory into the matrix cores' registers.  A block of 16 x 16 sums is R = 16
+// / P rows of x by R rows of W, each with P parts of K: index i of either operand
+// is part i / R of row i % R, and of the sums those of equal parts count.  A load
+// then reads P 64-byte pieces of R rows one behind another, which DRAM serves
+// faster than pieces of 16 rows, and few rows of W still fill the chip.  The waves'
+// sums and the parts are added in order in the LDS.
 // ---------------------------------------------------------------------------
-template <typename ST, int MT, int NT, int WAVES>
+template <typename ST, int P, int WAVES, int U>
 __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(DenseParams p) {
-    __shared__ __attribute__((aligned(16))) f32x4 join[WAVES][MT * NT][64];
+    constexpr int R = 16 / P;
+    __shared__ __attribute__((aligned(16))) float join[WAVES][16][20];   // [x's index][W's index]
     const int lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t n0 = (int64_t)blockIdx.x * NT * 16;
+    const int64_t n0 = (int64_t)blockIdx.x * R;
     // rows past the last read the last one, and are not stored
-    const char *W[NT], *X[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int64_t n = n0 + j * 16 + i16;
-        W[j] = p.B + (n < p.N ? n : p.N - 1) * p.b_pitch + g * 32;
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t m = i * 16 + i16;
-        X[i] = p.A + (m < p.M ? m : p.M - 1) * p.a_pitch + g * 32;
-    }
-    f32x4 acc[MT][NT] = {};
+    const int64_t n = n0 + i16 % R, m = i16 % R;
+    const int in = (i16 / R) * 128 + g * 16;   // the lane's first piece in a step of P 128 bytes
+    const char *W = p.B + (n < p.N ? n : p.N - 1) * p.b_pitch + in;
+    const char *X = p.A + (m < p.M ? m : p.M - 1) * p.a_pitch + in;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     const int64_t bytes = p.K * 2;
+    constexpr int STEP = P * 128;
     auto piece = [&](const char *row, const char *first, int64_t at, bool whole) -> i32x4 {
         i32x4 v;
         if (whole) {
             __builtin_memcpy(&v, row + at, 16);
             return v;
         }
-        const int64_t n = bytes - at - g * 32;
-        return load_piece(row + (n > 0 ? at : 0), n < 16 ? (int)(n < 0 ? 0 : n) : 16, first);
+        const int64_t left = bytes - at - in;
+        return load_piece(row + (left > 0 ? at : 0), left < 16 ? (int)(left < 0 ? 0 : left) : 16, first);
     };
-    // U steps, 128 bytes of K each: all loads, then the products
+    // UU steps: all loads, then the products
     auto steps = [&](int64_t at, auto u_, auto whole_) {
-        constexpr int U = decltype(u_)::value;
+        constexpr int UU = decltype(u_)::value;
         constexpr bool whole = decltype(whole_)::value;
-        i32x4 w[U][NT][2], x[U][MT][2];
+        i32x4 w[UU][2], x[UU][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < UU; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int64_t k = at + u * WAVES * 128 + 16 * h;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) w[u][j][h] = piece(W[j], p.B, k, whole);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) x[u][i][h] = piece(X[i], p.A, k, whole);
+                w[u][h] = piece(W, p.B, at + u * STEP + 64 * h, whole);
+                x[u][h] = piece(X, p.A, at + u * STEP + 64 * h, whole);
             }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < UU; ++u)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        acc[i][j] = mfma16(w[u][j][h], x[u][i][h], acc[i][j], ST{});
+            for (int h = 0; h < 2; ++h) acc = mfma16(w[u][h], x[u][h], acc, ST{});
     };
     using std::integral_constant;
-    constexpr int U = MT + NT <= 3 ? 4 : 2;
-    int64_t at = (int64_t)wave * 128;
-    for (; at + (U - 1) * WAVES * 128 + 128 <= bytes; at += U * WAVES * 128)
-        steps(at, integral_constant<int, U>{}, std::true_type{});
-    for (; at + 128 <= bytes; at += WAVES * 128)
-        steps(at, integral_constant<int, 1>{}, std::true_type{});
-    if (at < bytes) steps(at, integral_constant<int, 1>{}, std::false_type{});
+    const int64_t per = ((bytes + STEP - 1) / STEP + WAVES - 1) / WAVES * STEP;
+    int64_t at = per * wave;
+    const int64_t end = at + per < bytes ? at + per : bytes;
+    for (; at + U * STEP <= end; at += U * STEP) steps(at, integral_constant<int, U>{}, std::true_type{});
+    for (; at + STEP <= end; at += STEP) steps(at, integral_constant<int, 1>{}, std::true_type{});
+    if (at < end) steps(at, integral_constant<int, 1>{}, std::false_type{});
 
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) join[wave][i * NT + j][lane] = acc[i][j];
+    *(f32x4 *)&join[wave][i16][4 * g] = acc;
     __syncthreads();
-    // a lane has 4 columns of a row: two of them make the 8 of the epilogue
-    for (int o = threadIdx.x; o < MT * NT * 32; o += 64 * WAVES) {
-        const int b = o / 32, row = o % 32 / 2, half = o % 2;
+    // 8 columns of a row to a lane (R where that is less)
+    constexpr int C = R < 8 ? R : 8, GROUPS = R / C;
+    if (threadIdx.x < R * GROUPS) {
+        const int row = threadIdx.x / GROUPS, c0 = threadIdx.x % GROUPS * C;
         float v[8] = {};
 #pragma unroll
         for (int w = 0; w < WAVES; ++w)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const f32x4 s = join[w][b][(half * 2 + q) * 16 + row];
+            for (int q = 0; q < P; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[q * 4 + e] += s[e];
-            }
-        const int64_t m = b / NT * 16 + row, n = n0 + b % NT * 16 + half * 8;
-        const int left = p.N - n < 8 ? (int)(p.N - n) : 8;
-        if (m < p.M && left > 0) {
+                for (int e = 0; e < C; ++e) v[e] += join[w][q * R + row][q * R + c0 + e];
+        const int64_t col = n0 + c0;
+        const int left = p.N - col < C ? (int)(p.N - col) : C;
+        if (row < p.M && left > 0) {
             float bias[8];
-            bias_at<ST>(p, n, left, bias);
-            finish8<ST>(p, v, bias, res_at<ST>(p, m, n, left), m, n, left);
+            bias_at<ST>(p, col, left, bias);
+            finish8<ST>(p, v, bias, res_at<ST>(p, row, col, left), row, col, left);
         }
     }
 }
@@ -479,8 +463,6 @@ template <typename ST> __global__ __launch_bounds__(256) void dense_bias_kernel(
     }
 }
 
-bool dense_few(const DenseParams &p) { return !p.a_cols && !p.b_cols && p.M <= 64; }
-
 namespace {
 
 bool pieces(const DenseParams &p) {
@@ -499,25 +481,85 @@ hipError_t dense_go(const DenseParams &p, hipStream_t st) {
     dense_kernel<ST, Sh, DMA><<<dim3((uint32_t)((all + 7) / 8 * 8)), Sh::THREADS, Sh::LDS_BYTES, st>>>(p);
     return hipGetLastError();
 }
-template <typename ST, int MT, int NT> hipError_t few_go(const DenseParams &p, hipStream_t st) {
-    const int64_t blocks = (p.N + NT * 16 - 1) / (NT * 16);
+template <typename ST, int P, int WAVES, int U> hipError_t few_go(const DenseParams &p, hipStream_t st) {
+    const int64_t blocks = (p.N + 16 / P - 1) / (16 / P);
     if (blocks >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
-    dense_few_kernel<ST, MT, NT, 8><<<dim3((uint32_t)blocks), 512, 0, st>>>(p);
+    dense_few_kernel<ST, P, WAVES, U><<<dim3((uint32_t)blocks), 64 * WAVES, 0, st>>>(p);
     return hipGetLastError();
 }
+// Parts of K: as few as give three quarters of the CUs a workgroup.  Measured (us,
+// M x N x K, one part / two / four):
+//     1 x 4096 x 4096    8.9 / 10.0 / 12.2      1 x 1024 x 8192   12.2 / 8.0 / 6.4
+//     1 x 8192 x 8192   25.0 / 27.0 / 30.2      1 x 1000 x 2048    5.7 / 4.6 / 4.5
 template <typename ST> hipError_t few_plan(const DenseParams &p, hipStream_t st) {
-    if (p.M <= 16) return few_go<ST, 1, 1>(p, st);
-    if (p.M <= 32) return few_go<ST, 2, 1>(p, st);
-    return few_go<ST, 4, 1>(p, st);
+    int parts = 1;
+    while (parts < 4 && p.M * parts <= 8 && p.N * parts < 16 * 192) parts *= 2;
+    if (parts == 1) return few_go<ST, 1, 8, 8>(p, st);
+    if (parts == 2) return few_go<ST, 2, 8, 8>(p, st);
+    return few_go<ST, 4, 8, 4>(p, st);
+}
+
+// The tile and the K ranges of the shortest time: rounds of workgroups, so many at
+// once, by a round's time, `fixed` + `slope` K / 1024 us (fitted to 180 shapes of 32
+// to 8192 rows and columns, K = 512 to 4096, for operands along K and for a weight's
+// gradient); partial sums cost a launch and their way through memory.  Chosen so,
+// products of those shapes take 1% longer on average than with the best tile of
+// each.  Measured (us, M x N x K, operands along K; 32 x 16 / 32 x 32 / 64 x 32 / 64 x
+// 64 in two groups of waves / 64 x 64 / 128 x 128 / 256 x 128 / 256 x 256):
+//     32 x 4096 x 4096      12 / 14 / 19 / 23 / 43 / 44 / 79 / 125
+//     128 x 4096 x 4096     34 / 24 / 18 / 23 / 44 / 44 / 72 / 120
+//     512 x 4096 x 4096    132 / 93 / 69 / 43 / 39 / 41 / 66 / 112
+//     2048 x 4096 x 2048     - /  - / 117 / 71 / 63 / 49 / 41 / 69
+//     4096 x 4096 x 2048     - /  - / 233 / 139 / 120 / 97 / 79 / 68
+struct TileCost {
+    int bm, bn, at_once;
+    float fixed[2], slope[2];   // of operands along K, of a weight's gradient
+};
+constexpr TileCost kTiles[] = {
+    {32, 16, 256, {2.0f, 1.8f}, {1.45f, 2.4f}},     {32, 32, 256, {2.0f, 1.8f}, {2.25f, 3.3f}},
+    {64, 32, 256, {2.7f, 2.2f}, {2.85f, 3.25f}},    {64, 64, 256, {2.7f, 2.1f}, {3.7f, 4.05f}},
+    {64, 64, 512, {2.2f, 1.6f}, {6.5f, 7.2f}},      {128, 128, 256, {3.9f, 3.1f}, {7.4f, 7.8f}},
+    {256, 128, 256, {6.1f, 4.7f}, {12.2f, 14.2f}},  {256, 256, 256, {7.7f, 5.4f}, {21.5f, 21.0f}},
+};
+struct DensePlan {
+    int tile, splits;
+};
+DensePlan plan_tiles(const DenseParams &p) {
+    DensePlan best = {0, 1};
+    double least = 0;
+    for (int splits = 1; splits <= 16; splits *= 2) {
+        // ranges of 8 stages at least, sums that stay in the caches
+        if (splits > 1 && (p.K < 512 * splits || (double)splits * p.M * p.N > 1 << 24)) break;
+        const double join = splits > 1 ? 3.0 + 2e-6 * splits * p.M * p.N : 0.0;
+        for (int i = 0; i < (int)(sizeof kTiles / sizeof *kTiles); ++i) {
+            const TileCost &t = kTiles[i];
+            const double n = (double)tiles(p, t.bm, t.bn) * splits;
+            const double time = join + ceil(n / t.at_once) * (t.fixed[p.a_cols] + t.slope[p.a_cols] *
+                                                              (double)p.K / splits / 1024);
+            if ((i == 0 && splits == 1) || time < least) {
+                least = time;
+                best = {i, splits};
+            }
+        }
+    }
+    return best;
 }
 
 template <typename ST, bool AC, bool BC> hipError_t tile_plan(const DenseParams &p, hipStream_t st) {
-    if (!pieces(p)) return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 2, 2>, false>(p, st);
-    if (tiles(p, 256, 256) >= 256)
-        return dense_go<ST, TileShape<1, AC, BC, 256, 256, 2, 4, 2>, true>(p, st);
-    if (tiles(p, 128, 128) * p.splits >= 192)
-        return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 4, 2>, true>(p, st);
-    return dense_go<ST, TileShape<1, AC, BC, 64, 64, 2, 2, 2, 2>, true>(p, st);
+    if (!pieces(p)) {
+        if (p.M <= 32) return dense_go<ST, TileShape<1, AC, BC, 32, 64, 1, 4, 2>, false>(p, st);
+        return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 2, 2>, false>(p, st);
+    }
+    switch (plan_tiles(p).tile) {
+    case 0: return dense_go<ST, TileShape<1, AC, BC, 32, 16, 1, 1, 4, 4>, true>(p, st);
+    case 1: return dense_go<ST, TileShape<1, AC, BC, 32, 32, 1, 2, 4, 4>, true>(p, st);
+    case 2: return dense_go<ST, TileShape<1, AC, BC, 64, 32, 2, 1, 3, 4>, true>(p, st);
+    case 3: return dense_go<ST, TileShape<1, AC, BC, 64, 64, 2, 2, 4, 2>, true>(p, st);
+    case 4: return dense_go<ST, TileShape<1, AC, BC, 64, 64, 2, 2, 2, 2>, true>(p, st);
+    case 5: return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 4, 4>, true>(p, st);
+    case 6: return dense_go<ST, TileShape<1, AC, BC, 256, 128, 4, 2, 3>, true>(p, st);
+    default: return dense_go<ST, TileShape<1, AC, BC, 256, 256, 2, 4, 2>, true>(p, st);
+    }
 }
 template <typename ST> hipError_t dense_plan(const DenseParams &p, hipStream_t st) {
     if (dense_few(p)) return few_plan<ST>(p, st);
@@ -532,12 +574,13 @@ template <typename ST> hipError_t dense_plan(const DenseParams &p, hipStream_t s
 
 }  // namespace
 
+// Up to 4 rows, and up to 16 that the tiles' DMA cannot take (us, 4 x 4096 x 4096:
+// 9.7, tiles of 32 x 16 9.4; 16 x 4096 x 4096: 11.5 and 9.6)
+bool dense_few(const DenseParams &p) {
+    return !p.a_cols && !p.b_cols && (p.M <= 4 || (p.M <= 16 && !pieces(p)));
+}
 int dense_splits(const DenseParams &p) {
-    if (dense_few(p) || p.M == 0 || p.N == 0) return 1;
-    const int64_t n = tiles(p, 64, 64), stages = (p.K + 63) / 64;
-    int s = 1;
-    while (s < 16 && n * s < 256 && stages / (2 * s) >= 8) s *= 2;
-    return s;
+    return dense_few(p) || p.M == 0 || p.N == 0 ? 1 : plan_tiles(p).splits;
 }
 
 hipError_t launch_dense(const DenseParams &p, int dtype, hipStream_t st) {

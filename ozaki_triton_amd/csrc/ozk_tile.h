@@ -115,7 +115,8 @@ template <int RB> OZK_DEV int cols_swz(int k) {
     static_assert((RB & (RB - 1)) == 0, "the XOR leaves a chunk in its row");
     if constexpr (RB >= 256) return (k & 3) | ((k >> 1) & 4);
     else if constexpr (RB == 128) return ((k >> 1) & 1) | ((k >> 2) & 2);
-    else return (k >> 3) & 1;
+    else if constexpr (RB == 64) return (k >> 3) & 1;
+    else return 0;   // one chunk a row
 }
 
 // a value that is the same in every lane, in scalar registers: the DMA's buffer

@@ -9,13 +9,15 @@ NotImplementedError, tensors off the GPU RuntimeError.
 """
 from __future__ import annotations
 
-import ctypes
+from array import array
 
 import torch
 
 from . import _lib
-from .linear import _FLOAT, _bytes, _call, _no_grad, _on_one_gpu, _require_dtype, _workspace
+from .linear import _FLOAT, _bytes, _call, _no_tangent, _on_one_gpu, _require_dtype, _workspace
 from .ozaki import _TORCH_TO_OZK
+
+_CODES = {d: _TORCH_TO_OZK[d] for d in _FLOAT}
 
 
 def _is_dense(t: torch.Tensor) -> bool:
@@ -30,24 +32,32 @@ def _is_dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _tensors(name, grads):
-    grads = list(grads)
-    assert grads, f"{name} needs at least one tensor"
-    _on_one_gpu(*grads)
-    for t in grads:
-        if t.dtype not in _FLOAT:
-            _require_dtype(name, t.dtype, _FLOAT)
-    return grads
+def _checked(name, tensors):
+    """The tensors as a list, and the types' codes.  (Host time counts: a model has
+    hundreds of gradients.)"""
+    tensors = list(tensors)
+    assert tensors, f"{name} needs at least one tensor"
+    dev = tensors[0].get_device()
+    codes = [_CODES.get(t.dtype) for t in tensors]
+    if dev < 0 or any([t.get_device() != dev for t in tensors]):
+        _on_one_gpu(*tensors)
+    if None in codes:
+        _require_dtype(name, tensors[codes.index(None)].dtype, _FLOAT)
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or on "
+                           "detached tensors")
+    _no_tangent(name, *tensors)
+    return tensors, codes
 
 
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+class _Table:
+    """Host arrays of addresses, element counts and types, as the C calls take them."""
 
-
-def _described(tensors):
-    n = len(tensors)
-    return ((ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
-            (ctypes.c_int * n)(*[_TORCH_TO_OZK[t.dtype] for t in tensors]))
+    def __init__(self, ins, outs, codes):
+        self.held = (array("Q", [t.data_ptr() for t in ins]), array("q", [t.numel() for t in ins]),
+                     array("i", codes), None if outs is None else array("Q", [t.data_ptr() for t in outs]))
+        self.ins, self.counts, self.codes = (a.buffer_info()[0] for a in self.held[:3])
+        self.outs = None if outs is None else self.held[3].buffer_info()[0]
 
 
 def gradient_norm(grads) -> torch.Tensor:
@@ -56,14 +66,14 @@ def gradient_norm(grads) -> torch.Tensor:
 
     grads: tensors of any shapes, float32 / float16 / bfloat16 in any mix, on one GPU
     """
-    grads = _tensors("gradient_norm", grads)
-    _no_grad("gradient_norm", *grads)
-    grads = [t if _is_dense(t) else t.contiguous() for t in grads]
+    grads, codes = _checked("gradient_norm", grads)
+    grads = [t if t.is_contiguous() or _is_dense(t) else t.contiguous() for t in grads]
     dev, n = grads[0].device, len(grads)
+    table = _Table(grads, None, codes)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     size = _bytes("ozk_gradient_norm_workspace_bytes", n)
     ws, wsp = _workspace(size, dev)
-    _call("ozk_gradient_norm", dev, _pointers(grads), *_described(grads), n, norm.data_ptr(), wsp, size)
+    _call("ozk_gradient_norm", dev, table.ins, table.counts, table.codes, n, norm.data_ptr(), wsp, size)
     del ws
     return norm
 
@@ -79,39 +89,30 @@ def clip_gradients(grads, max_norm: float, *, out=None) -> torch.Tensor:
              the gradients themselves, in place
     A norm of infinity makes everything finite 0, one of NaN everything NaN.
     """
-    grads = _tensors("clip_gradients", grads)
-    outs = grads if out is None else list(out)
+    grads, codes = _checked("clip_gradients", grads)
     assert max_norm >= 0, f"max_norm must be >= 0, got {max_norm}"
-    if outs is not grads:
-        assert len(outs) == len(grads), f"out must have {len(grads)} tensors, got {len(outs)}"
-        for g, o in zip(grads, outs):
+    ins, to, back = grads, grads, ()
+    if out is None:
+        whole = all([t.is_contiguous() for t in grads])
+    else:
+        to, _ = _checked("clip_gradients", out)
+        assert len(to) == len(grads), f"out must have {len(grads)} tensors, got {len(to)}"
+        for g, o in zip(grads, to):
             assert o.shape == g.shape and o.dtype == g.dtype, \
                 f"out must match: {tuple(g.shape)} {g.dtype}, got {tuple(o.shape)} {o.dtype}"
-        _on_one_gpu(grads[0], *outs)
-    _no_grad("clip_gradients", *grads)
-    if outs is not grads:
-        _no_grad("clip_gradients", *outs)
-    # tensors with gaps, or laid out other than their result, go through copies
-    ins, to = grads, outs
-    back = []
-    for i, (g, o) in enumerate(zip(grads, outs)):
-        if g is o and _is_dense(g) or (g.is_contiguous() and o.is_contiguous()):
-            continue
-        if g.stride() == o.stride() and _is_dense(g):
-            continue
-        assert all(s or n <= 1 for s, n in zip(o.stride(), o.shape)), \
-            "out must not be expanded: its elements share memory"
-        if ins is grads:
-            ins, to = list(grads), list(outs)
-        ins[i] = g.contiguous()
-        to[i] = torch.empty_like(ins[i])
-        back.append((o, to[i]))
+        if grads[0].get_device() != to[0].get_device():
+            _on_one_gpu(grads[0], to[0])
+        whole = all([g.is_contiguous() and o.is_contiguous() for g, o in zip(grads, to)])
+    outs = to
+    if not whole:
+        ins, to, back = _through_copies(grads, to)
     dev, n = grads[0].device, len(grads)
+    table = _Table(ins, to, codes)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     size = _bytes("ozk_gradient_norm_workspace_bytes", n)
     ws, wsp = _workspace(size, dev)
     try:
-        _call("ozk_clip_gradients", dev, _pointers(ins), _pointers(to), *_described(ins), n,
+        _call("ozk_clip_gradients", dev, table.ins, table.outs, table.counts, table.codes, n,
               float(max_norm), norm.data_ptr(), wsp, size)
     except _lib.OzakiLibError as e:
         if e.status == _lib.OZK_ERR_SHAPE:
@@ -121,5 +122,20 @@ def clip_gradients(grads, max_norm: float, *, out=None) -> torch.Tensor:
     for o, t in back:
         o.copy_(t)
     # written behind autograd's back
-    torch.autograd.graph.increment_version([t for t in outs if not t.is_inference()])
+    torch.autograd.graph.increment_version(outs)
     return norm
+
+
+def _through_copies(grads, outs):
+    """Tensors with gaps, or laid out other than their result, by copies: the inputs,
+    the outputs, and (result, copy) to copy back."""
+    ins, to, back = list(grads), list(outs), []
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        if (g is o or g.stride() == o.stride()) and _is_dense(g) or (g.is_contiguous() and o.is_contiguous()):
+            continue
+        assert all(s or n <= 1 for s, n in zip(o.stride(), o.shape)), \
+            "out must not be expanded: its elements share memory"
+        ins[i] = g.contiguous()
+        to[i] = torch.empty_like(ins[i])
+        back.append((o, to[i]))
+    return ins, to, back

@@ -486,23 +486,29 @@ def _linear_forward(x, W, bias, residual, act, want_z):
 def _linear_backward(dy, z, x, W, act, want):
     """The gradients (dx, dW, db) that `want`, three truth values, asks for; x or W
     may be None where only the other's is wanted."""
-    M, N = dy.shape
-    K = (x if W is None else W).shape[1] if x is not None or W is not None else 0
-    dev, dtype = dy.device, dy.dtype
+    (M, N), dev, dtype = dy.shape, dy.device, dy.dtype
     dy, sy = _rows(dy)
-    (x, sx) = _rows(x) if x is not None else (None, 0)
-    (W, sw) = _weight(W) if W is not None else (None, (0, 1))
-    dx = dy.new_empty((M, K)) if want[0] else None
-    dW = dy.new_empty((N, K)) if want[1] else None
-    db = dy.new_empty((N,)) if want[2] else None
-    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
-    align = lambda t: 0 if t is None else t.data_ptr() & 15   # noqa: E731
-    mask = want[0] | want[1] << 1 | want[2] << 2
-    n = _bytes("ozk_linear_backward_workspace_bytes", align(dy), sy, align(x), sx, align(W), sw, act,
-               M, N, K, mask)
+    xp = wp = dx = dW = db = None
+    sw = (0, 1)
+    mask = K = sx = 0
+    if want[0]:
+        K, mask = W.shape[1], 1
+        W, sw = _weight(W)
+        wp, dx = W.data_ptr(), dy.new_empty((M, K))
+    if want[1]:
+        K, mask = x.shape[1], mask | 2
+        x, sx = _rows(x)
+        xp, dW = x.data_ptr(), dy.new_empty((N, K))
+    if want[2]:
+        mask |= 4
+        db = dy.new_empty((N,))
+    dp = dy.data_ptr()
+    n = _bytes("ozk_linear_backward_workspace_bytes", dp & 15, sy, (xp or 0) & 15, sx, (wp or 0) & 15,
+               sw, act, M, N, K, mask)
     ws, wsp = _workspace(n, dev)
-    _call("ozk_linear_backward", dev, ptr(dy), sy, ptr(z), ptr(x), sx, ptr(W), _i64(*sw), act, M, N,
-          K, _TORCH_TO_OZK[dtype], ptr(dx), K, ptr(dW), K, ptr(db), wsp, n)
+    _call("ozk_linear_backward", dev, dp, sy, None if z is None else z.data_ptr(), xp, sx, wp,
+          _i64(*sw), act, M, N, K, _TORCH_TO_OZK[dtype], None if dx is None else dx.data_ptr(), K,
+          None if dW is None else dW.data_ptr(), K, None if db is None else db.data_ptr(), wsp, n)
     del ws
     return dx, dW, db
 
@@ -511,20 +517,32 @@ class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, bias, residual, act):
         need = ctx.needs_input_grad
-        y, z = _linear_forward(x, W, bias, residual, act, act != 0 and any(need[:3]))
+        y, z = _linear_forward(x, W, bias, residual, act,
+                               act != 0 and (need[0] or need[1] or need[2]))
         ctx.save_for_backward(x if need[1] else None, W if need[0] else None, z)
         ctx.act = act
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        # (the wrapper that refuses a second derivative costs 4 us: only where one is asked for)
+        if torch.is_grad_enabled():
+            return _FusedLinear.backward_once(ctx, dy)
+        return _FusedLinear.gradients(ctx, dy)
+
+    @staticmethod
+    def gradients(ctx, dy):
         x, W, z = ctx.saved_tensors
         need = ctx.needs_input_grad
-        grads = (None, None, None)
-        if any(need[:3]):
-            grads = _linear_backward(dy, z, x, W, ctx.act, need[:3])
-        return (*grads, dy if need[3] else None, None)
+        dx = dW = db = None
+        if need[0] or need[1] or need[2]:
+            dx, dW, db = _linear_backward(dy, z, x, W, ctx.act, need)
+        return dx, dW, db, dy if need[3] else None, None
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward_once(ctx, dy):
+        return _FusedLinear.gradients(ctx, dy)
 
 
 def fused_linear(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor | None = None, *,

@@ -39,50 +39,61 @@ class Routing(NamedTuple):
 
 def _route_forward(logits, mask, k, normalize):
     T, E = logits.shape
-    dev = logits.device
-    ints = torch.empty(3 * T * k + 2 * E + 1, dtype=torch.int32, device=dev)
-    experts, order, place, offsets, counts = ints.split((T * k, T * k, T * k, E + 1, E))
-    experts, place = experts.view(T, k), place.view(T, k)
+    dev, n = logits.device, T * k
+    ints = torch.empty(3 * n + 2 * E + 1, dtype=torch.int32, device=dev)
+    experts, order, place, offsets, counts = ints.split_with_sizes((n, n, n, E + 1, E))
     weights = torch.empty((T, k), dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    n = _bytes("ozk_route_workspace_bytes", T, E, k)
-    ws, wsp = _workspace(n, dev)
+    at = ints.data_ptr()
+    size = _bytes("ozk_route_workspace_bytes", T, E, k)
+    ws, wsp = _workspace(size, dev)
     _call("ozk_route", dev, logits.data_ptr(), _TORCH_TO_OZK[logits.dtype], logits.stride(0),
-          None if mask is None else mask.data_ptr(), T, E, k, int(normalize), experts.data_ptr(),
-          weights.data_ptr(), order.data_ptr(), place.data_ptr(), offsets.data_ptr(),
-          counts.data_ptr(), loss.data_ptr(), wsp, n)
+          None if mask is None else mask.data_ptr(), T, E, k, 1 if normalize else 0, at,
+          weights.data_ptr(), at + 4 * n, at + 8 * n, at + 12 * n, at + 12 * n + 4 * (E + 1),
+          loss.data_ptr(), wsp, size)
     del ws
-    return experts, weights, order, place, offsets, counts, loss
+    return experts.view(T, k), weights, order, place.view(T, k), offsets, counts, loss
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, mask, k, normalize):
-        out = _route_forward(logits, mask, k, normalize)
-        experts, weights, order, place, offsets, counts, loss = out
-        ctx.save_for_backward(logits, mask, experts, weights, counts)
-        ctx.normalize = normalize
-        ctx.mark_non_differentiable(experts, order, place, offsets, counts)
+    def forward(ctx, logits, mask, k, normalize, rest):
+        """The differentiable two; the others go into the list `rest`."""
+        experts, weights, order, place, offsets, counts, loss = _route_forward(logits, mask, k, normalize)
+        rest += (experts, order, place, offsets, counts)
+        ctx.save_for_backward(logits, mask, weights)
+        ctx.whole = experts, counts, normalize
         ctx.set_materialize_grads(False)
-        return out
+        return weights, loss
+
+    @staticmethod
+    def backward(ctx, dweights, dloss):
+        # (the wrapper that refuses a second derivative costs 4 us: only where one is asked for)
+        if torch.is_grad_enabled():
+            return _Route.backward_once(ctx, dweights, dloss)
+        return _Route.gradients(ctx, dweights, dloss)
+
+    @staticmethod
+    def gradients(ctx, dweights, dloss):
+        if dweights is None and dloss is None:
+            return None, None, None, None, None
+        logits, mask, weights = ctx.saved_tensors
+        experts, counts, normalize = ctx.whole
+        T, k = experts.shape
+        if dweights is not None:
+            dweights = dweights.contiguous()
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _call("ozk_route_backward", logits.device, logits.data_ptr(), _TORCH_TO_OZK[logits.dtype],
+              logits.stride(0), None if mask is None else mask.data_ptr(), T, counts.shape[0], k,
+              1 if normalize else 0, experts.data_ptr(), weights.data_ptr(), counts.data_ptr(),
+              None if dweights is None else dweights.data_ptr(),
+              None if dloss is None else dloss.data_ptr(), dlogits.data_ptr())
+        return dlogits, None, None, None, None
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, _e, dweights, _o, _p, _f, _c, dloss):
-        if dweights is None and dloss is None:
-            return None, None, None, None
-        logits, mask, experts, weights, counts = ctx.saved_tensors
-        T, E = logits.shape
-        k = experts.shape[1]
-        if dweights is not None:
-            dweights = dweights.contiguous()
-        dlogits = logits.new_empty((T, E))
-        _call("ozk_route_backward", logits.device, logits.data_ptr(), _TORCH_TO_OZK[logits.dtype],
-              logits.stride(0), None if mask is None else mask.data_ptr(), T, E, k,
-              int(ctx.normalize), experts.data_ptr(), weights.data_ptr(), counts.data_ptr(),
-              None if dweights is None else dweights.data_ptr(),
-              None if dloss is None else dloss.data_ptr(), dlogits.data_ptr())
-        return dlogits, None, None, None
+    def backward_once(ctx, dweights, dloss):
+        return _Route.gradients(ctx, dweights, dloss)
 
 
 def route_tokens(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = None,
@@ -116,5 +127,8 @@ def route_tokens(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = No
     if mask is not None and mask.stride(0) != 1:
         mask = mask.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return Routing(*_Route.apply(logits, mask, k, normalize))
+        rest: list = []
+        weights, loss = _Route.apply(logits, mask, k, normalize, rest)
+        experts, order, place, offsets, counts = rest
+        return Routing(experts, weights, order, place, offsets, counts, loss)
     return Routing(*_route_forward(logits, mask, k, normalize))
