@@ -88,6 +88,7 @@ template <typename F> OZK_DEV void with_act(int act, F &&f) {
 // ---------------------------------------------------------------------------
 // 8 consecutive 16-bit values of a row, of which `n` exist
 // ---------------------------------------------------------------------------
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 OZK_DEV i32x4 load8(const char *p, int n) {
     i32x4 v = {0, 0, 0, 0};
     if (n >= 8) {
@@ -146,7 +147,9 @@ OZK_DEV void finish8(const DenseParams &p, float (&v)[8], const float (&bias)[8]
                 if ((e[i] & 0x7FFF) == 0 && v[i] != 0.f) e[i] |= 1;
             __builtin_memcpy(&z, e, 16);
         }
-        store8(p.Z + (m * p.N + n) * 2, left, z);
+        char *to = p.Z + (m * p.N + n) * 2;
+        if (left == 8) __builtin_nontemporal_store((i32x4_any)z, (i32x4_any *)to);   // not read soon
+        else store8(to, left, z);
     }
     with_act(p.act, [&](auto act) {
 #pragma unroll
@@ -226,12 +229,36 @@ OZK_DEV void finish_tile(const Loop &t, const DenseParams &p, char *smem, int64_
     }
 }
 
+// db for 16 columns: the partial sums' rows over groups of 16 lanes, added in 64 bits
+template <typename ST> OZK_DEV void add_bias(const DenseParams &p, int64_t block, int threads, double (*join)[16]) {
+    const int64_t c = block * 16 + threadIdx.x % 16;
+    const int groups = threads / 16, of = threadIdx.x / 16;   // 32 groups at most
+    double v = 0.0;
+    if (c < p.db_n)
+#pragma unroll 4
+        for (int64_t b = of; b < p.db_blocks; b += groups) v += (double)p.sums[b * p.db_n + c];
+    join[of][threadIdx.x % 16] = v;
+    __syncthreads();
+    if (threadIdx.x < 16 && c < p.db_n) {
+        v = 0.0;
+        for (int i = 0; i < groups; ++i) v += join[i][threadIdx.x];
+        store_value<ST>(p.db, c, (float)v);
+    }
+}
+
 template <typename ST, typename Sh, bool DMA>
 __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void dense_kernel(DenseParams p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int BM = Sh::BM, BN = Sh::BN;
     const uint32_t tiles_m = (uint32_t)((p.M + BM - 1) / BM), tiles_n = (uint32_t)((p.N + BN - 1) / BN);
     const uint32_t each = tiles_m * tiles_n;
+    if constexpr (Sh::ACOLS) {   // a weight's gradient: the bias' with it
+        const uint32_t own = (each * (uint32_t)p.splits + 7) / 8 * 8;
+        if (blockIdx.x >= own) {
+            add_bias<ST>(p, blockIdx.x - own, Sh::THREADS, (double(*)[16])smem);
+            return;
+        }
+    }
     const int64_t tile = xcd_tile(blockIdx.x, each * (uint32_t)p.splits);
     if (tile < 0) return;
     // 8 tile rows at a time, column by column: the workgroups of an XCD share a
@@ -446,21 +473,9 @@ template <typename ST> __global__ __launch_bounds__(256) void dense_grad_kernel(
         p.sums[(int64_t)blockIdx.y * p.N + c] = v;
     }
 }
-// db: the workgroups' sums, added in 64 bits
-template <typename ST> __global__ __launch_bounds__(256) void dense_bias_kernel(DenseGradParams p) {
-    __shared__ double join[4][64];
-    const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x % 64;
-    const int64_t blocks = (p.M + p.rows - 1) / p.rows;
-    double v = 0.0;
-    if (c < p.N)
-#pragma unroll 4
-        for (int64_t b = threadIdx.x / 64; b < blocks; b += 4) v += (double)p.sums[b * p.N + c];
-    join[threadIdx.x / 64][threadIdx.x % 64] = v;
-    __syncthreads();
-    if (threadIdx.x < 64 && c < p.N) {
-        const int i = threadIdx.x;
-        store_value<ST>(p.db, c, (float)(join[0][i] + join[1][i] + join[2][i] + join[3][i]));
-    }
+template <typename ST> __global__ __launch_bounds__(256) void dense_bias_kernel(DenseParams p) {
+    __shared__ double join[16][16];
+    add_bias<ST>(p, blockIdx.x, 256, join);
 }
 
 namespace {
@@ -478,7 +493,8 @@ hipError_t dense_go(const DenseParams &p, hipStream_t st) {
     const int64_t all = tiles(p, Sh::BM, Sh::BN) * p.splits;
     if (all >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
     if (hipError_t e = allow_lds<&dense_kernel<ST, Sh, DMA>>(Sh::LDS_BYTES); e != hipSuccess) return e;
-    dense_kernel<ST, Sh, DMA><<<dim3((uint32_t)((all + 7) / 8 * 8)), Sh::THREADS, Sh::LDS_BYTES, st>>>(p);
+    const int64_t blocks = (all + 7) / 8 * 8 + (Sh::ACOLS && p.db ? (p.db_n + 15) / 16 : 0);
+    dense_kernel<ST, Sh, DMA><<<dim3((uint32_t)blocks), Sh::THREADS, Sh::LDS_BYTES, st>>>(p);
     return hipGetLastError();
 }
 template <typename ST, int P, int WAVES, int U> hipError_t few_go(const DenseParams &p, hipStream_t st) {
@@ -505,7 +521,7 @@ template <typename ST> hipError_t few_plan(const DenseParams &p, hipStream_t st)
 // gradient); partial sums cost a launch and their way through memory.  Chosen so,
 // products of those shapes take 1% longer on average than with the best tile of
 // each.  Measured (us, M x N x K, operands along K; 32 x 16 / 32 x 32 / 64 x 32 / 64 x
-// 64 in two groups of waves / 64 x 64 / 128 x 128 / 256 x 128 / 256 x 256):
+// 64 in two groups of waves / 64 x 64 / 128 x 128 / 128 x 256 / 256 x 256):
 //     32 x 4096 x 4096      12 / 14 / 19 / 23 / 43 / 44 / 79 / 125
 //     128 x 4096 x 4096     34 / 24 / 18 / 23 / 44 / 44 / 72 / 120
 //     512 x 4096 x 4096    132 / 93 / 69 / 43 / 39 / 41 / 66 / 112
@@ -519,7 +535,8 @@ constexpr TileCost kTiles[] = {
     {32, 16, 256, {2.0f, 1.8f}, {1.45f, 2.4f}},     {32, 32, 256, {2.0f, 1.8f}, {2.25f, 3.3f}},
     {64, 32, 256, {2.7f, 2.2f}, {2.85f, 3.25f}},    {64, 64, 256, {2.7f, 2.1f}, {3.7f, 4.05f}},
     {64, 64, 512, {2.2f, 1.6f}, {6.5f, 7.2f}},      {128, 128, 256, {3.9f, 3.1f}, {7.4f, 7.8f}},
-    {256, 128, 256, {6.1f, 4.7f}, {12.2f, 14.2f}},  {256, 256, 256, {7.7f, 5.4f}, {21.5f, 21.0f}},
+    {128, 128, 512, {6.0f, 1.8f}, {12.6f, 13.1f}},  {128, 256, 256, {6.1f, 4.7f}, {12.2f, 14.2f}},
+    {256, 256, 256, {7.7f, 5.4f}, {21.5f, 21.0f}},
 };
 struct DensePlan {
     int tile, splits;
@@ -557,7 +574,8 @@ template <typename ST, bool AC, bool BC> hipError_t tile_plan(const DenseParams 
     case 3: return dense_go<ST, TileShape<1, AC, BC, 64, 64, 2, 2, 4, 2>, true>(p, st);
     case 4: return dense_go<ST, TileShape<1, AC, BC, 64, 64, 2, 2, 2, 2>, true>(p, st);
     case 5: return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 4, 4>, true>(p, st);
-    case 6: return dense_go<ST, TileShape<1, AC, BC, 256, 128, 4, 2, 3>, true>(p, st);
+    case 6: return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 4, 2>, true>(p, st);
+    case 7: return dense_go<ST, TileShape<1, AC, BC, 128, 256, 2, 4, 3>, true>(p, st);
     default: return dense_go<ST, TileShape<1, AC, BC, 256, 256, 2, 4, 2>, true>(p, st);
     }
 }
@@ -591,7 +609,7 @@ int64_t dense_grad_rows(int64_t M, int64_t N) {
     // 128 rows, or so many that there are about 1024 workgroups
     const int64_t across = (N + 255) / 256;
     int64_t rows = 128;
-    while (rows > 8 && ((M + rows - 1) / rows) * across < 512) rows /= 2;
+    while (rows > 16 && ((M + rows - 1) / rows) * across < 512) rows /= 2;
     while ((M + rows - 1) / rows >= 32768) rows *= 2;
     return rows;
 }
@@ -602,9 +620,14 @@ hipError_t launch_dense_grad(const DenseGradParams &p, int dtype, hipStream_t st
     return hipGetLastError();
 }
 hipError_t launch_dense_bias(const DenseGradParams &p, int dtype, hipStream_t st) {
-    const dim3 grid((uint32_t)((p.N + 63) / 64));
-    if (dtype == OZK_F16) dense_bias_kernel<_Float16><<<grid, 256, 0, st>>>(p);
-    else dense_bias_kernel<__bf16><<<grid, 256, 0, st>>>(p);
+    DenseParams q = {};
+    q.sums = p.sums;
+    q.db = p.db;
+    q.db_n = p.N;
+    q.db_blocks = (p.M + p.rows - 1) / p.rows;
+    const dim3 grid((uint32_t)((p.N + 15) / 16));
+    if (dtype == OZK_F16) dense_bias_kernel<_Float16><<<grid, 256, 0, st>>>(q);
+    else dense_bias_kernel<__bf16><<<grid, 256, 0, st>>>(q);
     return hipGetLastError();
 }
 

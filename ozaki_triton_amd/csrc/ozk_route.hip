@@ -10,11 +10,12 @@
 //   over the n tokens that are not masked out.  Masked ones have expert E, weight 0
 //   and the places behind the last group.
 //
-// Three launches: rows (softmax, choice, counts of each workgroup's tokens and
-// the slots' places among them), scan (the counts of the workgroups before) and
-// place (slots to their places); few tokens need one workgroup and one launch.
-// The sums over tokens are those of fixed parts in a fixed order, no atomics but
-// whole-number counts.
+// Two launches: rows (softmax, choice, counts of each workgroup's tokens and the
+// slots' places among them) and place (slots to their places: every workgroup adds
+// up the counts of those before it; where that is much to read, a third launch,
+// scan, does it once); few tokens need one workgroup and one launch.  The sums over
+// tokens are those of fixed parts in a fixed order, no atomics but whole-number
+// counts.
 //
 // A token takes GL lanes with V consecutive logits each, so that several share a
 // wave; the k choices are k rounds of a maximum over keys (the logits' bits in
@@ -52,22 +53,31 @@ template <int GL, typename T, typename F> OZK_DEV T over_group(T v, F &&f) {
 template <int GL> OZK_DEV uint32_t group_max(uint32_t v) {
     return over_group<GL>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
-template <int GL> OZK_DEV uint32_t group_min(uint32_t v) {
-    return over_group<GL>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-}
 template <int GL> OZK_DEV float group_sum(float v) {
     return over_group<GL>(v, [](float a, float b) { return a + b; });
 }
 
-// Whole numbers in the order of the values: -0 as 0, NaN above all; 0 is below
-// every logit's.
-OZK_DEV uint32_t key_of(float x) {
-    if (x != x) return 0xFFFFFFFFu;
-    const uint32_t u = __float_as_uint(x + 0.f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+// Keys: whole numbers in the order of the values, -0 as 0, NaN above all, 0 below
+// every logit's.  Of 16-bit logits a key has the index behind the value's bits,
+// the lowest greatest, so that a maximum finds both.
+template <typename T> OZK_DEV uint32_t key_of(float x, uint32_t index) {
+    if constexpr (sizeof(T) == 4) {
+        if (x != x) return 0xFFFFFFFFu;
+        const uint32_t u = __float_as_uint(x + 0.f);
+        return u & 0x80000000u ? ~u : u | 0x80000000u;
+    } else {
+        const uint32_t u = to_bits16(x + 0.f, T{});
+        const uint32_t key = x != x ? 0xFFFFu : u & 0x8000u ? ~u & 0xFFFFu : u | 0x8000u;
+        return key << 16 | (0xFFFFu - index);
+    }
 }
-OZK_DEV float value_of(uint32_t key) {
-    return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+template <typename T> OZK_DEV float value_of(uint32_t key) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+    } else {
+        const uint32_t k = key >> 16;
+        return from_bits16((uint16_t)(k & 0x8000u ? k & 0x7FFFu : ~k), T{});
+    }
 }
 
 // A token's V logits of a lane, from expert e0 on; -inf behind the last expert
@@ -91,20 +101,18 @@ constexpr int kRouteWaves = 16;   // of a workgroup
 struct RouteLds {
     uint32_t *wave_hist;   // [waves][E + 1]
     float *psum;           // [waves][E]
-    float *top;            // [per]: the greatest logit
-    float *scale;          // [per]: 1 over the sum that the weights are divided by
-    float *value;          // [per k]: the chosen logits
+    float *scale;          // [per]: what the weights are divided by
+    float *value;          // [per k]: e to the chosen logits less the greatest
     uint16_t *expert;      // [per k]
     OZK_DEV RouteLds(char *at, int E, int64_t per, int k) {
         wave_hist = (uint32_t *)at;
         psum = (float *)(wave_hist + kRouteWaves * (E + 1));
-        top = psum + kRouteWaves * E;
-        scale = top + per;
+        scale = psum + kRouteWaves * E;
         value = scale + per;
         expert = (uint16_t *)(value + per * k);
     }
     static size_t bytes(int E, int64_t per, int k) {
-        return 4 * (size_t)(kRouteWaves * (2 * E + 1)) + 8 * (size_t)per + 6 * (size_t)(per * k);
+        return 4 * (size_t)(kRouteWaves * (2 * E + 1)) + 4 * (size_t)per + 6 * (size_t)(per * k);
     }
 };
 
@@ -122,7 +130,8 @@ OZK_DEV uint32_t before_in_block(uint32_t v, uint32_t *parts) {
     if (lane == 63) parts[wave] = s;
     __syncthreads();
     uint32_t before = s - v;
-    for (int w = 0; w < wave; ++w) before += parts[w];
+#pragma unroll
+    for (int w = 0; w < kRouteWaves - 1; ++w) before += w < wave ? parts[w] : 0u;
     return before;
 }
 
@@ -152,6 +161,7 @@ OZK_DEV void finish_counts(const RouteParams &p, uint32_t total, double P, uint3
     __syncthreads();
     if (threadIdx.x == 0) {
         s = n = 0.0;
+#pragma unroll
         for (int w = 0; w < kRouteWaves; ++w) {
             s += sums[w];
             n += sums[kRouteWaves + w];
@@ -183,27 +193,55 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteParam
         logits_at<T, V>(p.logits + (t0 + t) * p.pitch * (int64_t)sizeof(T), e0, p.E, valid, l);
         uint32_t key[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = e0 + v < p.E ? key_of(l[v]) : 0u;
-        float top = 0.f, chosen = 0.f;
-        for (int j = 0; j < p.k; ++j) {
-            uint32_t best = key[0];
+        for (int v = 0; v < V; ++v) key[v] = e0 + v < p.E ? key_of<T>(l[v], e0 + v) : 0u;
+        // k rounds; lane j of the group keeps the j-th choice, GL of them at a time
+        float top = 0.f, chosen = 0.f, kept = 0.f;
+        uint32_t kept_at = 0;
+        for (int j0 = 0; j0 < p.k; j0 += GL) {
+            const int here = p.k - j0 < GL ? p.k - j0 : GL;
+            for (int j = 0; j < here; ++j) {
+                uint32_t own = key[0];
 #pragma unroll
-            for (int v = 1; v < V; ++v) best = key[v] > best ? key[v] : best;
-            best = group_max<GL>(best);
-            uint32_t at = 0xFFFFu;
+                for (int v = 1; v < V; ++v) own = key[v] > own ? key[v] : own;
+                const uint32_t best = group_max<GL>(own);
+                const float x = value_of<T>(best);
+                if (j0 + j == 0) top = x;
+                kept = in == j ? x : kept;
+                if constexpr (sizeof(T) == 4) {
+                    // the lowest lane of the group that has it, there the lowest slot
+                    const uint64_t has = __ballot(own == best);
+                    uint32_t lowest;
+                    if constexpr (GL == 64) lowest = (uint32_t)__builtin_ctzll(has);
+                    else lowest = __builtin_ctz((uint32_t)(has >> (lane & ~(GL - 1))) | (uint32_t)(1ull << GL));
+                    if ((uint32_t)in == lowest) {
+                        uint32_t at = 0;
+                        bool found = false;
 #pragma unroll
-            for (int v = V - 1; v >= 0; --v) at = key[v] == best ? (uint32_t)(e0 + v) : at;
-            at = group_min<GL>(at);
+                        for (int v = 0; v < V; ++v) {
+                            const bool hit = !found && key[v] == best;
+                            found |= hit;
+                            at = hit ? (uint32_t)(e0 + v) : at;
+                            key[v] = hit ? 0u : key[v];
+                        }
+                        if (there) lds.expert[t * p.k + j0 + j] = (uint16_t)(valid ? at : (uint32_t)p.E);
+                    }
+                } else {
+                    kept_at = in == j ? 0xFFFFu - (best & 0xFFFFu) : kept_at;
 #pragma unroll
-            for (int v = 0; v < V; ++v) key[v] = (uint32_t)(e0 + v) == at ? 0u : key[v];
-            const float x = value_of(best);
-            if (j == 0) top = x;
-            chosen += expf(x - top);
-            if (in == 0 && there) {
-                lds.value[t * p.k + j] = x;
-                lds.expert[t * p.k + j] = (uint16_t)(valid ? at : (uint32_t)p.E);
+                    for (int v = 0; v < V; ++v) key[v] = key[v] == best ? 0u : key[v];
+                }
+            }
+            if (in < here) {
+                const float e = expf(kept - top);
+                chosen += e;
+                if (there) {
+                    lds.value[t * p.k + j0 + in] = e;
+                    if constexpr (sizeof(T) == 2)
+                        lds.expert[t * p.k + j0 + in] = (uint16_t)(valid ? kept_at : (uint32_t)p.E);
+                }
             }
         }
+        chosen = group_sum<GL>(chosen);
         float q[V], sum = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -211,10 +249,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteParam
             sum += q[v];
         }
         sum = group_sum<GL>(sum);
-        if (in == 0 && there) {
-            lds.top[t] = top;
-            lds.scale[t] = p.normalize ? chosen : sum;
-        }
+        if (in == 0 && there) lds.scale[t] = p.normalize ? chosen : sum;
         if (valid) {
             const float by = 1.f / sum;
 #pragma unroll
@@ -240,7 +275,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteParam
         const int t = (int)((uint32_t)i / (uint32_t)p.k), e = lds.expert[i];
         atomicAdd(&hist[e], 1u);
         p.experts[s0 + i] = e;
-        p.weights[s0 + i] = e == p.E ? 0.f : expf(lds.value[i] - lds.top[t]) / lds.scale[t];
+        p.weights[s0 + i] = e == p.E ? 0.f : lds.value[i] / lds.scale[t];
     }
     __syncthreads();
     // over the waves, in order; the workgroup's counts and sums
@@ -348,38 +383,86 @@ __global__ __launch_bounds__(1024) void route_scan_kernel(RouteParams p) {
     }
 }
 
-__global__ __launch_bounds__(1024) void route_place_kernel(RouteParams p) {
+// (one workgroup more than there are, the first: it writes the counts, the offsets
+// and the loss)
+template <bool SCANNED> __global__ __launch_bounds__(1024) void route_place_kernel(RouteParams p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ __attribute__((aligned(16))) uint32_t parts[4 * kRouteWaves];
     uint32_t *start = (uint32_t *)smem;   // [E + 1]
     const int e = threadIdx.x;
-    const uint32_t total = e < p.E ? (uint32_t)p.counts[e] : 0u;
-    const uint32_t before = before_in_block(total, parts);
-    if (blockIdx.x == 0) finish_counts(p, total, e < p.E ? (double)p.psum[e] : 0.0, before, parts);
-    if (e < p.E) {
-        start[e] = before + p.hist[(int64_t)blockIdx.x * p.E + e];
-        if (e == p.E - 1) {
-            // behind the last group, and the masked slots of the workgroups before: all
-            // of their slots less those of the experts
-            start[p.E] = before + total;
+    const int block = (int)blockIdx.x - 1;
+    const bool rest = block < 0;   // counts, offsets, loss
+    const int64_t t0 = (int64_t)block * p.per, s0 = t0 * p.k;
+    const int tokens = (int)(p.T - t0 < p.per ? p.T - t0 : p.per), slots = rest ? 0 : tokens * p.k;
+    // on their way while the counts are added up
+    const int first = e < slots ? p.experts[s0 + e] : 0, first_at = e < slots ? p.place[s0 + e] : 0;
+    uint32_t total = 0, earlier = 0;      // of expert e: slots of all workgroups, of those before
+    double P = 0.0;
+    if constexpr (SCANNED) {
+        if (e < p.E) {
+            total = (uint32_t)p.counts[e];
+            if (rest) P = (double)p.psum[e];
+            else earlier = p.hist[(int64_t)block * p.E + e];
         }
+    } else {
+        // `ways` lanes to an expert, each every ways-th workgroup's counts
+        uint32_t *sums = start + (p.E + 2) / 2 * 2;   // [2][1024]
+        double *ps = (double *)(sums + 2048);         // [1024]
+        const int ways = 1024 / p.E, of = e % p.E, way = e / p.E;
+        if (way < ways) {
+#pragma unroll 8
+            for (int b = way; b < p.blocks; b += ways) {
+                const uint32_t n = p.hist[(int64_t)b * p.E + of];
+                total += n;
+                earlier += b < block ? n : 0u;
+            }
+            if (rest)
+#pragma unroll 8
+                for (int b = way; b < p.blocks; b += ways) P += (double)p.psum[(int64_t)b * p.E + of];
+            sums[e] = total;
+            sums[1024 + e] = earlier;
+            ps[e] = P;
+        }
+        __syncthreads();
+        total = earlier = 0;
+        P = 0.0;
+        if (e < p.E)
+#pragma unroll 4
+            for (int w = 0; w < ways; ++w) {
+                total += sums[w * p.E + e];
+                earlier += sums[1024 + w * p.E + e];
+                if (rest) P += ps[w * p.E + e];
+            }
+    }
+    const uint32_t before = before_in_block(total, parts);
+    if (rest) {
+        finish_counts(p, total, P, before, parts);
+        return;
+    }
+    if (e < p.E) {
+        start[e] = before + earlier;
+        if (e == p.E - 1) start[p.E] = before + total;   // behind the last group
     }
     __syncthreads();
-    const int64_t t0 = (int64_t)blockIdx.x * p.per, s0 = t0 * p.k;
-    const int tokens = (int)(p.T - t0 < p.per ? p.T - t0 : p.per), slots = tokens * p.k;
     if (p.mask) {
-        // the workgroups' slots before this one that have an expert
-        uint32_t n = e < p.E ? p.hist[(int64_t)blockIdx.x * p.E + e] : 0u;
-        const uint32_t upto = before_in_block(n, parts) + n;
+        // and the masked slots of the workgroups before: all of theirs less the experts'
+        const uint32_t upto = before_in_block(earlier, parts) + earlier;
         __syncthreads();
         if (e == 64 * kRouteWaves - 1) start[p.E] += (uint32_t)s0 - upto;
         __syncthreads();
     }
     for (int i = threadIdx.x; i < slots; i += 1024) {
-        const uint32_t at = start[p.experts[s0 + i]] + (uint32_t)p.place[s0 + i];
+        const uint32_t at = i == e ? start[first] + (uint32_t)first_at
+                                   : start[p.experts[s0 + i]] + (uint32_t)p.place[s0 + i];
         p.place[s0 + i] = (int32_t)at;
         p.order[at] = (int32_t)(s0 + i);
     }
+}
+
+// LDS writes of a wave's other lanes before reads, and back
+OZK_DEV void settle_wave() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // The logits' gradient.  With q = softmax(l), c_e the counts and n the tokens:
@@ -389,7 +472,9 @@ __global__ __launch_bounds__(1024) void route_place_kernel(RouteParams p) {
 template <typename T, int GL, int V>
 __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradParams p) {
     constexpr int TPW = 64 / GL;
+    __shared__ __attribute__((aligned(16))) float spread[4][TPW][GL * V];
     const int lane = threadIdx.x & 63, in = lane % GL, e0 = in * V;
+    float *at_experts = spread[threadIdx.x >> 6][lane / GL];
     float g0[V] = {};
     if (p.dloss) {
         uint32_t c[V], sum = 0;
@@ -428,21 +513,30 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradParams p) {
         }
         sum = group_sum<GL>(sum);
         const float by = 1.f / sum;
-        if (p.dw && valid) {
+        if (p.dw) {
+            // lane j has the token's j-th choice; through the LDS to its expert's lane
             const int64_t s = t * p.k;
             float mean = 0.f;
-            if (p.normalize)
-                for (int j = 0; j < p.k; ++j) mean = fmaf(p.weights[s + j], p.dw[s + j], mean);
-            for (int j = 0; j < p.k; ++j) {
-                const int e = p.experts[s + j];
-                const float dw = p.dw[s + j];
-                const float add = p.normalize ? p.weights[s + j] * (dw - mean) : dw;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (p.normalize) d[v] += e == e0 + v ? add : 0.f;
-                    else g[v] += e == e0 + v ? add : 0.f;
-                }
+            if (p.normalize) {
+                for (int j = in; j < p.k; j += GL)
+                    if (valid) mean = fmaf(p.weights[s + j], p.dw[s + j], mean);
+                mean = group_sum<GL>(mean);
             }
+#pragma unroll
+            for (int v = 0; v < V; ++v) at_experts[e0 + v] = 0.f;
+            settle_wave();
+            for (int j = in; j < p.k; j += GL)
+                if (valid)
+                    at_experts[p.experts[s + j]] =
+                        p.normalize ? p.weights[s + j] * (p.dw[s + j] - mean) : p.dw[s + j];
+            settle_wave();
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float add = at_experts[e0 + v];
+                if (p.normalize) d[v] = add;
+                else g[v] += add;
+            }
+            settle_wave();
         }
         float dot = 0.f;
 #pragma unroll
@@ -470,7 +564,10 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradParams p) {
 
 namespace {
 
-// lanes of a token and values of a lane, by E
+// Lanes of a token and values of a lane, by E.  4 values: with 8 a wave takes twice
+// the tokens at once, which pays only where there are many (rows alone, us, with 4 /
+// with 8: 32768 x 64, k = 8, fp32 13.4 / 12.5; 4099 x 40, k = 3, bf16 6.3 / 8.1; 16 x
+// 16, k = 2 6.8 / 7.8).
 template <typename F> hipError_t with_shape(int E, F &&f) {
     using std::integral_constant;
 #define OZK_ROUTE(GL, V) return f(integral_constant<int, GL>{}, integral_constant<int, V>{})
@@ -484,7 +581,11 @@ template <typename F> hipError_t with_shape(int E, F &&f) {
     OZK_ROUTE(64, 16);
 #undef OZK_ROUTE
 }
-int lanes_of(int E) { return E <= 8 ? 2 : E <= 16 ? 4 : E <= 32 ? 8 : E <= 64 ? 16 : E <= 128 ? 32 : 64; }
+int lanes_of(int E) {
+    int lanes = 2;
+    while (lanes < 64 && E > 4 * lanes) lanes *= 2;
+    return lanes;
+}
 
 template <typename T> hipError_t route_go(const RouteParams &p, hipStream_t st) {
     return with_shape(p.E, [&](auto gl, auto v) {
@@ -517,7 +618,7 @@ void plan_route(RouteParams &p) {
     // a workgroup's tokens: one step of its waves, more where that makes more
     // than 256 of them, as many as its LDS holds
     const int64_t step = (int64_t)kRouteWaves * 64 / lanes_of(p.E);
-    int64_t per = step, most = (150 * 1024 - (int64_t)RouteLds::bytes(p.E, 0, 0)) / (8 + 6 * p.k);
+    int64_t per = step, most = (150 * 1024 - (int64_t)RouteLds::bytes(p.E, 0, 0)) / (4 + 6 * p.k);
     while (per < most / 2 && (p.T + per - 1) / per > 256) per *= 2;
     if (per > most) per = most;
     p.per = per;
@@ -529,9 +630,15 @@ hipError_t launch_route(const RouteParams &p, int dtype, hipStream_t st) {
                    : dtype == OZK_F16 ? route_go<_Float16>(p, st)
                                       : route_go<__bf16>(p, st);
     if (e != hipSuccess || p.blocks == 1) return e;
+    // up to 32 counts to a lane are read again by every workgroup
+    if ((int64_t)p.blocks * p.E <= 32 * 1024) {
+        const size_t lds = 4 * ((p.E + 2) / 2 * 2) + 8 * 1024 + 8 * 1024;
+        route_place_kernel<false><<<(uint32_t)p.blocks + 1, 1024, lds, st>>>(p);
+        return hipGetLastError();
+    }
     route_scan_kernel<<<(uint32_t)((p.E + 15) / 16), 1024, 0, st>>>(p);
     if (e = hipGetLastError(); e != hipSuccess) return e;
-    route_place_kernel<<<(uint32_t)p.blocks, 1024, 4 * (p.E + 1), st>>>(p);
+    route_place_kernel<true><<<(uint32_t)p.blocks + 1, 1024, 4 * (p.E + 1), st>>>(p);
     return hipGetLastError();
 }
 hipError_t launch_route_grad(const RouteGradParams &p, int dtype, hipStream_t st) {

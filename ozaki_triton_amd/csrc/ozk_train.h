@@ -24,6 +24,10 @@ struct DenseParams {
     bool a_padded, b_padded;   // rows go on with zeros up to a whole 16-byte piece
     float *part;             // workspace [splits, M, N]: partial sums of the K ranges (splits > 1)
     int splits;
+    // where given, workgroups behind the tiles' add up db (DenseGradParams)
+    const float *sums;
+    char *db;
+    int64_t db_n, db_blocks;
 };
 // a product of a few rows, which is not cut into tiles
 bool dense_few(const DenseParams &p);
@@ -96,6 +100,7 @@ struct ClipParams {
     uint32_t part0, parts;   // first partial sum of this launch, and how many all have
     double *part;
     double max_norm;
+    bool past_caches;        // the tensors are more than the memory-side cache holds
     float *norm;             // written by the launch that has it, else null
 };
 hipError_t launch_square_sums(const ClipParams &p, uint32_t grid, hipStream_t st);

@@ -209,16 +209,17 @@ constexpr int64_t kClipGrid = 2048;
 size_t clip_bytes(int64_t tensors) { return 8 * (size_t)(kClipGrid + tensors + 1); }
 
 int clip_checks(const void *const *grads, void *const *outs, bool scaled, const int64_t *counts,
-                const int *dtypes, int64_t tensors, double &elements) {
+                const int *dtypes, int64_t tensors, double &elements, double &bytes) {
     if (tensors < 0) return OZK_ERR_SHAPE;
     if (tensors > (int64_t)1 << 28) return OZK_ERR_TOO_LARGE;
     if (tensors && (!grads || !counts || !dtypes || (scaled && !outs))) return OZK_ERR_NULL;
-    elements = 0;
+    elements = bytes = 0;
     for (int64_t i = 0; i < tensors; ++i) {
         if (!is_float(dtypes[i])) return OZK_ERR_DTYPE;
         if (counts[i] < 0 || counts[i] >= (int64_t)1 << 56) return OZK_ERR_SHAPE;
         if (counts[i] && (!grads[i] || (scaled && !outs[i]))) return OZK_ERR_NULL;
         elements += (double)counts[i];
+        bytes += (double)counts[i] * (dtypes[i] == OZK_F32 ? 4 : 2);
     }
     return OZK_OK;
 }
@@ -254,11 +255,12 @@ int overlap_checks(const void *const *grads, void *const *outs, const int64_t *c
 }
 
 int run_clip(const void *const *grads, void *const *outs, const int64_t *counts, const int *dtypes,
-             int64_t tensors, double elements, double max_norm, float *norm, double *part,
+             int64_t tensors, double elements, double bytes, double max_norm, float *norm, double *part,
              hipStream_t st) {
-    // pieces of 2^11 to 2^16 elements, at least about 4096 of them where there is enough
+    // pieces of 2^11 to 2^14 elements, at least about 4096 of them where there is enough:
+    // larger ones come out uneven over the workgroups
     uint32_t size = 1 << 11;
-    while (size < 1 << 16 && elements / (2 * size) >= 4096) size *= 2;
+    while (size < 1 << 14 && elements / (2 * size) >= 4096) size *= 2;
     // more than a launch counts: larger ones
     while (elements / size > (double)((int64_t)1 << 30)) {
         if (size >= 1u << 29) return OZK_ERR_TOO_LARGE;
@@ -269,6 +271,7 @@ int run_clip(const void *const *grads, void *const *outs, const int64_t *counts,
     p.size = size;
     p.part = part;
     p.max_norm = max_norm;
+    p.past_caches = bytes > 256e6;
     const double whole = elements / size + (double)tensors;   // at least all pieces
     for (int pass = 0; pass < (outs ? 2 : 1); ++pass) {
         uint32_t part0 = 0;
@@ -371,6 +374,8 @@ int ozk_linear_backward(const void *dy, int64_t dy_stride, const void *z, const 
         return OZK_ERR_WORKSPACE;
     char *ws = (char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
+    // db's partial sums are added up by workgroups of dW's product where there is one
+    const bool in_product = db && b.sums && (want & 2) && N > 0 && K > 0;
     if (N > 0) {
         b.d.z = (const char *)z;
         b.d.dz = b.dz ? ws : nullptr;
@@ -379,10 +384,16 @@ int ozk_linear_backward(const void *dy, int64_t dy_stride, const void *z, const 
         b.d.db = (char *)db;
         if (b.d.dz || b.d.sums)
             if (hipError_t e = ozk::launch_dense_grad(b.d, dtype, st); e != hipSuccess) return launched(e);
-        if (db)   // (no rows: zeros)
+        if (db && !in_product)   // (no rows: zeros)
             if (hipError_t e = ozk::launch_dense_bias(b.d, dtype, st); e != hipSuccess) return launched(e);
     }
     char *rest = ws ? ws + b.dz + b.sums : nullptr;
+    if (in_product) {
+        b.dw.sums = b.d.sums;
+        b.dw.db = b.d.db;
+        b.dw.db_n = N;
+        b.dw.db_blocks = (M + b.d.rows - 1) / b.d.rows;
+    }
     if (want & 1) {
         b.dx.C = (char *)dx;
         b.dx.c_pitch = dx_stride * 2;
@@ -485,29 +496,29 @@ int ozk_gradient_norm_workspace_bytes(int64_t tensors, size_t *bytes_out) {
 int ozk_gradient_norm(const void *const *grads, const int64_t *counts, const int *dtypes,
                       int64_t tensors, float *norm, void *workspace, size_t workspace_bytes,
                       void *stream) {
-    double elements;
-    if (int st = clip_checks(grads, nullptr, false, counts, dtypes, tensors, elements)) return st;
+    double elements, bytes;
+    if (int st = clip_checks(grads, nullptr, false, counts, dtypes, tensors, elements, bytes)) return st;
     if (!norm) return OZK_ERR_NULL;
     if (!workspace || workspace_bytes < clip_bytes(tensors) || ((uintptr_t)workspace & 15))
         return OZK_ERR_WORKSPACE;
-    return run_clip(grads, nullptr, counts, dtypes, tensors, elements, 0.0, norm, (double *)workspace,
+    return run_clip(grads, nullptr, counts, dtypes, tensors, elements, bytes, 0.0, norm, (double *)workspace,
                     (hipStream_t)stream);
 }
 
 int ozk_clip_gradients(const void *const *grads, void *const *outs, const int64_t *counts,
                        const int *dtypes, int64_t tensors, double max_norm, float *norm,
                        void *workspace, size_t workspace_bytes, void *stream) {
-    double elements;
-    if (int st = clip_checks(grads, outs, true, counts, dtypes, tensors, elements)) return st;
+    double elements, bytes;
+    if (int st = clip_checks(grads, outs, true, counts, dtypes, tensors, elements, bytes)) return st;
     if (!norm) return OZK_ERR_NULL;
     if (!(max_norm >= 0.0)) return OZK_ERR_SHAPE;
     if (!workspace || workspace_bytes < clip_bytes(tensors) || ((uintptr_t)workspace & 15))
         return OZK_ERR_WORKSPACE;
     if (!tensors)
-        return run_clip(grads, nullptr, counts, dtypes, 0, 0.0, 0.0, norm, (double *)workspace,
+        return run_clip(grads, nullptr, counts, dtypes, 0, 0.0, 0.0, 0.0, norm, (double *)workspace,
                         (hipStream_t)stream);
     if (int st = overlap_checks(grads, outs, counts, dtypes, tensors)) return st;
-    return run_clip(grads, outs, counts, dtypes, tensors, elements, max_norm, norm,
+    return run_clip(grads, outs, counts, dtypes, tensors, elements, bytes, max_norm, norm,
                     (double *)workspace, (hipStream_t)stream);
 }
 
