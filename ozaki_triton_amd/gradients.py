@@ -95,14 +95,15 @@ def clip_gradients(grads, max_norm: float, *, out=None) -> torch.Tensor:
     if out is None:
         whole = all([t.is_contiguous() for t in grads])
     else:
-        to, _ = _checked("clip_gradients", out)
+        to, kinds = _checked("clip_gradients", out)
         assert len(to) == len(grads), f"out must have {len(grads)} tensors, got {len(to)}"
-        for g, o in zip(grads, to):
-            assert o.shape == g.shape and o.dtype == g.dtype, \
-                f"out must match: {tuple(g.shape)} {g.dtype}, got {tuple(o.shape)} {o.dtype}"
+        if kinds != codes or [t.shape for t in to] != [t.shape for t in grads]:
+            for g, o in zip(grads, to):
+                assert o.shape == g.shape and o.dtype == g.dtype, \
+                    f"out must match: {tuple(g.shape)} {g.dtype}, got {tuple(o.shape)} {o.dtype}"
         if grads[0].get_device() != to[0].get_device():
             _on_one_gpu(grads[0], to[0])
-        whole = all([g.is_contiguous() and o.is_contiguous() for g, o in zip(grads, to)])
+        whole = all([t.is_contiguous() for t in grads]) and all([t.is_contiguous() for t in to])
     outs = to
     if not whole:
         ins, to, back = _through_copies(grads, to)
