@@ -2,12 +2,15 @@
 
     python examples/expert_layer.py [--steps 30] [--tokens 512] [--experts 8]
 
-Training: a router sends every token to its best expert; the tokens are sorted by
-expert and go through two grouped products with a ReLU between, a head gives the
-outputs.  The experts' and the head's weights move along their orthogonalised
-momentum.  Serving: the head and each expert's matrices are brought to 4 bits, and
-single tokens go through them; the example prints how far the outputs are from the
-unquantised layer's.
+Training: every token goes through a shared expert, two dense products with the
+activation and the residual in them, and through its own: a router chooses it and
+sorts the tokens by expert for two grouped products with a ReLU between, whose result
+is weighted with the router's probability.  A head gives the outputs.  The loss has
+the router's balance loss in it; the gradients are clipped to a common norm, and the
+experts' and the head's weights move along their orthogonalised momentum.  Serving:
+the head and each expert's matrices are brought to 4 bits, and single tokens go
+through them; the example prints how far the outputs are from the unquantised
+layer's.
 
 Everything stays on the GPU: the groups' offsets are made there and the host never
 reads them.
@@ -30,32 +33,44 @@ class ExpertLayer:
             w = torch.randn(*size, generator=g, device="cuda") * size[-2] ** -0.5
             return w.to(dtype).requires_grad_()
 
-        self.router = torch.randn(width, experts, generator=g, device="cuda")   # fixed
+        self.router = torch.randn(width, experts, generator=g, device="cuda").requires_grad_()
         self.up = weight(experts, width, hidden)
         self.down = weight(experts, hidden, width)
-        self.head = weight(1, width, outputs)
+        # of the shared expert and the head: [out, in], as fused_linear reads them
+        self.shared_up = weight(width, hidden).detach().mT.contiguous().requires_grad_()
+        self.shared_down = weight(hidden, width).detach().mT.contiguous().requires_grad_()
+        self.head = weight(width, outputs).detach().mT.contiguous().requires_grad_()
+        self.bias = torch.zeros(outputs, device="cuda", dtype=dtype, requires_grad=True)
         self.momentum = [torch.zeros_like(w) for w in self.weights()]
 
     def weights(self):
-        return [self.up, self.down, self.head]
+        """Those that move along their orthogonalised momentum."""
+        return [self.up, self.down, self.shared_up, self.shared_down, self.head]
+
+    def shared(self, x):
+        h = ozk.fused_linear(x, self.shared_up, activation="gelu")
+        return ozk.fused_linear(h, self.shared_down, residual=x)
 
     def __call__(self, x):
-        expert = (x.float() @ self.router).argmax(-1)
-        order = expert.argsort(stable=True)
-        ends = torch.bincount(expert, minlength=self.router.shape[1]).cumsum(0)
-        offsets = torch.nn.functional.pad(ends, (1, 0))
-        h = ozk.grouped_matmul(x[order], self.up, offsets).relu()
-        y = torch.empty_like(x).index_copy(0, order, ozk.grouped_matmul(h, self.down, offsets))
-        whole = torch.tensor([0, x.shape[0]], device=x.device)
-        return ozk.grouped_matmul(x + y, self.head, whole)
+        """The outputs and the router's balance loss."""
+        r = ozk.route_tokens(x.float() @ self.router, 1, normalize=False)
+        h = ozk.grouped_matmul(x[r.order], self.up, r.offsets).relu()
+        y = ozk.grouped_matmul(h, self.down, r.offsets)[r.place[:, 0]] * r.weights.to(x.dtype)
+        return ozk.fused_linear(self.shared(x) + y, self.head, self.bias), r.balance_loss
 
     def step(self, x, target, rate):
-        loss = (self(x).float() - target).square().mean()
-        loss.backward()
+        y, balance = self(x)
+        loss = (y.float() - target).square().mean()
+        (loss + 0.01 * balance).backward()
+        others = [self.router, self.bias]
         with torch.no_grad():
+            ozk.clip_gradients([w.grad for w in self.weights() + others], 1.0)
             for w, m in zip(self.weights(), self.momentum):
                 m.mul_(0.9).add_(w.grad)
                 w.sub_(ozk.orthogonalize(m), alpha=rate)
+            for w in others:
+                w.sub_(w.grad, alpha=5 * rate)
+            for w in self.weights() + others:
                 w.grad = None
         return loss.detach()
 
@@ -64,11 +79,11 @@ class ServedLayer:
     """The same layer with 4-bit weights, for a few tokens at a time."""
 
     def __init__(self, layer, group_size=64):
-        self.router, self.group_size = layer.router, group_size
+        self.layer, self.group_size = layer, group_size
         pack = lambda w: ozk.quantize_w4(w.detach().T, group_size, zeros=True)  # noqa: E731
         self.up = [pack(w) for w in layer.up]
         self.down = [pack(w) for w in layer.down]
-        self.head = pack(layer.head[0])
+        self.head = pack(layer.head.mT)
 
     def _times(self, x, weights):
         return ozk.matmul_w4(x, *weights, group_size=self.group_size)
@@ -77,7 +92,8 @@ class ServedLayer:
     def token(self, x, expert):
         """x [1, width], its expert known to the caller (a serving loop batches by it)."""
         y = self._times(self._times(x, self.up[expert]).relu(), self.down[expert])
-        return self._times(x + y, self.head)
+        p = (x.float() @ self.layer.router).softmax(-1)[:, expert:expert + 1]
+        return self._times(self.layer.shared(x) + y * p.to(x.dtype), self.head) + self.layer.bias
 
 
 def main(argv=None):
@@ -97,7 +113,7 @@ def main(argv=None):
 
     served = ServedLayer(layer)
     with torch.no_grad():
-        whole = layer(x)
+        whole, _ = layer(x)
     experts = (x.float() @ layer.router).argmax(-1)[:8].tolist()
     got = torch.cat([served.token(x[i:i + 1], e) for i, e in enumerate(experts)])
     off = float((got.float() - whole[:8].float()).norm() / whole[:8].float().norm())

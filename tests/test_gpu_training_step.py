@@ -1,0 +1,110 @@
+"""The operators of a training step together: router, grouped products, dense products
+with their epilogues, clipping, orthogonalised update; eager and captured."""
+import math
+
+import pytest
+import torch
+
+import ozaki_triton_amd as ozk
+
+pytestmark = pytest.mark.gpu
+
+F16 = torch.float16
+T, WIDTH, HIDDEN, OUT, E, K = 200, 64, 96, 40, 5, 2
+
+
+def _setup(seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    p = dict(router=r(WIDTH, E) / 8, up=(r(E, WIDTH, HIDDEN) / 8).to(F16), down=(r(E, HIDDEN, WIDTH) / 10).to(F16),
+             shared=(r(HIDDEN, WIDTH) / 8).to(F16), back=(r(WIDTH, HIDDEN) / 10).to(F16),
+             head=(r(OUT, WIDTH) / 8).to(F16), bias=r(OUT).to(F16))
+    return r(T, WIDTH).to(F16), torch.rand(T, generator=g, device="cuda") < 0.85, r(T, OUT).to(F16), p
+
+
+def _step(x, mask, dy, p):
+    """One layer's outputs, balance loss and gradients, these clipped to half their norm's bound."""
+    r = ozk.route_tokens(x.float() @ p["router"], K, mask=mask)
+    h = ozk.grouped_matmul(x[r.order // K], p["up"], r.offsets).relu()
+    y = ozk.grouped_matmul(h, p["down"], r.offsets)
+    y = (y[r.place].float() * r.weights[..., None]).sum(1).to(F16)
+    s = ozk.fused_linear(ozk.fused_linear(x, p["shared"], activation="gelu"), p["back"], residual=x)
+    out = ozk.fused_linear(s + y, p["head"], p["bias"], activation="silu")
+    grads = list(torch.autograd.grad([out, r.balance_loss], list(p.values()),
+                                     [dy, torch.full((), 30.0, device="cuda")]))
+    norm = ozk.clip_gradients(grads, 20.0)
+    with torch.no_grad():
+        update = ozk.orthogonalize(grads[5])
+    return [out.detach(), r.balance_loss.detach(), norm, update, *grads]
+
+
+def _exact(x, mask, dy, p):
+    """The same in 64 bits, every expert on every token."""
+    p = {n: v.detach().double().requires_grad_() for n, v in p.items()}
+    x, dy = x.double(), dy.double()
+    logits = x @ p["router"]
+    chosen = torch.sort(-logits.detach(), dim=1, stable=True).indices[:, :K]
+    w = torch.softmax(logits.gather(1, chosen), 1) * mask[:, None]
+    every = torch.stack([(x @ p["up"][e]).relu() @ p["down"][e] for e in range(E)], 1)
+    y = (every.gather(1, chosen[..., None].expand(T, K, WIDTH)) * w[..., None]).sum(1)
+    u = x @ p["shared"].T
+    s = (u * 0.5 * torch.erfc(-u / math.sqrt(2))) @ p["back"].T + x
+    z = (s + y) @ p["head"].T + p["bias"]
+    out = z * torch.sigmoid(z)
+    n = mask.sum()
+    counts = torch.bincount(chosen[mask].flatten(), minlength=E).double()
+    loss = E * (counts / (n * K) * torch.softmax(logits, 1)[mask].mean(0)).sum()
+    grads = torch.autograd.grad([out, loss], list(p.values()), [dy, torch.full_like(loss, 30.0)])
+    norm = math.sqrt(sum(float(v.square().sum()) for v in grads))
+    return out, loss, norm, [v * min(1.0, 20.0 / norm) for v in grads]
+
+
+def test_step_against_64_bits(gpu):
+    x, mask, dy, p = _setup()
+    for v in p.values():
+        v.requires_grad_()
+    out, loss, norm, update, *grads = _step(x, mask, dy, p)
+    want, want_loss, want_norm, want_grads = _exact(x, mask, dy, p)
+    # a path has about ten roundings to fp16, each half a step (2^-11) of its tensor's norm at
+    # most, through maps that do not enlarge norms much: three times their sum
+    tol = 30 * 2.0 ** -11
+    off = lambda a, b: float((a.detach().double() - b.detach()).norm() / b.detach().norm())  # noqa: E731
+    assert off(out, want) <= tol
+    # logits in fp32 (64 terms)
+    assert abs(float(loss) - float(want_loss.detach())) <= 1e-5 * float(want_loss.detach())
+    assert want_norm > 20.0                                # the gradients are scaled
+    assert abs(float(norm) - want_norm) <= tol * want_norm
+    for name, got, exact in zip(p, grads, want_grads):
+        assert off(got, exact) <= tol, name
+    # singular values near 1, along the gradient
+    s = torch.linalg.svdvals(update.float())
+    assert float(s.max()) < 1.3 and float((update.float() * grads[5].float()).sum()) > 0
+
+
+def test_step_captured(gpu):
+    """One graph of the whole step, replayed on new inputs between eager steps."""
+    x, mask, dy, p = _setup()
+    for v in p.values():
+        v.requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            _step(x, mask, dy, p)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = _step(x, mask, dy, p)
+    for seed in range(1, 5):
+        nx, nmask, ndy, np_ = _setup(seed)
+        with torch.no_grad():
+            for old, new in zip((x, mask, dy, *p.values()), (nx, nmask, ndy, *np_.values())):
+                old.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in results]
+        eager = _step(x, mask, dy, p)
+        for a, b in zip(got, eager):
+            # (torch's own reductions and scatters run in both)
+            assert float((a.double() - b.double()).norm()) <= 1e-3 * float(b.double().norm()) + 1e-12
+        assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
