@@ -525,10 +525,11 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradParams p) {
 #pragma unroll
             for (int v = 0; v < V; ++v) at_experts[e0 + v] = 0.f;
             settle_wave();
-            for (int j = in; j < p.k; j += GL)
-                if (valid)
-                    at_experts[p.experts[s + j]] =
-                        p.normalize ? p.weights[s + j] * (p.dw[s + j] - mean) : p.dw[s + j];
+            for (int j = in; j < p.k; j += GL) {
+                const uint32_t e = valid ? (uint32_t)p.experts[s + j] : 0xFFFFFFFFu;
+                if (e < (uint32_t)p.E)   // whatever the tensor holds
+                    at_experts[e] = p.normalize ? p.weights[s + j] * (p.dw[s + j] - mean) : p.dw[s + j];
+            }
             settle_wave();
 #pragma unroll
             for (int v = 0; v < V; ++v) {

@@ -327,7 +327,8 @@ int ozk_linear(const void *x, int64_t x_stride, const void *W, const int64_t w_s
     if (!is_half(dtype)) return OZK_ERR_DTYPE;
     ozk::DenseParams p;
     if (int st = linear_params(p, x, x_stride, W, w_strides, M, N, K)) return st;
-    if (activation < OZK_ACT_NONE || activation > OZK_ACT_SILU || y_stride < 0 || r_stride < 0)
+    if (activation < OZK_ACT_NONE || activation > OZK_ACT_SILU || r_stride < 0 ||
+        (M > 1 && y_stride < N))
         return OZK_ERR_SHAPE;
     if (M == 0 || N == 0) return OZK_OK;
     if (!y || (K > 0 && (!x || !W))) return OZK_ERR_NULL;
@@ -366,7 +367,7 @@ int ozk_linear_backward(const void *dy, int64_t dy_stride, const void *z, const 
     if (int st = backward_plan(b, dy, dy_stride, x, x_stride, W, w_strides, activation, M, N, K,
                                want, workspace))
         return st;
-    if (dx_stride < 0 || dw_stride < 0) return OZK_ERR_SHAPE;
+    if ((dx && M > 1 && dx_stride < K) || (dW && N > 1 && dw_stride < K)) return OZK_ERR_SHAPE;
     const bool some = M > 0 && N > 0;
     if (some && (!dy || (activation != OZK_ACT_NONE && !z))) return OZK_ERR_NULL;
     if (some && K > 0 && (((want & 1) && !W) || ((want & 2) && !x))) return OZK_ERR_NULL;

@@ -61,8 +61,8 @@ class _Route(torch.autograd.Function):
         """The differentiable two; the others go into the list `rest`."""
         experts, weights, order, place, offsets, counts, loss = _route_forward(logits, mask, k, normalize)
         rest += (experts, order, place, offsets, counts)
-        ctx.save_for_backward(logits, mask, weights)
-        ctx.whole = experts, counts, normalize
+        ctx.save_for_backward(logits, mask, weights, experts, counts)
+        ctx.normalize = normalize
         ctx.set_materialize_grads(False)
         return weights, loss
 
@@ -77,15 +77,14 @@ class _Route(torch.autograd.Function):
     def gradients(ctx, dweights, dloss):
         if dweights is None and dloss is None:
             return None, None, None, None, None
-        logits, mask, weights = ctx.saved_tensors
-        experts, counts, normalize = ctx.whole
+        logits, mask, weights, experts, counts = ctx.saved_tensors
         T, k = experts.shape
         if dweights is not None:
             dweights = dweights.contiguous()
         dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _call("ozk_route_backward", logits.device, logits.data_ptr(), _TORCH_TO_OZK[logits.dtype],
               logits.stride(0), None if mask is None else mask.data_ptr(), T, counts.shape[0], k,
-              1 if normalize else 0, experts.data_ptr(), weights.data_ptr(), counts.data_ptr(),
+              1 if ctx.normalize else 0, experts.data_ptr(), weights.data_ptr(), counts.data_ptr(),
               None if dweights is None else dweights.data_ptr(),
               None if dloss is None else dloss.data_ptr(), dlogits.data_ptr())
         return dlogits, None, None, None, None
