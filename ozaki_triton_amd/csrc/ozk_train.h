@@ -45,6 +45,7 @@ struct DenseGradParams {
     int64_t M, N, dy_pitch, dz_pitch;
     int act;
     int64_t rows;            // of a workgroup
+    int lanes;               // set by the launch
 };
 int64_t dense_grad_rows(int64_t M, int64_t N);   // rows of a workgroup
 hipError_t launch_dense_grad(const DenseGradParams &p, int dtype, hipStream_t st);

@@ -434,6 +434,14 @@ _ACTIVATIONS = {None: _lib.OZK_ACT_NONE, "relu": _lib.OZK_ACT_RELU, "gelu": _lib
 
 
 def _linear_checks(x, W, bias, activation, residual):
+    xs, ws, dtype, dev = x.shape, W.shape, x.dtype, x.device
+    if (len(ws) == 2 and len(xs) and xs[-1] == ws[1] and dtype in _HALF and W.dtype == dtype
+            and activation in _ACTIVATIONS and dev.type == "cuda" and W.device == dev
+            and (bias is None or (bias.shape == ws[:1] and bias.dtype == dtype and bias.device == dev))
+            and (residual is None or (residual.shape == (*xs[:-1], ws[0]) and residual.dtype == dtype
+                                      and residual.device == dev))):
+        return
+    # one of these says what is wrong
     assert x.dim() >= 1 and W.dim() == 2 and x.shape[-1] == W.shape[1], \
         f"x must be [..., K] and W [N, K], got {tuple(x.shape)} and {tuple(W.shape)}"
     assert activation in _ACTIVATIONS, \
@@ -463,13 +471,20 @@ def _linear_forward(x, W, bias, residual, act, want_z):
     """y for x [M, K], and where wanted what act is applied to."""
     M, K = x.shape
     N, dtype, dev = W.shape[0], x.dtype, x.device
-    x, sx = _rows(x)
-    W, sw = _weight(W)
+    # (the usual layouts without a call: host time counts)
+    sx, one = x.stride()
+    if one != 1 or sx >= _MAX_STRIDE:
+        x, sx = _rows(x)
+    sw = W.stride()
+    if sw[1] != 1 or sw[0] >= _MAX_STRIDE:
+        W, sw = _weight(W)
     if bias is not None and bias.stride(0) != 1:
         bias = bias.contiguous()
     rp = sr = 0
     if residual is not None:
-        residual, sr = _rows(residual)
+        sr, one = residual.stride()
+        if one != 1 or sr >= _MAX_STRIDE:
+            residual, sr = _rows(residual)
         rp = residual.data_ptr()
     y = x.new_empty((M, N))
     z = x.new_empty((M, N)) if want_z else None
@@ -487,17 +502,23 @@ def _linear_backward(dy, z, x, W, act, want):
     """The gradients (dx, dW, db) that `want`, three truth values, asks for; x or W
     may be None where only the other's is wanted."""
     (M, N), dev, dtype = dy.shape, dy.device, dy.dtype
-    dy, sy = _rows(dy)
+    sy, one = dy.stride()
+    if one != 1 or sy >= _MAX_STRIDE or M == 1:
+        dy, sy = _rows(dy)
     xp = wp = dx = dW = db = None
     sw = (0, 1)
     mask = K = sx = 0
     if want[0]:
         K, mask = W.shape[1], 1
-        W, sw = _weight(W)
+        sw = W.stride()
+        if sw[1] != 1 or sw[0] >= _MAX_STRIDE:
+            W, sw = _weight(W)
         wp, dx = W.data_ptr(), dy.new_empty((M, K))
     if want[1]:
         K, mask = x.shape[1], mask | 2
-        x, sx = _rows(x)
+        sx, one = x.stride()
+        if one != 1 or sx >= _MAX_STRIDE:
+            x, sx = _rows(x)
         xp, dW = x.data_ptr(), dy.new_empty((N, K))
     if want[2]:
         mask |= 4
