@@ -592,12 +592,13 @@ template <typename T> hipError_t route_go(const RouteParams &p, hipStream_t st) 
     return with_shape(p.E, [&](auto gl, auto v) {
         constexpr int GL = decltype(gl)::value, V = decltype(v)::value;
         const size_t lds = RouteLds::bytes(p.E, p.per, p.k);
+        const int all = (int)lds + 512;   // and the kernel's own
         if (p.blocks == 1) {
-            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, true>>((int)lds); e != hipSuccess)
+            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, true>>(all); e != hipSuccess)
                 return e;
             route_rows_kernel<T, GL, V, true><<<1, 64 * kRouteWaves, lds, st>>>(p);
         } else {
-            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, false>>((int)lds); e != hipSuccess)
+            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, false>>(all); e != hipSuccess)
                 return e;
             route_rows_kernel<T, GL, V, false><<<(uint32_t)p.blocks, 64 * kRouteWaves, lds, st>>>(p);
         }
