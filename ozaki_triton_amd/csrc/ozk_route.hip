@@ -99,20 +99,24 @@ constexpr int kRouteWaves = 16;   // of a workgroup
 
 // LDS of a workgroup: its slots' experts, those of each wave, sums
 struct RouteLds {
+    uint32_t *parts;       // [64], for prefix sums and the like
+    uint32_t *last;        // where the groups end
     uint32_t *wave_hist;   // [waves][E + 1]
     float *psum;           // [waves][E]
     float *scale;          // [per]: what the weights are divided by
     float *value;          // [per k]: e to the chosen logits less the greatest
     uint16_t *expert;      // [per k]
     OZK_DEV RouteLds(char *at, int E, int64_t per, int k) {
-        wave_hist = (uint32_t *)at;
+        parts = (uint32_t *)at;
+        last = parts + 4 * kRouteWaves;
+        wave_hist = last + 4;
         psum = (float *)(wave_hist + kRouteWaves * (E + 1));
         scale = psum + kRouteWaves * E;
         value = scale + per;
         expert = (uint16_t *)(value + per * k);
     }
     static size_t bytes(int E, int64_t per, int k) {
-        return 4 * (size_t)(kRouteWaves * (2 * E + 1)) + 4 * (size_t)per + 6 * (size_t)(per * k);
+        return 4 * (size_t)(4 * kRouteWaves + 4 + kRouteWaves * (2 * E + 1)) + 4 * (size_t)per + 6 * (size_t)(per * k);
     }
 };
 
@@ -175,7 +179,7 @@ OZK_DEV void finish_counts(const RouteParams &p, uint32_t total, double P, uint3
 template <typename T, int GL, int V, bool ONE>
 __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteParams p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ __attribute__((aligned(16))) uint32_t parts[4 * kRouteWaves];
+    // (all of it dynamic: the limit that the launch raises counts that alone)
     const RouteLds lds(smem, p.E, p.per, p.k);
     constexpr int TPW = 64 / GL;   // tokens of a wave at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -312,15 +316,14 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteParam
         }
     }
     if constexpr (ONE) {
-        __shared__ uint32_t last;   // where the groups end
-        const uint32_t before = before_in_block((int)threadIdx.x < p.E ? total : 0u, parts);
-        if ((int)threadIdx.x == p.E - 1) last = before + total;
-        finish_counts(p, total, P, before, parts);
+        const uint32_t before = before_in_block((int)threadIdx.x < p.E ? total : 0u, lds.parts);
+        if ((int)threadIdx.x == p.E - 1) *lds.last = before + total;
+        finish_counts(p, total, P, before, lds.parts);
         __syncthreads();
         if ((int)threadIdx.x < p.E)
 #pragma unroll
             for (int w = 0; w < kRouteWaves; ++w) lds.wave_hist[w * (p.E + 1) + threadIdx.x] += before;
-        if (threadIdx.x < kRouteWaves) lds.wave_hist[threadIdx.x * (p.E + 1) + p.E] += last;
+        if (threadIdx.x < kRouteWaves) lds.wave_hist[threadIdx.x * (p.E + 1) + p.E] += *lds.last;
     }
     __syncthreads();
     // the slots' places: those of the same expert before the range, then before it in it
@@ -592,13 +595,12 @@ template <typename T> hipError_t route_go(const RouteParams &p, hipStream_t st) 
     return with_shape(p.E, [&](auto gl, auto v) {
         constexpr int GL = decltype(gl)::value, V = decltype(v)::value;
         const size_t lds = RouteLds::bytes(p.E, p.per, p.k);
-        const int all = (int)lds + 512;   // and the kernel's own
         if (p.blocks == 1) {
-            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, true>>(all); e != hipSuccess)
+            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, true>>((int)lds); e != hipSuccess)
                 return e;
             route_rows_kernel<T, GL, V, true><<<1, 64 * kRouteWaves, lds, st>>>(p);
         } else {
-            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, false>>(all); e != hipSuccess)
+            if (hipError_t e = allow_lds<&route_rows_kernel<T, GL, V, false>>((int)lds); e != hipSuccess)
                 return e;
             route_rows_kernel<T, GL, V, false><<<(uint32_t)p.blocks, 64 * kRouteWaves, lds, st>>>(p);
         }

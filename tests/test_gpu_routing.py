@@ -65,7 +65,7 @@ def _logits(T, E, dtype, seed=0):
 CASES = [(1, 1, 1), (1, 2, 2), (1, 64, 8), (3, 5, 5), (16, 16, 2), (63, 7, 3), (64, 8, 1), (65, 9, 2), (100, 33, 4),
          (1000, 64, 8), (1025, 40, 3), (4099, 40, 3), (2000, 128, 8), (777, 129, 5), (500, 256, 8), (300, 300, 7),
          (200, 512, 2), (130, 1000, 10), (90, 1024, 4), (50, 1024, 1024), (5000, 4, 4), (70000, 8, 2),
-         (10, 300, 280), (40, 300, 280)]   # the last: 64 KiB of LDS, with the kernel's own a little more
+         (10, 300, 280), (40, 300, 280), (1, 600, 2), (5, 1024, 3)]   # the last: about 64 KiB of LDS
 
 
 @pytest.mark.parametrize("T, E, k", CASES)
