@@ -207,6 +207,24 @@ def load() -> ctypes.CDLL:
     return L
 
 
+_binding = None
+
+
+def torch_binding():
+    """The Python module of the calls that need PyTorch's C++ side (csrc/ozk_torch.cpp)."""
+    global _binding
+    if _binding is None:
+        load()
+        try:
+            from . import _ozk_torch
+        except ImportError as e:
+            raise ImportError(
+                f"{os.path.join(HERE, '_ozk_torch.so')} is not built for this interpreter and torch ({e}); "
+                "run `python -c 'import __graft_entry__ as g; g.build()'`") from e
+        _binding = _ozk_torch
+    return _binding
+
+
 def strerror(status: int) -> str:
     return load().ozk_strerror(int(status)).decode()
 

@@ -1,4 +1,5 @@
-"""Build libozaki_amd.so (HIP kernels + C ABI) in-tree for gfx950.
+"""Build libozaki_amd.so (HIP kernels + C ABI) in-tree for gfx950, and the Python
+module on top of it for the calls that need PyTorch's C++ side.
 
 Every source under csrc/ is compiled with hipcc; the shared library lands next
 to this file so that it travels with the source tree.  Flags:
@@ -105,6 +106,35 @@ def _check_no_undefined_own_symbols(lib: str) -> None:
         os.remove(lib)
         raise RuntimeError("libozaki_amd.so leaves symbols of its own undefined:\n" +
                            ("\n".join(own) if own else res.stdout))
+
+
+TORCH_NAME = "_ozk_torch.so"
+
+
+def build_torch_binding(verbose: bool = False) -> str:
+    """Compile csrc/ozk_torch.cpp, the Python module of the operators that need
+    PyTorch's C++ side, against this interpreter's torch and the in-tree library
+    (rpath to it).  Host code only."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    out = os.path.join(HERE, TORCH_NAME)
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-DTORCH_API_INCLUDE_EXTENSION_H",
+           *[f for d in includes for f in ("-isystem", d)],
+           os.path.join(CSRC, "ozk_torch.cpp"), "-o", out + ".tmp", "-L", HERE, "-lozaki_amd", "-L", libs,
+           "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"ozk_torch build failed:\n{res.stdout}")
+    os.replace(out + ".tmp", out)
+    return out
 
 
 def build_c_example(verbose: bool = False) -> str:

@@ -1,0 +1,333 @@
+// ozk_torch.cpp -- the operators around linear layers as PyTorch calls: a Python
+// module (_ozk_torch) that allocates results and workspaces, keeps what a backward
+// pass needs and calls the C ABI (include/ozaki_amd.h).
+//
+// In C++ because these calls are short: an autograd node in Python costs its two
+// passes 50 us of host time more than one here, and a list of a hundred tensors is
+// looked at in a few us.  Arguments are checked by the Python functions; what the
+// calls here do not take as it is they refuse by returning None, before anything has
+// happened, and the Python functions find out why.
+//
+// A stream comes as its handle.  A backward pass runs on the stream of its forward
+// pass, as autograd has it.
+#include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include "../../include/ozaki_amd.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+constexpr int64_t kMaxStride = (int64_t)1 << 22;   // the kernels' limit on the distance of two rows
+
+void check(const char *name, int status) {
+    if (status != OZK_OK)
+        throw std::runtime_error(std::string(name) + " failed: " + ozk_strerror(status) + " (status " +
+                                 std::to_string(status) + ")");
+}
+int code(at::ScalarType t) {
+    return t == at::kFloat      ? OZK_F32
+           : t == at::kHalf     ? OZK_F16
+           : t == at::kBFloat16 ? OZK_BF16
+                                : -1;
+}
+void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor workspace(size_t bytes, const Tensor &like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+// The results of a backward pass that is itself recorded: a second derivative would
+// be lost without a word, so taking one is an error.
+void refuse_second(const char *name, variable_list &grads) {
+    if (!at::GradMode::is_enabled()) return;
+    variable_list some;
+    for (const Tensor &g : grads)
+        if (g.defined()) some.push_back(g.detach().requires_grad_());
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string("trying to differentiate ") + name + " twice: its backward pass has no derivative",
+        (int64_t)some.size());
+    some = (*error)(std::move(some));
+    size_t i = 0;
+    for (Tensor &g : grads)
+        if (g.defined()) g = some[i++];
+}
+
+// t [rows, columns] with its columns contiguous, and its rows' distance within the
+// kernels' limit (strides of dims of size 1 mean nothing)
+Tensor rows(const Tensor &t, int64_t &stride) {
+    const int64_t n = t.size(0), c = t.size(1), s0 = t.stride(0), s1 = t.stride(1);
+    stride = n <= 1 ? 0 : s0;
+    if ((s1 == 1 || c <= 1) && stride < kMaxStride) return t;
+    stride = c;
+    return t.contiguous();
+}
+// W [N, K] with K or N contiguous, and its strides, the contiguous one 1
+Tensor weight(const Tensor &W, int64_t (&s)[2]) {
+    const int64_t N = W.size(0), K = W.size(1), s_n = N > 1 ? W.stride(0) : 0, s_k = W.stride(1);
+    if ((s_k == 1 || K <= 1) && s_n < kMaxStride) {
+        s[0] = s_n;
+        s[1] = 1;
+        return W;
+    }
+    if ((s_n == 1 || N <= 1) && s_k < kMaxStride) {
+        s[0] = 1;
+        s[1] = s_k;
+        return W;
+    }
+    s[0] = K;
+    s[1] = 1;
+    return W.contiguous();
+}
+
+// ---- the dense product ----
+
+Tensor linear_forward(const Tensor &x_, const Tensor &W_, const std::optional<Tensor> &bias_,
+                      const std::optional<Tensor> &residual_, int64_t act, int64_t stream, Tensor *z) {
+    const int64_t M = x_.size(0), K = x_.size(1), N = W_.size(0);
+    int64_t sx, sr = 0, sw[2];
+    const Tensor x = rows(x_, sx), W = weight(W_, sw);
+    const Tensor bias = bias_ ? bias_->contiguous() : Tensor();
+    const Tensor residual = residual_ ? rows(*residual_, sr) : Tensor();
+    Tensor y = at::empty({M, N}, x.options());
+    if (z) *z = at::empty({M, N}, x.options());
+    size_t bytes = 0;
+    check("ozk_linear_workspace_bytes",
+          ozk_linear_workspace_bytes(ptr(x), sx, ptr(W), sw, M, N, K, &bytes));
+    const Tensor ws = workspace(bytes, x);
+    check("ozk_linear", ozk_linear(ptr(x), sx, ptr(W), sw, ptr(bias), ptr(residual), sr, (int)act, M, N, K,
+                                   code(x.scalar_type()), ptr(y), N, z ? ptr(*z) : nullptr, ptr(ws), bytes,
+                                   (void *)stream));
+    return y;
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &W,
+                          const std::optional<Tensor> &bias, const std::optional<Tensor> &residual,
+                          int64_t act, int64_t stream) {
+        const bool need_x = x.requires_grad(), need_W = W.requires_grad();
+        const bool need_z = act != OZK_ACT_NONE && (need_x || need_W || (bias && bias->requires_grad()));
+        Tensor z;
+        const Tensor y = linear_forward(x, W, bias, residual, act, stream, need_z ? &z : nullptr);
+        ctx->save_for_backward({need_W ? x : Tensor(), need_x ? W : Tensor(), z});
+        ctx->saved_data["a"] =
+            std::vector<int64_t>{act, stream, bias.has_value(), residual.has_value(), x.size(1)};
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const auto a = ctx->saved_data["a"].toIntVector();
+        const int64_t act = a[0], stream = a[1], K = a[4];
+        const bool has_b = a[2], has_r = a[3];
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list out(6);
+        const Tensor &g = grads[0];
+        if (!g.defined()) return out;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const bool need_x = ctx->needs_input_grad(0), need_W = ctx->needs_input_grad(1);
+            const bool need_b = has_b && ctx->needs_input_grad(2);
+            const int64_t M = g.size(0), N = g.size(1);
+            int64_t sy, sx = 0, sw[2] = {0, 1};
+            const Tensor dy = rows(g, sy), z = saved[2];
+            const Tensor x = need_W ? rows(saved[0], sx) : Tensor(), W = need_x ? weight(saved[1], sw) : Tensor();
+            if (need_x) out[0] = at::empty({M, K}, dy.options());
+            if (need_W) out[1] = at::empty({N, K}, dy.options());
+            if (need_b) out[2] = at::empty({N}, dy.options());
+            if (need_x || need_W || need_b) {
+                const int want = (need_x ? 1 : 0) | (need_W ? 2 : 0) | (need_b ? 4 : 0);
+                size_t bytes = 0;
+                check("ozk_linear_backward_workspace_bytes",
+                      ozk_linear_backward_workspace_bytes(ptr(dy), sy, ptr(x), sx, ptr(W), sw, (int)act, M,
+                                                          N, K, want, &bytes));
+                const Tensor ws = workspace(bytes, dy);
+                check("ozk_linear_backward",
+                      ozk_linear_backward(ptr(dy), sy, ptr(z), ptr(x), sx, ptr(W), sw, (int)act, M, N, K,
+                                          code(dy.scalar_type()), ptr(out[0]), K, ptr(out[1]), K,
+                                          ptr(out[2]), ptr(ws), bytes, (void *)stream));
+            }
+        }
+        if (has_r && ctx->needs_input_grad(has_b ? 3 : 2)) out[3] = g;
+        variable_list mine = {out[0], out[1], out[2]};
+        refuse_second("fused_linear", mine);
+        for (int i = 0; i < 3; ++i) out[i] = mine[i];
+        return out;
+    }
+};
+
+bool linear_ok(const Tensor &x, const Tensor &W, const std::optional<Tensor> &bias,
+               const std::optional<Tensor> &residual) {
+    if (x.dim() != 2 || W.dim() != 2 || !x.is_cuda() || x.size(1) != W.size(1)) return false;
+    const auto t = x.scalar_type();
+    if ((t != at::kHalf && t != at::kBFloat16) || W.scalar_type() != t || W.device() != x.device())
+        return false;
+    if (bias && (bias->dim() != 1 || bias->size(0) != W.size(0) || bias->scalar_type() != t ||
+                 bias->device() != x.device()))
+        return false;
+    return !residual || (residual->dim() == 2 && residual->size(0) == x.size(0) &&
+                         residual->size(1) == W.size(0) && residual->scalar_type() == t &&
+                         residual->device() == x.device());
+}
+std::optional<Tensor> linear(const Tensor &x, const Tensor &W, const std::optional<Tensor> &bias,
+                             const std::optional<Tensor> &residual, int64_t act, int64_t stream) {
+    if (!linear_ok(x, W, bias, residual)) return std::nullopt;
+    if (at::GradMode::is_enabled() && (x.requires_grad() || W.requires_grad() || (bias && bias->requires_grad()) ||
+                                       (residual && residual->requires_grad())))
+        return Linear::apply(x, W, bias, residual, act, stream);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return linear_forward(x, W, bias, residual, act, stream, nullptr);
+}
+
+// ---- the router ----
+
+// experts, weights, order, place, offsets, counts, loss
+variable_list route_forward(const Tensor &logits_, const std::optional<Tensor> &mask_, int64_t k,
+                            bool normalize, int64_t stream) {
+    const int64_t T = logits_.size(0), E = logits_.size(1), n = T * k;
+    const Tensor logits = logits_.stride(1) == 1 || E == 1 ? logits_ : logits_.contiguous();
+    const Tensor mask = mask_ ? mask_->contiguous() : Tensor();
+    const auto ints = logits.options().dtype(at::kInt), floats = logits.options().dtype(at::kFloat);
+    const Tensor all = at::empty({3 * n + 2 * E + 1}, ints);
+    const Tensor experts = all.as_strided({T, k}, {k, 1}, 0), order = all.as_strided({n}, {1}, n);
+    const Tensor place = all.as_strided({T, k}, {k, 1}, 2 * n);
+    const Tensor offsets = all.as_strided({E + 1}, {1}, 3 * n);
+    const Tensor counts = all.as_strided({E}, {1}, 3 * n + E + 1);
+    const Tensor weights = at::empty({T, k}, floats), loss = at::empty({}, floats);
+    size_t bytes = 0;
+    check("ozk_route_workspace_bytes", ozk_route_workspace_bytes(T, E, k, &bytes));
+    const Tensor ws = workspace(bytes, logits);
+    check("ozk_route",
+          ozk_route(ptr(logits), code(logits.scalar_type()), logits.stride(0), ptr(mask), T, E, k, normalize,
+                    (int32_t *)ptr(experts), (float *)ptr(weights), (int32_t *)ptr(order),
+                    (int32_t *)ptr(place), (int32_t *)ptr(offsets), (int32_t *)ptr(counts),
+                    (float *)ptr(loss), ptr(ws), bytes, (void *)stream));
+    return {experts, weights, order, place, offsets, counts, loss};
+}
+
+struct Route : torch::autograd::Function<Route> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &logits, const std::optional<Tensor> &mask,
+                                 int64_t k, bool normalize, int64_t stream) {
+        const variable_list r = route_forward(logits, mask, k, normalize, stream);
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({r[0], r[2], r[3], r[4], r[5]});
+        ctx->save_for_backward({logits, mask ? *mask : Tensor(), r[0], r[1], r[5]});
+        ctx->saved_data["a"] = std::vector<int64_t>{normalize, stream};
+        return r;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        variable_list out(5);
+        const Tensor &gw = grads[1], &gl = grads[6];
+        if (!gw.defined() && !gl.defined()) return out;
+        const auto a = ctx->saved_data["a"].toIntVector();
+        const variable_list saved = ctx->get_saved_variables();
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const Tensor logits = saved[0].stride(1) == 1 || saved[0].size(1) == 1 ? saved[0]
+                                                                                   : saved[0].contiguous();
+            const Tensor mask = saved[1].defined() ? saved[1].contiguous() : Tensor(), &experts = saved[2];
+            const Tensor dw = gw.defined() ? gw.contiguous() : Tensor();
+            out[0] = at::empty({logits.size(0), logits.size(1)}, logits.options());
+            check("ozk_route_backward",
+                  ozk_route_backward(ptr(logits), code(logits.scalar_type()), logits.stride(0),
+                                     ptr(mask), logits.size(0), logits.size(1), experts.size(1),
+                                     (int)a[0], (int32_t *)ptr(experts), (float *)ptr(saved[3]),
+                                     (int32_t *)ptr(saved[4]), (float *)ptr(dw), (float *)ptr(gl),
+                                     ptr(out[0]), (void *)a[1]));
+        }
+        variable_list mine = {out[0]};
+        refuse_second("route_tokens", mine);
+        out[0] = mine[0];
+        return out;
+    }
+};
+
+std::optional<variable_list> route(const Tensor &logits, const std::optional<Tensor> &mask, int64_t k,
+                                   bool normalize, int64_t stream) {
+    if (logits.dim() != 2 || !logits.is_cuda() || code(logits.scalar_type()) < 0) return std::nullopt;
+    const int64_t E = logits.size(1);
+    if (E < 1 || E > OZK_MAX_EXPERTS || k < 1 || k > E) return std::nullopt;
+    if (mask && (mask->dim() != 1 || mask->size(0) != logits.size(0) ||
+                 mask->scalar_type() != at::kBool || mask->device() != logits.device()))
+        return std::nullopt;
+    if (at::GradMode::is_enabled() && logits.requires_grad())
+        return Route::apply(logits, mask, k, normalize, stream);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return route_forward(logits, mask, k, normalize, stream);
+}
+
+// ---- gradient norms ----
+
+struct Table {
+    std::vector<const void *> ins;
+    std::vector<void *> outs;
+    std::vector<int64_t> counts;
+    std::vector<int> codes;
+};
+// false: not all on one GPU, contiguous, of a type with a kernel, without a gradient
+bool table_of(const std::vector<Tensor> &in, const std::vector<Tensor> *out, Table &t) {
+    const size_t n = in.size();
+    if (!n || !in[0].is_cuda() || (out && out->size() != n)) return false;
+    const bool grad = at::GradMode::is_enabled();
+    t.ins.resize(n);
+    t.outs.resize(out ? n : 0);
+    t.counts.resize(n);
+    t.codes.resize(n);
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor &g = in[i];
+        t.codes[i] = code(g.scalar_type());
+        if (t.codes[i] < 0 || g.device() != in[0].device() || !g.is_contiguous() ||
+            (grad && g.requires_grad()))
+            return false;
+        t.ins[i] = g.data_ptr();
+        t.counts[i] = g.numel();
+        if (!out) continue;
+        const Tensor &o = (*out)[i];
+        if (o.scalar_type() != g.scalar_type() || o.device() != g.device() || !o.is_contiguous() ||
+            o.sizes() != g.sizes() || (grad && o.requires_grad()))
+            return false;
+        t.outs[i] = o.data_ptr();
+    }
+    return true;
+}
+Tensor norm_workspace(int64_t n, const Tensor &like, size_t &bytes) {
+    check("ozk_gradient_norm_workspace_bytes", ozk_gradient_norm_workspace_bytes(n, &bytes));
+    return workspace(bytes, like);
+}
+std::optional<Tensor> gradient_norm(const std::vector<Tensor> &grads, int64_t stream) {
+    Table t;
+    if (!table_of(grads, nullptr, t)) return std::nullopt;
+    const int64_t n = (int64_t)grads.size();
+    Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+    size_t bytes;
+    const Tensor ws = norm_workspace(n, norm, bytes);
+    check("ozk_gradient_norm", ozk_gradient_norm(t.ins.data(), t.counts.data(), t.codes.data(), n,
+                                                 norm.data_ptr<float>(), ptr(ws), bytes, (void *)stream));
+    return norm;
+}
+// nothing also where tensors share memory, which the Python function then says
+std::optional<Tensor> clip_gradients(const std::vector<Tensor> &grads, const std::vector<Tensor> &outs,
+                                     double max_norm, int64_t stream) {
+    Table t;
+    if (!(max_norm >= 0) || !table_of(grads, &outs, t)) return std::nullopt;
+    const int64_t n = (int64_t)grads.size();
+    Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+    size_t bytes;
+    const Tensor ws = norm_workspace(n, norm, bytes);
+    const int st = ozk_clip_gradients(t.ins.data(), t.outs.data(), t.counts.data(), t.codes.data(), n,
+                                      max_norm, norm.data_ptr<float>(), ptr(ws), bytes, (void *)stream);
+    if (st == OZK_ERR_SHAPE) return std::nullopt;
+    check("ozk_clip_gradients", st);
+    // written behind autograd's back
+    for (const Tensor &o : outs)
+        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+    return norm;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_ozk_torch, m) {
+    m.def("linear", &linear);
+    m.def("route", &route);
+    m.def("gradient_norm", &gradient_norm);
+    m.def("clip_gradients", &clip_gradients);
+}

@@ -12,9 +12,10 @@ from __future__ import annotations
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .linear import _FLOAT, _bytes, _call, _no_tangent, _on_one_gpu, _require_dtype, _workspace
+from .linear import _FLOAT, _bound, _bytes, _call, _no_tangent, _on_one_gpu, _require_dtype, _workspace
 from .ozaki import _TORCH_TO_OZK
 
 _CODES = {d: _TORCH_TO_OZK[d] for d in _FLOAT}
@@ -33,8 +34,7 @@ def _is_dense(t: torch.Tensor) -> bool:
 
 
 def _checked(name, tensors):
-    """The tensors as a list, and the types' codes.  (Host time counts: a model has
-    hundreds of gradients.)"""
+    """The tensors as a list, and the types' codes."""
     tensors = list(tensors)
     assert tensors, f"{name} needs at least one tensor"
     dev = tensors[0].get_device()
@@ -66,6 +66,11 @@ def gradient_norm(grads) -> torch.Tensor:
 
     grads: tensors of any shapes, float32 / float16 / bfloat16 in any mix, on one GPU
     """
+    grads = list(grads)
+    if grads and grads[0].is_cuda and forward_ad._current_level < 0:
+        norm = _bound("gradient_norm", grads[0].device, grads)
+        if norm is not None:
+            return norm
     grads, codes = _checked("gradient_norm", grads)
     grads = [t if t.is_contiguous() or _is_dense(t) else t.contiguous() for t in grads]
     dev, n = grads[0].device, len(grads)
@@ -89,6 +94,14 @@ def clip_gradients(grads, max_norm: float, *, out=None) -> torch.Tensor:
              the gradients themselves, in place
     A norm of infinity makes everything finite 0, one of NaN everything NaN.
     """
+    grads = list(grads)
+    out = None if out is None else list(out)
+    if grads and grads[0].is_cuda and forward_ad._current_level < 0:
+        norm = _bound("clip_gradients", grads[0].device, grads, grads if out is None else out,
+                      float(max_norm))
+        if norm is not None:
+            return norm
+    # what the call does not take as it is: layouts other than contiguous, and mistakes
     grads, codes = _checked("clip_gradients", grads)
     assert max_norm >= 0, f"max_norm must be >= 0, got {max_norm}"
     ins, to, back = grads, grads, ()

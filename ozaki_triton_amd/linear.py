@@ -81,6 +81,19 @@ def _call(name: str, dev: torch.device, *args) -> None:
         _lib.check(name, st)
 
 
+def _bound(name: str, dev: torch.device, *args):
+    """Call `name` of the module on PyTorch's C++ side on dev's current stream, its
+    last argument; None: it does not take these arguments as they are."""
+    fn = _FUNCTIONS.get("bound " + name)
+    if fn is None:
+        fn = _FUNCTIONS["bound " + name] = getattr(_lib.torch_binding(), name)
+    idx = dev.index
+    if _RAW_STREAM is not None and idx == _current_device():
+        return fn(*args, _RAW_STREAM(idx))
+    with torch.cuda.device(dev):
+        return fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+
+
 @functools.lru_cache(maxsize=1024)
 def _i64(*vals):
     return _lib.i64arr(vals)
@@ -434,14 +447,6 @@ _ACTIVATIONS = {None: _lib.OZK_ACT_NONE, "relu": _lib.OZK_ACT_RELU, "gelu": _lib
 
 
 def _linear_checks(x, W, bias, activation, residual):
-    xs, ws, dtype, dev = x.shape, W.shape, x.dtype, x.device
-    if (len(ws) == 2 and len(xs) and xs[-1] == ws[1] and dtype in _HALF and W.dtype == dtype
-            and activation in _ACTIVATIONS and dev.type == "cuda" and W.device == dev
-            and (bias is None or (bias.shape == ws[:1] and bias.dtype == dtype and bias.device == dev))
-            and (residual is None or (residual.shape == (*xs[:-1], ws[0]) and residual.dtype == dtype
-                                      and residual.device == dev))):
-        return
-    # one of these says what is wrong
     assert x.dim() >= 1 and W.dim() == 2 and x.shape[-1] == W.shape[1], \
         f"x must be [..., K] and W [N, K], got {tuple(x.shape)} and {tuple(W.shape)}"
     assert activation in _ACTIVATIONS, \
@@ -455,115 +460,6 @@ def _linear_checks(x, W, bias, activation, residual):
         f"residual must be {want} {dtype}, got {tuple(residual.shape)} {residual.dtype}"
     _on_one_gpu(x, W, bias, residual)
     _require_dtype("fused_linear", dtype, _HALF)
-
-
-def _weight(W):
-    """W [N, K] with K or N contiguous, and its strides, the contiguous one 1."""
-    (N, K), (s_n, s_k) = W.shape, W.stride()
-    if (s_k == 1 or K <= 1) and (s_n < _MAX_STRIDE or N <= 1):
-        return W, (s_n if N > 1 else 0, 1)
-    if (s_n == 1 or N <= 1) and s_k < _MAX_STRIDE:
-        return W, (1, s_k)
-    return W.contiguous(), (K, 1)
-
-
-def _linear_forward(x, W, bias, residual, act, want_z):
-    """y for x [M, K], and where wanted what act is applied to."""
-    M, K = x.shape
-    N, dtype, dev = W.shape[0], x.dtype, x.device
-    # (the usual layouts without a call: host time counts)
-    sx, one = x.stride()
-    if one != 1 or sx >= _MAX_STRIDE:
-        x, sx = _rows(x)
-    sw = W.stride()
-    if sw[1] != 1 or sw[0] >= _MAX_STRIDE:
-        W, sw = _weight(W)
-    if bias is not None and bias.stride(0) != 1:
-        bias = bias.contiguous()
-    rp = sr = 0
-    if residual is not None:
-        sr, one = residual.stride()
-        if one != 1 or sr >= _MAX_STRIDE:
-            residual, sr = _rows(residual)
-        rp = residual.data_ptr()
-    y = x.new_empty((M, N))
-    z = x.new_empty((M, N)) if want_z else None
-    xp, wp = x.data_ptr(), W.data_ptr()
-    n = _bytes("ozk_linear_workspace_bytes", xp & 15, sx, wp & 15, sw, M, N, K)
-    ws, wsp = _workspace(n, dev)
-    _call("ozk_linear", dev, xp, sx, wp, _i64(*sw), None if bias is None else bias.data_ptr(),
-          rp or None, sr, act, M, N, K, _TORCH_TO_OZK[dtype], y.data_ptr(), N,
-          z.data_ptr() if want_z else None, wsp, n)
-    del ws
-    return y, z
-
-
-def _linear_backward(dy, z, x, W, act, want):
-    """The gradients (dx, dW, db) that `want`, three truth values, asks for; x or W
-    may be None where only the other's is wanted."""
-    (M, N), dev, dtype = dy.shape, dy.device, dy.dtype
-    sy, one = dy.stride()
-    if one != 1 or sy >= _MAX_STRIDE or M == 1:
-        dy, sy = _rows(dy)
-    xp = wp = dx = dW = db = None
-    sw = (0, 1)
-    mask = K = sx = 0
-    if want[0]:
-        K, mask = W.shape[1], 1
-        sw = W.stride()
-        if sw[1] != 1 or sw[0] >= _MAX_STRIDE:
-            W, sw = _weight(W)
-        wp, dx = W.data_ptr(), dy.new_empty((M, K))
-    if want[1]:
-        K, mask = x.shape[1], mask | 2
-        sx, one = x.stride()
-        if one != 1 or sx >= _MAX_STRIDE:
-            x, sx = _rows(x)
-        xp, dW = x.data_ptr(), dy.new_empty((N, K))
-    if want[2]:
-        mask |= 4
-        db = dy.new_empty((N,))
-    dp = dy.data_ptr()
-    n = _bytes("ozk_linear_backward_workspace_bytes", dp & 15, sy, (xp or 0) & 15, sx, (wp or 0) & 15,
-               sw, act, M, N, K, mask)
-    ws, wsp = _workspace(n, dev)
-    _call("ozk_linear_backward", dev, dp, sy, None if z is None else z.data_ptr(), xp, sx, wp,
-          _i64(*sw), act, M, N, K, _TORCH_TO_OZK[dtype], None if dx is None else dx.data_ptr(), K,
-          None if dW is None else dW.data_ptr(), K, None if db is None else db.data_ptr(), wsp, n)
-    del ws
-    return dx, dW, db
-
-
-class _FusedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, W, bias, residual, act):
-        need = ctx.needs_input_grad
-        y, z = _linear_forward(x, W, bias, residual, act,
-                               act != 0 and (need[0] or need[1] or need[2]))
-        ctx.save_for_backward(x if need[1] else None, W if need[0] else None, z)
-        ctx.act = act
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        # (the wrapper that refuses a second derivative costs 4 us: only where one is asked for)
-        if torch.is_grad_enabled():
-            return _FusedLinear.backward_once(ctx, dy)
-        return _FusedLinear.gradients(ctx, dy)
-
-    @staticmethod
-    def gradients(ctx, dy):
-        x, W, z = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = dW = db = None
-        if need[0] or need[1] or need[2]:
-            dx, dW, db = _linear_backward(dy, z, x, W, ctx.act, need)
-        return dx, dW, db, dy if need[3] else None, None
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward_once(ctx, dy):
-        return _FusedLinear.gradients(ctx, dy)
 
 
 def fused_linear(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -583,18 +479,14 @@ def fused_linear(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor | None = N
         pass keeps x W^T + bias in x's dtype where there is an activation, and the
         gradient to it is rounded to that dtype.
     """
-    _linear_checks(x, W, bias, activation, residual)
     _no_tangent("fused_linear", x, W, bias, residual)
-    act = _ACTIVATIONS[activation]
-    shape = x.shape
-    if len(shape) != 2:
-        M = math.prod(shape[:-1])
-        x = x.reshape(M, shape[-1])
-        residual = None if residual is None else residual.reshape(M, W.shape[0])
-    if torch.is_grad_enabled() and (
-            x.requires_grad or W.requires_grad or (bias is not None and bias.requires_grad)
-            or (residual is not None and residual.requires_grad)):
-        y = _FusedLinear.apply(x, W, bias, residual, act)
-    else:
-        y, _ = _linear_forward(x, W, bias, residual, act, False)
-    return y if len(shape) == 2 else y.view(*shape[:-1], W.shape[0])
+    act = _ACTIVATIONS.get(activation, -1)
+    if act >= 0 and x.dim() == 2 and x.is_cuda:
+        y = _bound("linear", x.device, x, W, bias, residual, act)
+        if y is not None:
+            return y
+    _linear_checks(x, W, bias, activation, residual)
+    shape, N = x.shape[:-1], W.shape[0]
+    M = math.prod(shape)
+    residual = None if residual is None else residual.reshape(M, N)
+    return _bound("linear", x.device, x.reshape(M, W.shape[1]), W, bias, residual, act).view(*shape, N)

@@ -15,8 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .linear import _FLOAT, _bytes, _call, _no_tangent, _on_one_gpu, _require_dtype, _workspace
-from .ozaki import _TORCH_TO_OZK
+from .linear import _FLOAT, _bound, _no_tangent, _on_one_gpu, _require_dtype
 
 
 class Routing(NamedTuple):
@@ -37,64 +36,6 @@ class Routing(NamedTuple):
     balance_loss: torch.Tensor   # () float32
 
 
-def _route_forward(logits, mask, k, normalize):
-    T, E = logits.shape
-    dev, n = logits.device, T * k
-    ints = torch.empty(3 * n + 2 * E + 1, dtype=torch.int32, device=dev)
-    experts, order, place, offsets, counts = ints.split_with_sizes((n, n, n, E + 1, E))
-    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    at = ints.data_ptr()
-    size = _bytes("ozk_route_workspace_bytes", T, E, k)
-    ws, wsp = _workspace(size, dev)
-    _call("ozk_route", dev, logits.data_ptr(), _TORCH_TO_OZK[logits.dtype], logits.stride(0),
-          None if mask is None else mask.data_ptr(), T, E, k, 1 if normalize else 0, at,
-          weights.data_ptr(), at + 4 * n, at + 8 * n, at + 12 * n, at + 12 * n + 4 * (E + 1),
-          loss.data_ptr(), wsp, size)
-    del ws
-    return experts.view(T, k), weights, order, place.view(T, k), offsets, counts, loss
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, mask, k, normalize, rest):
-        """The differentiable two; the others go into the list `rest`."""
-        experts, weights, order, place, offsets, counts, loss = _route_forward(logits, mask, k, normalize)
-        rest += (experts, order, place, offsets, counts)
-        ctx.save_for_backward(logits, mask, weights, experts, counts)
-        ctx.normalize = normalize
-        ctx.set_materialize_grads(False)
-        return weights, loss
-
-    @staticmethod
-    def backward(ctx, dweights, dloss):
-        # (the wrapper that refuses a second derivative costs 4 us: only where one is asked for)
-        if torch.is_grad_enabled():
-            return _Route.backward_once(ctx, dweights, dloss)
-        return _Route.gradients(ctx, dweights, dloss)
-
-    @staticmethod
-    def gradients(ctx, dweights, dloss):
-        if dweights is None and dloss is None:
-            return None, None, None, None, None
-        logits, mask, weights, experts, counts = ctx.saved_tensors
-        T, k = experts.shape
-        if dweights is not None:
-            dweights = dweights.contiguous()
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _call("ozk_route_backward", logits.device, logits.data_ptr(), _TORCH_TO_OZK[logits.dtype],
-              logits.stride(0), None if mask is None else mask.data_ptr(), T, counts.shape[0], k,
-              1 if ctx.normalize else 0, experts.data_ptr(), weights.data_ptr(), counts.data_ptr(),
-              None if dweights is None else dweights.data_ptr(),
-              None if dloss is None else dloss.data_ptr(), dlogits.data_ptr())
-        return dlogits, None, None, None, None
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward_once(ctx, dweights, dloss):
-        return _Route.gradients(ctx, dweights, dloss)
-
-
 def route_tokens(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = None,
                  normalize: bool = True) -> Routing:
     """Each token's k experts, their weights, and the slots' order for grouped_matmul.
@@ -112,6 +53,12 @@ def route_tokens(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = No
         that are not left out (0 if there is none).  weights and balance_loss are
         differentiable in logits (reverse mode, once; f as a constant).
     """
+    _no_tangent("route_tokens", logits)
+    if logits.is_cuda:
+        out = _bound("route", logits.device, logits, mask, k, normalize)
+        if out is not None:
+            return Routing(*out)
+    # one of these says what is wrong
     assert logits.dim() == 2, f"logits must be [tokens, experts], got {tuple(logits.shape)}"
     T, E = logits.shape
     assert 1 <= E <= _lib.OZK_MAX_EXPERTS, f"experts must be 1 .. {_lib.OZK_MAX_EXPERTS}, got {E}"
@@ -120,14 +67,4 @@ def route_tokens(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = No
         f"mask must be {(T,)} bool, got {tuple(mask.shape)} {mask.dtype}"
     _on_one_gpu(logits, mask)
     _require_dtype("route_tokens", logits.dtype, _FLOAT)
-    _no_tangent("route_tokens", logits)
-    if logits.stride(1) != 1 and E != 1:
-        logits = logits.contiguous()
-    if mask is not None and mask.stride(0) != 1:
-        mask = mask.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        rest: list = []
-        weights, loss = _Route.apply(logits, mask, k, normalize, rest)
-        experts, order, place, offsets, counts = rest
-        return Routing(experts, weights, order, place, offsets, counts, loss)
-    return Routing(*_route_forward(logits, mask, k, normalize))
+    raise AssertionError("route_tokens: arguments not taken")
