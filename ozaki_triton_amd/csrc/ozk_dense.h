@@ -85,6 +85,7 @@ template <typename F> OZK_DEV void with_act(int act, F &&f) {
 // 8 consecutive 16-bit values of a row, of which `n` exist
 // ---------------------------------------------------------------------------
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef int i32x4_words __attribute__((ext_vector_type(4), aligned(4)));
 OZK_DEV i32x4 load8(const char *p, int n) {
     i32x4 v = {0, 0, 0, 0};
     if (n >= 8) {
@@ -346,8 +347,12 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseParams p) {
 // then reads P 64-byte pieces of R rows one behind another, which DRAM serves
 // faster than pieces of 16 rows, and few rows of W still fill the chip.  The waves'
 // sums and the parts are added in order in the LDS.
+// Loads off a 4-byte address take two to three times as long, so rows of odd
+// addresses (WORDS false) are read as the words that hold them and shifted (1 x 4096
+// x 4097: 16.0 -> 11.7 us, 16 rows 27 -> 16).  More than 16 rows, which such operands may have: so many
+// workgroups beside each other.
 // ---------------------------------------------------------------------------
-template <typename ST, int P, int WAVES, int U>
+template <typename ST, int P, int WAVES, int U, bool WORDS>
 __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(DenseParams p) {
     constexpr int R = 16 / P;
     __shared__ __attribute__((aligned(16))) float join[WAVES][16][20];   // [x's index][W's index]
@@ -355,7 +360,7 @@ __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(DenseParams p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t n0 = (int64_t)blockIdx.x * R;
     // rows past the last read the last one, and are not stored
-    const int64_t n = n0 + i16 % R, m = i16 % R;
+    const int64_t m0 = (int64_t)blockIdx.y * 16, n = n0 + i16 % R, m = m0 + i16 % R;
     const int in = (i16 / R) * 128 + g * 16;   // the lane's first piece in a step of P 128 bytes
     const char *W = p.B + (n < p.N ? n : p.N - 1) * p.b_pitch + in;
     const char *X = p.A + (m < p.M ? m : p.M - 1) * p.a_pitch + in;
@@ -364,9 +369,19 @@ __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(DenseParams p) {
     constexpr int STEP = P * 128;
     auto piece = [&](const char *row, const char *first, int64_t at, bool whole) -> i32x4 {
         i32x4 v;
-        if (whole) {
+        if (whole && WORDS) {
             __builtin_memcpy(&v, row + at, 16);
             return v;
+        }
+        if (whole) {
+            const uintptr_t p = (uintptr_t)(row + at);
+            const uint32_t *w = (const uint32_t *)(p & ~(uintptr_t)3);
+            const uint32_t by = (uint32_t)(p & 2) * 8, e = w[4];
+            i32x4_words u = *(const i32x4_words *)w;
+            return i32x4{(int)__builtin_amdgcn_alignbit((uint32_t)u.y, (uint32_t)u.x, by),
+                         (int)__builtin_amdgcn_alignbit((uint32_t)u.z, (uint32_t)u.y, by),
+                         (int)__builtin_amdgcn_alignbit((uint32_t)u.w, (uint32_t)u.z, by),
+                         (int)__builtin_amdgcn_alignbit(e, (uint32_t)u.w, by)};
         }
         const int64_t left = bytes - at - in;
         return load_piece(row + (left > 0 ? at : 0), left < 16 ? (int)(left < 0 ? 0 : left) : 16, first);
@@ -392,9 +407,11 @@ __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(DenseParams p) {
     const int64_t per = ((bytes + STEP - 1) / STEP + WAVES - 1) / WAVES * STEP;
     int64_t at = per * wave;
     const int64_t end = at + per < bytes ? at + per : bytes;
-    for (; at + U * STEP <= end; at += U * STEP) steps(at, integral_constant<int, U>{}, std::true_type{});
-    for (; at + STEP <= end; at += STEP) steps(at, integral_constant<int, 1>{}, std::true_type{});
-    if (at < end) steps(at, integral_constant<int, 1>{}, std::false_type{});
+    // (the word behind a shifted piece has to exist)
+    const int64_t whole = WORDS || end + 4 <= bytes ? end : bytes - 4;
+    for (; at + U * STEP <= whole; at += U * STEP) steps(at, integral_constant<int, U>{}, std::true_type{});
+    for (; at + STEP <= whole; at += STEP) steps(at, integral_constant<int, 1>{}, std::true_type{});
+    for (; at < end; at += STEP) steps(at, integral_constant<int, 1>{}, std::false_type{});
 
     *(f32x4 *)&join[wave][i16][4 * g] = acc;
     __syncthreads();
@@ -411,10 +428,10 @@ __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(DenseParams p) {
                 for (int e = 0; e < C; ++e) v[e] += join[w][q * R + row][q * R + c0 + e];
         const int64_t col = n0 + c0;
         const int left = p.N - col < C ? (int)(p.N - col) : C;
-        if (row < p.M && left > 0) {
+        if (m0 + row < p.M && left > 0) {
             float bias[8];
             bias_at<ST>(p, col, left, bias);
-            finish8<ST>(p, v, bias, res_at<ST>(p, row, col, left), row, col, left);
+            finish8<ST>(p, v, bias, res_at<ST>(p, m0 + row, col, left), m0 + row, col, left);
         }
     }
 }
@@ -517,7 +534,11 @@ hipError_t dense_go(const DenseParams &p, hipStream_t st) {
 template <typename ST, int P, int WAVES, int U> hipError_t few_go(const DenseParams &p, hipStream_t st) {
     const int64_t blocks = (p.N + 16 / P - 1) / (16 / P);
     if (blocks >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
-    dense_few_kernel<ST, P, WAVES, U><<<dim3((uint32_t)blocks), 64 * WAVES, 0, st>>>(p);
+    const dim3 grid((uint32_t)blocks, (uint32_t)((p.M + 15) / 16));
+    if ((((uintptr_t)p.A | (uintptr_t)p.B | (uintptr_t)p.a_pitch | (uintptr_t)p.b_pitch) & 3) == 0)
+        dense_few_kernel<ST, P, WAVES, U, true><<<grid, 64 * WAVES, 0, st>>>(p);
+    else
+        dense_few_kernel<ST, P, WAVES, U, false><<<grid, 64 * WAVES, 0, st>>>(p);
     return hipGetLastError();
 }
 // Parts of K: as few as give three quarters of the CUs a workgroup.  Measured (us,
@@ -609,10 +630,10 @@ template <typename ST> hipError_t dense_plan(const DenseParams &p, hipStream_t s
 
 }  // namespace
 
-// Up to 4 rows, and up to 16 that the tiles' DMA cannot take (us, 4 x 4096 x 4096:
-// 9.7, tiles of 32 x 16 9.4; 16 x 4096 x 4096: 11.5 and 9.6)
+// Up to 4 rows, and up to 32 that the tiles' DMA cannot take (us, this / tiles: 4 x
+// 4096 x 4096 9.7 / 9.4, 16 x 4096 x 4096 11.5 / 9.6, 32 x 4096 x 4097 25 / 52)
 bool dense_few(const DenseParams &p) {
-    return !p.a_cols && !p.b_cols && (p.M <= 4 || (p.M <= 16 && !pieces(p)));
+    return !p.a_cols && !p.b_cols && (p.M <= 4 || (p.M <= 32 && !pieces(p)));
 }
 int dense_splits(const DenseParams &p) {
     return dense_few(p) || p.M == 0 || p.N == 0 ? 1 : plan_tiles(p).splits;

@@ -69,7 +69,7 @@ SHAPES = [
     (1, 4096, 4096), (1, 1, 1), (1, 17, 100), (3, 1000, 2047), (16, 64, 512), (17, 250, 129), (31, 96, 8),
     (33, 512, 1000), (64, 40, 4100), (65, 128, 256), (100, 1, 72), (128, 256, 4096), (200, 72, 2056),
     (257, 300, 64), (500, 1030, 200), (1999, 520, 1000), (1024, 2048, 1024), (4096, 4100, 136),
-    (700, 333, 1001), (90, 90, 4097), (2300, 8, 3000), (70, 2000, 7)]
+    (700, 333, 1001), (90, 90, 4097), (2, 60, 4097), (20, 48, 1025), (9, 50, 2049), (32, 33, 4159), (2300, 8, 3000), (70, 2000, 7)]
 
 
 @pytest.mark.parametrize("M, N, K", SHAPES)
