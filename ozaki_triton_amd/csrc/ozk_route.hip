@@ -488,9 +488,11 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradParams p) {
         }
         sum = over_group<GL>(sum, [](uint32_t a, uint32_t b) { return a + b; });
         const double n = (double)sum / p.k;
+        // less their mean, which changes nothing in g - sum q g: balanced counts would
+        // cancel there in 32 bits
         const double by = sum ? (double)*p.dloss * p.E / ((double)sum * n) : 0.0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) g0[v] = (float)(by * (double)c[v]);
+        for (int v = 0; v < V; ++v) g0[v] = (float)(by * ((double)c[v] - (double)sum / p.E));
     }
     const int64_t step = (int64_t)gridDim.x * 4 * TPW;
     for (int64_t r = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * TPW; r < p.T; r += step) {
