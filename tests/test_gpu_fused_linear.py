@@ -373,3 +373,45 @@ def test_refusals_on_the_gpu(gpu):
     g, = torch.autograd.grad(ozk.fused_linear(t, W.to(BF)).sum(), t, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_gradients_without_a_bias(gpu):
+    x, W, b, res, dy = _inputs(120, 96, 72, BF)
+    for need in ((1, 1, 1), (0, 0, 1), (1, 0, 0), (0, 1, 1)):
+        for act in (None, "gelu_tanh"):
+            ts = [t.clone().requires_grad_(bool(n)) for t, n in zip((x, W, res), need)]
+            ozk.fused_linear(ts[0], ts[1], activation=act, residual=ts[2]).backward(dy)
+            zero = torch.zeros_like(b).requires_grad_()
+            us = [t.clone().requires_grad_() for t in (x, W, res)]
+            want = torch.autograd.grad(ozk.fused_linear(us[0], us[1], zero, activation=act, residual=us[2]), us, dy)
+            for t, n, w in zip(ts, need, want):
+                assert (t.grad is None) == (not n) and (not n or torch.equal(t.grad, w))
+
+
+def test_backward_twice_and_recorded(gpu):
+    """A kept graph gives the same gradients again; a recorded backward pass has their values and
+    refuses a second derivative, in a sum with something that has one too."""
+    x, W, b, _, dy = _inputs(120, 96, 72, BF)
+    leaves = [t.requires_grad_() for t in (x, W, b)]
+    y = ozk.fused_linear(x, W, b, activation="silu")
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    recorded = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    for a, c, d in zip(first, again, recorded):
+        assert torch.equal(a, c) and torch.equal(a, d.detach())
+    with pytest.raises(RuntimeError, match="twice"):
+        (recorded[0].float().square().sum() + x.float().sum()).backward()
+    # a saved operand that has changed meanwhile is noticed
+    y = ozk.fused_linear(x, W, b, activation="silu")
+    with torch.no_grad():
+        W.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward(dy)
+
+
+def test_inference_mode(gpu):
+    x, W, b, res, _ = _inputs(70, 96, 72, BF)
+    want = ozk.fused_linear(x, W, b, activation="gelu", residual=res)
+    with torch.inference_mode():
+        y = ozk.fused_linear(x, W.requires_grad_(), b, activation="gelu", residual=res)
+    assert torch.equal(y, want) and not y.requires_grad

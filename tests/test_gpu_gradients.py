@@ -198,3 +198,17 @@ def test_past_32_bits(gpu):
     assert float(ozk.gradient_norm([t])) == 13.0
     ozk.clip_gradients([t], 6.5)
     assert [float(t[i]) for i in (n - 1, 0, n // 2)] == [1.5, 2.0, 6.0]
+
+
+def test_parameters_gradients_in_place(gpu):
+    """As a training loop calls it: the .grad of parameters, the parameters' own flags unchanged."""
+    ps = [torch.randn(40, 30, device="cuda").to(BF).requires_grad_(), torch.randn(30, device="cuda", requires_grad=True)]
+    sum(p.float().square().sum() for p in ps).backward()
+    before = [p.grad.clone() for p in ps]
+    norm = ozk.clip_gradients((p.grad for p in ps), 1.0)      # any iterable
+    _check(before, [p.grad for p in ps], 1.0, norm)
+    assert all(p.requires_grad and not p.grad.requires_grad for p in ps)
+    with torch.inference_mode():
+        t = [torch.ones(10, device="cuda")]
+        ozk.clip_gradients(t, 1.0)
+    assert abs(float(t[0].norm()) - 1) < 1e-6

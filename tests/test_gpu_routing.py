@@ -309,3 +309,23 @@ def test_layer_of_experts(gpu):
     assert not out[~mask].any()
     tol = 2.0 ** -7 * full.abs().sum(2).amax(1)[:, None] + 1e-5
     assert bool(((logits.grad.double() - l.grad).abs() <= tol).all())
+
+
+def test_recorded_and_changed(gpu):
+    """A recorded backward pass has the same values; what it needs and was changed is noticed."""
+    logits = _logits(200, 16, F32).requires_grad_()
+    r = ozk.route_tokens(logits, 3)
+    dw = torch.randn(200, 3, device="cuda")
+    a, = torch.autograd.grad(r.weights, logits, dw, retain_graph=True)
+    b, = torch.autograd.grad(r.weights, logits, dw, create_graph=True)
+    assert torch.equal(a, b.detach())
+    with pytest.raises(RuntimeError, match="twice"):
+        b.sum().backward()
+    for name in ("experts", "counts"):
+        r = ozk.route_tokens(logits, 3)
+        getattr(r, name).add_(1000)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            (r.weights * dw).sum().backward()
+    with torch.inference_mode():
+        q = ozk.route_tokens(logits, 3)
+    assert torch.equal(q.order, r.order) and not q.weights.requires_grad
