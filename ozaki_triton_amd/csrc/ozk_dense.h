@@ -554,17 +554,21 @@ template <typename ST> hipError_t few_plan(const DenseParams &p, hipStream_t st)
 }
 
 // The tile and the K ranges of the shortest time: rounds of workgroups, so many at
-// once, by a round's time, `fixed` + `slope` K / 1024 us (fitted to 180 shapes of 32
-// to 8192 rows and columns, K = 512 to 4096, for operands along K and for a weight's
-// gradient); partial sums cost a launch and their way through memory.  Chosen so,
-// products of those shapes take 1% longer on average than with the best tile of
-// each.  Measured (us, M x N x K, operands along K; 32 x 16 / 32 x 32 / 64 x 32 / 64 x
-// 64 in two groups of waves / 64 x 64 / 128 x 128 / 128 x 256 / 256 x 256):
-//     32 x 4096 x 4096      12 / 14 / 19 / 23 / 43 / 44 / 79 / 125
-//     128 x 4096 x 4096     34 / 24 / 18 / 23 / 44 / 44 / 72 / 120
-//     512 x 4096 x 4096    132 / 93 / 69 / 43 / 39 / 41 / 66 / 112
-//     2048 x 4096 x 2048     - /  - / 117 / 71 / 63 / 49 / 41 / 69
-//     4096 x 4096 x 2048     - /  - / 233 / 139 / 120 / 97 / 79 / 68
+// once, by a round's time, `fixed` + `slope` K / 1024 us (fitted to 477 shapes of 32
+// to 8192 rows and columns, K = 512 to 4096, of operands along K, along N, and of a
+// weight's gradient); partial sums cost a launch and their way through memory.
+// Chosen so, products of those shapes take 1 to 2% longer on average than with the
+// best tile of each.  Measured (us, M x N x K, operands along K, gelu; 32 x 16 / 32 x
+// 32 / 64 x 32 / 64 x 64 in two groups of waves / 64 x 64 / 128 x 128 of 4 stages / 128
+// x 128 / 128 x 256 / 256 x 256):
+//     32 x 4096 x 4096      12 / 14 / 15 / 20 / 33 / 31 / 60 / 51 / 96
+//     128 x 4096 x 4096     34 / 24 / 18 / 23 / 34 / 42 / 64 / 61 / 103
+//     512 x 4096 x 4096    124 / 86 / 61 / 42 / 39 / 40 / 63 / 59 / 111
+//     1024 x 4096 x 1024   122 / 70 / 48 / 30 / 23 / 16 / 19 / 23 / 38
+//     2048 x 4096 x 2048   303 / 206 / 139 / 93 / 76 / 48 / 45 / 42 / 66
+//     4096 x 4096 x 2048   588 / 369 / 275 / 183 / 147 / 93 / 84 / 77 / 69
+// and a weight's gradient of 8192 rows, 4096 x 2048, in its training step: 128 x 128
+// 404 us a step, 128 x 256 413, 256 x 256 431.
 struct TileCost {
     int bm, bn, at_once;
     float fixed[2], slope[2];   // of operands along K, of a weight's gradient
