@@ -133,6 +133,24 @@ def test_infinities_and_nan(gpu):
         assert torch.isfinite(d).all() and not d[7].any()
 
 
+def test_lowest_values(gpu):
+    """Experts switched off by the type's lowest value, some or all of them."""
+    for dtype in (F32, BF, F16):
+        low = torch.finfo(dtype).min
+        logits = _logits(500, 24, dtype)
+        logits[:, 5:20] = low
+        logits[3] = low
+        logits[4] = torch.finfo(dtype).max
+        logits[5, ::2] = torch.finfo(dtype).max
+        logits[5, 1::2] = low
+        logits.requires_grad_()
+        r, want, p, *_ = _check(logits, 6)
+        assert torch.isfinite(r.weights).all() and torch.isfinite(r.balance_loss)
+        d, = torch.autograd.grad(r.balance_loss * 500 + r.weights.square().sum(), logits)
+        assert torch.isfinite(d).all()
+        assert not d[6:, 5:20].any()
+
+
 def test_nothing_left(gpu):
     for T in (0, 1, 70, 5000):
         logits = _logits(T, 12, F32).requires_grad_()

@@ -166,3 +166,27 @@ def test_gradient_c_calls_check_before_they_launch():
                  ((a, a + 64), (a + 4096, a + 4100)),  # results on each other
                  ((a, a + 64), (a + 4096, a + 32))):   # a result on another tensor
         assert c(g, o, n=room) == _lib.OZK_ERR_SHAPE, (g, o)
+
+
+def test_module_on_pytorchs_side():
+    """It is built for this interpreter and torch, and takes nothing that is off the GPU."""
+    m = _lib.torch_binding()
+    x, W = _z(2, 8), _z(3, 8)
+    assert m.linear(x, W, None, None, 0, 0) is None
+    assert m.route(torch.zeros(4, 8), None, 2, True, 0) is None
+    assert m.gradient_norm([torch.zeros(4)], 0) is None and m.gradient_norm([], 0) is None
+    assert m.clip_gradients([torch.zeros(4)], [torch.zeros(4)], 1.0, 0) is None
+
+
+def test_a_missing_module_is_named(monkeypatch):
+    import builtins
+    real = builtins.__import__
+
+    def absent(name, globals=None, locals=None, fromlist=(), level=0):
+        if fromlist and "_ozk_torch" in fromlist:
+            raise ImportError("absent")
+        return real(name, globals, locals, fromlist, level)
+    monkeypatch.setattr(_lib, "_binding", None)
+    monkeypatch.setattr(builtins, "__import__", absent)
+    with pytest.raises(ImportError, match="_ozk_torch.so is not built"):
+        _lib.torch_binding()
