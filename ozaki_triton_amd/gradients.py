@@ -144,6 +144,8 @@ def _through_copies(grads, outs):
     """Tensors with gaps, or laid out other than their result, by copies: the inputs,
     the outputs, and (result, copy) to copy back."""
     ins, to, back = list(grads), list(outs), []
+    assert len({(o.data_ptr(), o.shape, o.stride()) for o in outs if o.numel()}) == \
+        sum(1 for o in outs if o.numel()), "tensors to clip share memory"
     for i, (g, o) in enumerate(zip(grads, outs)):
         if (g is o or g.stride() == o.stride()) and _is_dense(g) or (g.is_contiguous() and o.is_contiguous()):
             continue

@@ -85,6 +85,18 @@ def test_range(gpu):
     assert abs(float(ozk.gradient_norm(big)) / _norm(big) - 1) <= 2 * U
 
 
+def test_factors_below_32_bits(gpu):
+    """max_norm over the norm below fp32's least: results that are ordinary values."""
+    for dtype, value, limit in ((BF, 3e38, 1e-5), (BF, 1e30, 1e-20), (F32, 3e38, 1e-30)):
+        t = [torch.full((n,), value, device="cuda").to(dtype) for n in (3000, 13)]
+        want = [a.double() * (limit / _norm(t)) for a in t]
+        ozk.clip_gradients(t, limit)
+        for a, w in zip(t, want):
+            # one rounding to the type, those of the factor and of 32 bits far below it
+            u = torch.finfo(dtype).eps / 2
+            assert bool(((a.double() - w).abs() <= (u + 4 * U) * w).all())
+
+
 def test_infinite_nan_and_zero(gpu):
     inf, nan = float("inf"), float("nan")
     for bad in (inf, -inf):
@@ -137,6 +149,10 @@ def test_refusals_on_the_gpu(gpu):
     assert abs(float(ozk.gradient_norm([t, t])) - math.sqrt(200)) < 1e-5
     with pytest.raises(AssertionError):
         ozk.clip_gradients([t[:1].expand(5)], 1.0)
+    gaps = torch.ones(10, 10, device="cuda")
+    with pytest.raises(AssertionError):
+        ozk.clip_gradients([gaps[:, ::2], gaps[:, ::2]], 1.0)
+    assert bool((gaps == 1).all())
     with pytest.raises(AssertionError):
         ozk.clip_gradients([t], 1.0, out=[t, t])
     with pytest.raises(AssertionError):
