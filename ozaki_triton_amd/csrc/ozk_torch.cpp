@@ -54,6 +54,12 @@ void refuse_second(const char *name, variable_list &grads) {
         if (g.defined()) g = some[i++];
 }
 
+// A hook may give back anything for a saved tensor: what the kernels take on trust
+void saved_as(const Tensor &t, at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) {
+    if (t.sizes() != sizes || t.scalar_type() != type || t.device() != like.device() || t.layout() != at::kStrided)
+        throw std::runtime_error("a saved tensor came back with another shape, type or device");
+}
+
 // t [rows, columns] with its columns contiguous, and its rows' distance within the
 // kernels' limit (strides of dims of size 1 mean nothing)
 Tensor rows(const Tensor &t, int64_t &stride) {
@@ -128,8 +134,11 @@ struct Linear : torch::autograd::Function<Linear> {
             const bool need_x = ctx->needs_input_grad(0), need_W = ctx->needs_input_grad(1);
             const bool need_b = has_b && ctx->needs_input_grad(2);
             const int64_t M = g.size(0), N = g.size(1);
+            if (need_W) saved_as(saved[0], {M, K}, g.scalar_type(), g);
+            if (need_x) saved_as(saved[1], {N, K}, g.scalar_type(), g);
+            if (saved[2].defined()) saved_as(saved[2], {M, N}, g.scalar_type(), g);
             int64_t sy, sx = 0, sw[2] = {0, 1};
-            const Tensor dy = rows(g, sy), z = saved[2];
+            const Tensor dy = rows(g, sy), z = saved[2].defined() ? saved[2].contiguous() : Tensor();
             const Tensor x = need_W ? rows(saved[0], sx) : Tensor(), W = need_x ? weight(saved[1], sw) : Tensor();
             if (need_x) out[0] = at::empty({M, K}, dy.options());
             if (need_W) out[1] = at::empty({N, K}, dy.options());
@@ -207,11 +216,17 @@ variable_list route_forward(const Tensor &logits_, const std::optional<Tensor> &
 struct Route : torch::autograd::Function<Route> {
     static variable_list forward(AutogradContext *ctx, const Tensor &logits, const std::optional<Tensor> &mask,
                                  int64_t k, bool normalize, int64_t stream) {
-        const variable_list r = route_forward(logits, mask, k, normalize, stream);
+        variable_list r;
+        {
+            // (views of one tensor that do not count each other's changes)
+            at::AutoDispatchBelowADInplaceOrView below;
+            r = route_forward(logits, mask, k, normalize, stream);
+        }
         ctx->set_materialize_grads(false);
         ctx->mark_non_differentiable({r[0], r[2], r[3], r[4], r[5]});
         ctx->save_for_backward({logits, mask ? *mask : Tensor(), r[0], r[1], r[5]});
-        ctx->saved_data["a"] = std::vector<int64_t>{normalize, stream};
+        ctx->saved_data["a"] = std::vector<int64_t>{
+            normalize, stream, mask.has_value(), logits.size(0), logits.size(1), k, (int64_t)logits.scalar_type()};
         return r;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -222,17 +237,23 @@ struct Route : torch::autograd::Function<Route> {
         const variable_list saved = ctx->get_saved_variables();
         {
             at::AutoDispatchBelowADInplaceOrView below;
-            const Tensor logits = saved[0].stride(1) == 1 || saved[0].size(1) == 1 ? saved[0]
-                                                                                   : saved[0].contiguous();
-            const Tensor mask = saved[1].defined() ? saved[1].contiguous() : Tensor(), &experts = saved[2];
+            const Tensor &like = gw.defined() ? gw : gl;
+            const int64_t T = a[3], E = a[4], k = a[5];
+            saved_as(saved[0], {T, E}, (at::ScalarType)a[6], like);
+            if (a[2]) saved_as(saved[1], {T}, at::kBool, like);
+            saved_as(saved[2], {T, k}, at::kInt, like);
+            saved_as(saved[3], {T, k}, at::kFloat, like);
+            saved_as(saved[4], {E}, at::kInt, like);
+            const Tensor logits = saved[0].stride(1) == 1 || E == 1 ? saved[0] : saved[0].contiguous();
+            const Tensor mask = a[2] ? saved[1].contiguous() : Tensor(), experts = saved[2].contiguous();
+            const Tensor weights = saved[3].contiguous(), counts = saved[4].contiguous();
             const Tensor dw = gw.defined() ? gw.contiguous() : Tensor();
-            out[0] = at::empty({logits.size(0), logits.size(1)}, logits.options());
+            out[0] = at::empty({T, E}, logits.options());
             check("ozk_route_backward",
-                  ozk_route_backward(ptr(logits), code(logits.scalar_type()), logits.stride(0),
-                                     ptr(mask), logits.size(0), logits.size(1), experts.size(1),
-                                     (int)a[0], (int32_t *)ptr(experts), (float *)ptr(saved[3]),
-                                     (int32_t *)ptr(saved[4]), (float *)ptr(dw), (float *)ptr(gl),
-                                     ptr(out[0]), (void *)a[1]));
+                  ozk_route_backward(ptr(logits), code(logits.scalar_type()), logits.stride(0), ptr(mask), T, E,
+                                     k, (int)a[0], (int32_t *)ptr(experts), (float *)ptr(weights),
+                                     (int32_t *)ptr(counts), (float *)ptr(dw), (float *)ptr(gl), ptr(out[0]),
+                                     (void *)a[1]));
         }
         variable_list mine = {out[0]};
         refuse_second("route_tokens", mine);

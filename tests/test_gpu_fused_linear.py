@@ -415,3 +415,23 @@ def test_inference_mode(gpu):
     with torch.inference_mode():
         y = ozk.fused_linear(x, W.requires_grad_(), b, activation="gelu", residual=res)
     assert torch.equal(y, want) and not y.requires_grad
+
+
+def test_saved_tensor_hooks(gpu):
+    """Saved tensors that travel to the host and back; ones that come back as something else."""
+    x, W, b, _, dy = _inputs(70, 96, 72, BF)
+    leaves = [t.requires_grad_() for t in (x, W, b)]
+
+    def grads():
+        return torch.autograd.grad(ozk.fused_linear(x, W, b, activation="gelu"), leaves, dy)
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        assert all(torch.equal(a, c) for a, c in zip(grads(), want))
+    # same values, other strides
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.mT.contiguous().mT):
+        for a, c in zip(grads(), want):
+            assert bool(((a.double() - c.double()).abs() <= 2.0 ** -7 * c.double().abs() + 1e-2).all())
+    for back in (lambda t: t.cpu(), lambda t: t[:1], lambda t: t.half(), lambda t: t[..., None]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+            with pytest.raises(RuntimeError, match="saved"):
+                grads()

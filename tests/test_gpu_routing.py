@@ -347,3 +347,34 @@ def test_recorded_and_changed(gpu):
     with torch.inference_mode():
         q = ozk.route_tokens(logits, 3)
     assert torch.equal(q.order, r.order) and not q.weights.requires_grad
+
+
+def test_results_are_each_others_own(gpu):
+    """What the backward pass does not need may be changed in place before it."""
+    logits = _logits(200, 16, F32).requires_grad_()
+    dw = torch.randn(200, 3, device="cuda")
+    want, = torch.autograd.grad(ozk.route_tokens(logits, 3).weights, logits, dw)
+    r = ozk.route_tokens(logits, 3)
+    r.order.div_(3, rounding_mode="floor")
+    r.place.add_(7)
+    r.offsets.zero_()
+    got, = torch.autograd.grad(r.weights, logits, dw)
+    assert torch.equal(got, want)
+
+
+def test_saved_tensor_hooks(gpu):
+    """Saved tensors that travel to the host and back; ones that come back as something else."""
+    logits = _logits(300, 20, BF).requires_grad_()
+    mask = torch.rand(300, device="cuda") < 0.9
+    dw = torch.randn(300, 4, device="cuda")
+
+    def grad():
+        r = ozk.route_tokens(logits, 4, mask=mask)
+        return torch.autograd.grad([r.weights, r.balance_loss], logits, [dw, dw[0, 0]])[0]
+    want = grad()
+    with torch.autograd.graph.save_on_cpu():
+        assert torch.equal(grad(), want)
+    for back in (lambda t: t.cpu(), lambda t: t[:1], lambda t: t.double(), lambda t: t[..., None]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+            with pytest.raises(RuntimeError, match="saved"):
+                grad()
