@@ -435,3 +435,43 @@ def test_saved_tensor_hooks(gpu):
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
             with pytest.raises(RuntimeError, match="saved"):
                 grads()
+
+
+@pytest.mark.parametrize("M, N, K", [(1, 64, 64), (3, 70, 100), (4, 33, 4097), (20, 50, 1025), (33, 65, 72), (130, 200, 136),
+                                     (300, 72, 2056), (64, 40, 99)])
+@pytest.mark.parametrize("offset", [0, 1, 8])
+def test_nothing_beside_the_operands_counts(gpu, M, N, K, offset):
+    """Operands inside tensors of NaN: neither results nor gradients have one."""
+    def inside(rows, columns):
+        big = torch.full((rows + 3, columns + 24), math.nan, device="cuda", dtype=BF)
+        big[1:1 + rows, offset:offset + columns] = torch.randn(rows, columns, device="cuda").to(BF)
+        return big[1:1 + rows, offset:offset + columns]
+    for W in (inside(N, K), inside(K, N).mT):
+        x, b, res = inside(M, K), inside(1, N)[0], inside(M, N)
+        leaves = [t.detach().requires_grad_() for t in (x, W, b, res)]
+        y = ozk.fused_linear(leaves[0], leaves[1], leaves[2], activation="gelu", residual=leaves[3])
+        _check(y.detach(), x, W, b, res, "gelu")
+        for g in torch.autograd.grad(y, leaves, inside(M, N)):
+            assert bool(torch.isfinite(g).all())
+
+
+def test_past_32_bits(gpu):
+    """More than 2^31 results: the first, middle and last rows and columns, and their gradients."""
+    M, N, K = 70000, 31000, 16
+    x, W, b = (torch.randn(*s, device="cuda").to(BF) for s in ((M, K), (N, K), (N,)))
+    dy = torch.randn(N, device="cuda").to(BF).expand(M, N)
+    leaves = [t.requires_grad_() for t in (x, W, b)]
+    y = ozk.fused_linear(x, W, b, activation="relu")
+    for rows in (slice(0, 100), slice(34600, 34800), slice(M - 100, M)):
+        _check(y[rows].detach(), x[rows].detach(), W.detach(), b.detach(), None, "relu")
+    dx, dW, db = torch.autograd.grad(y, leaves, dy)
+    last = slice(M - 50, M)
+    dz = torch.where(y[last].detach() > 0, dy[last].double(), 0.0)   # relu's side as computed
+    size = dz.abs() @ W.detach().double().abs()
+    want = dz @ W.detach().double()
+    assert bool(((dx[last].double() - want).abs() <= (1.13 * N * U + 2.0 ** -8) * size).all())
+    columns = slice(N - 40, N)
+    dz = torch.where(y[:, columns].detach() > 0, dy[:, columns].double(), 0.0).mT.contiguous()
+    size = dz.abs() @ x.detach().double().abs()
+    assert bool(((dW[columns].double() - dz @ x.detach().double()).abs() <= (1.13 * M * U + 2.0 ** -8) * size).all())
+    assert bool(((db[columns].double() - dz.sum(1)).abs() <= (M * U + 2.0 ** -8) * dz.abs().sum(1)).all())

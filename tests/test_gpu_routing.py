@@ -378,3 +378,32 @@ def test_saved_tensor_hooks(gpu):
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
             with pytest.raises(RuntimeError, match="saved"):
                 grad()
+
+
+def test_past_32_bits(gpu):
+    """More than 2^31 logits: the first and the last tokens, the whole order, their gradients."""
+    T, E, k = 4300000, 512, 2
+    logits = torch.randn(T, E, device="cuda").to(BF).requires_grad_()
+    r = ozk.route_tokens(logits, k)
+    ends = [slice(0, 500), slice(T - 500, T)]
+    for s in ends:
+        want, *_ = _plain(logits[s].detach(), k, None, True)
+        assert torch.equal(r.experts[s].long(), want["experts"])
+        # (2 spread U as above, spread below 64)
+        assert bool(((r.weights[s].double() - want["weights"]).abs() <= 128 * U).all())
+    slots = torch.arange(T * k, device="cuda")
+    sorted_experts = r.experts.flatten()[r.order.long()]
+    assert torch.equal(r.order[r.place.flatten().long()].long(), slots)
+    assert bool((sorted_experts.diff() >= 0).all())
+    assert bool(((r.order.diff() > 0) | (sorted_experts.diff() > 0)).all())   # their own order within one
+    assert torch.equal(r.counts.long(), torch.bincount(r.experts.flatten(), minlength=E))
+    assert torch.equal(r.offsets.diff(), r.counts)
+    dw = torch.randn(T, k, device="cuda")
+    d, = torch.autograd.grad(r.weights, logits, dw)
+    for s in ends:
+        w, g = r.weights[s].detach().double(), dw[s].double()
+        want = torch.zeros(500, E, device="cuda", dtype=torch.float64).scatter_(
+            1, r.experts[s].long(), w * (g - (w * g).sum(1, keepdim=True)))
+        # a weight's error by the difference of two terms that have it, too
+        tol = 2.0 ** -8 * want.abs() + 3 * 128 * U * g.abs().sum(1, keepdim=True)
+        assert bool(((d[s].double() - want).abs() <= tol).all())

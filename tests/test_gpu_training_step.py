@@ -1,6 +1,7 @@
 """The operators of a training step together: router, grouped products, dense products
 with their epilogues, clipping, orthogonalised update; eager and captured."""
 import math
+import threading
 
 import pytest
 import torch
@@ -108,3 +109,36 @@ def test_step_captured(gpu):
             # (torch's own reductions and scatters run in both)
             assert float((a.double() - b.double()).norm()) <= 1e-3 * float(b.double().norm()) + 1e-12
         assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
+
+
+def test_threads(gpu):
+    """Steps of several threads at once, each on a stream of its own, have the same bits."""
+    x, W = (torch.randn(*s, device="cuda").to(torch.bfloat16) for s in ((333, 520), (700, 520)))
+    logits = torch.randn(3000, 64, device="cuda")
+
+    def step():
+        a, w, t = (v.detach().requires_grad_() for v in (x, W, logits))
+        y = ozk.fused_linear(a, w, activation="gelu")
+        r = ozk.route_tokens(t, 4)
+        (y.float().square().sum() + r.balance_loss + r.weights.square().sum()).backward()
+        norm = ozk.clip_gradients([a.grad, w.grad, t.grad], 1.0)
+        return [y.detach(), a.grad, w.grad, t.grad, norm, *(v.detach() for v in r)]
+    want = step()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = step()
+                stream.synchronize()
+                if not all(torch.equal(u, v) for u, v in zip(got, want)):
+                    wrong.append(i)
+        wrong.append(None)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [None] * 4
