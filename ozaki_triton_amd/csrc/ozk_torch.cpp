@@ -10,6 +10,7 @@
 //
 // A stream comes as its handle.  A backward pass runs on the stream of its forward
 // pass, as autograd has it.
+#include <hip/hip_runtime_api.h>
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -52,6 +53,26 @@ void refuse_second(const char *name, variable_list &grads) {
     size_t i = 0;
     for (Tensor &g : grads)
         if (g.defined()) g = some[i++];
+}
+
+// A backward pass that is captured on `stream` and goes on at a node of the default
+// stream, as a leaf has while an earlier graph of it is alive: the engine would make the
+// default stream wait for the capture, which ends the process.
+void refuse_default_stream(const char *name, int64_t stream) {
+    const auto node = torch::autograd::get_current_node();
+    if (!stream || !node) return;
+    bool found = false;
+    for (const auto &edge : node->next_edges())
+        if (edge.function) {
+            const auto s = edge.function->stream();
+            found |= s && s->id() == 0;
+        }
+    if (!found) return;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone)
+        return;
+    throw std::runtime_error(std::string(name) + ": a captured backward pass reaches a tensor that has a graph on "
+                             "the default stream; delete that graph (its results) before the capture");
 }
 
 // A hook may give back anything for a saved tensor: what the kernels take on trust
@@ -129,6 +150,7 @@ struct Linear : torch::autograd::Function<Linear> {
         variable_list out(6);
         const Tensor &g = grads[0];
         if (!g.defined()) return out;
+        refuse_default_stream("fused_linear", stream);
         {
             at::AutoDispatchBelowADInplaceOrView below;
             const bool need_x = ctx->needs_input_grad(0), need_W = ctx->needs_input_grad(1);
@@ -234,6 +256,7 @@ struct Route : torch::autograd::Function<Route> {
         const Tensor &gw = grads[1], &gl = grads[6];
         if (!gw.defined() && !gl.defined()) return out;
         const auto a = ctx->saved_data["a"].toIntVector();
+        refuse_default_stream("route_tokens", a[1]);
         const variable_list saved = ctx->get_saved_variables();
         {
             at::AutoDispatchBelowADInplaceOrView below;

@@ -142,3 +142,36 @@ def test_threads(gpu):
     for t in threads:
         t.join()
     assert wrong == [None] * 4
+
+
+def test_capture_beside_an_eager_graph(gpu):
+    """A captured backward pass of leaves that an eager graph holds is refused, and works once that is gone."""
+    x = torch.randn(64, 64, device="cuda").to(F16)
+    W = torch.randn(64, 64, device="cuda").to(F16).requires_grad_()
+    logits = torch.randn(40, 8, device="cuda").requires_grad_()
+    dy, dw = torch.randn(64, 64, device="cuda").to(F16), torch.randn(40, 2, device="cuda")
+    calls = [(lambda: ozk.fused_linear(x, W), W, dy), (lambda: ozk.route_tokens(logits, 2).weights, logits, dw)]
+    for forward, leaf, seed in calls:
+        want, = torch.autograd.grad(forward(), leaf, seed)
+        keep = forward()
+        # on another stream, but not captured: as ever
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got, = torch.autograd.grad(forward(), leaf, seed)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="default stream"):
+            with torch.cuda.graph(graph):
+                torch.autograd.grad(forward(), leaf, seed)
+        torch.cuda.synchronize()
+        del keep
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(forward(), leaf, seed)
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
