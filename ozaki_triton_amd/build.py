@@ -121,8 +121,7 @@ def build_torch_binding(verbose: bool = False) -> str:
     from torch.utils import cpp_extension
     out = os.path.join(HERE, TORCH_NAME)
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
-    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"],
-                os.path.join(os.path.dirname(os.path.dirname(_hipcc())), "include")]
+    includes = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"]]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__",
