@@ -413,10 +413,12 @@ template <bool SCANNED> __global__ __launch_bounds__(1024) void route_place_kern
             else earlier = p.hist[(int64_t)block * p.E + e];
         }
     } else {
-        // `ways` lanes to an expert, each every ways-th workgroup's counts
+        // `ways` lanes to an expert, each every ways-th workgroup's counts; 32 of them at
+        // most, as theirs are added up one after the other (rows and place of 4096 x 2, us:
+        // 512 ways 37, 32 ways 11; 4096 x 16: 64 ways 13.5, 32 ways 11.7)
         uint32_t *sums = start + (p.E + 2) / 2 * 2;   // [2][1024]
         double *ps = (double *)(sums + 2048);         // [1024]
-        const int ways = 1024 / p.E, of = e % p.E, way = e / p.E;
+        const int ways = p.E > 32 ? 1024 / p.E : 32, of = e % p.E, way = e / p.E;
         if (way < ways) {
 #pragma unroll 8
             for (int b = way; b < p.blocks; b += ways) {
