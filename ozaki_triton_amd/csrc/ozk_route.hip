@@ -189,6 +189,10 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteParam
     constexpr int TPW = 64 / GL;   // tokens of a wave at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int in = lane % GL, e0 = in * V;
+    // a lane's keys greatest first, so that a round looks at one of them (with 4 of them, us,
+    // unsorted / sorted: 300000 x 64, k = 8, fp32 145 / 129; 32768 x 64 20.4 / 19.4)
+    constexpr bool SORTED = V == 4;
+    const uint64_t below = (((uint64_t)1 << in) - 1) << (lane - in);   // the group's lanes before this
     const int64_t t0 = (int64_t)blockIdx.x * p.per;
     const int tokens = (int)(p.T - t0 < p.per ? p.T - t0 : p.per);
     for (int i = threadIdx.x; i < kRouteWaves * (p.E + 1); i += 64 * kRouteWaves) lds.wave_hist[i] = 0;
@@ -203,53 +207,72 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteParam
         uint32_t key[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) key[v] = e0 + v < p.E ? key_of<T>(l[v], e0 + v) : 0u;
+        uint32_t expert[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) expert[v] = e0 + v;
+        if constexpr (SORTED) {   // exchanges of neighbours only, so that equal ones stay in order
+            auto order = [&](int i) {
+                const bool swap = key[i + 1] > key[i];
+                const uint32_t k0 = key[i], k1 = key[i + 1], x0 = expert[i], x1 = expert[i + 1];
+                key[i] = swap ? k1 : k0;
+                key[i + 1] = swap ? k0 : k1;
+                expert[i] = swap ? x1 : x0;
+                expert[i + 1] = swap ? x0 : x1;
+            };
+#pragma unroll
+            for (int n = 0; n < V; ++n)
+#pragma unroll
+                for (int i = n & 1; i + 1 < V; i += 2) order(i);
+        }
         // k rounds; lane j of the group keeps the j-th choice, GL of them at a time
-        float top = 0.f, chosen = 0.f, kept = 0.f;
-        uint32_t kept_at = 0;
+        float chosen = 0.f;
+        uint32_t first = 0, kept = 0;
         for (int j0 = 0; j0 < p.k; j0 += GL) {
             const int here = p.k - j0 < GL ? p.k - j0 : GL;
             for (int j = 0; j < here; ++j) {
                 uint32_t own = key[0];
+                if constexpr (!SORTED)
 #pragma unroll
-                for (int v = 1; v < V; ++v) own = key[v] > own ? key[v] : own;
+                    for (int v = 1; v < V; ++v) own = key[v] > own ? key[v] : own;
                 const uint32_t best = group_max<GL>(own);
-                const float x = value_of<T>(best);
-                if (j0 + j == 0) top = x;
-                kept = in == j ? x : kept;
-                if constexpr (sizeof(T) == 4) {
-                    // the lowest lane of the group that has it, there the lowest slot
-                    const uint64_t has = __ballot(own == best);
-                    uint32_t lowest;
-                    if constexpr (GL == 64) lowest = (uint32_t)__builtin_ctzll(has);
-                    else lowest = __builtin_ctz((uint32_t)(has >> (lane & ~(GL - 1))) | (uint32_t)(1ull << GL));
-                    if ((uint32_t)in == lowest) {
-                        uint32_t at = 0;
+                first = j0 + j == 0 ? best : first;
+                kept = in == j ? best : kept;
+                bool mine = own == best;
+                if constexpr (sizeof(T) == 4) mine = mine && !(__ballot(mine) & below);
+                if (mine) {
+                    uint32_t at = expert[0];
+                    if constexpr (SORTED) {
+#pragma unroll
+                        for (int v = 0; v + 1 < V; ++v) {
+                            key[v] = key[v + 1];
+                            expert[v] = expert[v + 1];
+                        }
+                        key[V - 1] = 0;
+                    } else {   // the lowest that has it
                         bool found = false;
 #pragma unroll
                         for (int v = 0; v < V; ++v) {
                             const bool hit = !found && key[v] == best;
                             found |= hit;
-                            at = hit ? (uint32_t)(e0 + v) : at;
+                            at = hit ? expert[v] : at;
                             key[v] = hit ? 0u : key[v];
                         }
-                        if (there) lds.expert[t * p.k + j0 + j] = (uint16_t)(valid ? at : (uint32_t)p.E);
                     }
-                } else {
-                    kept_at = in == j ? 0xFFFFu - (best & 0xFFFFu) : kept_at;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) key[v] = key[v] == best ? 0u : key[v];
+                    if constexpr (sizeof(T) == 4)
+                        if (there) lds.expert[t * p.k + j0 + j] = (uint16_t)(valid ? at : (uint32_t)p.E);
                 }
             }
             if (in < here) {
-                const float e = expf(kept - top);
+                const float e = expf(value_of<T>(kept) - value_of<T>(first));
                 chosen += e;
                 if (there) {
                     lds.value[t * p.k + j0 + in] = e;
                     if constexpr (sizeof(T) == 2)
-                        lds.expert[t * p.k + j0 + in] = (uint16_t)(valid ? kept_at : (uint32_t)p.E);
+                        lds.expert[t * p.k + j0 + in] = (uint16_t)(valid ? 0xFFFFu - (kept & 0xFFFFu) : (uint32_t)p.E);
                 }
             }
         }
+        const float top = value_of<T>(first);
         chosen = group_sum<GL>(chosen);
         float q[V], sum = 0.f;
 #pragma unroll
@@ -628,12 +651,18 @@ template <typename T> hipError_t route_grad_go(const RouteGradParams &p, hipStre
 }  // namespace
 
 void plan_route(RouteParams &p) {
-    // a workgroup's tokens: one step of its waves, more where that makes more
-    // than 256 of them, as many as its LDS holds
+    // a workgroup's tokens: whole steps of its waves, a workgroup to a CU, or two where
+    // that leaves 6 steps each, as many as the LDS of two or of one holds (rows and place,
+    // us, 256 / 512 workgroups: 32768 x 64, k = 8, fp32 19.3 / 22.3; 300000 x 64 84 / 76;
+    // 65536 x 256, k = 8, bf16 64 / 61)
     const int64_t step = (int64_t)kRouteWaves * 64 / lanes_of(p.E);
-    int64_t per = step, most = (150 * 1024 - (int64_t)RouteLds::bytes(p.E, 0, 0)) / (4 + 6 * p.k);
-    while (per < most / 2 && (p.T + per - 1) / per > 256) per *= 2;
-    if (per > most) per = most;
+    const int64_t fixed = (int64_t)RouteLds::bytes(p.E, 0, 0), each = 4 + 6 * p.k;
+    const int64_t room = fixed + step * each <= 78 * 1024 ? 78 * 1024 : 150 * 1024;
+    const int64_t most = (room - fixed) / each;
+    const int64_t blocks = p.T > 256 * 12 * step ? 512 : 256;
+    int64_t per = ((p.T + blocks - 1) / blocks + step - 1) / step * step;
+    if (per > most) per = most < step ? most : most / step * step;
+    if (per == 0) per = step;
     p.per = per;
     p.blocks = p.T > per ? (int)((p.T + per - 1) / per) : 1;
 }
