@@ -634,10 +634,15 @@ template <typename ST> hipError_t dense_plan(const DenseParams &p, hipStream_t s
 
 }  // namespace
 
-// Up to 4 rows, and up to 32 that the tiles' DMA cannot take (us, this / tiles: 4 x
-// 4096 x 4096 9.7 / 9.4, 16 x 4096 x 4096 11.5 / 9.6, 32 x 4096 x 4097 25 / 52)
+// Up to 4 rows; of those that the tiles' DMA cannot take up to 32, and up to 128 where
+// W, read once for 16 of them, is small (us, this / tiles: 4 x 4096 x 4096 9.7 / 9.4, 16
+// x 4096 x 4096 11.5 / 9.6; 32 x 4096 x 4097 24 / 52, 48 x 4096 x 4097 35 / 26, 40 x 3648
+// x 1810 11.7 / 40, 96 x 3648 x 1810 17.9 / 18.2, 128 x 1024 x 1001 7.6 / 10.6)
 bool dense_few(const DenseParams &p) {
-    return !p.a_cols && !p.b_cols && (p.M <= 4 || (p.M <= 32 && !pieces(p)));
+    if (p.a_cols || p.b_cols) return false;
+    if (p.M <= 4) return true;
+    const int64_t groups = (p.M + 15) / 16;
+    return (groups <= 2 || (groups <= 8 && (double)groups * p.N * p.K <= 35e6)) && !pieces(p);
 }
 int dense_splits(const DenseParams &p) {
     return dense_few(p) || p.M == 0 || p.N == 0 ? 1 : plan_tiles(p).splits;

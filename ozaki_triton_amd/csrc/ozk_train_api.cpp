@@ -78,7 +78,12 @@ ozk::GroupedGradParams as_grad(const ozk::DenseParams &p) {   // K rows of M and
 ozk::PackedSizes copies(const ozk::DenseParams &p) {
     // few rows go past the tiles
     if (ozk::dense_few(p)) return {0, 0};
-    return p.a_cols ? ozk::plan_grad_pack(as_grad(p)) : ozk::plan_grouped_pack(as_grouped(p));
+    if (p.a_cols) return ozk::plan_grad_pack(as_grad(p));
+    ozk::GroupedParams g = as_grouped(p);
+    // a grouped product has smaller tiles for fewer than 48 rows, this one does not (40 x
+    // 6592 x 2861, us: read as they are 59, copied 25)
+    if (g.T > 32 && g.T < 48) g.T = 48;
+    return ozk::plan_grouped_pack(g);
 }
 size_t part_bytes(const ozk::DenseParams &p, int splits) {
     return splits > 1 ? (size_t)round_up((int64_t)splits * p.M * p.N * 4, 16) : 0;

@@ -475,3 +475,15 @@ def test_past_32_bits(gpu):
     size = dz.abs() @ x.detach().double().abs()
     assert bool(((dW[columns].double() - dz @ x.detach().double()).abs() <= (1.13 * M * U + 2.0 ** -8) * size).all())
     assert bool(((db[columns].double() - dz.sum(1)).abs() <= (M * U + 2.0 ** -8) * dz.abs().sum(1)).all())
+
+
+@pytest.mark.parametrize("M, N, K", [(33, 70, 1001), (40, 2500, 2861), (45, 7000, 2861), (64, 129, 515), (100, 60, 4097),
+                                     (113, 33, 1810), (128, 1000, 999), (129, 1000, 999), (47, 90, 8191), (97, 1, 77)])
+def test_rows_off_16_bytes(gpu, M, N, K):
+    """Whole range of rows that are no 16-byte pieces: with few of them, copied, and read as they are."""
+    for dtype, act in ((BF, "gelu"), (F16, None)):
+        x, W, b, res, _ = _inputs(M, N, K, dtype)
+        _check(ozk.fused_linear(x, W, b, activation=act, residual=res), x, W, b, res, act)
+        # rows that are whole pieces apart but begin off them
+        x, W = (torch.nn.functional.pad(t, (1, 16 - (K + 1) % 8))[:, 1:1 + K] for t in (x, W))
+        _check(ozk.fused_linear(x, W, b, activation=act), x, W, b, None, act)
