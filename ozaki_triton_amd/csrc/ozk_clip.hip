@@ -128,12 +128,14 @@ __global__ __launch_bounds__(256) void norm_kernel(ClipParams p) {
     if (threadIdx.x == 0) *p.norm = (float)norm;
 }
 
-// WIDE: the products in 64 bits, rounded once, as fp32 needs them.  Else in 32 bits,
-// whose rounding is 2^-13 of a 16-bit type's, for factors that lose no bits there (a
-// bf16 value of 3e38 times 1e-45 is an ordinary number).
-template <typename T, bool NT, bool WIDE> OZK_DEV void piece_scale(const Piece &c, double by) {
+// fp32: the product in 64 bits, rounded once.  16 bits: in 32 bits, whose rounding is
+// 2^-13 of theirs, by's exponent apart, as by itself may be below 32 bits' range (a bf16
+// value of 3e38 times 1e-45 is an ordinary number).
+template <typename T, bool NT> OZK_DEV void piece_scale(const Piece &c, double by) {
     constexpr int V = 16 / sizeof(T);
     const int parts = c.n / V;
+    int exponent;
+    const float mantissa = (float)frexp(by, &exponent);
     auto scaled = [&](i32x4 v) {
         float f[V];
         values<T>(v, f);
@@ -146,7 +148,7 @@ template <typename T, bool NT, bool WIDE> OZK_DEV void piece_scale(const Piece &
             uint16_t e[V];
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                e[i] = to_bits16(WIDE ? (float)((double)f[i] * by) : f[i] * (float)by, T{});
+                e[i] = to_bits16(__builtin_ldexpf(f[i] * mantissa, exponent), T{});
             __builtin_memcpy(&r, e, 16);
         }
         return r;
@@ -177,10 +179,9 @@ template <bool NT> __global__ __launch_bounds__(256) void scale_kernel(ClipParam
     for (uint32_t j = blockIdx.x; j < p.pieces; j += gridDim.x) {
         const Piece c = piece_of(p, p.pieces - 1 - j);
         if (by == 1.0 && c.in == c.out) continue;
-        if (c.dtype == OZK_F32) piece_scale<float, NT, true>(c, by);
-        else if (c.dtype == OZK_F16) piece_scale<_Float16, NT, false>(c, by);   // (0 long before)
-        else if (by >= 0x1p-100) piece_scale<__bf16, NT, false>(c, by);
-        else piece_scale<__bf16, NT, true>(c, by);
+        if (c.dtype == OZK_F32) piece_scale<float, NT>(c, by);
+        else if (c.dtype == OZK_F16) piece_scale<_Float16, NT>(c, by);
+        else piece_scale<__bf16, NT>(c, by);
     }
 }
 
