@@ -9,8 +9,8 @@
 // Tensors are cut into pieces of one size, which the workgroups take in turn; a
 // launch carries its tensors' addresses in its arguments (so a captured graph
 // keeps them), kClipTensors at most.  Bound by memory: every element read once
-// for the norm, read and written once more for the scaling (268M bf16 elements: 82 us,
-// 6.5 TB/s, and 193 us, 5.6 TB/s).
+// for the norm, read and written once more for the scaling (268M bf16 elements: 83 us,
+// 6.5 TB/s, and 192 us, 5.6 TB/s).
 #include "../../include/ozaki_amd.h"
 #include "ozk_train.h"
 #include "ozk_tile.h"

@@ -23,7 +23,7 @@
 //
 // Bound by latency and instructions, not by the bytes (22 MB of the first line are
 // 4.5 us of a copy).  Measured (us, T x E, k; rows / place / gradient):
-//     32768 x 64, 8, fp32   13.5 / 8.2 / 8.8      4099 x 40, 3, bf16   6.3 / 6.8 / 4.4
+//     32768 x 64, 8, fp32   12.3 / 8.3 / 8.8      4099 x 40, 3, bf16   6.2 / 6.9 / 4.4
 //     16 x 16, 2, bf16       6.9 (one launch)
 #include "../../include/ozaki_amd.h"
 #include "ozk_train.h"
@@ -602,8 +602,8 @@ namespace {
 
 // Lanes of a token and values of a lane, by E.  4 values: with 8 a wave takes twice
 // the tokens at once, which pays only where there are many (rows alone, us, with 4 /
-// with 8: 32768 x 64, k = 8, fp32 13.4 / 12.5; 4099 x 40, k = 3, bf16 6.3 / 8.1; 16 x
-// 16, k = 2 6.8 / 7.8).
+// with 8, unsorted: 32768 x 64, k = 8, fp32 13.4 / 12.5, 12.3 with 4 sorted; 4099 x 40,
+// k = 3, bf16 6.3 / 8.1; 16 x 16, k = 2 6.8 / 7.8).
 template <typename F> hipError_t with_shape(int E, F &&f) {
     using std::integral_constant;
 #define OZK_ROUTE(GL, V) return f(integral_constant<int, GL>{}, integral_constant<int, V>{})
