@@ -14,6 +14,9 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
+#include <numeric>
+
 #include "../../include/ozaki_amd.h"
 
 namespace {
@@ -367,6 +370,98 @@ std::optional<Tensor> clip_gradients(const std::vector<Tensor> &grads, const std
     return norm;
 }
 
+// ---- tensors with gaps that lie in the same memory ----
+
+// Whether sum of step k over the terms, each k within its lo .. hi, can be from `lo` to
+// `hi` (with `moved`: any; else: with some k that is not 0).  Largest steps first, each k
+// as far as the rest can make up for; what a common divisor leaves out is left out.
+// Past `budget` steps the answer is yes.
+struct Term {
+    int64_t step, lo, hi;
+};
+bool reaches(const Term *t, size_t n, int64_t lo, int64_t hi, bool moved, int64_t &budget) {
+    if (!n) return moved && lo <= 0 && hi >= 0;
+    if (--budget < 0) return true;
+    int64_t least = 0, most = 0, common = 0;   // of the rest; of all
+    for (size_t i = 0; i < n; ++i) {
+        common = std::gcd(common, t[i].step);
+        if (!i) continue;
+        least += t[i].step * t[i].lo;
+        most += t[i].step * t[i].hi;
+    }
+    auto floor_of = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    if (floor_of(hi, common) * common < lo) return false;
+    const int64_t step = t->step, first = std::max(t->lo, -floor_of(most - lo, step));
+    const int64_t last = std::min(t->hi, floor_of(hi - least, step));
+    for (int64_t k = first; k <= last; ++k)
+        if (reaches(t + 1, n - 1, lo - step * k, hi - step * k, moved || k, budget)) return true;
+    return false;
+}
+constexpr int64_t kReachBudget = 1 << 16;
+
+struct Span {
+    int64_t lo, hi, item;      // bytes
+    std::vector<Term> dims;    // one element to the next, in bytes
+    size_t of;                 // its place in the list
+    bool out;
+};
+Span span_of(const Tensor &t, size_t of, bool out) {
+    Span s = {(int64_t)(uintptr_t)t.data_ptr(), 0, (int64_t)t.element_size(), {}, of, out};
+    s.hi = s.lo + s.item;
+    for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) > 1) {
+            s.dims.push_back({t.stride(d) * s.item, 0, t.size(d) - 1});
+            s.hi += s.dims.back().step * s.dims.back().hi;
+        }
+    return s;
+}
+// whether two indices are one element, or elements that overlap
+bool meets_itself(const Span &s) {
+    std::vector<Term> t;
+    for (const Term &d : s.dims) {
+        if (!d.step) return true;
+        t.push_back({d.step, -d.hi, d.hi});
+    }
+    std::sort(t.begin(), t.end(), [](const Term &a, const Term &b) { return a.step > b.step; });
+    int64_t budget = kReachBudget;
+    return reaches(t.data(), t.size(), 1 - s.item, s.item - 1, false, budget);
+}
+bool meet(const Span &a, const Span &b) {
+    std::vector<Term> t;
+    for (const Term &d : a.dims)
+        if (d.step) t.push_back(d);
+    for (const Term &d : b.dims)
+        if (d.step) t.push_back({d.step, -d.hi, 0});
+    std::sort(t.begin(), t.end(), [](const Term &x, const Term &y) { return x.step > y.step; });
+    size_t n = 0;   // those of one step as one
+    for (size_t i = 0; i < t.size(); ++i)
+        if (n && t[n - 1].step == t[i].step) {
+            t[n - 1].lo += t[i].lo;
+            t[n - 1].hi += t[i].hi;
+        } else {
+            t[n++] = t[i];
+        }
+    const int64_t d = a.lo - b.lo;
+    int64_t budget = kReachBudget;
+    return reaches(t.data(), n, 1 - a.item - d, b.item - 1 - d, true, budget);
+}
+// Whether an element of outs is in one of the other tensors, of ins or outs, or there
+// twice (or cannot be shown not to be).
+bool share_memory(const std::vector<Tensor> &ins, const std::vector<Tensor> &outs) {
+    std::vector<Span> s;
+    for (size_t i = 0; i < outs.size(); ++i) {
+        if (!outs[i].numel()) continue;
+        s.push_back(span_of(outs[i], i, true));
+        if (meets_itself(s.back())) return true;
+        if (!ins[i].is_same(outs[i])) s.push_back(span_of(ins[i], i, false));
+    }
+    std::sort(s.begin(), s.end(), [](const Span &a, const Span &b) { return a.lo < b.lo; });
+    for (size_t i = 0; i < s.size(); ++i)
+        for (size_t j = i + 1; j < s.size() && s[j].lo < s[i].hi; ++j)
+            if ((s[i].out || s[j].out) && s[i].of != s[j].of && meet(s[i], s[j])) return true;
+    return false;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ozk_torch, m) {
@@ -374,4 +469,5 @@ PYBIND11_MODULE(_ozk_torch, m) {
     m.def("route", &route);
     m.def("gradient_norm", &gradient_norm);
     m.def("clip_gradients", &clip_gradients);
+    m.def("share_memory", &share_memory);
 }

@@ -228,3 +228,21 @@ def test_parameters_gradients_in_place(gpu):
         t = [torch.ones(10, device="cuda")]
         ozk.clip_gradients(t, 1.0)
     assert abs(float(t[0].norm()) - 1) < 1e-6
+
+
+def test_overlaps_of_tensors_with_gaps(gpu):
+    """Refused like those of contiguous ones, before anything is written."""
+    base = torch.ones(64, 48, device="cuda")
+    for bad in ([base, base[:, ::2]], [base[:, :4], base[:, 2:6]], [base[:8], base[::2]],
+                [base.as_strided((5, 5), (3, 2))]):
+        with pytest.raises(AssertionError, match="share memory"):
+            ozk.clip_gradients(bad, 1.0)
+    g = [torch.ones(64, 4, device="cuda") for _ in range(2)]
+    for out in ([base[:, :4], base[:, 2:6]], [base[:, 44:], base[:1, 44:].expand(64, 4)]):
+        with pytest.raises(AssertionError, match="share memory"):
+            ozk.clip_gradients(g, 1.0, out=out)
+    assert bool((base == 1).all()) and all(bool((t == 1).all()) for t in g)
+    # columns of one tensor, apart
+    views = [base[:, i::3] for i in range(3)]
+    before = [v.clone() for v in views]
+    _check(before, views, 3.0, ozk.clip_gradients(views, 3.0))
