@@ -14,14 +14,24 @@
 namespace ozk {
 
 // ---------------------------------------------------------------------------
-// Activations.  Results are rounded to 8 or 11 bits: exp2 and the reciprocal of
-// the hardware (1 ulp) and the rounding of exp2's argument, |z| 2^-24 relative,
-// stay far below that.
+// Activations.  Results are rounded to 8 or 11 bits: exp2 and the reciprocal of the
+// hardware (1 ulp each) and the roundings of exp2's argument stay far below that.  The
+// latter are worth 2^-24 of the argument's size each, which grows with z in silu, with
+// z^2 in gelu and z^3 in gelu_tanh: up to 7e-6, 8e-6 and 1.7e-5 of the smallest normal
+// results (fp32 steps against 64 bits, 2e6 values of z each).
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.44269504f, kGelu2 = 1.59576912f /* 2 sqrt(2 / pi) */, kGelu3 = 0.044715f;
 
-OZK_DEV float sigmoid(float z) {   // 1 / (1 + e^-z)
-    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * z));
+// Far below 0 the exponentials leave fp32's normal range, where exp2 and the reciprocal
+// give 0, before the results do (bf16 has that range, too; silu(-88) is -5.3e-37): they
+// are 2^64 times as large there, and the results brought back last.
+struct Scaled {
+    float v, by;   // v * by, by 1 or 2^-64
+};
+OZK_DEV Scaled sigmoid(float z) {   // 1 / (1 + e^-z)
+    const float t = -kLog2e * z;
+    const bool far = t > 96.f;
+    return {__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(far ? t - 64.f : t)), far ? 0x1p-64f : 1.f};
 }
 // Phi(-a) of the normal distribution for a = |z| is e^(-a a / 2) times something
 // smooth, here a polynomial in t = 1 / (1 + 0.3 a) fitted to it over 0 .. 14 (beyond,
@@ -37,7 +47,13 @@ OZK_DEV float tail_factor(float z) {
     q = fmaf(q, t, 0.12127471715211868f);
     return fmaf(q, t, -7.979064685059711e-05f);
 }
+// (gelu itself: where e^(-z z / 2) is 0 here it is below 2^-127; its derivative is not)
 OZK_DEV float gauss(float z) { return __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z); }
+OZK_DEV Scaled gauss_scaled(float z) {
+    const float t = -0.5f * kLog2e * z * z;
+    const bool far = t < -96.f;
+    return {__builtin_amdgcn_exp2f(far ? t + 64.f : t), far ? 0x1p-64f : 1.f};
+}
 // |z| and z within 1e4, where every formula below has reached its limit and no
 // infinity is left to be multiplied with 0; a NaN is carried by the other factors
 OZK_DEV float near_abs(float z) { return fminf(fabsf(z), 1e4f); }
@@ -45,9 +61,14 @@ OZK_DEV float near(float z) { return __builtin_amdgcn_fmed3f(z, -1e4f, 1e4f); }
 
 template <int ACT> OZK_DEV float activation(float z) {
     if constexpr (ACT == OZK_ACT_RELU) return z < 0.f ? 0.f : z;   // NaN stays
-    if constexpr (ACT == OZK_ACT_SILU) return z * sigmoid(z);
-    if constexpr (ACT == OZK_ACT_GELU_TANH)
-        return z * sigmoid(kGelu2 * fmaf(kGelu3 * z * z, z, z));   // (1 + tanh u) / 2 = sigmoid(2u)
+    if constexpr (ACT == OZK_ACT_SILU) {
+        const Scaled s = sigmoid(z);
+        return z * s.v * s.by;
+    }
+    if constexpr (ACT == OZK_ACT_GELU_TANH) {   // (1 + tanh u) / 2 = sigmoid(2u)
+        const Scaled s = sigmoid(kGelu2 * fmaf(kGelu3 * z * z, z, z));
+        return z * s.v * s.by;
+    }
     if constexpr (ACT == OZK_ACT_GELU)                             // z Phi(z)
         return fmaf(-near_abs(z), tail_factor(z) * gauss(z), fmaxf(z, 0.f));
     return z;
@@ -57,16 +78,17 @@ template <int ACT> OZK_DEV float activation(float z) {
 template <int ACT> OZK_DEV float derivative(float z) {
     if constexpr (ACT == OZK_ACT_RELU) return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;   // NaN stays
     if constexpr (ACT == OZK_ACT_SILU) {
-        const float s = sigmoid(z);
-        return s * fmaf(near(z), 1.f - s, 1.f);
+        const Scaled s = sigmoid(z);
+        return s.v * fmaf(near(z), 1.f - s.v * s.by, 1.f) * s.by;
     }
     if constexpr (ACT == OZK_ACT_GELU_TANH) {
         const float c = near(z), zz = kGelu3 * c * c;
-        const float s = sigmoid(kGelu2 * fmaf(zz, z, z));
-        return s * fmaf(c * (1.f - s), kGelu2 * fmaf(3.f, zz, 1.f), 1.f);
+        const Scaled s = sigmoid(kGelu2 * fmaf(zz, z, z));
+        return s.v * fmaf(c * (1.f - s.v * s.by), kGelu2 * fmaf(3.f, zz, 1.f), 1.f) * s.by;
     }
     if constexpr (ACT == OZK_ACT_GELU) {   // Phi(z) + z phi(z): d below 0, 1 - d above
-        const float d = gauss(z) * fmaf(-0.398942280f, near_abs(z), tail_factor(z));
+        const Scaled s = gauss_scaled(z);
+        const float d = s.v * fmaf(-0.398942280f, near_abs(z), tail_factor(z)) * s.by;
         return z < 0.f ? d : 1.f - d;
     }
     return 1.f;

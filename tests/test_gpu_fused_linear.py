@@ -487,3 +487,37 @@ def test_rows_off_16_bytes(gpu, M, N, K):
         # rows that are whole pieces apart but begin off them
         x, W = (torch.nn.functional.pad(t, (1, 16 - (K + 1) % 8))[:, 1:1 + K] for t in (x, W))
         _check(ozk.fused_linear(x, W, b, activation=act), x, W, b, None, act)
+
+
+@pytest.mark.parametrize("act", ACTS[2:])
+def test_smallest_results(gpu, act):
+    """Far below 0 results and derivatives keep their relative accuracy as long as they are normal
+    numbers: bf16 has fp32's range, and the exponentials in them leave it first.
+
+    exp2's argument, up to 2^7 in size there, has at most 8 roundings of 2^-24 (gelu_tanh): 2^-14
+    relative in the result; then one rounding to bf16, of the derivative one more factor of that size."""
+    bits = torch.arange(-32768, 0, dtype=torch.int32, device="cuda").to(torch.int16)
+    x = bits.view(BF)
+    x = x[(x.float() <= -8) & (x.float() > -300)]
+    z, h = x.double(), _half(BF)[0]
+    if act == "gelu_tanh":
+        slope = 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z * z)
+        s = torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+        want, steep = z * s, s * (1 + z * slope * (1 - s))
+    else:
+        want, steep = _act(z, act)
+        if act == "gelu":        # Phi + z phi, of which the second is larger
+            steep = 0.5 * torch.erfc(z * -math.sqrt(0.5)) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    for rows in (x, x[:3], x[-40:]):
+        n = rows.shape[0]
+        first = 0 if rows.data_ptr() == x.data_ptr() else x.shape[0] - n
+        a = rows[:, None].contiguous().requires_grad_()
+        y = ozk.fused_linear(a, torch.ones(1, 1, dtype=BF, device="cuda"), activation=act)
+        d, = torch.autograd.grad(y, a, torch.ones_like(y))
+        for got, exact in ((y, want), (d, steep)):
+            exact = exact[first:first + n]
+            off = (got.detach().double()[:, 0] - exact).abs()
+            # (below 2^-126 they may come out as 0)
+            tol = torch.where(exact.abs() >= 2.0 ** -126, (h + 2.0 ** -13) * exact.abs(), 2.0 ** -126)
+            assert bool((off <= tol).all()), [(float(z[first + i]), float(got[i]), float(exact[i]))
+                                              for i in torch.nonzero(off > tol)[:5, 0].tolist()]
