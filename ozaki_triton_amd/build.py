@@ -127,7 +127,7 @@ def build_torch_binding(verbose: bool = False) -> str:
            "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__",
            *[f for d in includes for f in ("-isystem", d)],
            os.path.join(CSRC, "ozk_torch.cpp"), "-o", out + ".tmp", "-L", HERE, "-lozaki_amd", "-L", libs,
-           "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+           "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)

@@ -8,8 +8,10 @@
 // calls here do not take as it is they refuse by returning None, before anything has
 // happened, and the Python functions find out why.
 //
-// A stream comes as its handle.  A backward pass runs on the stream of its forward
-// pass, as autograd has it.
+// A stream comes as its handle.  A backward pass runs on its gradient's device and the
+// current stream there, which its memory comes from, too: autograd has made it that of
+// the forward pass, a caller of the node itself may have another.
+#include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -56,6 +58,10 @@ void refuse_second(const char *name, variable_list &grads) {
     size_t i = 0;
     for (Tensor &g : grads)
         if (g.defined()) g = some[i++];
+}
+
+int64_t current_stream(const Tensor &t) {
+    return (int64_t)c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
 // A backward pass that is captured on `stream` and goes on at a node of the default
@@ -142,17 +148,19 @@ struct Linear : torch::autograd::Function<Linear> {
         const Tensor y = linear_forward(x, W, bias, residual, act, stream, need_z ? &z : nullptr);
         ctx->save_for_backward({need_W ? x : Tensor(), need_x ? W : Tensor(), z});
         ctx->saved_data["a"] =
-            std::vector<int64_t>{act, stream, bias.has_value(), residual.has_value(), x.size(1)};
+            std::vector<int64_t>{act, bias.has_value(), residual.has_value(), x.size(1)};
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const auto a = ctx->saved_data["a"].toIntVector();
-        const int64_t act = a[0], stream = a[1], K = a[4];
-        const bool has_b = a[2], has_r = a[3];
+        const int64_t act = a[0], K = a[3];
+        const bool has_b = a[1], has_r = a[2];
         const variable_list saved = ctx->get_saved_variables();
         variable_list out(6);
         const Tensor &g = grads[0];
         if (!g.defined()) return out;
+        const c10::OptionalDeviceGuard device(g.device());
+        const int64_t stream = current_stream(g);
         refuse_default_stream("fused_linear", stream);
         {
             at::AutoDispatchBelowADInplaceOrView below;
@@ -251,7 +259,7 @@ struct Route : torch::autograd::Function<Route> {
         ctx->mark_non_differentiable({r[0], r[2], r[3], r[4], r[5]});
         ctx->save_for_backward({logits, mask ? *mask : Tensor(), r[0], r[1], r[5]});
         ctx->saved_data["a"] = std::vector<int64_t>{
-            normalize, stream, mask.has_value(), logits.size(0), logits.size(1), k, (int64_t)logits.scalar_type()};
+            normalize, mask.has_value(), logits.size(0), logits.size(1), k, (int64_t)logits.scalar_type()};
         return r;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -259,19 +267,21 @@ struct Route : torch::autograd::Function<Route> {
         const Tensor &gw = grads[1], &gl = grads[6];
         if (!gw.defined() && !gl.defined()) return out;
         const auto a = ctx->saved_data["a"].toIntVector();
-        refuse_default_stream("route_tokens", a[1]);
+        const Tensor &like = gw.defined() ? gw : gl;
+        const c10::OptionalDeviceGuard device(like.device());
+        const int64_t stream = current_stream(like);
+        refuse_default_stream("route_tokens", stream);
         const variable_list saved = ctx->get_saved_variables();
         {
             at::AutoDispatchBelowADInplaceOrView below;
-            const Tensor &like = gw.defined() ? gw : gl;
-            const int64_t T = a[3], E = a[4], k = a[5];
-            saved_as(saved[0], {T, E}, (at::ScalarType)a[6], like);
-            if (a[2]) saved_as(saved[1], {T}, at::kBool, like);
+            const int64_t T = a[2], E = a[3], k = a[4];
+            saved_as(saved[0], {T, E}, (at::ScalarType)a[5], like);
+            if (a[1]) saved_as(saved[1], {T}, at::kBool, like);
             saved_as(saved[2], {T, k}, at::kInt, like);
             saved_as(saved[3], {T, k}, at::kFloat, like);
             saved_as(saved[4], {E}, at::kInt, like);
             const Tensor logits = saved[0].stride(1) == 1 || E == 1 ? saved[0] : saved[0].contiguous();
-            const Tensor mask = a[2] ? saved[1].contiguous() : Tensor(), experts = saved[2].contiguous();
+            const Tensor mask = a[1] ? saved[1].contiguous() : Tensor(), experts = saved[2].contiguous();
             const Tensor weights = saved[3].contiguous(), counts = saved[4].contiguous();
             const Tensor dw = gw.defined() ? gw.contiguous() : Tensor();
             out[0] = at::empty({T, E}, logits.options());
@@ -279,7 +289,7 @@ struct Route : torch::autograd::Function<Route> {
                   ozk_route_backward(ptr(logits), code(logits.scalar_type()), logits.stride(0), ptr(mask), T, E,
                                      k, (int)a[0], (int32_t *)ptr(experts), (float *)ptr(weights),
                                      (int32_t *)ptr(counts), (float *)ptr(dw), (float *)ptr(gl), ptr(out[0]),
-                                     (void *)a[1]));
+                                     (void *)stream));
         }
         variable_list mine = {out[0]};
         refuse_second("route_tokens", mine);

@@ -175,3 +175,49 @@ def test_capture_beside_an_eager_graph(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+
+
+def test_nodes_called_by_hand(gpu):
+    """A backward node called outside autograd's engine runs where it is called: in a capture on
+    another stream than its forward pass's it is captured, and behind work on its own stream."""
+    x, W = (torch.randn(*s, device="cuda").to(F16).requires_grad_() for s in ((64, 72), (80, 72)))
+    logits = torch.randn(40, 8, device="cuda").requires_grad_()
+    y, r = ozk.fused_linear(x, W, activation="silu"), ozk.route_tokens(logits, 2)
+    dy, dw = torch.randn(64, 80, device="cuda").to(F16), torch.randn(40, 2, device="cuda")
+    nothing = [None] * 7
+
+    def route(dw):
+        grads = list(nothing)
+        grads[1] = dw
+        return r.weights.grad_fn(*grads)      # one result: not a tuple
+
+    def calls():
+        dx, dW = y.grad_fn(dy)[:2]
+        return [dx, dW, route(dw)]
+
+    def want():
+        return [*torch.autograd.grad(y, (x, W), dy, retain_graph=True),
+                *torch.autograd.grad(r.weights, logits, dw, retain_graph=True)]
+    assert all(torch.equal(a, b) for a, b in zip(calls(), want()))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for seed in range(3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        dy.copy_(torch.randn(64, 80, device="cuda", generator=g))
+        dw.copy_(torch.randn(40, 2, device="cuda", generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want()))
+    # 40 products of 4096 before dy is there
+    side, a = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(40):
+            a = a @ a * 1e-2
+        dy.copy_(torch.where(a[:64, :80] == a[:64, :80], 2.0, 3.0))
+        dw.fill_(0.5)
+        got = calls()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want()))
