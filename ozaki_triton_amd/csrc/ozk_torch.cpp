@@ -84,6 +84,13 @@ void refuse_default_stream(const char *name, int64_t stream) {
                              "the default stream; delete that graph (its results) before the capture");
 }
 
+// The engine hands a node gradients of its results' shape, type and device; who calls it
+// by hand may not
+void gradient_as(const Tensor &t, at::IntArrayRef sizes, at::ScalarType type, int64_t device) {
+    if (!t.is_cuda() || t.device().index() != device || t.layout() != at::kStrided || t.sizes() != sizes ||
+        t.scalar_type() != type)
+        throw std::runtime_error("a gradient has another shape, type or device than its result");
+}
 // A hook may give back anything for a saved tensor: what the kernels take on trust
 void saved_as(const Tensor &t, at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) {
     if (t.sizes() != sizes || t.scalar_type() != type || t.device() != like.device() || t.layout() != at::kStrided)
@@ -148,17 +155,19 @@ struct Linear : torch::autograd::Function<Linear> {
         const Tensor y = linear_forward(x, W, bias, residual, act, stream, need_z ? &z : nullptr);
         ctx->save_for_backward({need_W ? x : Tensor(), need_x ? W : Tensor(), z});
         ctx->saved_data["a"] =
-            std::vector<int64_t>{act, bias.has_value(), residual.has_value(), x.size(1)};
+            std::vector<int64_t>{act, bias.has_value(), residual.has_value(), x.size(0), W.size(0), x.size(1),
+                                 (int64_t)x.scalar_type(), x.device().index()};
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const auto a = ctx->saved_data["a"].toIntVector();
-        const int64_t act = a[0], K = a[3];
+        const int64_t act = a[0], M = a[3], N = a[4], K = a[5];
         const bool has_b = a[1], has_r = a[2];
         const variable_list saved = ctx->get_saved_variables();
         variable_list out(6);
         const Tensor &g = grads[0];
         if (!g.defined()) return out;
+        gradient_as(g, {M, N}, (at::ScalarType)a[6], a[7]);
         const c10::OptionalDeviceGuard device(g.device());
         const int64_t stream = current_stream(g);
         refuse_default_stream("fused_linear", stream);
@@ -166,7 +175,6 @@ struct Linear : torch::autograd::Function<Linear> {
             at::AutoDispatchBelowADInplaceOrView below;
             const bool need_x = ctx->needs_input_grad(0), need_W = ctx->needs_input_grad(1);
             const bool need_b = has_b && ctx->needs_input_grad(2);
-            const int64_t M = g.size(0), N = g.size(1);
             if (need_W) saved_as(saved[0], {M, K}, g.scalar_type(), g);
             if (need_x) saved_as(saved[1], {N, K}, g.scalar_type(), g);
             if (saved[2].defined()) saved_as(saved[2], {M, N}, g.scalar_type(), g);
@@ -259,7 +267,8 @@ struct Route : torch::autograd::Function<Route> {
         ctx->mark_non_differentiable({r[0], r[2], r[3], r[4], r[5]});
         ctx->save_for_backward({logits, mask ? *mask : Tensor(), r[0], r[1], r[5]});
         ctx->saved_data["a"] = std::vector<int64_t>{
-            normalize, mask.has_value(), logits.size(0), logits.size(1), k, (int64_t)logits.scalar_type()};
+            normalize, mask.has_value(), logits.size(0), logits.size(1), k, (int64_t)logits.scalar_type(),
+            logits.device().index()};
         return r;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -268,13 +277,15 @@ struct Route : torch::autograd::Function<Route> {
         if (!gw.defined() && !gl.defined()) return out;
         const auto a = ctx->saved_data["a"].toIntVector();
         const Tensor &like = gw.defined() ? gw : gl;
+        const int64_t T = a[2], E = a[3], k = a[4];
+        if (gw.defined()) gradient_as(gw, {T, k}, at::kFloat, a[6]);
+        if (gl.defined()) gradient_as(gl, {}, at::kFloat, a[6]);
         const c10::OptionalDeviceGuard device(like.device());
         const int64_t stream = current_stream(like);
         refuse_default_stream("route_tokens", stream);
         const variable_list saved = ctx->get_saved_variables();
         {
             at::AutoDispatchBelowADInplaceOrView below;
-            const int64_t T = a[2], E = a[3], k = a[4];
             saved_as(saved[0], {T, E}, (at::ScalarType)a[5], like);
             if (a[1]) saved_as(saved[1], {T}, at::kBool, like);
             saved_as(saved[2], {T, k}, at::kInt, like);

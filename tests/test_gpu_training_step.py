@@ -221,3 +221,26 @@ def test_nodes_called_by_hand(gpu):
         got = calls()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want()))
+
+
+def test_nodes_called_by_hand_with_other_gradients(gpu):
+    """Gradients of another shape, type or device than the results raise before a launch."""
+    x, b = torch.randn(16, 24, device="cuda").to(F16), torch.zeros(40, device="cuda", dtype=F16).requires_grad_()
+    W = torch.randn(40, 24, device="cuda").to(F16)
+    logits = torch.randn(16, 8, device="cuda").requires_grad_()
+    r = ozk.route_tokens(logits, 2)
+    ok = torch.ones(16, 40, device="cuda", dtype=F16)
+    for y in (ozk.fused_linear(x, W, b), ozk.fused_linear(x, W, b, activation="silu"),
+              ozk.fused_linear(x.clone().requires_grad_(), W)):
+        y.grad_fn(ok)
+        for bad in (ok[:15], ok[:, :39], ok[0], ok.float(), ok.cpu(), ok[None]):
+            with pytest.raises(RuntimeError, match="another shape, type or device"):
+                y.grad_fn(bad)
+    dw, dl = torch.ones(16, 2, device="cuda"), torch.ones((), device="cuda")
+    call = lambda w, l: r.weights.grad_fn(None, w, None, None, None, None, l)  # noqa: E731
+    want, = torch.autograd.grad([r.weights, r.balance_loss], logits, [dw, dl], retain_graph=True)
+    assert torch.equal(call(dw, dl), want)
+    for w, l in ((dw[:15], dl), (dw[:, :1], None), (dw.half(), dl), (dw.cpu(), None), (dw, dl.cpu()),
+                 (None, dl.double()), (None, dl[None])):
+        with pytest.raises(RuntimeError, match="another shape, type or device"):
+            call(w, l)
