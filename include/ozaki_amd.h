@@ -371,7 +371,8 @@ int ozk_orthogonalize(const void *G, int dtype, int64_t batch, int64_t M, int64_
  *   dx = dz W [M, K], dW = dz^T x [N, K], db = sum of the unrounded dz over the
  *   rows [N]; each where its pointer is given.  z as above; not read without act.
  * Its workspace is 256-byte aligned; `want` of the query: 1 dx, 2 dW, 4 db.
- * Rows of 2^22 or more elements apart return OZK_ERR_TOO_LARGE.
+ * Rows of 2^22 or more elements apart return OZK_ERR_TOO_LARGE; with an activation the
+ * backward call has rows of N, rounded up to 8, of its own (from two rows on).
  */
 #define OZK_ACT_NONE 0
 #define OZK_ACT_RELU 1

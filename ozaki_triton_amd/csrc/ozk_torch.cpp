@@ -221,8 +221,14 @@ bool linear_ok(const Tensor &x, const Tensor &W, const std::optional<Tensor> &bi
 std::optional<Tensor> linear(const Tensor &x, const Tensor &W, const std::optional<Tensor> &bias,
                              const std::optional<Tensor> &residual, int64_t act, int64_t stream) {
     if (!linear_ok(x, W, bias, residual)) return std::nullopt;
-    if (at::GradMode::is_enabled() && (x.requires_grad() || W.requires_grad() || (bias && bias->requires_grad()) ||
-                                       (residual && residual->requires_grad())))
+    const bool grad = at::GradMode::is_enabled();
+    const bool products = grad && (x.requires_grad() || W.requires_grad() || (bias && bias->requires_grad()));
+    // what the backward pass would refuse: its dz has rows of N, with an activation padded
+    const int64_t N = W.size(0);
+    if (products && x.size(0) > 1 && (act == OZK_ACT_NONE ? N : (N + 7) / 8 * 8) >= kMaxStride)
+        throw std::runtime_error("fused_linear: results of more than one row have gradients for fewer than 2^22 "
+                                 "columns, got " + std::to_string(N));
+    if (products || (grad && residual && residual->requires_grad()))
         return Linear::apply(x, W, bias, residual, act, stream);
     at::AutoDispatchBelowADInplaceOrView below;
     return linear_forward(x, W, bias, residual, act, stream, nullptr);

@@ -165,7 +165,7 @@ int backward_plan(BackwardPlan &b, const void *dy, int64_t dy_stride, const void
     if (int st = stride_status({dy_stride})) return st;
     const bool act = activation != OZK_ACT_NONE, products = (want & 3) != 0 && M > 0 && N > 0;
     const int64_t padded = round_up(N, 8);
-    if (act && padded >= kMaxStride) return OZK_ERR_TOO_LARGE;
+    if (act && M > 1 && padded >= kMaxStride) return OZK_ERR_TOO_LARGE;
     b = {};
     b.d.dy = (const char *)dy;
     b.d.dy_pitch = dy_stride * 2;
@@ -176,7 +176,7 @@ int backward_plan(BackwardPlan &b, const void *dy, int64_t dy_stride, const void
     b.dz = act && products ? (size_t)round_up(M * padded * 2, 256) : 0;
     b.sums = (want & 4) && M > 0 ? (size_t)round_up((M + b.d.rows - 1) / b.d.rows * N * 4, 256) : 0;
     const char *dz = act ? (const char *)ws : (const char *)dy;
-    const int64_t pitch = act ? padded * 2 : dy_stride * 2;
+    const int64_t pitch = M <= 1 ? 0 : act ? padded * 2 : dy_stride * 2;
     // dx = dz W: the contraction runs along N
     b.dx = {};
     b.dx.A = dz;

@@ -478,6 +478,8 @@ def fused_linear(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor | None = N
         Differentiable in x, W, bias and residual (reverse mode, once): the backward
         pass keeps x W^T + bias in x's dtype where there is an activation, and the
         gradient to it is rounded to that dtype.
+    Rows of 2^22 or more columns are taken one at a time: x of them has one row or W does,
+    and y of them has one where it has a gradient in x, W or bias (RuntimeError).
     """
     _no_tangent("fused_linear", x, W, bias, residual)
     act = _ACTIVATIONS.get(activation, -1)

@@ -521,3 +521,40 @@ def test_smallest_results(gpu, act):
             tol = torch.where(exact.abs() >= 2.0 ** -126, (h + 2.0 ** -13) * exact.abs(), 2.0 ** -126)
             assert bool((off <= tol).all()), [(float(z[first + i]), float(got[i]), float(exact[i]))
                                               for i in torch.nonzero(off > tol)[:5, 0].tolist()]
+
+
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_wide_results(gpu, act):
+    """Rows of 2^22 results and more: a gradient that the backward pass does not take is refused
+    before the forward pass, that of one row has the formula's values."""
+    N, K = (1 << 22) + 3, 8
+    x, W, b, _, dy = _inputs(2, N, K, F16)
+    _check(ozk.fused_linear(x, W, b, activation=act), x, W, b, None, act)
+    for leaf in (x, W, b):
+        leaf.requires_grad_()
+        with pytest.raises(RuntimeError, match="columns"):
+            ozk.fused_linear(x, W, b, activation=act)
+        with torch.no_grad():
+            assert ozk.fused_linear(x, W, b, activation=act).shape == (2, N)
+        leaf.requires_grad_(False)
+    res = dy.clone().requires_grad_()       # its gradient is dy
+    g, = torch.autograd.grad(ozk.fused_linear(x, W, b, activation=act, residual=res), res, dy)
+    assert torch.equal(g, dy)
+    x, dy = x[:1], dy[:1]
+    leaves = [t.requires_grad_() for t in (x, W, b)]
+    dx, dW, db = torch.autograd.grad(ozk.fused_linear(*leaves, activation=act), leaves, dy)
+    x, W, b = (t.detach() for t in leaves)
+    h, least = _half(F16)
+    z = x.double() @ W.double().mT.contiguous() + b.double()
+    dz = dy.double() * _act(z, act)[1]
+    # as in test_gradients: z in 16 bits, dz rounded, the sums of N or one product
+    e = (h * dz.abs() + least + dy.double().abs() * (0.8 * (h * z.abs() + least + (K + 4) * U * 4) + 2 ** -17)
+         if act else torch.zeros_like(dz))
+    for got, want, tol in ((dx, dz @ W.double(), e @ W.double().abs() + (N + 2) * U * ((dz.abs() + e) @ W.double().abs())),
+                           (dW, dz.mT.contiguous() @ x.double(), e.mT.contiguous() @ x.double().abs()),
+                           (db, dz[0], e[0])):
+        tol = tol + (h + U) * (want.abs() + tol) + 2 * least
+        assert bool(((got.double() - want).abs() <= tol).all())
+    # (N terms whose roundings are as good as independent)
+    want = dz @ W.double()
+    assert float((dx.double() - want).norm()) <= 2 * h * float(want.norm()) + 4 * h * float((dz.mT.contiguous() * W.double()).norm())

@@ -190,3 +190,15 @@ def test_a_missing_module_is_named(monkeypatch):
     monkeypatch.setattr(builtins, "__import__", absent)
     with pytest.raises(ImportError, match="_ozk_torch.so is not built"):
         _lib.torch_binding()
+
+
+def test_wide_results_have_the_gradients_of_one_row():
+    """Rows of 2^22 elements: one row of them needs no distance between rows, with an activation as without."""
+    L, n = _lib.load(), ctypes.c_size_t(0)
+    q = lambda M, N, act, dy: L.ozk_linear_backward_workspace_bytes(  # noqa: E731
+        None, dy, None, 8, None, _b(8, 1), act, M, N, 8, 7, ctypes.byref(n))
+    for act in (0, 2):
+        for N in (1 << 22, (1 << 22) - 3, (1 << 23) + 5):
+            assert q(1, N, act, 0) == _lib.OZK_OK
+    assert q(2, 1 << 22, 0, 1 << 22) == q(2, 1 << 22, 2, 1 << 22) == _lib.OZK_ERR_TOO_LARGE
+    assert q(2, (1 << 22) - 8, 2, (1 << 22) - 8) == q(2, (1 << 22) - 1, 0, (1 << 22) - 1) == _lib.OZK_OK
