@@ -136,19 +136,22 @@ template <typename T, bool NT> OZK_DEV void piece_scale(const Piece &c, double b
     const int parts = c.n / V;
     int exponent;
     const float mantissa = (float)frexp(by, &exponent);
+    auto one = [&](float f) {   // the same for every element, wherever it lies
+        if constexpr (sizeof(T) == 4) return (float)((double)f * by);
+        else return __builtin_ldexpf(f * mantissa, exponent);
+    };
     auto scaled = [&](i32x4 v) {
         float f[V];
         values<T>(v, f);
         i32x4 r;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = (float)((double)f[i] * by);
+            for (int i = 0; i < V; ++i) f[i] = one(f[i]);
             __builtin_memcpy(&r, f, 16);
         } else {
             uint16_t e[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                e[i] = to_bits16(__builtin_ldexpf(f[i] * mantissa, exponent), T{});
+            for (int i = 0; i < V; ++i) e[i] = to_bits16(one(f[i]), T{});
             __builtin_memcpy(&r, e, 16);
         }
         return r;
@@ -166,7 +169,7 @@ template <typename T, bool NT> OZK_DEV void piece_scale(const Piece &c, double b
         store16<NT>(c.out + (int64_t)i * 16, scaled(load16<NT>(c.in + (int64_t)i * 16)));
     if ((int)threadIdx.x < c.n - parts * V) {
         const int64_t at = parts * V + threadIdx.x;
-        store_value<T>(c.out, at, (float)((double)load_value<T>(c.in, at) * by));
+        store_value<T>(c.out, at, one(load_value<T>(c.in, at)));
     }
 }
 

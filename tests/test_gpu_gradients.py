@@ -246,3 +246,27 @@ def test_overlaps_of_tensors_with_gaps(gpu):
     views = [base[:, i::3] for i in range(3)]
     before = [v.clone() for v in views]
     _check(before, views, 3.0, ozk.clip_gradients(views, 3.0))
+
+
+def _split_cases(dtype, n):
+    """Values and limits where a factor rounded to 32 bits first and one in 64 bits lead to
+    neighbouring values of the dtype."""
+    g = torch.Generator().manual_seed(3)
+    v = (1 + torch.rand(1 << 20, generator=g)).to(dtype)
+    limit = torch.rand(1 << 20, generator=g, dtype=torch.float64) * math.sqrt(n)
+    by = limit / (math.sqrt(n) * v.double())
+    mantissa, exponent = torch.frexp(by)
+    first = torch.ldexp(v.float() * mantissa.float(), exponent).to(dtype)
+    at = torch.nonzero(first != (v.double() * by).float().to(dtype))[:8, 0]
+    assert len(at) >= 4
+    return [(float(v[i]), float(limit[i])) for i in at]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_equal_values_stay_equal(gpu, dtype):
+    """Wherever they lie: a tensor's last elements are no 16 bytes."""
+    n = 4099
+    for value, limit in _split_cases(dtype, n):
+        t = torch.full((n,), value, device="cuda").to(dtype)
+        ozk.clip_gradients([t], limit)
+        assert bool((t == t[0]).all()), (value, limit)
