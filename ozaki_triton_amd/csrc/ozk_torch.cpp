@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <numeric>
+#include <unordered_set>
 
 #include "../../include/ozaki_amd.h"
 
@@ -64,24 +65,32 @@ int64_t current_stream(const Tensor &t) {
     return (int64_t)c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
-// A backward pass that is captured on `stream` and goes on at a node of the default
-// stream, as a leaf has while an earlier graph of it is alive: the engine would make the
-// default stream wait for the capture, which ends the process.
+// A backward pass that is captured on `stream` and reaches a node of the default stream
+// further on (behind a reshape of x, say), as a leaf has while an earlier graph of it is
+// alive: the engine would make the default stream wait for the capture, which ends the
+// process.
 void refuse_default_stream(const char *name, int64_t stream) {
     const auto node = torch::autograd::get_current_node();
     if (!stream || !node) return;
-    bool found = false;
-    for (const auto &edge : node->next_edges())
-        if (edge.function) {
-            const auto s = edge.function->stream();
-            found |= s && s->id() == 0;
-        }
-    if (!found) return;
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone)
         return;
-    throw std::runtime_error(std::string(name) + ": a captured backward pass reaches a tensor that has a graph on "
-                             "the default stream; delete that graph (its results) before the capture");
+    std::unordered_set<torch::autograd::Node *> seen;
+    std::vector<torch::autograd::Node *> todo = {node.get()};
+    while (!todo.empty()) {
+        torch::autograd::Node *at = todo.back();
+        todo.pop_back();
+        for (size_t i = 0; i < at->next_edges().size(); ++i) {
+            torch::autograd::Node *next = at->next_edge(i).function.get();
+            if (!next || !at->task_should_compute_output(i) || !seen.insert(next).second) continue;
+            const auto s = next->stream();
+            if (s && s->id() == 0)
+                throw std::runtime_error(std::string(name) + ": a captured backward pass reaches a tensor that has a "
+                                         "graph on the default stream; delete that graph (its results) before the "
+                                         "capture");
+            todo.push_back(next);
+        }
+    }
 }
 
 // The engine hands a node gradients of its results' shape, type and device; who calls it

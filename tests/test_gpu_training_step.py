@@ -244,3 +244,43 @@ def test_nodes_called_by_hand_with_other_gradients(gpu):
                  (None, dl.double()), (None, dl[None])):
         with pytest.raises(RuntimeError, match="another shape, type or device"):
             call(w, l)
+
+
+def test_capture_beside_an_eager_graph_further_on(gpu):
+    """The same where the leaf lies behind other nodes: behind the reshape of an x of three dims, or
+    the caller's own operations; a leaf whose gradient is not wanted does not matter."""
+    x = torch.randn(4, 16, 64, device="cuda").to(F16).requires_grad_()
+    W = torch.randn(64, 64, device="cuda").to(F16).requires_grad_()
+    logits = torch.randn(40, 8, device="cuda").requires_grad_()
+    dy, dw = torch.randn(4, 16, 64, device="cuda").to(F16), torch.randn(40, 2, device="cuda")
+    calls = [(lambda: ozk.fused_linear(x, W.detach(), activation="gelu"), x, dy),
+             (lambda: ozk.fused_linear(x.detach(), (2 * W).mT.contiguous()), W, dy),
+             (lambda: ozk.route_tokens(3 * logits.view(8, 40).view(40, 8), 2).weights, logits, dw)]
+    for forward, leaf, seed in calls:
+        want, = torch.autograd.grad(forward(), leaf, seed)
+        keep = forward()
+        with pytest.raises(RuntimeError, match="default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(forward(), leaf, seed)
+        torch.cuda.synchronize()
+        del keep
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(forward(), leaf, seed)
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+    # not wanted: the eager graph holds W alone, the gradient is x's
+    want, = torch.autograd.grad(ozk.fused_linear(x, W), x, dy)
+    keep = ozk.fused_linear(x.detach(), W)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(ozk.fused_linear(x, W), x, dy)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    assert keep.requires_grad
