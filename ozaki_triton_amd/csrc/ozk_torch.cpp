@@ -112,7 +112,7 @@ Tensor rows(const Tensor &t, int64_t &stride) {
     const int64_t n = t.size(0), c = t.size(1), s0 = t.stride(0), s1 = t.stride(1);
     stride = n <= 1 ? 0 : s0;
     if ((s1 == 1 || c <= 1) && stride < kMaxStride) return t;
-    stride = c;
+    stride = n <= 1 ? 0 : c;
     return t.contiguous();
 }
 // W [N, K] with K or N contiguous, and its strides, the contiguous one 1
@@ -128,7 +128,7 @@ Tensor weight(const Tensor &W, int64_t (&s)[2]) {
         s[1] = s_k;
         return W;
     }
-    s[0] = K;
+    s[0] = N > 1 ? K : 0;
     s[1] = 1;
     return W.contiguous();
 }

@@ -558,3 +558,15 @@ def test_wide_results(gpu, act):
     # (N terms whose roundings are as good as independent)
     want = dz @ W.double()
     assert float((dx.double() - want).norm()) <= 2 * h * float(want.norm()) + 4 * h * float((dz.mT.contiguous() * W.double()).norm())
+
+
+def test_one_long_row(gpu):
+    """One row of 2^22 elements has no distance to a next one, also where it comes with gaps."""
+    K = 1 << 22
+    x = torch.randn(K, 2, device="cuda").to(F16)[:, :1].mT
+    V = (torch.randn(K, 3, device="cuda") / math.sqrt(K)).to(F16)
+    _check(ozk.fused_linear(x, V.mT), x, V.mT, None, None, None)
+    w = torch.randn(K, 2, device="cuda").to(F16)[:, 1:].mT / 64
+    _check(ozk.fused_linear(x, w.contiguous()), x, w, None, None, None)
+    w = (torch.randn(K, 2, device="cuda") / 64).to(F16)[:, 1:].mT
+    _check(ozk.fused_linear(x, w), x, w, None, None, None)
