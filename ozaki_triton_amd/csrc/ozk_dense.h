@@ -627,7 +627,7 @@ DensePlan plan_tiles(const DenseParams &p) {
 }
 
 template <typename ST, bool AC, bool BC> hipError_t tile_plan(const DenseParams &p, hipStream_t st) {
-    if (!pieces(p)) {
+    if (!pieces(p)) {   // through registers (and with plan_tiles' K ranges, which know the others)
         if (p.M <= 32) return dense_go<ST, TileShape<1, AC, BC, 32, 64, 1, 4, 2>, false>(p, st);
         return dense_go<ST, TileShape<1, AC, BC, 128, 128, 2, 2, 2>, false>(p, st);
     }

@@ -4,12 +4,14 @@ u = 2^-24 is half a step of fp32, h half a step of the dtype, both relative.  A 
 of n products in fp32, in any order, is off by at most n u times the sum of their
 sizes; activations by their slope (at most 1.13) times that and 2^-18 |z| of their
 own (exp2's argument, the fitted tail); each rounding to the dtype by h."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 import ozaki_triton_amd as ozk
+from ozaki_triton_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -570,3 +572,32 @@ def test_one_long_row(gpu):
     _check(ozk.fused_linear(x, w.contiguous()), x, w, None, None, None)
     w = (torch.randn(K, 2, device="cuda") / 64).to(F16)[:, 1:].mT
     _check(ozk.fused_linear(x, w), x, w, None, None, None)
+
+
+@pytest.mark.parametrize("M, N, K", [(130, 64, 8191), (200, 72, 4099), (129, 520, 16383), (33, 3000, 8191), (500, 64, 16385)])
+@pytest.mark.parametrize("wt", [False, True])
+def test_partial_sums_without_copies(gpu, M, N, K, wt):
+    """The C call with room for the partial sums of K ranges but not for copies of rows off 16 bytes."""
+    L, n = _lib.load(), ctypes.c_size_t(0)
+    for dtype, act in ((BF, "gelu"), (F16, None)):
+        x, W, b, res, _ = _inputs(M, N, K, dtype, wt=wt)
+        s = _lib.i64arr(W.stride())
+        size = lambda k, *strides: (L.ozk_linear_workspace_bytes(  # noqa: E731
+            x.data_ptr(), strides[0], W.data_ptr(), _lib.i64arr(strides[1:]), M, N // 8 * 8, k, ctypes.byref(n)), n.value)
+        # rows that are whole 16 bytes need the partial sums alone
+        status, sums = size(K // 8 * 8, K // 8 * 8, *((1, N // 8 * 8) if wt else (K // 8 * 8, 1)))
+        assert status == _lib.OZK_OK and sums >= 2 * M * (N // 8 * 8) * 4
+        assert L.ozk_linear_workspace_bytes(x.data_ptr(), K, W.data_ptr(), s, M, N, K, ctypes.byref(n)) == _lib.OZK_OK
+        assert n.value > sums
+        for room in (n.value, n.value - 1):
+            ws = torch.full((room + 64,), 0xAB, dtype=torch.uint8, device="cuda")
+            y = torch.full((M, N), math.nan, device="cuda", dtype=dtype)
+            z = torch.full((M, N), math.nan, device="cuda", dtype=dtype)
+            assert L.ozk_linear(x.data_ptr(), K, W.data_ptr(), s, b.data_ptr(), res.data_ptr(), N, ACTS.index(act), M, N, K,
+                                _lib.OZK_BF16 if dtype == BF else _lib.OZK_F16, y.data_ptr(), N, z.data_ptr(),
+                                ws.data_ptr(), room, torch.cuda.current_stream().cuda_stream) == _lib.OZK_OK
+            _check(y, x, W, b, res, act)
+            _check(z, x, W, b, None, None)
+            assert bool((ws[room:] == 0xAB).all())
+        assert L.ozk_linear(x.data_ptr(), K, W.data_ptr(), s, None, None, 0, 0, M, N, K, _lib.OZK_F16, y.data_ptr(), N, None,
+                            ws.data_ptr(), sums // 2, None) == _lib.OZK_ERR_WORKSPACE
