@@ -284,3 +284,35 @@ def test_capture_beside_an_eager_graph_further_on(gpu):
         torch.cuda.synchronize()
         assert torch.equal(got, want)
     assert keep.requires_grad
+
+
+def test_transforms_are_refused(gpu):
+    """Tensors of torch.func's transforms have no memory of their own: an error, never a wrong result."""
+    x, W = torch.randn(4, 16, 24, device="cuda").to(F16), torch.randn(40, 24, device="cuda").to(F16)
+    b, logits = torch.zeros(4, 40, device="cuda", dtype=F16), torch.randn(4, 16, 8, device="cuda")
+    masks = torch.ones(4, 16, dtype=torch.bool, device="cuda")
+    grads = torch.ones(4, 100, device="cuda")
+    calls = [
+        lambda: torch.func.vmap(lambda t: ozk.fused_linear(t, W))(x),
+        lambda: torch.func.vmap(lambda t: ozk.fused_linear(x[0], W, t))(b),
+        lambda: torch.func.vmap(lambda t: ozk.fused_linear(x[0], W, residual=t))(x.new_zeros(4, 16, 40)),
+        lambda: torch.func.vmap(lambda t: ozk.route_tokens(t, 2).weights)(logits),
+        lambda: torch.func.vmap(lambda t: ozk.route_tokens(logits[0], 2, mask=t).weights)(masks),
+        lambda: torch.func.vmap(lambda t: ozk.gradient_norm([t]))(grads),
+        lambda: torch.func.vmap(lambda t: ozk.clip_gradients([t], 1.0))(grads),
+        lambda: torch.func.grad(lambda t: ozk.fused_linear(t, W).float().sum())(x[0]),
+        lambda: torch.func.grad(lambda t: ozk.fused_linear(x[0], t).float().sum())(W),
+        lambda: torch.func.grad(lambda t: ozk.route_tokens(t, 2).balance_loss)(logits[0]),
+        lambda: torch.func.jvp(lambda t: ozk.fused_linear(t, W), (x[0],), (x[1],)),
+    ]
+    t, r = x[0].clone().requires_grad_(), logits[0].clone().requires_grad_()
+    y, w = ozk.fused_linear(t, W, activation="silu"), ozk.route_tokens(r, 2).weights
+    calls += [
+        lambda: torch.autograd.grad(y, t, torch.ones(3, 16, 40, device="cuda", dtype=F16), is_grads_batched=True),
+        lambda: torch.autograd.grad(w, r, torch.ones(3, 16, 2, device="cuda"), is_grads_batched=True),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(RuntimeError):
+            call()
+            print("taken:", i)
+    assert bool((grads == 1).all())
