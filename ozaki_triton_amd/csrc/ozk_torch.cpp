@@ -8,6 +8,9 @@
 // calls here do not take as it is they refuse by returning None, before anything has
 // happened, and the Python functions find out why.
 //
+// A tensor that stands for its memory's negative (the imaginary part of a conjugate) is
+// written out first.
+//
 // A stream comes as its handle.  A backward pass runs on its gradient's device and the
 // current stream there, which its memory comes from, too: autograd has made it that of
 // the forward pass, a caller of the node itself may have another.
@@ -42,6 +45,7 @@ int code(at::ScalarType t) {
                                 : -1;
 }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor written_out(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 Tensor workspace(size_t bytes, const Tensor &like) {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
@@ -104,6 +108,12 @@ void gradient_as(const Tensor &t, at::IntArrayRef sizes, at::ScalarType type, in
 void saved_as(const Tensor &t, at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) {
     if (t.sizes() != sizes || t.scalar_type() != type || t.device() != like.device() || t.layout() != at::kStrided)
         throw std::runtime_error("a saved tensor came back with another shape, type or device");
+}
+
+variable_list saved_of(AutogradContext *ctx) {
+    variable_list saved = ctx->get_saved_variables();
+    for (Tensor &t : saved) t = written_out(t);
+    return saved;
 }
 
 // t [rows, columns] with its columns contiguous, and its rows' distance within the
@@ -172,10 +182,10 @@ struct Linear : torch::autograd::Function<Linear> {
         const auto a = ctx->saved_data["a"].toIntVector();
         const int64_t act = a[0], M = a[3], N = a[4], K = a[5];
         const bool has_b = a[1], has_r = a[2];
-        const variable_list saved = ctx->get_saved_variables();
+        const variable_list saved = saved_of(ctx);
         variable_list out(6);
-        const Tensor &g = grads[0];
-        if (!g.defined()) return out;
+        if (!grads[0].defined()) return out;
+        const Tensor g = written_out(grads[0]);
         gradient_as(g, {M, N}, (at::ScalarType)a[6], a[7]);
         const c10::OptionalDeviceGuard device(g.device());
         const int64_t stream = current_stream(g);
@@ -230,6 +240,10 @@ bool linear_ok(const Tensor &x, const Tensor &W, const std::optional<Tensor> &bi
 std::optional<Tensor> linear(const Tensor &x, const Tensor &W, const std::optional<Tensor> &bias,
                              const std::optional<Tensor> &residual, int64_t act, int64_t stream) {
     if (!linear_ok(x, W, bias, residual)) return std::nullopt;
+    if (x.is_neg() || W.is_neg() || (bias && bias->is_neg()) || (residual && residual->is_neg())) {
+        auto written = [](const std::optional<Tensor> &t) { return t ? t->resolve_neg() : t; };
+        return linear(x.resolve_neg(), W.resolve_neg(), written(bias), written(residual), act, stream);
+    }
     const bool grad = at::GradMode::is_enabled();
     const bool products = grad && (x.requires_grad() || W.requires_grad() || (bias && bias->requires_grad()));
     // what the backward pass would refuse: its dz has rows of N, with an activation padded
@@ -249,7 +263,8 @@ std::optional<Tensor> linear(const Tensor &x, const Tensor &W, const std::option
 variable_list route_forward(const Tensor &logits_, const std::optional<Tensor> &mask_, int64_t k,
                             bool normalize, int64_t stream) {
     const int64_t T = logits_.size(0), E = logits_.size(1), n = T * k;
-    const Tensor logits = logits_.stride(1) == 1 || E == 1 ? logits_ : logits_.contiguous();
+    const Tensor signs = written_out(logits_);
+    const Tensor logits = signs.stride(1) == 1 || E == 1 ? signs : signs.contiguous();
     const Tensor mask = mask_ ? mask_->contiguous() : Tensor();
     const auto ints = logits.options().dtype(at::kInt), floats = logits.options().dtype(at::kFloat);
     const Tensor all = at::empty({3 * n + 2 * E + 1}, ints);
@@ -288,7 +303,7 @@ struct Route : torch::autograd::Function<Route> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         variable_list out(5);
-        const Tensor &gw = grads[1], &gl = grads[6];
+        const Tensor gw = written_out(grads[1]), gl = written_out(grads[6]);
         if (!gw.defined() && !gl.defined()) return out;
         const auto a = ctx->saved_data["a"].toIntVector();
         const Tensor &like = gw.defined() ? gw : gl;
@@ -298,7 +313,7 @@ struct Route : torch::autograd::Function<Route> {
         const c10::OptionalDeviceGuard device(like.device());
         const int64_t stream = current_stream(like);
         refuse_default_stream("route_tokens", stream);
-        const variable_list saved = ctx->get_saved_variables();
+        const variable_list saved = saved_of(ctx);
         {
             at::AutoDispatchBelowADInplaceOrView below;
             saved_as(saved[0], {T, E}, (at::ScalarType)a[5], like);
@@ -359,14 +374,14 @@ bool table_of(const std::vector<Tensor> &in, const std::vector<Tensor> *out, Tab
         const Tensor &g = in[i];
         t.codes[i] = code(g.scalar_type());
         if (t.codes[i] < 0 || g.device() != in[0].device() || !g.is_contiguous() ||
-            (grad && g.requires_grad()))
+            g.is_neg() || (grad && g.requires_grad()))
             return false;
         t.ins[i] = g.data_ptr();
         t.counts[i] = g.numel();
         if (!out) continue;
         const Tensor &o = (*out)[i];
         if (o.scalar_type() != g.scalar_type() || o.device() != g.device() || !o.is_contiguous() ||
-            o.sizes() != g.sizes() || (grad && o.requires_grad()))
+            o.is_neg() || o.sizes() != g.sizes() || (grad && o.requires_grad()))
             return false;
         t.outs[i] = o.data_ptr();
     }

@@ -23,6 +23,8 @@ _CODES = {d: _TORCH_TO_OZK[d] for d in _FLOAT}
 
 def _is_dense(t: torch.Tensor) -> bool:
     """Whether t's elements, in some order, are one range of memory."""
+    if t.is_neg():      # they are the negatives of what is there
+        return False
     if t.is_contiguous():
         return True
     at = 1
@@ -72,7 +74,7 @@ def gradient_norm(grads) -> torch.Tensor:
         if norm is not None:
             return norm
     grads, codes = _checked("gradient_norm", grads)
-    grads = [t if t.is_contiguous() or _is_dense(t) else t.contiguous() for t in grads]
+    grads = [t if t.is_contiguous() or _is_dense(t) else t.contiguous() for t in grads]   # (of any sign)
     dev, n = grads[0].device, len(grads)
     table = _Table(grads, None, codes)
     norm = torch.empty((), dtype=torch.float32, device=dev)
@@ -108,7 +110,7 @@ def clip_gradients(grads, max_norm: float, *, out=None) -> torch.Tensor:
     assert max_norm >= 0, f"max_norm must be >= 0, got {max_norm}"
     ins, to, back = grads, grads, ()
     if out is None:
-        whole = all([t.is_contiguous() for t in grads])
+        whole = all([t.is_contiguous() and not t.is_neg() for t in grads])
     else:
         to, kinds = _checked("clip_gradients", out)
         assert len(to) == len(grads), f"out must have {len(grads)} tensors, got {len(to)}"
@@ -118,7 +120,7 @@ def clip_gradients(grads, max_norm: float, *, out=None) -> torch.Tensor:
                     f"out must match: {tuple(g.shape)} {g.dtype}, got {tuple(o.shape)} {o.dtype}"
         if grads[0].get_device() != to[0].get_device():
             _on_one_gpu(grads[0], to[0])
-        whole = all([t.is_contiguous() for t in grads]) and all([t.is_contiguous() for t in to])
+        whole = all([t.is_contiguous() and not t.is_neg() for t in grads + to])
     outs = to
     if not whole:
         ins, to, back = _through_copies(grads, to)
@@ -149,9 +151,10 @@ def _through_copies(grads, outs):
     assert not _lib.torch_binding().share_memory(grads, outs), "tensors to clip share memory"
     ins, to, back = list(grads), list(outs), []
     for i, (g, o) in enumerate(zip(grads, outs)):
-        if (g is o or g.stride() == o.stride()) and _is_dense(g) or (g.is_contiguous() and o.is_contiguous()):
+        if (g is o or g.stride() == o.stride() or g.is_contiguous() and o.is_contiguous()) \
+                and _is_dense(g) and _is_dense(o):
             continue
-        ins[i] = g.contiguous()
+        ins[i] = g.resolve_neg().contiguous()
         to[i] = torch.empty_like(ins[i])
         back.append((o, to[i]))
     return ins, to, back
