@@ -441,7 +441,9 @@ int ozk_route_backward(const void *logits, int dtype, int64_t l_stride, const vo
  *            with any tensor (OZK_ERR_SHAPE).
  *   norm     one float on the device; the sum of squares is taken in 64 bits, in
  *            the same order every time
- * With a norm of infinity everything finite becomes 0, with NaN everything NaN.
+ * The scaling goes by the norm in 64 bits, also where a float holds it as infinity.
+ * With an infinite element everything finite becomes 0 (with an infinite max_norm
+ * nothing changes), with a NaN everything NaN.
  */
 int ozk_gradient_norm_workspace_bytes(int64_t tensors, size_t *bytes_out);
 

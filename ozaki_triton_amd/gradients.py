@@ -96,7 +96,9 @@ def clip_gradients(grads, max_norm: float, *, out=None) -> torch.Tensor:
         max_norm: >= 0
         out: tensors of the same shapes and dtypes that take the results; default:
              the gradients themselves, in place
-    A norm of infinity makes everything finite 0, one of NaN everything NaN.
+    The scaling goes by the norm in 64 bits, also where float32 holds it as infinity.
+    An infinite element makes everything finite 0 (with an infinite max_norm nothing
+    changes), a NaN everything NaN.
     """
     grads = list(grads)
     out = None if out is None else list(out)

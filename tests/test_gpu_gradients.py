@@ -270,3 +270,19 @@ def test_equal_values_stay_equal(gpu, dtype):
         t = torch.full((n,), value, device="cuda").to(dtype)
         ozk.clip_gradients([t], limit)
         assert bool((t == t[0]).all()), (value, limit)
+
+
+def test_norms_past_float32(gpu):
+    """A norm that float32 holds as infinity scales by its value; an infinite limit changes nothing."""
+    for dtype in (F32, BF):
+        t = [torch.full((n,), 3e38, device="cuda").to(dtype) for n in (3000, 13)]
+        before = [a.clone() for a in t]
+        assert float(ozk.clip_gradients(t, 1.0)) == math.inf
+        u = torch.finfo(dtype).eps / 2 + 4 * U
+        for a, b in zip(t, before):
+            want = b.double() / _norm(before)
+            assert bool(((a.double() - want).abs() <= u * want).all())
+        t = [torch.tensor([1.0, math.inf, -2.0], device="cuda").to(dtype)]
+        before = [a.clone() for a in t]
+        assert float(ozk.clip_gradients(t, math.inf)) == math.inf
+        assert torch.equal(t[0], before[0])
