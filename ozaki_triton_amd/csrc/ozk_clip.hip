@@ -50,8 +50,8 @@ template <typename T> OZK_DEV void values(i32x4 v, float (&f)[16 / sizeof(T)]) {
 
 // 16 bytes of any alignment.  NT: past the caches, for tensors of more than these
 // hold: reads then need not wait for the dirty lines that they would push out of the
-// memory-side cache (512 MiB, norm / norm and scaling: 120 / 297 us without, 81 / 257
-// with).
+// memory-side cache (512 MiB in 60 tensors, a call, norm / norm and scaling in place: 94 /
+// 321 us without, 85 / 274 with).
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <bool NT> OZK_DEV i32x4 load16(const char *p) {
     if constexpr (NT) return __builtin_nontemporal_load((const i32x4_any *)p);

@@ -1,6 +1,7 @@
 // ozk_dense.h -- the product of a linear layer, y = act(x W^T + b) + r, and
 // what its gradients need beside products.  Part of the unit of the grouped
-// products (ozk_grouped.hip), whose tiles and copies it shares.
+// products (ozk_grouped.hip), whose tiles and copies it shares: included there, and
+// nowhere else.
 //
 // Three kernels compute the sums: tiles on the matrix cores (ozk_tile.h) with
 // the epilogue in them, the same with K cut into ranges whose fp32 sums a second
@@ -376,17 +377,16 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Up to 16 rows: bound by reading W once.  A wave takes a range of K; operands go
-// from memory into the matrix cores' registers.  A block of 16 x 16 sums is R = 16
-// / P rows of x by R rows of W, each with P parts of K: index i of either operand
-// is part i / R of row i % R, and of the sums those of equal parts count.  A load
-// then reads P 64-byte pieces of R rows one behind another, which DRAM serves
+// A few rows (dense_few says how many): bound by reading W, once for every 16 of them,
+// which are a row of the grid.  A wave takes a range of K; operands go from memory into
+// the matrix cores' registers.  A block of 16 x 16 sums is R = 16 / P rows of x by R
+// rows of W, each with P parts of K: index i of either operand is part i / R of row
+// i % R, and of the sums those of equal parts count.  A load then reads P 64-byte pieces of R rows one behind another, which DRAM serves
 // faster than pieces of 16 rows, and few rows of W still fill the chip.  The waves'
 // sums and the parts are added in order in the LDS.
 // Loads off a 4-byte address take two to three times as long, so rows of odd
 // addresses (WORDS false) are read as the words that hold them and shifted (1 x 4096
-// x 4097: 16.0 -> 11.7 us, 16 rows 27 -> 16).  More than 16 rows, which such operands may have: so many
-// workgroups beside each other.
+// x 4097: 16.0 -> 11.7 us, 16 rows 27 -> 16).
 // ---------------------------------------------------------------------------
 template <typename ST, int P, int WAVES, int U, bool WORDS>
 __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(DenseParams p) {
@@ -591,10 +591,11 @@ template <typename ST> hipError_t few_plan(const DenseParams &p, hipStream_t st)
 
 // The tile and the K ranges of the shortest time: rounds of workgroups, so many at
 // once, by a round's time, `fixed` + `slope` K / 1024 us (fitted to 477 shapes of 32
-// to 8192 rows and columns, K = 512 to 4096, of operands along K, along N, and of a
-// weight's gradient); partial sums cost a launch and their way through memory.
-// Chosen so, products of those shapes take 1 to 2% longer on average than with the
-// best tile of each.  Measured (us, M x N x K, operands along K, gelu; 32 x 16 / 32 x
+// to 8192 rows and columns, K = 512 to 4096; operands along N have the times of those
+// along K); partial sums cost a launch and their way through memory.  Chosen so,
+// products of those shapes take longer than with the best tile of each, on average / at
+// worst, of operands along K 0.6 / 10%, along N 1.7 / 41% (32 rows: 32 x 16 tiles read 32
+// bytes of a row), of a weight's gradient 1.9 / 18%.  Measured (us, M x N x K, operands along K, gelu; 32 x 16 / 32 x
 // 32 / 64 x 32 / 64 x 64 in two groups of waves / 64 x 64 / 128 x 128 of 4 stages / 128
 // x 128 / 128 x 256 / 256 x 256):
 //     32 x 4096 x 4096      12 / 14 / 15 / 20 / 33 / 31 / 60 / 51 / 96
@@ -672,8 +673,10 @@ template <typename ST> hipError_t dense_plan(const DenseParams &p, hipStream_t s
 
 // Up to 4 rows; of those that the tiles' DMA cannot take up to 32, and up to 128 where
 // W, read once for 16 of them, is small (us, this / tiles: 4 x 4096 x 4096 9.7 / 9.4, 16
-// x 4096 x 4096 11.5 / 9.6; 32 x 4096 x 4097 24 / 52, 48 x 4096 x 4097 35 / 26, 40 x 3648
-// x 1810 11.7 / 40, 96 x 3648 x 1810 17.9 / 18.2, 128 x 1024 x 1001 7.6 / 10.6)
+// x 4096 x 4096 11.5 / 9.6; then this / tiles through registers / tiles on copies: 32 x
+// 4096 x 4097 24 / 45 / 22, 48 x 4096 x 4097 34 / 27 / 26, 40 x 3648 x 1810 12 / 39 / 16, 96 x
+// 3648 x 1810 18 / 39 / 18, 128 x 1024 x 1001 8 / 24 / 11).  Of a large W that costs: 32 x 8192 x
+// 8190 75 / 109 / 64, 32 x 16384 x 4095 116 / 64 / 65.
 bool dense_few(const DenseParams &p) {
     if (p.a_cols || p.b_cols) return false;
     if (p.M <= 4) return true;

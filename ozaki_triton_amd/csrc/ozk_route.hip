@@ -21,8 +21,10 @@
 // wave; the k choices are k rounds of a maximum over keys (the logits' bits in
 // the order of their values, NaN greatest) in lane exchanges.
 //
-// Bound by latency and instructions, not by the bytes (22 MB of the first line are
-// 4.5 us of a copy).  Measured (us, T x E, k; rows / place / gradient):
+// Bound by latency and, with many tokens, instructions, not by the bytes (22 MB of the
+// first line are 4.5 us of a copy): the vector units of the rows kernel are busy 36% of the
+// time with 32768 tokens, where waves wait for each other and for lane exchanges 55% of
+// theirs, and 83% with 300000.  Measured (us, T x E, k; rows / place / gradient):
 //     32768 x 64, 8, fp32   12.3 / 8.3 / 8.8      4099 x 40, 3, bf16   6.2 / 6.9 / 4.4
 //     16 x 16, 2, bf16       6.9 (one launch)
 #include "../../include/ozaki_amd.h"

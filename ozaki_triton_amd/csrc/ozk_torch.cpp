@@ -3,8 +3,8 @@
 // pass needs and calls the C ABI (include/ozaki_amd.h).
 //
 // In C++ because these calls are short: an autograd node in Python costs its two
-// passes 50 us of host time more than one here, and a list of a hundred tensors is
-// looked at in a few us.  Arguments are checked by the Python functions; what the
+// passes 40 us of host time more than one here (a training step through 1999 x 520 x 1000
+// 109 against 69), and a list of a hundred tensors is looked at in a few us.  Arguments are checked by the Python functions; what the
 // calls here do not take as it is they refuse by returning None, before anything has
 // happened, and the Python functions find out why.
 //

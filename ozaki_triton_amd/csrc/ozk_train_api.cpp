@@ -80,8 +80,9 @@ ozk::PackedSizes copies(const ozk::DenseParams &p) {
     if (ozk::dense_few(p)) return {0, 0};
     if (p.a_cols) return ozk::plan_grad_pack(as_grad(p));
     ozk::GroupedParams g = as_grouped(p);
-    // a grouped product has smaller tiles for fewer than 48 rows, this one does not (40 x
-    // 6592 x 2861, us: read as they are 59, copied 25)
+    // a grouped product has smaller tiles for fewer than 48 rows, this one does not (us,
+    // read as they are / copied: 40 x 6592 x 2861 59 / 25, 40 x 4096 x 4097 28 / 26, but 40 x
+    // 8192 x 8190 58 / 69; the rule does not know the K ranges)
     if (g.T > 32 && g.T < 48) g.T = 48;
     return ozk::plan_grouped_pack(g);
 }
