@@ -381,9 +381,10 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseParams p) {
 // which are a row of the grid.  A wave takes a range of K; operands go from memory into
 // the matrix cores' registers.  A block of 16 x 16 sums is R = 16 / P rows of x by R
 // rows of W, each with P parts of K: index i of either operand is part i / R of row
-// i % R, and of the sums those of equal parts count.  A load then reads P 64-byte pieces of R rows one behind another, which DRAM serves
-// faster than pieces of 16 rows, and few rows of W still fill the chip.  The waves'
-// sums and the parts are added in order in the LDS.
+// i % R, and of the sums those of equal parts count.  A load then reads P 64-byte
+// pieces of R rows one behind another, which DRAM serves faster than pieces of 16 rows,
+// and few rows of W still fill the chip.  The waves' sums and the parts are added in
+// order in the LDS.
 // Loads off a 4-byte address take two to three times as long, so rows of odd
 // addresses (WORDS false) are read as the words that hold them and shifted (1 x 4096
 // x 4097: 16.0 -> 11.7 us, 16 rows 27 -> 16).
@@ -595,9 +596,10 @@ template <typename ST> hipError_t few_plan(const DenseParams &p, hipStream_t st)
 // along K); partial sums cost a launch and their way through memory.  Chosen so,
 // products of those shapes take longer than with the best tile of each, on average / at
 // worst, of operands along K 0.6 / 10%, along N 1.7 / 41% (32 rows: 32 x 16 tiles read 32
-// bytes of a row), of a weight's gradient 1.9 / 18%.  Measured (us, M x N x K, operands along K, gelu; 32 x 16 / 32 x
-// 32 / 64 x 32 / 64 x 64 in two groups of waves / 64 x 64 / 128 x 128 of 4 stages / 128
-// x 128 / 128 x 256 / 256 x 256):
+// bytes of a row), of a weight's gradient 1.9 / 18%.
+// Measured (us, M x N x K, operands along K, gelu; 32 x 16 / 32 x 32 / 64 x 32 / 64 x 64 in
+// two groups of waves / 64 x 64 / 128 x 128 of 4 stages / 128 x 128 / 128 x 256 / 256 x
+// 256):
 //     32 x 4096 x 4096      12 / 14 / 15 / 20 / 33 / 31 / 60 / 51 / 96
 //     128 x 4096 x 4096     34 / 24 / 18 / 23 / 34 / 42 / 64 / 61 / 103
 //     512 x 4096 x 4096    124 / 86 / 61 / 42 / 39 / 40 / 63 / 59 / 111

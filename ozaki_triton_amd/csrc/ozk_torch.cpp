@@ -4,9 +4,10 @@
 //
 // In C++ because these calls are short: an autograd node in Python costs its two
 // passes 40 us of host time more than one here (a training step through 1999 x 520 x 1000
-// 109 against 69), and a list of a hundred tensors is looked at in a few us.  Arguments are checked by the Python functions; what the
-// calls here do not take as it is they refuse by returning None, before anything has
-// happened, and the Python functions find out why.
+// 109 against 69), and a list of a hundred tensors is looked at in a few us.  Arguments
+// are checked by the Python functions; what the calls here do not take as it is they
+// refuse by returning None, before anything has happened, and the Python functions find
+// out why.
 //
 // A tensor that stands for its memory's negative (the imaginary part of a conjugate) is
 // written out first.
